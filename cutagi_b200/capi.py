@@ -58,6 +58,18 @@ _SIGNATURES = {
     "tagi_avgpool2d_fwd": [C.POINTER(ConvGeom), _p, _p, _p, _p, _p],
     "tagi_avgpool2d_bwd_state": [C.POINTER(ConvGeom), _p, _p, _p, _p, _p, _p],
     "tagi_add_shortcut": [_p, _p, _p, C.c_size_t, _p, _p, _p],
+    "tagi_ln_fwd": [_i, _i, _i, C.c_float] + [_p] * 11,
+    "tagi_ln_bwd_workspace_bytes": [_i, _i],
+    "tagi_ln_bwd": [_i, _i, _i, _i, C.c_float] + [_p] * 16 + [C.c_size_t, _p],
+    "tagi_route_workspace_bytes": [_i, _i, _i],
+    "tagi_route_fwd": [_i, _i, _i] + [_p] * 9 + [C.c_size_t, _p],
+    "tagi_route_bwd": [_i, _i, _i] + [_p] * 7,
+    "tagi_grouped_linear_fwd": [_i] * 6 + [_p] * 11,
+    "tagi_grouped_linear_bwd_state": [_i] * 4 + [_p] * 8,
+    "tagi_grouped_linear_bwd_param": [_i] * 6 + [_p] * 12,
+    "tagi_combine_fwd": [_i] * 4 + [_p] * 8,
+    "tagi_combine_bwd": [_i] * 4 + [_p] * 11,
+    "tagi_dispatch_bwd": [_i] * 4 + [_p] * 7,
     "tagi_io_create": [C.c_size_t, C.c_size_t, C.c_size_t, C.c_size_t, _i, C.POINTER(_p)],
     "tagi_io_destroy": [_p],
     "tagi_io_host_buffers": [_p, _i, C.POINTER(_p), C.POINTER(_p), C.POINTER(_p)],
@@ -88,7 +100,7 @@ def load():
         for name, args in _SIGNATURES.items():
             fn = getattr(_lib, name)
             fn.argtypes = args
-            fn.restype = _i
+            fn.restype = C.c_size_t if name.endswith("_workspace_bytes") else _i
     return _lib
 
 
@@ -97,8 +109,8 @@ class _Lib:
 
     def __getattr__(self, name):
         fn = getattr(load(), name)
-        if name in ("tagi_get_impl", "tagi_version", "tagi_last_error_string", "tagi_conv2d_workspace_bytes",
-                    "tagi_scratch_bytes"):
+        if name in ("tagi_get_impl", "tagi_version", "tagi_last_error_string", "tagi_scratch_bytes") \
+                or name.endswith("_workspace_bytes"):
             return fn
 
         def checked(*args):

@@ -1,6 +1,6 @@
 """Device-side mirror of the part of the pytagi API that surrounds the hot path (Linear, Conv2d, ReLU, BatchNorm2d,
-AvgPool2d, LayerBlock, ResNetBlock, Sequential, OutputUpdater), with the same names and argument meaning, so that whole
-TAGI training steps run through the C ABI.
+AvgPool2d, LayerNorm, LayerBlock, ResNetBlock, Sequential, OutputUpdater), with the same names and argument meaning, so that
+whole TAGI training steps run through the C ABI; and MixtureOfExperts, the expert layer of token models, which pytagi lacks.
 
 Every arithmetic step is a call into libtagi_b200.so; torch is used for device memory only. The mirror exists for
 parity tests and measurements. Inside cuTAGI the same entry points are reached through the reference's own classes
@@ -12,7 +12,7 @@ import math
 import numpy as np
 import torch
 
-from . import capi
+from . import capi, ops
 from .capi import lib
 
 
@@ -312,6 +312,135 @@ class AvgPool2d(_NoParams):
         return dmu_a, dvar_a
 
 
+class LayerNorm(Linear):
+    """cutagi.LayerNorm(normalized_shape, eps, bias): every sample (token) normalised over all of its features. Parameters
+    start as BatchNorm2d's: mu_w = 1, var_w = 1 / features, mu_b = 0, var_b = 1 / features."""
+
+    def __init__(self, normalized_shape, eps=1e-4, bias=True, gain_weight=1.0, gain_bias=1.0):
+        n = int(np.prod(normalized_shape))
+        self.input_size = self.output_size = n
+        self.eps, self.bias = eps, bias
+        self.load(dict(mu_w=np.ones(n, np.float32), var_w=np.full(n, gain_weight * gain_weight / n, np.float32),
+                       mu_b=np.zeros(n, np.float32), var_b=np.full(n, gain_bias * gain_bias / n, np.float32)))
+
+    def load(self, p):
+        super().load(p)
+        self.mu_w, self.var_w = self.mu_w.reshape(-1), self.var_w.reshape(-1)
+        self.delta_mu_w, self.delta_var_w = self.delta_mu_w.reshape(-1), self.delta_var_w.reshape(-1)
+
+    def init_shape(self, shape):
+        if int(np.prod(shape)) != self.input_size:
+            raise RuntimeError(f"Input size mismatch: {self.input_size} vs {int(np.prod(shape))}")
+        return shape
+
+    def forward(self, mu_a, var_a, jcb, train=True):
+        mu_z, var_z, mu_row, var_row = ops.layer_norm(self.mu_w, self.var_w, self.mu_b, self.var_b, mu_a, var_a, self.eps)
+        self.saved = (mu_a, jcb, mu_row, var_row)
+        return mu_z, var_z, None
+
+    def backward(self, dmu, dvar, state_update=True):
+        mu_a, jcb, mu_row, var_row = self.saved
+        dmu_a, dvar_a = ops.layer_norm_backward(
+            self.mu_w, self.var_w, self.var_b, mu_a, jcb, mu_row, var_row, dmu, dvar, self.eps, state_update,
+            (self.delta_mu_w, self.delta_var_w, self.delta_mu_b, self.delta_var_b))[:2]
+        if self.on_ready is not None:
+            self.on_ready()
+        return dmu_a, dvar_a
+
+
+class GroupedLinear(Linear):
+    """The Linear layers of `experts` experts, one after the other in memory ([experts][outputs][inputs]), run on rows in
+    dispatch order (ops.route). Initialised as Linear. A part of MixtureOfExperts: it is told the dispatch order."""
+
+    def __init__(self, experts, input_size, output_size, bias=True, gain_weight=1.0, gain_bias=1.0, seed=None):
+        self.shape = (experts, output_size, input_size)
+        self.input_size, self.output_size, self.bias = input_size, experts * output_size, bias   # rows that load() expects
+        rng = np.random.default_rng(seed)
+        scale = math.sqrt(1.0 / input_size)
+        rows = self.output_size
+        self.load(dict(mu_w=(rng.standard_normal((rows, input_size)) * gain_weight * scale).astype(np.float32),
+                       var_w=np.full((rows, input_size), (gain_weight * scale) ** 2, np.float32),
+                       mu_b=(rng.standard_normal(rows) * gain_bias * scale).astype(np.float32),
+                       var_b=np.full(rows, (gain_bias * scale) ** 2, np.float32)))
+
+    def load(self, p):
+        super().load(p)
+        for a in ("mu_w", "var_w", "delta_mu_w", "delta_var_w"):
+            setattr(self, a, getattr(self, a).reshape(self.shape))
+        if self.bias:
+            for a in ("mu_b", "var_b", "delta_mu_b", "delta_var_b"):
+                setattr(self, a, getattr(self, a).reshape(self.shape[:2]))
+
+    def forward(self, mu_a, var_a, offsets, token=None):
+        self.saved = (mu_a, offsets, token)
+        return ops.grouped_linear(self.mu_w, self.var_w, self.mu_b, self.var_b, mu_a, var_a, offsets, token)
+
+    def backward(self, dmu, dvar, jcb=None, state_update=True):
+        """State deltas of the rows in dispatch order; jcb: the Jacobian of the same rows."""
+        mu_a, offsets, token = self.saved
+        ops.grouped_linear_param(self.var_w, self.var_b, mu_a, dmu, dvar, offsets, token,
+                                 (self.delta_mu_w, self.delta_var_w, self.delta_mu_b, self.delta_var_b))
+        if self.on_ready is not None:
+            self.on_ready()
+        return ops.grouped_linear_state(self.mu_w, jcb, dmu, dvar, offsets) if state_update else (None, None)
+
+
+class MixtureOfExperts:
+    """An expert layer: a Linear router scores the experts, every token goes through its `top_k` best (Linear, ReLU, Linear),
+    and their outputs are joined with the softmax of the chosen scores as products of Gaussians. Router and experts are
+    updated together: the gates' deltas reach the router through the softmax's Jacobian."""
+
+    def __init__(self, input_size, hidden_size, output_size, num_experts, top_k, bias=True, gain_weight=1.0, gain_bias=1.0,
+                 seed=None):
+        if not 1 <= top_k <= num_experts:
+            raise ValueError(f"top_k: expected 1 to {num_experts} (num_experts), got {top_k}")
+        self.input_size, self.output_size, self.top_k = input_size, output_size, top_k
+        s = [None if seed is None else seed + 1000003 * i for i in range(3)]
+        self.router = Linear(input_size, num_experts, bias, gain_weight, gain_bias, seed=s[0])
+        self.up = GroupedLinear(num_experts, input_size, hidden_size, bias, gain_weight, gain_bias, seed=s[1])
+        self.down = GroupedLinear(num_experts, hidden_size, output_size, bias, gain_weight, gain_bias, seed=s[2])
+        self.act = ReLU()
+
+    def init_shape(self, shape):
+        if int(np.prod(shape)) != self.input_size:
+            raise RuntimeError(f"Input size mismatch: {self.input_size} vs {int(np.prod(shape))}")
+        return (self.output_size,)
+
+    def forward(self, mu_a, var_a, jcb, train=True):
+        mu_s, var_s, _ = self.router.forward(mu_a, var_a, jcb, train)
+        r = ops.route(mu_s, var_s, self.top_k)
+        mu_h, var_h, jcb_h = self.act.forward(*self.up.forward(mu_a, var_a, r.offsets, r.token), None)
+        mu_x, var_x = self.down.forward(mu_h, var_h, r.offsets)
+        self.saved = (r, jcb, jcb_h, mu_x)
+        return (*ops.combine(r.pos, r.mu_g, r.var_g, mu_x, var_x), None)
+
+    def backward(self, dmu, dvar, state_update=True):
+        r, jcb, jcb_h, mu_x = self.saved
+        dmu_x, dvar_x, dmu_g, dvar_g = ops.combine_backward(r.pos, r.mu_g, mu_x, None, dmu, dvar)
+        dmu_h, dvar_h = self.down.backward(dmu_x, dvar_x, jcb_h)
+        dmu_r, dvar_r = self.up.backward(dmu_h, dvar_h, None, state_update)
+        dmu_a, dvar_a = self.router.backward(*ops.route_backward(r, dmu_g, dvar_g), state_update)
+        if not state_update:
+            return None, None
+        dmu_t, dvar_t = ops.dispatch_backward(r.pos, jcb, dmu_r, dvar_r)
+        lib.tagi_add_shortcut(_p(dmu_t), _p(dvar_t), None, dmu_a.numel(), _p(dmu_a), _p(dvar_a), _stream())
+        return dmu_a, dvar_a
+
+    def step(self, batch_size):
+        for layer in (self.router, self.up, self.down):
+            layer.step(batch_size)
+
+    def named(self, prefix, idx):
+        name = f"MixtureOfExperts.{prefix}{idx}"
+        return {f"{name}.router": self.router, f"{name}.up": self.up, f"{name}.down": self.down}
+
+    def _delta_slots(self):
+        return self.down._delta_slots() + self.up._delta_slots() + self.router._delta_slots()
+
+    def delta_tensors(self):
+        return [getattr(o, a) for o, a in self._delta_slots()]
+
+
 fuse_relu = True   # run a Linear / Conv2d layer and the ReLU layer directly behind it as one call
 
 
@@ -580,7 +709,8 @@ class OutputUpdater:
 
 def build(spec, in_shape, seed=None):
     """Sequential from a spec (list of tuples): ("conv", fi, fo, k, stride, pad, pad_type, bias), ("linear", K, N, bias),
-    ("relu",), ("bn", C), ("pool", k, stride, pad, pad_type), ("res", [main spec], [shortcut spec] or None)."""
+    ("relu",), ("bn", C), ("pool", k, stride, pad, pad_type), ("res", [main spec], [shortcut spec] or None), ("ln", n),
+    ("moe", K, hidden, N, experts, top_k, bias)."""
     count = [0]
 
     def next_seed():   # one seed per parameterised layer, so that equally shaped layers do not start identical
@@ -602,6 +732,10 @@ def build(spec, in_shape, seed=None):
                 out.append(MixtureReLU())
             elif kind == "bn":
                 out.append(BatchNorm2d(a[0]))
+            elif kind == "ln":
+                out.append(LayerNorm(a[0]))
+            elif kind == "moe":
+                out.append(MixtureOfExperts(*a[:5], bias=a[5], seed=next_seed()))
             elif kind == "pool":
                 out.append(AvgPool2d(*a))
             elif kind == "res":

@@ -309,6 +309,88 @@ int tagi_avgpool2d_bwd_state(const tagi_conv2d_geom *g, const float *jcb, const 
 int tagi_add_shortcut(const float *mu_s, const float *var_s, const float *jcb, size_t n, float *mu_a, float *var_a,
                       void *stream);
 
+/* ---- Layers of token models: rows (tokens) of features, [rows][n] ------------------------------------------------------
+ * LayerNorm and the parts of an expert layer: the router picks k experts for every token (tagi_route_fwd), each expert's
+ * rows go through its own Linear layer (tagi_grouped_linear_*), and a token's expert rows are joined with their gates
+ * (tagi_combine_fwd); the backward calls take the deltas the other way. cuTAGI has no expert layer; its LayerNorm is
+ * src/layernorm_layer.cpp.
+ * All tensors are contiguous and row-major on the current device. No call keeps state or touches the library's scratch
+ * memory: temporaries live in the caller's workspace (16-byte aligned; its contents mean nothing before or after a call,
+ * and calls that may overlap on the GPU need one each), so calls on several streams and CUDA graphs replayed at the same
+ * time do not meet. No call waits for the host, allocates, or uses floating-point atomics: results repeat bit for bit.
+ * Row counts may be zero (pointers to empty tensors may then be NULL). Any alignment of 4 bytes is accepted; tensors that
+ * are 16-byte aligned with rows of a multiple of four floats are faster. */
+
+/* LayerNorm of every row over its n >= 2 features: mean = sum mu_a / n, var = (sum (mu_a - mean)^2 + sum var_a) / (n - 1),
+ * written to mu_row / var_row [R]; inv = 1 / sqrt(var + eps); mu_z = inv * (mu_a - mean) * mu_w + mu_b;
+ * var_z = inv^2 * (var_a * (mu_w^2 + var_w) + var_w * (mu_a - mean)^2) + var_b. The moments are those of tagi_bn2d_fwd with
+ * the statistics taken along a row. mu_b / var_b may be NULL when has_bias == 0. */
+int tagi_ln_fwd(int R, int n, int has_bias, float eps, const float *mu_w, const float *var_w, const float *mu_b,
+                const float *var_b, const float *mu_a, const float *var_a, float *mu_row, float *var_row, float *mu_z,
+                float *var_z, void *stream);
+/* LayerNorm backward. State deltas (state_update != 0): t = inv * mu_w * jcb; dmu = t * dmu_o; dvar = t^2 * dvar_o (jcb
+ * NULL = 1). Parameter deltas: dmu_w = sum_r u * dmu_o, dvar_w = sum_r u^2 * dvar_o with u = inv * (mu_a - mean) * var_w;
+ * dmu_b = var_b * sum_r dmu_o, dvar_b = var_b^2 * sum_r dvar_o; zeros for R == 0. mu_a / jcb are the layer's saved input,
+ * mu_row / var_row what tagi_ln_fwd wrote. workspace: tagi_ln_bwd_workspace_bytes(R, n) bytes (host helper; 0 = NULL is
+ * fine). */
+size_t tagi_ln_bwd_workspace_bytes(int R, int n);
+int tagi_ln_bwd(int R, int n, int has_bias, int state_update, float eps, const float *mu_w, const float *var_w,
+                const float *var_b, const float *mu_a, const float *jcb, const float *mu_row, const float *var_row,
+                const float *dmu_o, const float *dvar_o, float *dmu, float *dvar, float *dmu_w, float *dvar_w, float *dmu_b,
+                float *dvar_b, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Routing of T tokens to k of E experts (E <= 1024, k <= 32, k <= E) by the score means mu_s [T][E]. Slot j of token t
+ * holds its j-th best expert (equal scores: the lower index first; -0 equals 0); a score of -inf or NaN bars the expert.
+ * Slots that find no expert hold -1 and gates of zero.
+ *   expert [T][k]; gates: mu_g [T][k] = softmax over the token's chosen scores (scores of +inf share evenly),
+ *   var_g_i = sum_j J_ij^2 var_s_j with J_ij = mu_g_i * ((i == j) - mu_g_j); var_s [T][E] may be NULL (zero variances).
+ * Dispatch order: the slots sorted by expert, in slot order within one. offsets [E + 1]: expert e has rows offsets[e] to
+ * offsets[e + 1] - 1, offsets[E] of them in all; token [T * k]: the token of every row, -1 behind the last one; pos
+ * [T][k]: the row of every slot, -1 where it has no expert. workspace: tagi_route_workspace_bytes(T, E, k) bytes. */
+size_t tagi_route_workspace_bytes(int T, int E, int k);
+int tagi_route_fwd(int T, int E, int k, const float *mu_s, const float *var_s, int *expert, float *mu_g, float *var_g,
+                   int *offsets, int *token, int *pos, void *workspace, size_t workspace_bytes, void *stream);
+/* Deltas of the scores [T][E] from deltas of the gates [T][k]: dmu_s_j = sum_i J_ij dmu_g_i, dvar_s_j = sum_i J_ij^2
+ * dvar_g_i over the token's slots; zero for experts that were not chosen. expert, mu_g: what tagi_route_fwd wrote. Deltas
+ * of slots without an expert are not read. */
+int tagi_route_bwd(int T, int E, int k, const int *expert, const float *mu_g, const float *dmu_g, const float *dvar_g,
+                   float *dmu_s, float *dvar_s, void *stream);
+
+/* tagi_linear_fwd for E experts (E <= 1024) at once: weights [E][N][K], biases [E][N]; rows offsets[e] to offsets[e + 1] - 1
+ * of mu_z / var_z [S][N] are expert e's outputs. offsets is a DEVICE array of E + 1 non-decreasing row numbers in [0, S];
+ * rows from offsets[E] on and rows before offsets[0] are left as they were. token (device, S entries) names the row of
+ * mu_a / var_a [R][K] that each output row reads, so the tokens need no copy in dispatch order; NULL: row p reads row p
+ * (then R == S). Bad device data does no harm: offsets are clamped into range, a token outside [0, R) reads as a row of
+ * zeros. */
+int tagi_grouped_linear_fwd(int E, int S, int R, int K, int N, int has_bias, const int *offsets, const int *token,
+                            const float *mu_w, const float *var_w, const float *mu_b, const float *var_b, const float *mu_a,
+                            const float *var_a, float *mu_z, float *var_z, void *stream);
+/* tagi_linear_bwd_state per expert: deltas dmu_z / dvar_z [S][N] and outputs dmu_a / dvar_a [S][K] in dispatch order, jcb
+ * [S][K] the Jacobian of the same rows (NULL = 1; where the input was gathered by token, tagi_dispatch_bwd applies it). */
+int tagi_grouped_linear_bwd_state(int E, int S, int K, int N, const int *offsets, const float *mu_w, const float *jcb,
+                                  const float *dmu_z, const float *dvar_z, float *dmu_a, float *dvar_a, void *stream);
+/* tagi_linear_bwd_param per expert: dmu_w / dvar_w [E][N][K] and, when has_bias, dmu_b / dvar_b [E][N] are written for
+ * every expert, zeros for one without rows. token / R as for the forward pass: the rows of mu_a [R][K] that were read. */
+int tagi_grouped_linear_bwd_param(int E, int S, int R, int K, int N, int has_bias, const int *offsets, const int *token,
+                                  const float *var_w, const float *var_b, const float *mu_a, const float *dmu_z,
+                                  const float *dvar_z, float *dmu_w, float *dvar_w, float *dmu_b, float *dvar_b, void *stream);
+
+/* A token's expert rows joined with its gates, as products of independent Gaussians: over the token's slots with a row
+ * p = pos[t][j] in [0, S): mu_y = sum mu_g * mu_x[p]; var_y = sum var_g * (mu_x[p]^2 + var_x[p]) + mu_g^2 * var_x[p].
+ * mu_x / var_x [S][N], mu_y / var_y [T][N]; zeros for a token without a row. */
+int tagi_combine_fwd(int T, int k, int N, int S, const int *pos, const float *mu_g, const float *var_g, const float *mu_x,
+                     const float *var_x, float *mu_y, float *var_y, void *stream);
+/* Its backward pass: dmu_x[p] = mu_g * jcb[p] * dmu_y[t], dvar_x[p] = (mu_g * jcb[p])^2 * dvar_y[t] (jcb [S][N], NULL = 1;
+ * rows that no slot names are left as they were); gates: dmu_g = sum_n mu_x[p] * dmu_y[t], dvar_g = sum_n mu_x[p]^2 *
+ * dvar_y[t], zero for slots without a row. No two slots may name the same row. */
+int tagi_combine_bwd(int T, int k, int N, int S, const int *pos, const float *mu_g, const float *mu_x, const float *jcb,
+                     const float *dmu_y, const float *dvar_y, float *dmu_x, float *dvar_x, float *dmu_g, float *dvar_g,
+                     void *stream);
+/* Deltas of the tokens from the deltas of the rows they were sent to: dmu_a[t] = jcb[t] * sum dmu_x[p], dvar_a[t] =
+ * jcb[t]^2 * sum dvar_x[p] over the token's slots with a row (jcb [T][N], NULL = 1). */
+int tagi_dispatch_bwd(int T, int k, int N, int S, const int *pos, const float *jcb, const float *dmu_x, const float *dvar_x,
+                      float *dmu_a, float *dvar_a, void *stream);
+
 /* ---- Host I/O path of a training step ------------------------------------------------------------------------------
  * A pipeline owns `depth` slots. A slot holds, in pinned host memory and mirrored on the device, one batch's inputs
  * (in_floats), observations (obs_floats) and selected indices (idx_ints), and a pinned buffer for 2 * out_floats output
