@@ -50,6 +50,7 @@ int linear_tc_set_chunked(int on);
 int linear_tc_set_sm_budget(int sms);
 int linear_tc_set_variant(int v);
 int linear_tc_status(int *out, int reset);
+int grouped_tc_status(int *out, int reset);  // tagi_grouped_tc.cu
 // Implicit Conv2d operand for the pair kernel's A side (forward: receptive fields of the activations; state pass at
 // stride 1: the deltas each input pixel receives). Row R of A is pixel (b, py, px) of a pixel grid OHW / OW per image,
 // column kc = (c, ky, kx); its value is src[b][c][y0 + sign * ky][x0 + sign * kx] with

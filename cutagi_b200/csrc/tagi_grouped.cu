@@ -1,138 +1,10 @@
 // Linear layers grouped by expert: rows [offsets[e], offsets[e + 1]) of the dispatch order go through expert e's weights.
 // The offsets and the gather index are device data, so no pass waits for the host; both are checked where they are read
 // (offsets are clamped to [0, S] and made non-decreasing, a row whose token lies outside [0, R) reads as zero).
-#include "tagi_common.h"
+#include "tagi_grouped.h"
 
 namespace tagi {
 namespace {
-
-enum { FWD = 0, STATE = 1, PARAM = 2 };
-
-struct GroupedArgs {
-    int E, S, R, K, N;
-    const int *offsets, *token;
-    const float *mu_w, *var_w, *mu_b, *var_b, *a0, *a1, *jcb;  // a0, a1: activations (forward) or deltas; x: parameter pass
-    const float *x;
-    float *o0, *o1, *ob0, *ob1;
-};
-
-__device__ __forceinline__ void expert_rows(const GroupedArgs &a, int e, int &r0, int &r1) {
-    r0 = min(max(__ldg(a.offsets + e), 0), a.S);
-    r1 = min(max(__ldg(a.offsets + e + 1), r0), a.S);
-}
-
-// Input row of dispatch row p: -1 when its token is outside the tensor.
-__device__ __forceinline__ int input_row(const GroupedArgs &a, int p) {
-    const int r = a.token ? __ldg(a.token + p) : p;
-    return (unsigned)r < (unsigned)a.R ? r : -1;
-}
-
-constexpr int TILE = 64, KT = 16;
-
-// 64 x 64 tile of both outputs, 256 threads, 4 x 4 outputs each.
-template <int PASS>
-__global__ void __launch_bounds__(256) grouped_tile_kernel(const GroupedArgs a) {
-    __shared__ float sa[2][KT][TILE + 1], sb[2][KT][TILE + 1];
-    int e, r0, r1, m0;
-    if (PASS == PARAM) {
-        e = blockIdx.z;
-        expert_rows(a, e, r0, r1);
-        m0 = blockIdx.y * TILE;
-    } else {
-        int tile = blockIdx.x;
-        for (e = 0; e < a.E; e++) {
-            expert_rows(a, e, r0, r1);
-            const int tiles = (r1 - r0 + TILE - 1) / TILE;
-            if (tile < tiles) break;
-            tile -= tiles;
-        }
-        if (e == a.E) return;
-        m0 = r0 + tile * TILE;
-    }
-    const int c0 = (PASS == PARAM ? blockIdx.x : blockIdx.y) * TILE;
-    const int depth = PASS == FWD ? a.K : PASS == STATE ? a.N : r1 - r0;
-    const int rows = PASS == PARAM ? a.N : r1, cols = PASS == FWD ? a.N : a.K;
-    const size_t wbase = (size_t)e * a.N * a.K;
-    float acc0[4][4] = {}, acc1[4][4] = {};
-    const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
-    for (int k0 = 0; k0 < depth; k0 += KT) {
-        for (int i = threadIdx.x; i < TILE * KT; i += 256) {
-            // consecutive threads run along the dimension that is contiguous in memory
-            const int kk = PASS == PARAM ? i / TILE : i % KT, m = PASS == PARAM ? i % TILE : i / KT;
-            float v0 = 0.f, v1 = 0.f;
-            if (m0 + m < rows && k0 + kk < depth) {
-                if (PASS == FWD) {
-                    const int r = input_row(a, m0 + m);
-                    if (r >= 0) v0 = __ldg(a.a0 + (size_t)r * a.K + k0 + kk), v1 = __ldg(a.a1 + (size_t)r * a.K + k0 + kk);
-                } else if (PASS == STATE) {
-                    v0 = __ldg(a.a0 + (size_t)(m0 + m) * a.N + k0 + kk);
-                    v1 = __ldg(a.a1 + (size_t)(m0 + m) * a.N + k0 + kk);
-                } else {
-                    v0 = __ldg(a.a0 + (size_t)(r0 + k0 + kk) * a.N + m0 + m);
-                    v1 = __ldg(a.a1 + (size_t)(r0 + k0 + kk) * a.N + m0 + m);
-                }
-            }
-            sa[0][kk][m] = v0;
-            sa[1][kk][m] = v1;
-            const int kb = PASS == FWD ? i % KT : i / TILE, c = PASS == FWD ? i / KT : i % TILE;
-            v0 = v1 = 0.f;
-            if (c0 + c < cols && k0 + kb < depth) {
-                if (PASS == FWD) {
-                    v0 = __ldg(a.mu_w + wbase + (size_t)(c0 + c) * a.K + k0 + kb);
-                    v1 = __ldg(a.var_w + wbase + (size_t)(c0 + c) * a.K + k0 + kb);
-                } else if (PASS == STATE) {
-                    v0 = __ldg(a.mu_w + wbase + (size_t)(k0 + kb) * a.K + c0 + c);
-                } else {
-                    const int r = input_row(a, r0 + k0 + kb);
-                    if (r >= 0) v0 = __ldg(a.x + (size_t)r * a.K + c0 + c);
-                }
-            }
-            sb[0][kb][c] = v0;
-            sb[1][kb][c] = PASS == FWD ? v1 : v0 * v0;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int kk = 0; kk < KT; kk++) {
-            float x[4], v[4], w[4], u[4];
-#pragma unroll
-            for (int q = 0; q < 4; q++) {
-                x[q] = sa[0][kk][ty * 4 + q], v[q] = sa[1][kk][ty * 4 + q];
-                w[q] = sb[0][kk][tx * 4 + q], u[q] = sb[1][kk][tx * 4 + q];
-            }
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    acc0[i][j] += x[i] * w[j];
-                    if (PASS == FWD) acc1[i][j] += v[i] * (w[j] * w[j]) + (x[i] * x[i] + v[i]) * u[j];
-                    else acc1[i][j] += v[i] * u[j];
-                }
-        }
-        __syncthreads();
-    }
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int m = m0 + ty * 4 + i, c = c0 + tx * 4 + j;
-            if (m >= rows || c >= cols) continue;
-            float z = acc0[i][j], vz = acc1[i][j];
-            if (PASS == FWD) {
-                if (a.mu_b) z += __ldg(a.mu_b + (size_t)e * a.N + c), vz += __ldg(a.var_b + (size_t)e * a.N + c);
-                a.o0[(size_t)m * a.N + c] = z;
-                a.o1[(size_t)m * a.N + c] = vz;
-            } else if (PASS == STATE) {
-                const float q = a.jcb ? __ldg(a.jcb + (size_t)m * a.K + c) : 1.f;
-                a.o0[(size_t)m * a.K + c] = z * q;
-                a.o1[(size_t)m * a.K + c] = vz * q * q;
-            } else {
-                const size_t o = wbase + (size_t)m * a.K + c;
-                const float s = __ldg(a.var_w + o);
-                a.o0[o] = z * s;
-                a.o1[o] = vz * s * s;
-            }
-        }
-}
 
 // dmu_b = var_b sum dmu_z, dvar_b = var_b^2 sum dvar_z over an expert's rows: 32 features x 8 groups of rows per CTA.
 __global__ void __launch_bounds__(256) grouped_bias_kernel(const GroupedArgs a) {
@@ -201,8 +73,7 @@ int tagi_grouped_linear_fwd(int E, int S, int R, int K, int N, int has_bias, con
     GroupedArgs a{};
     a.E = E, a.S = S, a.R = R, a.K = K, a.N = N, a.offsets = offsets, a.token = token, a.mu_w = mu_w, a.var_w = var_w;
     a.mu_b = has_bias ? mu_b : nullptr, a.var_b = has_bias ? var_b : nullptr, a.a0 = mu_a, a.a1 = var_a, a.o0 = mu_z, a.o1 = var_z;
-    grouped_tile_kernel<FWD><<<dim3(S / TILE + E, (N + TILE - 1) / TILE), 256, 0, static_cast<cudaStream_t>(stream)>>>(a);
-    return launched("grouped_tile_kernel launch");
+    return grouped_tc(FWD, a, static_cast<cudaStream_t>(stream));
 }
 
 int tagi_grouped_linear_bwd_state(int E, int S, int K, int N, const int *offsets, const float *mu_w, const float *jcb,
@@ -219,8 +90,7 @@ int tagi_grouped_linear_bwd_state(int E, int S, int K, int N, const int *offsets
     GroupedArgs a{};
     a.E = E, a.S = S, a.R = S, a.K = K, a.N = N, a.offsets = offsets, a.mu_w = mu_w, a.jcb = jcb, a.a0 = dmu_z, a.a1 = dvar_z;
     a.o0 = dmu_a, a.o1 = dvar_a;
-    grouped_tile_kernel<STATE><<<dim3(S / TILE + E, (K + TILE - 1) / TILE), 256, 0, static_cast<cudaStream_t>(stream)>>>(a);
-    return launched("grouped_tile_kernel launch");
+    return grouped_tc(STATE, a, static_cast<cudaStream_t>(stream));
 }
 
 int tagi_grouped_linear_bwd_param(int E, int S, int R, int K, int N, int has_bias, const int *offsets, const int *token,
@@ -249,8 +119,7 @@ int tagi_grouped_linear_bwd_param(int E, int S, int R, int K, int N, int has_bia
     a.E = E, a.S = S, a.R = R, a.K = K, a.N = N, a.offsets = offsets, a.token = token, a.var_w = var_w, a.x = mu_a;
     a.var_b = has_bias ? var_b : nullptr, a.a0 = dmu_z, a.a1 = dvar_z, a.o0 = dmu_w, a.o1 = dvar_w, a.ob0 = dmu_b, a.ob1 = dvar_b;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    grouped_tile_kernel<PARAM><<<dim3((K + TILE - 1) / TILE, (N + TILE - 1) / TILE, E), 256, 0, st>>>(a);
-    rc = launched("grouped_tile_kernel launch");
+    rc = grouped_tc(PARAM, a, st);
     if (rc != TAGI_OK || !has_bias) return rc;
     grouped_bias_kernel<<<dim3((N + 31) / 32, E), 256, 0, st>>>(a);
     return launched("grouped_bias_kernel launch");

@@ -913,7 +913,11 @@ int linear_tc_status(int *out, int reset) {
     cudaError_t e = cudaMemcpy(out, w, sizeof(int), cudaMemcpyDeviceToHost);
     if (e != cudaSuccess) return cuda_fail(e, "cudaMemcpy(status)");
     if (reset && *out) cudaMemset(w, 0, sizeof(int));
-    return TAGI_OK;
+    // the grouped Linear kernels keep a word of their own (part of the library image: their calls allocate nothing)
+    int grouped = 0;
+    const int rc = grouped_tc_status(&grouped, reset);
+    if (*out == 0) *out = grouped;
+    return rc;
 }
 
 int linear_fwd_tc(const float *mu_w, const float *var_w, const float *mu_b, const float *var_b, const float *mu_a,
