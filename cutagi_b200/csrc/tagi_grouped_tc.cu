@@ -15,12 +15,13 @@
 // followed by mu_w^2.var_a as one contraction of twice the length), done one after the other by the same pair, which
 // finds the second's operands in L2.
 //
-// Roles. Sixteen warps fetch both operands from global memory into registers (gathered rows, ragged edges and any
+// Roles. Eight converter warps fetch both operands from global memory into registers (gathered rows, ragged edges and any
 // alignment cost nothing extra there), form squares, split and store the parts to shared memory in the swizzled layouts
-// the tensor core reads; every chunk later they add its accumulator to their registers. One thread issues the MMAs. Two
-// slots of 64 contraction steps hold 2 x 96 KiB of operands and two accumulators of 256 columns fill tensor memory, so
-// a slot's barriers cover its operands and its accumulator: "full" says both are the MMA's, "done" both are the
-// workers'. The loop runs on across tiles: a tile is written out while the next one's first chunks multiply.
+// the tensor core reads; half a chunk ahead is in flight. Eight summing warps add each chunk's accumulator to their
+// registers and write finished tiles out. One thread issues the MMAs. Two slots of 64 contraction steps hold 2 x 96 KiB of
+// operands and two accumulators of 256 columns fill tensor memory; a slot's "full" barrier counts the converters (operands
+// written) and the summing warps (accumulator read), its "done" barrier the MMAs' completion. Nothing stops at a tile's
+// end: the next tile's operands are converted while the last one's chunks multiply and its sums are written.
 #include "tagi_grouped.h"
 #include "tagi_tc_ptx.cuh"
 
@@ -29,12 +30,14 @@ namespace {
 
 using namespace ptx;
 
-constexpr int WORKERS = 16, THREADS = 32 * (WORKERS + 4);   // the fifth warpgroup: its first warp issues the MMAs
-// Registers of a thread: 640 threads are launched with 96 each; the fifth warpgroup gives up 72, of which each of the
-// other four takes 16 (4 x 128 x 112 + 128 x 24 = 60416 of the 61440 launched).
-constexpr int LAUNCH_REGS = 96, WORKER_REGS = 112, ISSUER_REGS = 24;
-static_assert(WORKERS * WORKER_REGS + 4 * ISSUER_REGS <= (WORKERS + 4) * LAUNCH_REGS, "more registers than the launch has");
+constexpr int SUMMERS = 8, CONVERTERS = 8, ISSUER = SUMMERS + CONVERTERS;   // warps 0-7, 8-15, 16 (17-19 idle)
+constexpr int THREADS = 32 * (ISSUER + 4);
+// Registers of a thread: 640 threads are launched with 96 each; each warpgroup then takes what its role needs.
+constexpr int LAUNCH_REGS = 96, SUMMER_REGS = 144, CONVERTER_REGS = 80, ISSUER_REGS = 24;
+static_assert(SUMMERS * SUMMER_REGS + CONVERTERS * CONVERTER_REGS + 4 * ISSUER_REGS <= (ISSUER + 4) * LAUNCH_REGS,
+              "more registers than the launch has");
 constexpr int KC = 64;                          // contraction steps of a chunk
+constexpr int TASKS = 8;                        // groups of four values a converter thread handles of each operand of a chunk
 constexpr uint32_t PART = 128 * KC * 2;         // one bf16 part of 128 rows (or columns) of a chunk: 16 KiB
 constexpr uint32_t SLOT = 6 * PART;             // hi, mid, lo of A, then of B
 constexpr uint32_t ACC = 256;                   // tensor-memory columns of a slot's accumulator
@@ -51,22 +54,13 @@ struct Item {
 
 __device__ __forceinline__ int round_up(int a, int b) { return (a + b - 1) / b * b; }
 
-// Item j of pair `pair`. With at least two tiles for every pair, a pair does both kinds of a tile in a row; with fewer, the
-// kinds go to different pairs.
+// Item j of pair `pair`. The two kinds of a tile are neighbours, so two pairs work on the same weights at the same time, and
+// a pair's kinds alternate from one item to the next (in the forward pass a variance costs twice a mean).
 template <int PASS>
 __device__ __forceinline__ bool get_item(const GroupedArgs &a, const int *before, int pair, int pairs, int j, Item &it) {
-    const int tiles = before[a.E];
-    int t;
-    if (tiles >= 2 * pairs) {
-        t = pair + (j >> 1) * pairs;
-        it.kind = (j & 1) ? MEAN : VAR;
-        if (t >= tiles) return false;
-    } else {
-        t = pair + j * pairs;
-        if (t >= 2 * tiles) return false;
-        it.kind = t < tiles ? VAR : MEAN;
-        if (t >= tiles) t -= tiles;
-    }
+    const int i = pair + j * pairs, t = i >> 1;
+    if (t >= before[a.E]) return false;
+    it.kind = (i + 2 * t / pairs) & 1;
     int lo = 0, hi = a.E - 1;   // the last expert whose tiles begin at or before t
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
@@ -108,18 +102,31 @@ __device__ __forceinline__ uint32_t top_halves(float a, float b) {   // a's uppe
     asm("prmt.b32 %0, %1, %2, 0x7632;" : "=r"(r) : "r"(__float_as_uint(a)), "r"(__float_as_uint(b)));
     return r;
 }
-__device__ __forceinline__ float rest(float x) { return x - __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
+__device__ __forceinline__ float truncated(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
+// two 32-bit operations as one instruction
+__device__ __forceinline__ void add2(float &a, float &b, float x, float y) {
+    asm("{\n\t.reg .b64 s, t;\n\tmov.b64 s, {%0, %1};\n\tmov.b64 t, {%2, %3};\n\tadd.rn.f32x2 s, s, t;\n\tmov.b64 {%0, %1}, s;\n\t}"
+        : "+f"(a), "+f"(b)
+        : "f"(x), "f"(y));
+}
+__device__ __forceinline__ void subtract_truncated2(float &a, float &b) {
+    const float x = truncated(a), y = truncated(b);
+    asm("{\n\t.reg .b64 s, t;\n\tmov.b64 s, {%0, %1};\n\tmov.b64 t, {%2, %3};\n\tsub.rn.f32x2 s, s, t;\n\tmov.b64 {%0, %1}, s;\n\t}"
+        : "+f"(a), "+f"(b)
+        : "f"(x), "f"(y));
+}
 __device__ __forceinline__ void sts64(uint32_t at, uint32_t a, uint32_t b) {
     asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(a), "r"(b) : "memory");
 }
 // hi, mid, lo of four values to their part tiles
 __device__ __forceinline__ void store_split(uint32_t at, float4 v) {
     sts64(at, top_halves(v.x, v.y), top_halves(v.z, v.w));
-    v.x = rest(v.x), v.y = rest(v.y), v.z = rest(v.z), v.w = rest(v.w);
+    subtract_truncated2(v.x, v.y), subtract_truncated2(v.z, v.w);
     sts64(at + PART, top_halves(v.x, v.y), top_halves(v.z, v.w));
-    v.x = rest(v.x), v.y = rest(v.y), v.z = rest(v.z), v.w = rest(v.w);
+    subtract_truncated2(v.x, v.y), subtract_truncated2(v.z, v.w);
     sts64(at + 2 * PART, top_halves(v.x, v.y), top_halves(v.z, v.w));
 }
+__device__ __forceinline__ float4 squared(float4 v) { return make_float4(v.x * v.x, v.y * v.y, v.z * v.z, v.w * v.w); }
 
 // kind::f16 instruction descriptor: FP32 accumulation, bf16 operands (see make_idesc_tf32 for the fields)
 __host__ __device__ constexpr uint32_t make_idesc_bf16(int M, int N, int a_mn, int b_mn) {
@@ -144,10 +151,11 @@ __device__ __forceinline__ void mma_bf16_pair(uint32_t d, uint32_t a_lo, uint32_
 template <bool MN>
 struct Place {
     // line (row or step) and position (step or row) of the first of this thread's four tasks; tasks are LINES apart
-    static constexpr int LINES = MN ? 16 : 32;
+    static constexpr int LINES = MN ? CONVERTERS : 2 * CONVERTERS;
     static constexpr uint32_t STRIDE = LINES * 128;
     static constexpr uint32_t KSTEP = (MN ? 16 * 128 : 32) >> 4;             // 16 contraction steps, in 16-byte units
     static constexpr uint32_t LBO = MN ? 64 * 128 : 16, SBO = 1024;
+    // warp: 0 .. CONVERTERS - 1
     __device__ static int line(int warp, int lane) { return MN ? warp : warp * 2 + (lane >> 4); }
     __device__ static int along(int lane) { return MN ? lane * 4 : (lane & 15) * 4; }
     __device__ static uint32_t offset(int warp, int lane) {
@@ -173,13 +181,13 @@ __global__ void __launch_bounds__(THREADS, 1) grouped_tc_kernel(const GroupedArg
     const int cta = (int)cluster_ctarank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     if (threadIdx.x == 0) {
         for (int s = 0; s < 2; s++) {
-            mbar_init(full + s, 2 * WORKERS);   // counted in CTA 0
+            mbar_init(full + s, 2 * (SUMMERS + CONVERTERS));   // counted in CTA 0
             mbar_init(done + s, 1);             // commit, multicast to both CTAs
         }
         *abort_flag = 0;
         mbar_init_fence();
     }
-    if (warp == WORKERS) tmem_alloc_pair(tmem_slot, 2 * ACC);
+    if (warp == ISSUER) tmem_alloc_pair(tmem_slot, 2 * ACC);
     if (warp == 0) {
         const int mt = ((PASS == FWD ? a.N : a.K) + 255) / 256;
         int carry = 0;
@@ -211,10 +219,10 @@ __global__ void __launch_bounds__(THREADS, 1) grouped_tc_kernel(const GroupedArg
         tc_fence_after_sync();
     };
 
-    if (warp >= WORKERS) {
+    if (warp >= ISSUER) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(ISSUER_REGS));
         // ---------------------------------------------------------------------------------------------- MMA (CTA 0)
-        if (warp == WORKERS && lane == 0 && cta == 0) {
+        if (warp == ISSUER && lane == 0 && cta == 0) {
             constexpr uint32_t HI = desc_hi(1024, SWZ_128B);
             Item it;
             int i = 0;
@@ -247,162 +255,220 @@ __global__ void __launch_bounds__(THREADS, 1) grouped_tc_kernel(const GroupedArg
         }
         __syncwarp();
         finish();
-        if (warp == WORKERS) tmem_dealloc_pair(*tmem_slot, 2 * ACC);
-    } else {
-        // -------------------------------------------------------------------------------------------------- workers
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(WORKER_REGS));
+        if (warp == ISSUER) tmem_dealloc_pair(*tmem_slot, 2 * ACC);
+    } else if (warp < SUMMERS) {
+        // ------------------------------------------------------------------------------------------- sums and output
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SUMMER_REGS));
         const int quad = warp & 3, group = warp >> 2;
         const uint32_t lane_addr = tmem + ((uint32_t)(quad * 32) << 16);
-        const int a_line = PA::line(warp, lane), a_along = PA::along(lane), b_line = PB::line(warp, lane), b_along = PB::along(lane);
-        const uint32_t a_off = PA::offset(warp, lane), b_off = 3 * PART + PB::offset(warp, lane);
-        float acc[64];
+        float acc[128];
 #pragma unroll
-        for (int x = 0; x < 64; x++) acc[x] = 0.f;
+        for (int x = 0; x < 128; x++) acc[x] = 0.f;
+        if (lane == 0) {   // both accumulators are free
+            mbar_arrive_cluster(full, 0);
+            mbar_arrive_cluster(full + 1, 0);
+        }
         Item it;
-        int j = 0, c = 0;            // item and chunk that is produced
-        int dj = 0, dc = 0, dbn = 0, dchunks = 0;   // item and chunk that is drained
-        bool more = get_item<PASS>(a, before, pair, pairs, 0, it), ok = true;
-        if (more) dbn = it.bn, dchunks = it.chunks;
-        int total = -1;              // chunks in all, once the last one has been produced
-        for (int i = 0; ok; i++) {
-            const int s = i & 1;
-            if (!more) {
-                if (total < 0) total = i;
-                if (i >= total + 2) break;
-            }
-            const uint32_t slot = smem_base + s * SLOT;
-            float4 va[4];
-            int half = 0, kc = 0;
-            if (more) {
-                half = c >= it.nk;
-                kc = (half ? c - it.nk : c) * KC;
-                // A: this CTA's 128 features
-#pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    const int line = a_line + q * PA::LINES;
-                    if (PASS == FWD) {
-                        const int m = it.m0 + cta * 128 + line, k = kc + a_along;
-                        const float *src = it.kind == VAR && !half ? a.var_w : a.mu_w;
-                        va[q] = ld4<VEC>(src + ((size_t)it.e * a.N + m) * a.K + k, m < a.N ? a.K - k : 0);
-                    } else {
-                        const int m = it.m0 + cta * 128 + a_along, k = kc + line;
-                        if (PASS == STATE) {
-                            va[q] = ld4<VEC>(a.mu_w + ((size_t)it.e * a.N + k) * a.K + m, k < a.N ? a.K - m : 0);
-                        } else {
-                            const int r = k < it.depth ? input_row(a, it.p0 + k) : -1;
-                            va[q] = ld4<VEC>(a.x + (size_t)max(r, 0) * a.K + m, r >= 0 ? a.K - m : 0);
-                        }
-                    }
-                }
-            }
-            if (i >= 2) {
-                // the accumulator of chunk i - 2, whose slot becomes free
-                ok = mbar_wait(done + s, ((i - 2) >> 1) & 1, abort_flag, &g_status, ST_TIMEOUT_ACC);
+        int i = 0;
+        bool ok = true;
+        for (int j = 0; ok && get_item<PASS>(a, before, pair, pairs, j, it); j++) {
+            const int per = it.bn >> 1;
+            for (int c = 0; c < it.chunks; c++, i++) {
+                const int s = i & 1;
+                ok = mbar_wait(done + s, (i >> 1) & 1, abort_flag, &g_status, ST_TIMEOUT_ACC);
                 if (!ok) break;
                 tc_fence_after_sync();
-                const int per = dbn >> 2;
                 const uint32_t at = lane_addr + s * ACC + group * per;
 #pragma unroll
-                for (int g = 0; g < 4; g++)
-                    if (g * 16 < per) {
-                        float v[16];
-                        tmem_ld_32x16(at + g * 16, v);
+                for (int g = 0; g < 128; g += 8)
+                    if (g < per) {
+                        float v[8];
+                        tmem_ld_32x8(at + g, v);
 #pragma unroll
-                        for (int x = 0; x < 16; x++) acc[g * 16 + x] += v[x];
+                        for (int x = 0; x < 8; x += 2) add2(acc[g + x], acc[g + x + 1], v[x], v[x + 1]);
                     }
-                if (++dc == dchunks) {
-                    Item o;
-                    get_item<PASS>(a, before, pair, pairs, dj, o);
-                    const int m = o.m0 + cta * 128 + quad * 32 + lane, first = group * per, n = min(per, o.cols - first);
-                    const int ld = PASS == FWD ? a.N : a.K;
-                    if (m < ld) {
-                        const size_t base = ((PASS == PARAM ? (size_t)o.e * a.N : 0) + o.c0 + first) * ld + m;
-                        float *out = (o.kind == VAR ? a.o1 : a.o0) + base;
-                        const float *aux = PASS == PARAM ? a.var_w + base : PASS == STATE && a.jcb ? a.jcb + base : nullptr;
-                        float bias = 0.f;
-                        if (PASS == FWD && a.mu_b) bias = __ldg((o.kind == VAR ? a.var_b : a.mu_b) + (size_t)o.e * a.N + m);
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(full + s, 0);
+            }
+            if (!ok) break;
+            const int m = it.m0 + cta * 128 + quad * 32 + lane, first = group * per, n = min(per, it.cols - first);
+            const int ld = PASS == FWD ? a.N : a.K;
+            const size_t base = ((PASS == PARAM ? (size_t)it.e * a.N : 0) + it.c0 + first) * ld + m;
+            float *out = (it.kind == VAR ? a.o1 : a.o0) + base;
+            const float *aux = PASS == PARAM ? a.var_w + base : PASS == STATE && a.jcb ? a.jcb + base : nullptr;
+            const bool live = m < ld;
+            float bias = 0.f;
+            if (PASS == FWD && a.mu_b && live) bias = __ldg((it.kind == VAR ? a.var_b : a.mu_b) + (size_t)it.e * a.N + m);
 #pragma unroll
-                        for (int g = 0; g < 64; g += 8) {
-                            float f[8];
+            for (int g = 0; g < 128; g += 8) {
+                if (g >= n || !live) break;
+                float f[8];
 #pragma unroll
-                            for (int x = 0; x < 8; x++) {
-                                f[x] = 1.f;
-                                if (PASS != FWD && aux && g + x < n) f[x] = __ldg(aux + (size_t)(g + x) * ld);
-                            }
+                for (int x = 0; x < 8; x++) {
+                    f[x] = 1.f;
+                    if (PASS != FWD && aux && g + x < n) f[x] = __ldg(aux + (size_t)(g + x) * ld);
+                }
 #pragma unroll
-                            for (int x = 0; x < 8; x++)
-                                if (g + x < n) {
-                                    float z = acc[g + x];
-                                    if (PASS == FWD) z += bias;
-                                    else z = o.kind == VAR ? z * f[x] * f[x] : z * f[x];
-                                    out[(size_t)(g + x) * ld] = z;
-                                }
-                        }
+                for (int x = 0; x < 8; x++)
+                    if (g + x < n) {
+                        float z = acc[g + x];
+                        if (PASS == FWD) z += bias;
+                        else z = it.kind == VAR ? z * f[x] * f[x] : z * f[x];
+                        out[(size_t)(g + x) * ld] = z;
                     }
+            }
 #pragma unroll
-                    for (int x = 0; x < 64; x++) acc[x] = 0.f;
-                    dc = 0;
-                    if (get_item<PASS>(a, before, pair, pairs, ++dj, o)) dbn = o.bn, dchunks = o.chunks;
+            for (int x = 0; x < 128; x++) acc[x] = 0.f;
+        }
+        finish();
+    } else {
+        // ------------------------------------------------------------------------------------------------- converters
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CONVERTER_REGS));
+        const int w = warp - SUMMERS;
+        const int a_line = PA::line(w, lane), a_along = PA::along(lane), b_line = PB::line(w, lane), b_along = PB::along(lane);
+        const uint32_t a_off = smem_base + PA::offset(w, lane), b_off = smem_base + 3 * PART + PB::offset(w, lane);
+        float4 va[TASKS], vb[4];
+        // Loads run ahead of the conversion, into registers that were just stored: the item and chunk they belong to are
+        // `nx` and `nc`. rows: the input rows that this lane looked up for its warp (gathered operands).
+        Item nx;
+        int nc = 0, nj = 0, a_rows = -1, b_rows = -1;
+        bool more = get_item<PASS>(a, before, pair, pairs, 0, nx);
+
+        auto chunk_k = [&](const Item &t, int c, int &half) {
+            half = PASS == FWD && c >= t.nk;
+            return (half ? c - t.nk : c) * KC;
+        };
+        auto look_up_a = [&]() {   // parameter pass: lane q < 8 knows the input row of step q * LINES + w of the chunk
+            if (PASS == PARAM) {
+                const int k = nc * KC + a_line + (lane & 7) * PA::LINES;
+                a_rows = k < nx.depth ? input_row(a, nx.p0 + k) : -1;
+            }
+        };
+        auto load_a = [&](int q0) {   // four tasks of the 128 features of this CTA
+            int half;
+            const int kc = chunk_k(nx, nc, half);
+#pragma unroll
+            for (int q = q0; q < q0 + 4; q++) {
+                if (PASS == FWD) {
+                    const int m = nx.m0 + cta * 128 + a_line + q * PA::LINES, k = kc + a_along;
+                    const float *src = nx.kind == VAR && !half ? a.var_w : a.mu_w;
+                    va[q] = ld4<VEC>(src + ((size_t)nx.e * a.N + m) * a.K + k, m < a.N ? a.K - k : 0);
+                } else if (PASS == STATE) {
+                    const int m = nx.m0 + cta * 128 + a_along, k = kc + a_line + q * PA::LINES;
+                    va[q] = ld4<VEC>(a.mu_w + ((size_t)nx.e * a.N + k) * a.K + m, k < a.N ? a.K - m : 0);
+                } else {
+                    const int m = nx.m0 + cta * 128 + a_along, r = __shfl_sync(0xffffffffu, a_rows, q);
+                    va[q] = ld4<VEC>(a.x + (size_t)max(r, 0) * a.K + m, r >= 0 ? a.K - m : 0);
                 }
             }
-            if (!more) continue;
-            const int half_bn = it.bn >> 1;
-            // B: this CTA's half of the columns, two tasks at a time
-            float4 vb[2], vc[2];
-            auto load_b = [&](int h) {
-#pragma unroll
-                for (int q = 0; q < 2; q++) {
-                    const int line = b_line + (h * 2 + q) * PB::LINES;
-                    vc[q] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (PASS == PARAM) {
-                        const int k = kc + line, n = cta * half_bn + b_along;
-                        const float *src = it.kind == VAR ? a.a1 : a.a0;
-                        vb[q] = ld4<VEC>(src + (size_t)(it.p0 + k) * a.N + it.c0 + n, k < it.depth && b_along < half_bn ? it.cols - n : 0);
-                    } else {
-                        const int p = cta * half_bn + line, k = kc + b_along;
-                        const bool live = line < half_bn && p < it.cols;
-                        if (PASS == FWD) {
-                            const int r = live ? input_row(a, it.c0 + p) : -1;
-                            const int valid = r >= 0 ? a.K - k : 0;
-                            const size_t o = (size_t)max(r, 0) * a.K + k;
-                            vb[q] = ld4<VEC>((it.kind == VAR && half ? a.a1 : a.a0) + o, valid);
-                            if (it.kind == VAR && !half) vc[q] = ld4<VEC>(a.a1 + o, valid);
-                        } else {
-                            vb[q] = ld4<VEC>((it.kind == VAR ? a.a1 : a.a0) + (size_t)(it.c0 + p) * a.N + k, live ? a.N - k : 0);
-                        }
-                    }
-                }
-            };
-            auto store_b = [&](int h) {
-#pragma unroll
-                for (int q = 0; q < 2; q++) {
-                    float4 v = vb[q];
-                    if (PASS == FWD && it.kind == VAR && !half) {
-                        v.x = fmaf(v.x, v.x, vc[q].x), v.y = fmaf(v.y, v.y, vc[q].y);
-                        v.z = fmaf(v.z, v.z, vc[q].z), v.w = fmaf(v.w, v.w, vc[q].w);
-                    }
-                    if (PASS == PARAM ? b_along < round_up(half_bn, 64) : b_line + (h * 2 + q) * PB::LINES < half_bn)
-                        store_split(slot + b_off + (h * 2 + q) * PB::STRIDE, v);
-                }
-            };
-            load_b(0);
-            const bool square = it.kind == VAR && (PASS != FWD || half);
-#pragma unroll
-            for (int q = 0; q < 4; q++) {
-                if (square) va[q].x *= va[q].x, va[q].y *= va[q].y, va[q].z *= va[q].z, va[q].w *= va[q].w;
-                store_split(slot + a_off + q * PA::STRIDE, va[q]);
+        };
+        auto look_up_b = [&]() {   // forward pass: lane knows the input row of column lane >> 1 of the warp's tasks
+            if (PASS == FWD) {
+                const int line = (lane >> 1) * PB::LINES + w * 2 + (lane & 1), half_bn = nx.bn >> 1, p = cta * half_bn + line;
+                b_rows = lane < 2 * TASKS && line < half_bn && p < nx.cols ? input_row(a, nx.c0 + p) : -1;
             }
-            store_b(0);
-            load_b(1);
-            store_b(1);
+        };
+        // one task of this CTA's half of the columns; second: the variances that belong to the means (forward pass)
+        auto load_b = [&](int q, bool second) {
+            int half;
+            const int kc = chunk_k(nx, nc, half), half_bn = nx.bn >> 1, line = b_line + q * PB::LINES;
+            if (PASS == PARAM) {
+                const int k = kc + line, n = cta * half_bn + b_along;
+                return ld4<VEC>((nx.kind == VAR ? a.a1 : a.a0) + (size_t)(nx.p0 + k) * a.N + nx.c0 + n,
+                                k < nx.depth && b_along < half_bn ? nx.cols - n : 0);
+            }
+            const int k = kc + b_along;
+            if (PASS == FWD) {
+                const int r = __shfl_sync(0xffffffffu, b_rows, q * 2 + (lane >> 4));
+                return ld4<VEC>((second || (nx.kind == VAR && half) ? a.a1 : a.a0) + (size_t)max(r, 0) * a.K + k, r >= 0 ? a.K - k : 0);
+            }
+            const int p = cta * half_bn + line;
+            return ld4<VEC>((nx.kind == VAR ? a.a1 : a.a0) + (size_t)(nx.c0 + p) * a.N + k, line < half_bn && p < nx.cols ? a.N - k : 0);
+        };
+        // vb: four tasks from q0, or (sums) the means and variances of two
+        auto load_b4 = [&](int q0, bool sums) {
+            if (PASS == FWD && sums) {
+                vb[0] = load_b(q0, false), vb[1] = load_b(q0 + 1, false);
+                vb[2] = load_b(q0, true), vb[3] = load_b(q0 + 1, true);
+            } else {
+#pragma unroll
+                for (int q = 0; q < 4; q++) vb[q] = load_b(q0 + q, false);
+            }
+        };
+        bool ok = true;
+        if (more) {
+            look_up_a();
+            look_up_b();
+            load_b4(0, PASS == FWD && nx.kind == VAR);
+            load_a(0);
+            load_a(4);
+        }
+        for (int i = 0; ok && more; i++) {
+            const int s = i & 1;
+            int half;
+            chunk_k(nx, nc, half);
+            const bool sums = PASS == FWD && nx.kind == VAR && !half, square = nx.kind == VAR && !sums;
+            const int lines = PASS == PARAM ? round_up(nx.bn >> 1, 64) : nx.bn >> 1;   // columns that this CTA holds
+            if (i >= 2) {
+                ok = mbar_wait(done + s, ((i - 2) >> 1) & 1, abort_flag, &g_status, ST_TIMEOUT_EMPTY);
+                if (!ok) break;
+            }
+            auto store_a = [&](int q0) {
+#pragma unroll
+                for (int q = q0; q < q0 + 4; q++)
+                    store_split(a_off + s * SLOT + q * PA::STRIDE, square ? squared(va[q]) : va[q]);
+            };
+            auto store_b = [&](int q, float4 v) {
+                if (PASS == PARAM ? b_along < lines : b_line + q * PB::LINES < lines) store_split(b_off + s * SLOT + q * PB::STRIDE, v);
+            };
+            auto store_b4 = [&](int q0) {
+                if (PASS == FWD && sums) {
+#pragma unroll
+                    for (int q = 0; q < 2; q++) {
+                        const float4 x = vb[q], v = vb[q + 2];
+                        store_b(q0 + q, make_float4(fmaf(x.x, x.x, v.x), fmaf(x.y, x.y, v.y), fmaf(x.z, x.z, v.z), fmaf(x.w, x.w, v.w)));
+                    }
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 4; q++) store_b(q0 + q, vb[q]);
+                }
+            };
+            // Every load is issued two groups of stores before its values are needed. With sums, columns take twice the
+            // registers: they come in four groups, the last two of this chunk (the next cannot be looked up earlier).
+            store_b4(0);
+            load_b4(sums ? 2 : 4, sums);
+            if (PASS == FWD && sums) {
+                store_a(0);
+                store_b4(2);
+                load_b4(4, true);
+                store_a(4);
+                store_b4(4);
+                load_b4(6, true);
+            } else {
+                store_a(0);
+                store_a(4);
+            }
+            Item cur_next = nx;   // the next chunk's item
+            int c_next = nc + 1, j_next = nj;
+            bool has_next = true;
+            if (c_next == nx.chunks) {
+                c_next = 0;
+                has_next = get_item<PASS>(a, before, pair, pairs, ++j_next, cur_next);
+            }
+            store_b4(sums ? 6 : 4);
+            nx = cur_next, nc = c_next, more = has_next;
+            if (more) {
+                look_up_a();
+                if (j_next != nj) look_up_b();
+                load_b4(0, PASS == FWD && nx.kind == VAR && nc < nx.nk);
+                load_a(0);
+                load_a(4);
+            }
+            nj = j_next;
             fence_proxy_async_smem();
-            tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(full + s, 0);
-            if (++c == it.chunks) {
-                c = 0;
-                more = get_item<PASS>(a, before, pair, pairs, ++j, it);
-            }
         }
         finish();
     }
