@@ -50,9 +50,14 @@ using namespace tagi;
 
 extern "C" {
 
+size_t tagi_grouped_linear_workspace_bytes(int S, int R, int K) {
+    if (S <= 0 || R <= 0 || K <= 0) return 0;
+    return (size_t)R * K * sizeof(float);
+}
+
 int tagi_grouped_linear_fwd(int E, int S, int R, int K, int N, int has_bias, const int *offsets, const int *token,
                             const float *mu_w, const float *var_w, const float *mu_b, const float *var_b, const float *mu_a,
-                            const float *var_a, float *mu_z, float *var_z, void *stream) {
+                            const float *var_a, float *mu_z, float *var_z, void *workspace, size_t workspace_bytes, void *stream) {
     int rc = check_grouped(__func__, E, S, K, N, offsets);
     if (rc != TAGI_OK) return rc;
     TAGI_PTR(mu_w);
@@ -70,9 +75,13 @@ int tagi_grouped_linear_fwd(int E, int S, int R, int K, int N, int has_bias, con
     TAGI_PTR(var_a);
     TAGI_PTR(mu_z);
     TAGI_PTR(var_z);
+    const size_t need = tagi_grouped_linear_workspace_bytes(S, R, K);
+    TAGI_REQUIRE(need == 0 || (workspace != nullptr && aligned16(workspace) && workspace_bytes >= need),
+                 "workspace is null, not 16-byte aligned or smaller than tagi_grouped_linear_workspace_bytes");
     GroupedArgs a{};
     a.E = E, a.S = S, a.R = R, a.K = K, a.N = N, a.offsets = offsets, a.token = token, a.mu_w = mu_w, a.var_w = var_w;
     a.mu_b = has_bias ? mu_b : nullptr, a.var_b = has_bias ? var_b : nullptr, a.a0 = mu_a, a.a1 = var_a, a.o0 = mu_z, a.o1 = var_z;
+    a.second = static_cast<float *>(workspace);
     return grouped_tc(FWD, a, static_cast<cudaStream_t>(stream));
 }
 

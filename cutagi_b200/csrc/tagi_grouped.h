@@ -11,6 +11,7 @@ struct GroupedArgs {
     const int *offsets, *token;
     // a0, a1: activations (forward) or deltas (backward); x: input means of the parameter pass
     const float *mu_w, *var_w, *mu_b, *var_b, *a0, *a1, *jcb, *x;
+    float *second;   // forward: workspace for mu_a^2 + var_a, [R][K], 16-byte aligned
     float *o0, *o1, *ob0, *ob1;
 };
 

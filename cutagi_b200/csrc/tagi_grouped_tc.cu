@@ -23,6 +23,9 @@
 // written) and the summing warps (accumulator read), its "done" barrier the MMAs' completion. Nothing stops at a tile's
 // end: the next tile's operands are converted while the last one's chunks multiply and its sums are written.
 #include "tagi_grouped.h"
+
+#include <cstddef>
+
 #include "tagi_tc_ptx.cuh"
 
 namespace tagi {
@@ -30,14 +33,14 @@ namespace {
 
 using namespace ptx;
 
-constexpr int SUMMERS = 8, CONVERTERS = 8, ISSUER = SUMMERS + CONVERTERS;   // warps 0-7, 8-15, 16 (17-19 idle)
+constexpr int SUMMERS = 8, CONVERTERS = 8, ISSUER = SUMMERS + CONVERTERS;   // warps 0-7; 8-11 (A), 12-15 (B); 16 (17-19 idle)
 constexpr int THREADS = 32 * (ISSUER + 4);
 // Registers of a thread: 640 threads are launched with 96 each; each warpgroup then takes what its role needs.
-constexpr int LAUNCH_REGS = 96, SUMMER_REGS = 144, CONVERTER_REGS = 80, ISSUER_REGS = 24;
-static_assert(SUMMERS * SUMMER_REGS + CONVERTERS * CONVERTER_REGS + 4 * ISSUER_REGS <= (ISSUER + 4) * LAUNCH_REGS,
+constexpr int LAUNCH_REGS = 96, SUMMER_REGS = 144, A_REGS = 80, B_REGS = 88, ISSUER_REGS = 24;
+static_assert(SUMMERS * SUMMER_REGS + CONVERTERS / 2 * (A_REGS + B_REGS) + 4 * ISSUER_REGS <= (ISSUER + 4) * LAUNCH_REGS,
               "more registers than the launch has");
 constexpr int KC = 64;                          // contraction steps of a chunk
-constexpr int TASKS = 8;                        // groups of four values a converter thread handles of each operand of a chunk
+constexpr int TASKS = 16;                       // times four values: a converter thread's part of its operand of a chunk
 constexpr uint32_t PART = 128 * KC * 2;         // one bf16 part of 128 rows (or columns) of a chunk: 16 KiB
 constexpr uint32_t SLOT = 6 * PART;             // hi, mid, lo of A, then of B
 constexpr uint32_t ACC = 256;                   // tensor-memory columns of a slot's accumulator
@@ -47,10 +50,28 @@ constexpr int PAIRS = 74;
 __device__ int g_status;  // first wait that ran out, read and cleared by grouped_tc_status
 
 struct Item {
-    int e, m0, c0, cols, bn, kind, depth, p0, nk, chunks;
-    // expert; first feature; first column (row of the output, or output feature in the parameter pass); live columns;
-    // tile width; MEAN or VAR; contraction length; first contraction row (parameter pass); chunks of a contraction; of the item
+    int chunks;                 // of the item; 0: there are no more items
+    int e, m0, c0, cols, bn;    // expert; first feature; first column (output row, or feature in the parameter pass); live columns; width
+    int kind, depth, p0, nk;    // MEAN or VAR; contraction length; first contraction row (parameter pass); chunks of one contraction
 };
+// A warp of each CTA works out the items ahead of the others and hands them over through shared memory.
+struct Record {
+    Item item;
+    int pad[2];
+    int rows[128];              // forward pass: input rows of this CTA's columns, -1 where there is none
+};
+constexpr int RECORDS = 8;
+
+struct Shared {                 // behind the slots
+    uint64_t full[2], done[2], item_full[RECORDS], item_empty[RECORDS];
+    uint32_t tmem;
+    volatile int abort_flag;
+    Record record[RECORDS];
+    alignas(16) int rows[4][16];      // parameter pass: input rows of a chunk's steps, per warp of A
+    float aux[8][3][8][32];     // scale entries on their way to the summing warps: three groups of eight columns each
+    int before[];               // tiles of the experts before e, E + 1 entries
+};
+static_assert(offsetof(Shared, rows) % 16 == 0 && sizeof(Shared) % 8 == 0, "rows are read 16 bytes at a time");
 
 __device__ __forceinline__ int round_up(int a, int b) { return (a + b - 1) / b * b; }
 
@@ -133,61 +154,232 @@ __host__ __device__ constexpr uint32_t make_idesc_bf16(int M, int N, int a_mn, i
     return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(N >> 3) << 17) |
            ((uint32_t)(M >> 4) << 24);
 }
-__device__ __forceinline__ void mma_bf16_pair(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi,
-                                              uint32_t idesc, uint32_t accumulate) {
+// The six products of 16 contraction steps of a slot: operand parts lie PART bytes apart, the high descriptor words are the
+// same for all. One asm block each: building descriptors between the instructions costs the issuing thread more than the
+// tensor core needs for a narrow tile.
+#define GROUPED_MMA(AP, BP, P)                                                        \
+    "add.u32 ra, %1, " AP ";\n\tadd.u32 rb, %2, " BP ";\n\t"                          \
+    "mov.b64 da, {ra, %3};\n\tmov.b64 db, {rb, %3};\n\t"                              \
+    "tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %4, " P ";\n\t"
+static_assert((PART >> 4) == 1024, "part distance in the asm blocks");
+// lo hi, hi lo, mid mid, mid hi, hi mid; accumulate == 0: the first overwrites the accumulator
+__device__ __forceinline__ void mma_small_products(uint32_t d, uint32_t x, uint32_t y, uint32_t hi, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "mov.b64 da, {%1, %2};\n\tmov.b64 db, {%3, %4};\n\t"
-        "tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %5, p;\n\t}"
-        ::"r"(d), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p, t;\n\t.reg .b32 ra, rb;\n\t.reg .b64 da, db;\n\t"
+        "setp.ne.b32 p, %5, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
+        GROUPED_MMA("2048", "0", "p") GROUPED_MMA("0", "2048", "t") GROUPED_MMA("1024", "1024", "t")
+        GROUPED_MMA("1024", "0", "t") GROUPED_MMA("0", "1024", "t") "}"
+        ::"r"(d), "r"(x), "r"(y), "r"(hi), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void mma_large_product(uint32_t d, uint32_t x, uint32_t y, uint32_t hi, uint32_t idesc) {
+    asm volatile(
+        "{\n\t.reg .pred t;\n\t.reg .b32 ra, rb;\n\t.reg .b64 da, db;\n\tsetp.eq.b32 t, 0, 0;\n\t" GROUPED_MMA("0", "0", "t") "}"
+        ::"r"(d), "r"(x), "r"(y), "r"(hi), "r"(idesc)
         : "memory");
 }
 
 // Operands of 128 rows x 64 contraction steps as the tensor core reads them (128-byte swizzle: 16-byte chunk c of line r
-// lies at chunk c ^ (r & 7)).
-//  K-major: line = row, 64 steps of 2 bytes. A lane loads 4 steps; 16 lanes fill a line.
-//  MN-major: line = 64 rows of one step; the 64 lines of rows 0..63 come before those of rows 64..127.
+// lies at chunk c ^ (r & 7)), and which 16 groups of four values each of an operand's 128 threads brings there.
+//  K-major: line = row, 64 steps of 2 bytes. Task t = 4 g + s: row g * 32 + row(), steps s * 16 + 0..3 + along(); a warp
+//  loads 64 consecutive bytes of eight rows and stores to all banks.
+//  MN-major: line = 64 rows of one step; the 64 lines of rows 0..63 come before those of rows 64..127. Task t: step
+//  4 t + row(), rows along() + 0..3; a warp loads 512 consecutive bytes.
 template <bool MN>
 struct Place {
-    // line (row or step) and position (step or row) of the first of this thread's four tasks; tasks are LINES apart
-    static constexpr int LINES = MN ? CONVERTERS : 2 * CONVERTERS;
-    static constexpr uint32_t STRIDE = LINES * 128;
     static constexpr uint32_t KSTEP = (MN ? 16 * 128 : 32) >> 4;             // 16 contraction steps, in 16-byte units
     static constexpr uint32_t LBO = MN ? 64 * 128 : 16, SBO = 1024;
-    // warp: 0 .. CONVERTERS - 1
-    __device__ static int line(int warp, int lane) { return MN ? warp : warp * 2 + (lane >> 4); }
-    __device__ static int along(int lane) { return MN ? lane * 4 : (lane & 15) * 4; }
-    __device__ static uint32_t offset(int warp, int lane) {
-        const uint32_t l = line(warp, lane), c = (lane & 15) >> 1;
-        return (MN ? (lane >> 4) * 8192u : 0u) + l * 128 + ((c ^ (l & 7)) << 4) + (lane & 1) * 8;
+    __device__ static int row(int warp, int lane) { return MN ? warp : warp * 8 + ((lane >> 2) & 3) * 2 + (lane >> 4); }
+    __device__ static int along(int lane) { return MN ? lane * 4 : (lane & 3) * 4; }
+    __device__ static uint32_t base(int warp, int lane) {
+        const uint32_t r = row(warp, lane), c = MN ? (lane & 15) >> 1 : (lane & 3) >> 1;
+        return (MN ? (lane >> 4) * 8192u : 0u) + r * 128 + ((c ^ (r & 7)) << 4) + (lane & 1) * 8;
+    }
+    // where task t goes, from base(): the swizzle's exclusive or with the bits of t that change the chunk or the line
+    __device__ static uint32_t at(uint32_t base, int t) {
+        return MN ? (base ^ ((t & 1) << 6)) + t * 512 : (base ^ ((t & 3) << 5)) + (t >> 2) * 4096;
     }
 };
+
+// Item j, as it was handed over; false when the CTA is aborting. release(): this warp needs the record no longer.
+__device__ __forceinline__ bool take(Shared &sh, int j, Item &t) {
+    t.chunks = 0;
+    if (!mbar_wait(sh.item_full + j % RECORDS, (j / RECORDS) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_RAW)) return false;
+    t = sh.record[j % RECORDS].item;
+    return true;
+}
+__device__ __forceinline__ void release(Shared &sh, int j, int lane) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(sh.item_empty + j % RECORDS);
+}
+
+// What both operands' converters follow: the chunk that is loaded next. It runs ahead of the chunk that is stored.
+struct Cursor {
+    int j, c, chunks, kc;
+    bool var, half;   // of a variance; second half of a forward variance (mu_w^2 . var_a)
+};
+
+// A: 128 features of this CTA. A chunk is fetched whole as soon as the registers of the one before have been stored (one
+// latency a chunk: loads that are waited for in turn would cost one each).
+template <int PASS, bool VEC>
+__device__ __forceinline__ void convert_a(const GroupedArgs &a, Shared &sh, int cta, int w, int lane, uint32_t smem_base) {
+    constexpr bool MN = PASS != FWD;
+    using P = Place<MN>;
+    const int row = P::row(w, lane), along = P::along(lane);
+    const uint32_t to = smem_base + P::base(w, lane);
+    float4 v[TASKS];
+    Cursor cu;
+    size_t base = 0;         // the thread's first element at contraction step 0, without the source
+    int left = 0, nk = 0, depth = 0, p0 = 0;   // left: features from the thread's first one to the end (0: load nothing)
+    int mine = -1;           // parameter pass: the input row that this lane looked up, of step 4 * lane + row of the cursor's chunk
+    auto look_up = [&]() {
+        if (PASS == PARAM) {
+            const int k = cu.kc + (lane & 15) * 4 + row;
+            mine = k < depth ? input_row(a, p0 + k) : -1;
+        }
+    };
+    auto seek = [&](int j) {
+        Item t;
+        take(sh, j, t);
+        release(sh, j, lane);
+        cu.j = j, cu.c = cu.kc = 0, cu.chunks = t.chunks;
+        left = depth = 0;
+        if (t.chunks == 0) return;
+        const int m = t.m0 + cta * 128 + (MN ? along : row);
+        base = PASS == FWD ? ((size_t)t.e * a.N + m) * a.K + along : PASS == STATE ? ((size_t)t.e * a.N + row) * a.K + m : m;
+        left = (PASS == FWD ? a.N : a.K) - m;
+        cu.var = t.kind == VAR, cu.half = false;
+        nk = t.nk, depth = t.depth, p0 = t.p0;
+    };
+    auto advance = [&]() {
+        cu.kc += KC;
+        if (++cu.c == cu.chunks) seek(cu.j + 1);
+        else if (PASS == FWD && cu.c == nk) cu.kc = 0, cu.half = true;
+        look_up();
+    };
+    auto load = [&]() {
+        if (PASS == PARAM) {   // the looked up rows, for all lanes of the warp
+            __syncwarp();
+            if (lane < 16) sh.rows[w][lane] = mine;
+            __syncwarp();
+        }
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            const float *src = PASS == FWD ? (cu.var && !cu.half ? a.var_w : a.mu_w) + base + cu.kc + (size_t)(g * 32) * a.K
+                               : PASS == STATE ? a.mu_w + base + (size_t)(cu.kc + g * 16) * a.K : a.x + base;
+            int4 r = make_int4(-1, -1, -1, -1);
+            if (PASS == PARAM) r = *reinterpret_cast<const int4 *>(&sh.rows[w][g * 4]);
+#pragma unroll
+            for (int s = 0; s < 4; s++) {
+                const int rs = s == 0 ? r.x : s == 1 ? r.y : s == 2 ? r.z : r.w;
+                if (PASS == FWD) v[g * 4 + s] = ld4<VEC>(src + s * 16, g * 32 < left ? a.K - cu.kc - along - s * 16 : 0);
+                else if (PASS == STATE) v[g * 4 + s] = ld4<VEC>(src + (size_t)(s * 4) * a.K, cu.kc + (g * 4 + s) * 4 + row < a.N ? left : 0);
+                else v[g * 4 + s] = ld4<VEC>(src + (size_t)max(rs, 0) * a.K, rs >= 0 ? left : 0);
+            }
+        }
+    };
+    seek(0);
+    look_up();
+    for (int i = 0; cu.chunks > 0; i++) {
+        const int s = i & 1;
+        const bool square = cu.var && (PASS != FWD || cu.half);
+        load();
+        advance();   // and looks up what the next load needs
+        if (i >= 2 && !mbar_wait(sh.done + s, ((i - 2) >> 1) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_EMPTY)) return;
+#pragma unroll
+        for (int q = 0; q < TASKS; q++) store_split(P::at(to + s * SLOT, q), square ? squared(v[q]) : v[q]);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(sh.full + s, 0);
+    }
+}
+
+// B: this CTA's half of the tile's columns, as A.
+template <int PASS, bool VEC>
+__device__ __forceinline__ void convert_b(const GroupedArgs &a, Shared &sh, int cta, int w, int lane, uint32_t smem_base) {
+    constexpr bool MN = PASS == PARAM;
+    using P = Place<MN>;
+    const int row = P::row(w, lane), along = P::along(lane);
+    const uint32_t to = smem_base + 3 * PART + P::base(w, lane);
+    float4 v[TASKS];
+    Cursor cu;
+    int rows[4];             // forward pass: input rows of the thread's four columns
+    size_t base = 0;         // state, parameter pass: the thread's first element at contraction step 0
+    int left = 0, half_bn = 0, nk = 0, depth = 0;   // left: columns from the thread's first one to the end of the CTA's
+    auto seek = [&](int j) {
+        Item t;
+        take(sh, j, t);
+        cu.j = j, cu.c = cu.kc = 0, cu.chunks = t.chunks, cu.var = t.kind == VAR, cu.half = false;
+        half_bn = t.chunks ? t.bn >> 1 : 0;
+        const int n = cta * half_bn + (MN ? along : row);
+        left = t.chunks == 0 ? 0 : MN ? (along < half_bn ? t.cols - n : 0) : min(half_bn - row, t.cols - n);
+        nk = t.nk, depth = t.chunks ? t.depth : 0;
+        if (PASS == FWD) {
+#pragma unroll
+            for (int g = 0; g < 4; g++) rows[g] = g * 32 < left ? sh.record[j % RECORDS].rows[g * 32 + row] : -1;
+        } else {
+            base = PASS == STATE ? (size_t)(t.c0 + n) * a.N + along : (size_t)(t.p0 + row) * a.N + t.c0 + n;
+        }
+        release(sh, j, lane);
+    };
+    auto advance = [&]() {
+        cu.kc += KC;
+        if (++cu.c == cu.chunks) seek(cu.j + 1);
+        else if (PASS == FWD && cu.c == nk) cu.kc = 0, cu.half = true;
+    };
+    auto load = [&](int g) {
+        const float *src = PASS == FWD ? (!cu.var ? a.a0 : cu.half ? a.a1 : a.second) + (size_t)max(rows[g], 0) * a.K + cu.kc + along
+                                       : (cu.var ? a.a1 : a.a0) + base + (PASS == STATE ? (size_t)(g * 32) * a.N + cu.kc : (size_t)(cu.kc + g * 16) * a.N);
+#pragma unroll
+        for (int s = 0; s < 4; s++) {
+            if (PASS == FWD) v[g * 4 + s] = ld4<VEC>(src + s * 16, rows[g] >= 0 ? a.K - cu.kc - along - s * 16 : 0);
+            else if (PASS == STATE) v[g * 4 + s] = ld4<VEC>(src + s * 16, g * 32 < left ? a.N - cu.kc - along - s * 16 : 0);
+            else v[g * 4 + s] = ld4<VEC>(src + (size_t)(s * 4) * a.N, cu.kc + (g * 4 + s) * 4 + row < depth ? left : 0);
+        }
+    };
+    seek(0);
+    for (int i = 0; cu.chunks > 0; i++) {
+        const int s = i & 1, lines = half_bn;
+#pragma unroll
+        for (int g = 0; g < 4; g++) load(g);
+        advance();
+        if (i >= 2 && !mbar_wait(sh.done + s, ((i - 2) >> 1) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_EMPTY)) return;
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+            if (MN || g * 32 < lines) {   // narrow tiles have no columns for the later groups
+#pragma unroll
+                for (int q = g * 4; q < g * 4 + 4; q++)
+                    if (MN ? along < round_up(lines, 64) : g * 32 + row < lines) store_split(P::at(to + s * SLOT, q), v[q]);
+            }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(sh.full + s, 0);
+    }
+}
 
 template <int PASS, bool VEC>
 __global__ void __launch_bounds__(THREADS, 1) grouped_tc_kernel(const GroupedArgs a) {
     constexpr bool A_MN = PASS != FWD, B_MN = PASS == PARAM;
-    using PA = Place<A_MN>;
+    using PA = Place<A_MN>;   // layouts of the operands
     using PB = Place<B_MN>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    uint8_t *behind = smem_raw + (smem_base - smem_u32(smem_raw)) + 2 * SLOT;
-    uint64_t *full = reinterpret_cast<uint64_t *>(behind), *done = full + 2;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(done + 2);
-    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
-    int *before = reinterpret_cast<int *>(tmem_slot + 2);   // tiles of the experts before e, E + 1 entries
-
+    Shared &sh = *reinterpret_cast<Shared *>(smem_raw + (smem_base - smem_u32(smem_raw)) + 2 * SLOT);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int cta = (int)cluster_ctarank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     if (threadIdx.x == 0) {
         for (int s = 0; s < 2; s++) {
-            mbar_init(full + s, 2 * (SUMMERS + CONVERTERS));   // counted in CTA 0
-            mbar_init(done + s, 1);             // commit, multicast to both CTAs
+            mbar_init(sh.full + s, 2 * (SUMMERS + CONVERTERS));   // counted in CTA 0
+            mbar_init(sh.done + s, 1);                            // commit, multicast to both CTAs
         }
-        *abort_flag = 0;
+        for (int s = 0; s < RECORDS; s++) {
+            mbar_init(sh.item_full + s, 1);
+            mbar_init(sh.item_empty + s, SUMMERS + CONVERTERS + (cta == 0));   // CTA 0: and the issuing thread
+        }
+        sh.abort_flag = 0;
         mbar_init_fence();
     }
-    if (warp == ISSUER) tmem_alloc_pair(tmem_slot, 2 * ACC);
+    if (warp == ISSUER) tmem_alloc_pair(&sh.tmem, 2 * ACC);
     if (warp == 0) {
         const int mt = ((PASS == FWD ? a.N : a.K) + 255) / 256;
         int carry = 0;
@@ -201,16 +393,16 @@ __global__ void __launch_bounds__(THREADS, 1) grouped_tc_kernel(const GroupedArg
                 const int u = __shfl_up_sync(0xffffffffu, s, o);
                 if (lane >= o) s += u;
             }
-            if (e0 + lane < a.E) before[e0 + lane] = carry + s - v;
+            if (e0 + lane < a.E) sh.before[e0 + lane] = carry + s - v;
             carry += __shfl_sync(0xffffffffu, s, 31);
         }
-        if (lane == 0) before[a.E] = carry;
+        if (lane == 0) sh.before[a.E] = carry;
     }
     tc_fence_before_sync();
     __syncthreads();
     cluster_sync_all();   // the peer's barriers exist before anyone arrives on them
     tc_fence_after_sync();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = sh.tmem;
     // neither CTA frees tensor memory or leaves while the other may still signal or read it
     auto finish = [&]() {
         tc_fence_before_sync();
@@ -227,35 +419,46 @@ __global__ void __launch_bounds__(THREADS, 1) grouped_tc_kernel(const GroupedArg
             Item it;
             int i = 0;
             bool ok = true;
-            for (int j = 0; ok && get_item<PASS>(a, before, pair, pairs, j, it); j++) {
+            for (int j = 0; ok && take(sh, j, it) && it.chunks > 0; j++) {
+                mbar_arrive(sh.item_empty + j % RECORDS);
                 const uint32_t idesc = make_idesc_bf16(256, it.bn, A_MN, B_MN);
                 for (int c = 0; c < it.chunks; c++, i++) {
                     const int s = i & 1, left = it.depth - (c >= it.nk ? c - it.nk : c) * KC;
                     const int steps = max(1, min(KC / 16, (left + 15) / 16));
-                    ok = mbar_wait_cluster(full + s, (i >> 1) & 1, abort_flag, &g_status, ST_TIMEOUT_CONV);
+                    ok = mbar_wait_cluster(sh.full + s, (i >> 1) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_CONV);
                     if (!ok) break;
                     tc_fence_after_sync();
                     const uint32_t al = desc_lo(smem_base + s * SLOT, PA::LBO), bl = desc_lo(smem_base + s * SLOT + 3 * PART, PB::LBO);
                     const uint32_t d = tmem + s * ACC;
-                    constexpr uint32_t P = PART >> 4;
-                    uint32_t acc = 0;
-                    for (int k = 0; k < steps; k++) {
-                        const uint32_t x = al + k * PA::KSTEP, y = bl + k * PB::KSTEP;
-                        mma_bf16_pair(d, x + 2 * P, HI, y, HI, idesc, acc);        // lo hi
-                        acc = 1;
-                        mma_bf16_pair(d, x, HI, y + 2 * P, HI, idesc, 1);          // hi lo
-                        mma_bf16_pair(d, x + P, HI, y + P, HI, idesc, 1);          // mid mid
-                        mma_bf16_pair(d, x + P, HI, y, HI, idesc, 1);              // mid hi
-                        mma_bf16_pair(d, x, HI, y + P, HI, idesc, 1);              // hi mid
-                    }
-                    for (int k = 0; k < steps; k++) mma_bf16_pair(d, al + k * PA::KSTEP, HI, bl + k * PB::KSTEP, HI, idesc, 1);
-                    mma_commit_pair(done + s);
+                    for (int k = 0; k < steps; k++) mma_small_products(d, al + k * PA::KSTEP, bl + k * PB::KSTEP, HI, idesc, k);
+                    for (int k = 0; k < steps; k++) mma_large_product(d, al + k * PA::KSTEP, bl + k * PB::KSTEP, HI, idesc);
+                    mma_commit_pair(sh.done + s);
                 }
+            }
+        }
+        if (warp == ISSUER + 1) {
+            // ------------------------------------------------------------------------------------------------- items
+            bool more = true;
+            for (int j = 0; more; j++) {
+                Record &r = sh.record[j % RECORDS];
+                if (j >= RECORDS && !mbar_wait(sh.item_empty + j % RECORDS, (j / RECORDS - 1) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_EMPTY))
+                    break;
+                Item t;
+                more = get_item<PASS>(a, sh.before, pair, pairs, j, t);
+                if (!more) t.chunks = 0;
+                if (lane == 0) r.item = t;
+                if (PASS == FWD && more)
+                    for (int l = lane; l < t.bn >> 1; l += 32) {
+                        const int p = cta * (t.bn >> 1) + l;
+                        r.rows[l] = p < t.cols ? input_row(a, t.c0 + p) : -1;
+                    }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(sh.item_full + j % RECORDS);
             }
         }
         __syncwarp();
         finish();
-        if (warp == ISSUER) tmem_dealloc_pair(*tmem_slot, 2 * ACC);
+        if (warp == ISSUER) tmem_dealloc_pair(sh.tmem, 2 * ACC);
     } else if (warp < SUMMERS) {
         // ------------------------------------------------------------------------------------------- sums and output
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SUMMER_REGS));
@@ -265,17 +468,54 @@ __global__ void __launch_bounds__(THREADS, 1) grouped_tc_kernel(const GroupedArg
 #pragma unroll
         for (int x = 0; x < 128; x++) acc[x] = 0.f;
         if (lane == 0) {   // both accumulators are free
-            mbar_arrive_cluster(full, 0);
-            mbar_arrive_cluster(full + 1, 0);
+            mbar_arrive_cluster(sh.full, 0);
+            mbar_arrive_cluster(sh.full + 1, 0);
         }
+        const bool scaled = PASS == PARAM || (PASS == STATE && a.jcb != nullptr);
+        const uint32_t aux_at = smem_u32(&sh.aux[warp][0][0][lane]);
+        // Where a thread's part of a tile lies. Worked out from the record when it is needed (the record is kept until then):
+        // the accumulators leave no registers to remember it in.
+        struct Output {
+            size_t base;   // first entry of the thread's column `first`
+            int n, m, ld, kind, e;   // live columns of the warp's part; feature; pitch
+        };
+        auto locate = [&](int j) {
+            const volatile Item &t = sh.record[j % RECORDS].item;
+            Output o;
+            const int per = t.bn >> 1, first = group * per;
+            o.n = min(per, t.cols - first);
+            o.m = t.m0 + cta * 128 + quad * 32 + lane;
+            o.ld = PASS == FWD ? a.N : a.K;
+            o.kind = t.kind, o.e = t.e;
+            if (o.m >= o.ld) o.n = 0;
+            o.base = ((PASS == PARAM ? (size_t)o.e * a.N : 0) + t.c0 + first) * o.ld + o.m;
+            return o;
+        };
+        // Scale entries (Jacobian, prior variances) come from HBM and there are no registers to wait for them in either: a
+        // lane copies its own to shared memory, 24 columns ahead, the first before the last chunk is done.
+        auto fetch = [&](const Output &o, int g) {   // columns g .. g + 7
+            if (scaled) {
+                const float *aux = (PASS == PARAM ? a.var_w : a.jcb) + o.base + (size_t)g * o.ld;
+#pragma unroll
+                for (int x = 0; x < 8; x++)
+                    if (g + x < o.n) cp_async_f32(aux_at + ((g / 8 % 3) * 8 + x) * 128, aux + (size_t)x * o.ld, true);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
         Item it;
         int i = 0;
         bool ok = true;
-        for (int j = 0; ok && get_item<PASS>(a, before, pair, pairs, j, it); j++) {
-            const int per = it.bn >> 1;
-            for (int c = 0; c < it.chunks; c++, i++) {
+        for (int j = 0; ok && take(sh, j, it) && it.chunks > 0; j++) {
+            const int per = it.bn >> 1, chunks = it.chunks;
+            for (int c = 0; c < chunks; c++, i++) {
                 const int s = i & 1;
-                ok = mbar_wait(done + s, (i >> 1) & 1, abort_flag, &g_status, ST_TIMEOUT_ACC);
+                if (PASS != FWD && c == chunks - 1) {
+                    const Output o = locate(j);
+                    fetch(o, 0);
+                    fetch(o, 8);
+                    fetch(o, 16);
+                }
+                ok = mbar_wait(sh.done + s, (i >> 1) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_ACC);
                 if (!ok) break;
                 tc_fence_after_sync();
                 const uint32_t at = lane_addr + s * ACC + group * per;
@@ -289,196 +529,85 @@ __global__ void __launch_bounds__(THREADS, 1) grouped_tc_kernel(const GroupedArg
                     }
                 tc_fence_before_sync();
                 __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(full + s, 0);
+                if (lane == 0) mbar_arrive_cluster(sh.full + s, 0);
             }
             if (!ok) break;
-            const int m = it.m0 + cta * 128 + quad * 32 + lane, first = group * per, n = min(per, it.cols - first);
-            const int ld = PASS == FWD ? a.N : a.K;
-            const size_t base = ((PASS == PARAM ? (size_t)it.e * a.N : 0) + it.c0 + first) * ld + m;
-            float *out = (it.kind == VAR ? a.o1 : a.o0) + base;
-            const float *aux = PASS == PARAM ? a.var_w + base : PASS == STATE && a.jcb ? a.jcb + base : nullptr;
-            const bool live = m < ld;
+            const Output o = locate(j);
+            release(sh, j, lane);
+            float *out = (o.kind == VAR ? a.o1 : a.o0) + o.base;
             float bias = 0.f;
-            if (PASS == FWD && a.mu_b && live) bias = __ldg((it.kind == VAR ? a.var_b : a.mu_b) + (size_t)it.e * a.N + m);
+            if (PASS == FWD && a.mu_b && o.n > 0) bias = __ldg((o.kind == VAR ? a.var_b : a.mu_b) + (size_t)o.e * a.N + o.m);
 #pragma unroll
             for (int g = 0; g < 128; g += 8) {
-                if (g >= n || !live) break;
-                float f[8];
-#pragma unroll
-                for (int x = 0; x < 8; x++) {
-                    f[x] = 1.f;
-                    if (PASS != FWD && aux && g + x < n) f[x] = __ldg(aux + (size_t)(g + x) * ld);
-                }
+                if (g >= o.n) break;
+                if (PASS != FWD) asm volatile("cp.async.wait_group 2;" ::: "memory");
 #pragma unroll
                 for (int x = 0; x < 8; x++)
-                    if (g + x < n) {
+                    if (g + x < o.n) {
                         float z = acc[g + x];
-                        if (PASS == FWD) z += bias;
-                        else z = it.kind == VAR ? z * f[x] * f[x] : z * f[x];
-                        out[(size_t)(g + x) * ld] = z;
+                        if (PASS == FWD) {
+                            z += bias;
+                        } else if (scaled) {
+                            float f;
+                            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f) : "r"(aux_at + ((g / 8 % 3) * 8 + x) * 128));
+                            z = o.kind == VAR ? z * f * f : z * f;
+                        }
+                        out[(size_t)x * o.ld] = z;
                     }
+                out += (size_t)8 * o.ld;
+                if (PASS != FWD) fetch(o, g + 24);
             }
+            if (PASS != FWD) cp_async_wait_all();
 #pragma unroll
             for (int x = 0; x < 128; x++) acc[x] = 0.f;
         }
         finish();
     } else {
         // ------------------------------------------------------------------------------------------------- converters
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CONVERTER_REGS));
-        const int w = warp - SUMMERS;
-        const int a_line = PA::line(w, lane), a_along = PA::along(lane), b_line = PB::line(w, lane), b_along = PB::along(lane);
-        const uint32_t a_off = smem_base + PA::offset(w, lane), b_off = smem_base + 3 * PART + PB::offset(w, lane);
-        float4 va[TASKS], vb[4];
-        // Loads run ahead of the conversion, into registers that were just stored: the item and chunk they belong to are
-        // `nx` and `nc`. rows: the input rows that this lane looked up for its warp (gathered operands).
-        Item nx;
-        int nc = 0, nj = 0, a_rows = -1, b_rows = -1;
-        bool more = get_item<PASS>(a, before, pair, pairs, 0, nx);
-
-        auto chunk_k = [&](const Item &t, int c, int &half) {
-            half = PASS == FWD && c >= t.nk;
-            return (half ? c - t.nk : c) * KC;
-        };
-        auto look_up_a = [&]() {   // parameter pass: lane q < 8 knows the input row of step q * LINES + w of the chunk
-            if (PASS == PARAM) {
-                const int k = nc * KC + a_line + (lane & 7) * PA::LINES;
-                a_rows = k < nx.depth ? input_row(a, nx.p0 + k) : -1;
-            }
-        };
-        auto load_a = [&](int q0) {   // four tasks of the 128 features of this CTA
-            int half;
-            const int kc = chunk_k(nx, nc, half);
-#pragma unroll
-            for (int q = q0; q < q0 + 4; q++) {
-                if (PASS == FWD) {
-                    const int m = nx.m0 + cta * 128 + a_line + q * PA::LINES, k = kc + a_along;
-                    const float *src = nx.kind == VAR && !half ? a.var_w : a.mu_w;
-                    va[q] = ld4<VEC>(src + ((size_t)nx.e * a.N + m) * a.K + k, m < a.N ? a.K - k : 0);
-                } else if (PASS == STATE) {
-                    const int m = nx.m0 + cta * 128 + a_along, k = kc + a_line + q * PA::LINES;
-                    va[q] = ld4<VEC>(a.mu_w + ((size_t)nx.e * a.N + k) * a.K + m, k < a.N ? a.K - m : 0);
-                } else {
-                    const int m = nx.m0 + cta * 128 + a_along, r = __shfl_sync(0xffffffffu, a_rows, q);
-                    va[q] = ld4<VEC>(a.x + (size_t)max(r, 0) * a.K + m, r >= 0 ? a.K - m : 0);
-                }
-            }
-        };
-        auto look_up_b = [&]() {   // forward pass: lane knows the input row of column lane >> 1 of the warp's tasks
-            if (PASS == FWD) {
-                const int line = (lane >> 1) * PB::LINES + w * 2 + (lane & 1), half_bn = nx.bn >> 1, p = cta * half_bn + line;
-                b_rows = lane < 2 * TASKS && line < half_bn && p < nx.cols ? input_row(a, nx.c0 + p) : -1;
-            }
-        };
-        // one task of this CTA's half of the columns; second: the variances that belong to the means (forward pass)
-        auto load_b = [&](int q, bool second) {
-            int half;
-            const int kc = chunk_k(nx, nc, half), half_bn = nx.bn >> 1, line = b_line + q * PB::LINES;
-            if (PASS == PARAM) {
-                const int k = kc + line, n = cta * half_bn + b_along;
-                return ld4<VEC>((nx.kind == VAR ? a.a1 : a.a0) + (size_t)(nx.p0 + k) * a.N + nx.c0 + n,
-                                k < nx.depth && b_along < half_bn ? nx.cols - n : 0);
-            }
-            const int k = kc + b_along;
-            if (PASS == FWD) {
-                const int r = __shfl_sync(0xffffffffu, b_rows, q * 2 + (lane >> 4));
-                return ld4<VEC>((second || (nx.kind == VAR && half) ? a.a1 : a.a0) + (size_t)max(r, 0) * a.K + k, r >= 0 ? a.K - k : 0);
-            }
-            const int p = cta * half_bn + line;
-            return ld4<VEC>((nx.kind == VAR ? a.a1 : a.a0) + (size_t)(nx.c0 + p) * a.N + k, line < half_bn && p < nx.cols ? a.N - k : 0);
-        };
-        // vb: four tasks from q0, or (sums) the means and variances of two
-        auto load_b4 = [&](int q0, bool sums) {
-            if (PASS == FWD && sums) {
-                vb[0] = load_b(q0, false), vb[1] = load_b(q0 + 1, false);
-                vb[2] = load_b(q0, true), vb[3] = load_b(q0 + 1, true);
-            } else {
-#pragma unroll
-                for (int q = 0; q < 4; q++) vb[q] = load_b(q0 + q, false);
-            }
-        };
-        bool ok = true;
-        if (more) {
-            look_up_a();
-            look_up_b();
-            load_b4(0, PASS == FWD && nx.kind == VAR);
-            load_a(0);
-            load_a(4);
+        const int w = (warp - SUMMERS) & 3;
+        if (warp < SUMMERS + 4) {
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(A_REGS));
+            convert_a<PASS, VEC>(a, sh, cta, w, lane, smem_base);
+            finish();
+        } else {
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(B_REGS));
+            convert_b<PASS, VEC>(a, sh, cta, w, lane, smem_base);
+            finish();
         }
-        for (int i = 0; ok && more; i++) {
-            const int s = i & 1;
-            int half;
-            chunk_k(nx, nc, half);
-            const bool sums = PASS == FWD && nx.kind == VAR && !half, square = nx.kind == VAR && !sums;
-            const int lines = PASS == PARAM ? round_up(nx.bn >> 1, 64) : nx.bn >> 1;   // columns that this CTA holds
-            if (i >= 2) {
-                ok = mbar_wait(done + s, ((i - 2) >> 1) & 1, abort_flag, &g_status, ST_TIMEOUT_EMPTY);
-                if (!ok) break;
-            }
-            auto store_a = [&](int q0) {
-#pragma unroll
-                for (int q = q0; q < q0 + 4; q++)
-                    store_split(a_off + s * SLOT + q * PA::STRIDE, square ? squared(va[q]) : va[q]);
-            };
-            auto store_b = [&](int q, float4 v) {
-                if (PASS == PARAM ? b_along < lines : b_line + q * PB::LINES < lines) store_split(b_off + s * SLOT + q * PB::STRIDE, v);
-            };
-            auto store_b4 = [&](int q0) {
-                if (PASS == FWD && sums) {
-#pragma unroll
-                    for (int q = 0; q < 2; q++) {
-                        const float4 x = vb[q], v = vb[q + 2];
-                        store_b(q0 + q, make_float4(fmaf(x.x, x.x, v.x), fmaf(x.y, x.y, v.y), fmaf(x.z, x.z, v.z), fmaf(x.w, x.w, v.w)));
-                    }
-                } else {
-#pragma unroll
-                    for (int q = 0; q < 4; q++) store_b(q0 + q, vb[q]);
-                }
-            };
-            // Every load is issued two groups of stores before its values are needed. With sums, columns take twice the
-            // registers: they come in four groups, the last two of this chunk (the next cannot be looked up earlier).
-            store_b4(0);
-            load_b4(sums ? 2 : 4, sums);
-            if (PASS == FWD && sums) {
-                store_a(0);
-                store_b4(2);
-                load_b4(4, true);
-                store_a(4);
-                store_b4(4);
-                load_b4(6, true);
-            } else {
-                store_a(0);
-                store_a(4);
-            }
-            Item cur_next = nx;   // the next chunk's item
-            int c_next = nc + 1, j_next = nj;
-            bool has_next = true;
-            if (c_next == nx.chunks) {
-                c_next = 0;
-                has_next = get_item<PASS>(a, before, pair, pairs, ++j_next, cur_next);
-            }
-            store_b4(sums ? 6 : 4);
-            nx = cur_next, nc = c_next, more = has_next;
-            if (more) {
-                look_up_a();
-                if (j_next != nj) look_up_b();
-                load_b4(0, PASS == FWD && nx.kind == VAR && nc < nx.nk);
-                load_a(0);
-                load_a(4);
-            }
-            nj = j_next;
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(full + s, 0);
-        }
-        finish();
     }
+}
+
+// mu_a^2 + var_a, the forward variance's operand
+__global__ void __launch_bounds__(256) grouped_second_moment_kernel(const float *__restrict__ mu, const float *__restrict__ var,
+                                                                    size_t n, float *__restrict__ out) {
+    const size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i + 4 <= n) {
+        const float4 m = __ldg(reinterpret_cast<const float4 *>(mu + i)), v = __ldg(reinterpret_cast<const float4 *>(var + i));
+        *reinterpret_cast<float4 *>(out + i) =
+            make_float4(fmaf(m.x, m.x, v.x), fmaf(m.y, m.y, v.y), fmaf(m.z, m.z, v.z), fmaf(m.w, m.w, v.w));
+    } else {
+        for (size_t j = i; j < n; j++) out[j] = fmaf(__ldg(mu + j), __ldg(mu + j), __ldg(var + j));
+    }
+}
+__global__ void __launch_bounds__(256) grouped_second_moment_unaligned_kernel(const float *__restrict__ mu, const float *__restrict__ var,
+                                                                              size_t n, float *__restrict__ out) {
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (i < n) out[i] = fmaf(__ldg(mu + i), __ldg(mu + i), __ldg(var + i));
 }
 
 template <int PASS>
 int launch_pass(const GroupedArgs &a, cudaStream_t st) {
+    if (PASS == FWD) {
+        const size_t n = (size_t)a.R * a.K;
+        if (aligned16(a.a0) && aligned16(a.a1))
+            grouped_second_moment_kernel<<<(unsigned)((n + 1023) / 1024), 256, 0, st>>>(a.a0, a.a1, n, a.second);
+        else
+            grouped_second_moment_unaligned_kernel<<<(unsigned)((n + 255) / 256), 256, 0, st>>>(a.a0, a.a1, n, a.second);
+        TAGI_CUDA(cudaGetLastError());
+    }
     const bool vec = a.K % 4 == 0 && a.N % 4 == 0 && aligned16(a.mu_w) && aligned16(a.var_w) && aligned16(a.a0) && aligned16(a.a1) &&
                      aligned16(a.x);
-    const size_t smem = 2 * SLOT + 1024 + 64 + (a.E + 1) * sizeof(int);
+    const size_t smem = 2 * SLOT + 1024 + sizeof(Shared) + (a.E + 1) * sizeof(int);
     const long mt = ((PASS == FWD ? a.N : a.K) + 255) / 256;
     const long most = 2 * mt * (PASS == PARAM ? (long)a.E * ((a.N + 255) / 256) : a.S / 256 + (a.E < a.S ? a.E : a.S));
     cudaLaunchConfig_t cfg = {};

@@ -145,8 +145,10 @@ def grouped_linear(mu_w, var_w, mu_b, var_b, mu_a, var_a, offsets, token=None):
     _check(d, mu_w=(mu_w, (E, N, K), _F), var_w=(var_w, (E, N, K), _F), mu_b=(mu_b, (E, N), _F), var_b=(var_b, (E, N), _F),
            mu_a=(mu_a, (R, K), _F), var_a=(var_a, (R, K), _F), offsets=(offsets, (E + 1,), _I), token=(token, (S,), _I))
     mu_z, var_z = torch.empty(2, S, N, dtype=_F, device=d)
+    nbytes = capi.load().tagi_grouped_linear_workspace_bytes(S, R, K)
+    ws = _workspace(nbytes, d)
     _run("tagi_grouped_linear_fwd", d, E, S, R, K, N, bias, _p(offsets), _p(token), _p(mu_w), _p(var_w), _p(mu_b), _p(var_b),
-         _p(mu_a), _p(var_a), _p(mu_z), _p(var_z))
+         _p(mu_a), _p(var_a), _p(mu_z), _p(var_z), _p(ws), nbytes)
     return mu_z, var_z
 
 

@@ -364,7 +364,8 @@ int tagi_route_bwd(int T, int E, int k, const int *expert, const float *mu_g, co
  * zeros. */
 int tagi_grouped_linear_fwd(int E, int S, int R, int K, int N, int has_bias, const int *offsets, const int *token,
                             const float *mu_w, const float *var_w, const float *mu_b, const float *var_b, const float *mu_a,
-                            const float *var_a, float *mu_z, float *var_z, void *stream);
+                            const float *var_a, float *mu_z, float *var_z, void *workspace, size_t workspace_bytes, void *stream);
+size_t tagi_grouped_linear_workspace_bytes(int S, int R, int K); /* of the forward pass; host helper */
 /* tagi_linear_bwd_state per expert: deltas dmu_z / dvar_z [S][N] and outputs dmu_a / dvar_a [S][K] in dispatch order, jcb
  * [S][K] the Jacobian of the same rows (NULL = 1; where the input was gathered by token, tagi_dispatch_bwd applies it). */
 int tagi_grouped_linear_bwd_state(int E, int S, int K, int N, const int *offsets, const float *mu_w, const float *jcb,

@@ -76,8 +76,8 @@ def test_route_refusals():
 
 
 def test_grouped_linear_refusals():
-    def fwd(E=4, S=8, R_=8, K=16, N=16, bias=1, p=None):
-        return (E, S, R_, K, N, bias, *(p or [P] * 10), None)
+    def fwd(E=4, S=8, R_=8, K=16, N=16, bias=1, p=None, ws=P, size=1 << 30):
+        return (E, S, R_, K, N, bias, *(p or [P] * 10), ws, size, None)
     for kw in (dict(E=0), dict(E=1025), dict(S=-1), dict(R_=-1), dict(K=0), dict(N=0), dict(K=(1 << 20) + 1),
                dict(S=(1 << 28) + 1), dict(R_=0)):
         refused("tagi_grouped_linear_fwd", *fwd(**kw))
@@ -85,6 +85,10 @@ def test_grouped_linear_refusals():
         if i != 1:      # the gather index may be NULL
             refused("tagi_grouped_linear_fwd", *fwd(p=[None if j == i else P for j in range(10)]))
         refused("tagi_grouped_linear_fwd", *fwd(p=[P + 2 if j == i else P for j in range(10)]))
+    need = lib.tagi_grouped_linear_workspace_bytes(1000, 500, 64)
+    assert need >= 500 * 64 * 4 and lib.tagi_grouped_linear_workspace_bytes(0, 500, 64) == 0
+    for kw in (dict(ws=None), dict(ws=P + 4), dict(size=need - 1)):
+        refused("tagi_grouped_linear_fwd", *fwd(S=1000, R_=500, K=64, **kw))
     refused("tagi_grouped_linear_fwd", *fwd(R_=7, p=[P, None] + [P] * 8))     # no gather index: R must equal S
 
     def state(E=4, S=8, K=16, N=16, p=None):
@@ -137,7 +141,7 @@ def test_tensor_functions_refuse_what_the_kernels_cannot_read():
 
 def test_empty_calls_touch_nothing():
     assert lib.tagi_ln_fwd(*ln_args(R=0, p=[P] * 4 + [None] * 6)) == 0
-    assert lib.tagi_grouped_linear_fwd(4, 0, 0, 16, 16, 1, P, None, P, P, P, P, None, None, None, None, None) == 0
+    assert lib.tagi_grouped_linear_fwd(4, 0, 0, 16, 16, 1, P, None, P, P, P, P, None, None, None, None, None, 0, None) == 0
     assert lib.tagi_grouped_linear_bwd_state(4, 0, 16, 16, P, P, None, None, None, None, None, None) == 0
     assert lib.tagi_combine_fwd(0, 2, 8, 0, *[None] * 8) == 0
     assert lib.tagi_combine_bwd(0, 2, 8, 0, *[None] * 11) == 0

@@ -95,6 +95,14 @@ def test_layer_norm_forward(lib, rows, n, bias, misalign):
         R.check(name, got.get(), pair, R.U)
 
 
+def grouped_fwd(lib, E, S, rows, K, N, *args):
+    """tagi_grouped_linear_fwd with a guarded workspace."""
+    size = lib.tagi_grouped_linear_workspace_bytes(S, rows, K)
+    ws = torch.full((size // 4 + 32,), SENT, device="cuda")
+    lib.tagi_grouped_linear_fwd(E, S, rows, K, N, *args, p(ws), size, st())
+    assert bool((ws[size // 4:] == SENT).all())
+
+
 def test_layer_norm_forward_of_a_constant_row(lib):
     """No spread at all: the variance is what the inputs' own variances give, zero with them at zero."""
     n = 256
@@ -246,8 +254,8 @@ def test_grouped_linear(lib, counts, K, N, bias, gather, misalign, lead, tail):
     mb, vb = (g.n(E, N, scale=0.1), g.u(E, N, lo=0.001, hi=0.1)) if bias else (None, None)
     ma, va = g.n(rows, K), g.u(rows, K, lo=0.001, hi=0.2)
     z, vz = Guard(S, N, misalign=misalign), Guard(S, N, misalign=misalign)
-    lib.tagi_grouped_linear_fwd(E, S, rows, K, N, int(bias), p(offsets), p(token), p(mw), p(vw), p(mb), p(vb), p(ma), p(va),
-                                z.ptr(), vz.ptr(), st())
+    grouped_fwd(lib, E, S, rows, K, N, int(bias), p(offsets), p(token), p(mw), p(vw), p(mb), p(vb), p(ma), p(va),
+                                z.ptr(), vz.ptr())
     ref = R.grouped_fwd(mw, vw, mb, vb, ma, va, offsets, token)
     R.check("mu_z", guard_rows(z, r0, r1), sub(ref[0], r0, r1), R.sum_tol(K))
     R.check("var_z", guard_rows(vz, r0, r1), sub(ref[1], r0, r1), R.sum_tol(2 * K))
@@ -287,7 +295,7 @@ def test_grouped_linear_bad_device_data_stays_in_range(lib, rows):
     offsets = torch.tensor([-5, rows // 2, 2 ** 31 - 1], dtype=i32, device="cuda")
     mw, vw, ma, va = g.n(2, N, K), g.u(2, N, K), g.n(rows, K), g.u(rows, K)
     z, vz = Guard(rows, N), Guard(rows, N)
-    lib.tagi_grouped_linear_fwd(2, rows, rows, K, N, 0, p(offsets), p(token), p(mw), p(vw), None, None, p(ma), p(va), z.ptr(), vz.ptr(), st())
+    grouped_fwd(lib, 2, rows, rows, K, N, 0, p(offsets), p(token), p(mw), p(vw), None, None, p(ma), p(va), z.ptr(), vz.ptr())
     ref = R.grouped_fwd(mw, vw, None, None, ma, va, offsets, token)
     assert bool((z.get()[:3] == 0).all())
     R.check("mu_z", z.get(), ref[0], R.sum_tol(K))
@@ -315,7 +323,7 @@ def test_grouped_linear_rows_of_other_experts_do_not_leak(lib, counts):
     z, vz, da, dva = Guard(S, N), Guard(S, N), Guard(S, K), Guard(S, K)
     o = [Guard(E, N, K) for _ in range(2)] + [Guard(E, N) for _ in range(2)]
     vb = g.u(E, N)
-    lib.tagi_grouped_linear_fwd(E, S, S, K, N, 0, p(offsets), None, p(mw), p(vw), None, None, p(ma), p(va), z.ptr(), vz.ptr(), st())
+    grouped_fwd(lib, E, S, S, K, N, 0, p(offsets), None, p(mw), p(vw), None, None, p(ma), p(va), z.ptr(), vz.ptr())
     lib.tagi_grouped_linear_bwd_state(E, S, K, N, p(offsets), p(mw), None, p(dm), p(dv), da.ptr(), dva.ptr(), st())
     lib.tagi_grouped_linear_bwd_param(E, S, S, K, N, 1, p(offsets), None, p(vw), p(vb), p(ma), p(dm), p(dv), *[x.ptr() for x in o], st())
     rows = torch.cat([torch.arange(lo, a), torch.arange(b, hi)]).cuda()
@@ -338,7 +346,7 @@ def test_grouped_linear_wide_range_of_values(lib, rows):
     ma, va = g.n(rows, K) * scale, g.u(rows, K, lo=0.1) * scale.square()
     offsets, _ = spread([rows])
     z, vz = Guard(rows, N), Guard(rows, N)
-    lib.tagi_grouped_linear_fwd(1, rows, rows, K, N, 0, p(offsets), None, p(mw), p(vw), None, None, p(ma), p(va), z.ptr(), vz.ptr(), st())
+    grouped_fwd(lib, 1, rows, rows, K, N, 0, p(offsets), None, p(mw), p(vw), None, None, p(ma), p(va), z.ptr(), vz.ptr())
     ref = R.grouped_fwd(mw, vw, None, None, ma, va, offsets, None)
     R.check("mu_z", z.get(), ref[0], R.sum_tol(K))
     R.check("var_z", vz.get(), ref[1], R.sum_tol(2 * K))
