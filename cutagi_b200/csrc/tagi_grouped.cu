@@ -6,12 +6,14 @@
 namespace tagi {
 namespace {
 
-// dmu_b = var_b sum dmu_z, dvar_b = var_b^2 sum dvar_z over an expert's rows: 32 features x 8 groups of rows per CTA.
+// dmu_b = var_b sum dmu_z, dvar_b = var_b^2 sum dvar_z over the rows of the experts that run on the tensor cores: 32 features
+// x 8 groups of rows per CTA.
 __global__ void __launch_bounds__(256) grouped_bias_kernel(const GroupedArgs a) {
     __shared__ float2 red[8][32];
     const int c = threadIdx.x & 31, g = threadIdx.x >> 5, n = blockIdx.x * 32 + c, e = blockIdx.y;
     int r0, r1;
     expert_rows(a, e, r0, r1);
+    if (r1 - r0 <= FEW_PARAM_ROWS) return;
     float s = 0.f, v = 0.f;
     if (n < a.N)
         for (int r = r0 + g; r < r1; r += 8) s += __ldg(a.a0 + (size_t)r * a.N + n), v += __ldg(a.a1 + (size_t)r * a.N + n);
@@ -29,6 +31,11 @@ __global__ void __launch_bounds__(256) grouped_bias_kernel(const GroupedArgs a) 
 inline int launched(const char *what) {
     cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? TAGI_OK : cuda_fail(e, what);
+}
+
+int run(int pass, const GroupedArgs &a, cudaStream_t st) {
+    const int rc = grouped_few(pass, a, st);
+    return rc != TAGI_OK || a.S <= few_rows(pass) ? rc : grouped_tc(pass, a, st);
 }
 
 int check_grouped(const char *who, int E, int S, int K, int N, const int *offsets) {
@@ -51,7 +58,7 @@ using namespace tagi;
 extern "C" {
 
 size_t tagi_grouped_linear_workspace_bytes(int S, int R, int K) {
-    if (S <= 0 || R <= 0 || K <= 0) return 0;
+    if (S <= FEW_ROWS || R <= 0 || K <= 0) return 0;
     return (size_t)R * K * sizeof(float);
 }
 
@@ -82,7 +89,7 @@ int tagi_grouped_linear_fwd(int E, int S, int R, int K, int N, int has_bias, con
     a.E = E, a.S = S, a.R = R, a.K = K, a.N = N, a.offsets = offsets, a.token = token, a.mu_w = mu_w, a.var_w = var_w;
     a.mu_b = has_bias ? mu_b : nullptr, a.var_b = has_bias ? var_b : nullptr, a.a0 = mu_a, a.a1 = var_a, a.o0 = mu_z, a.o1 = var_z;
     a.second = static_cast<float *>(workspace);
-    return grouped_tc(FWD, a, static_cast<cudaStream_t>(stream));
+    return run(FWD, a, static_cast<cudaStream_t>(stream));
 }
 
 int tagi_grouped_linear_bwd_state(int E, int S, int K, int N, const int *offsets, const float *mu_w, const float *jcb,
@@ -99,7 +106,7 @@ int tagi_grouped_linear_bwd_state(int E, int S, int K, int N, const int *offsets
     GroupedArgs a{};
     a.E = E, a.S = S, a.R = S, a.K = K, a.N = N, a.offsets = offsets, a.mu_w = mu_w, a.jcb = jcb, a.a0 = dmu_z, a.a1 = dvar_z;
     a.o0 = dmu_a, a.o1 = dvar_a;
-    return grouped_tc(STATE, a, static_cast<cudaStream_t>(stream));
+    return run(STATE, a, static_cast<cudaStream_t>(stream));
 }
 
 int tagi_grouped_linear_bwd_param(int E, int S, int R, int K, int N, int has_bias, const int *offsets, const int *token,
@@ -128,8 +135,8 @@ int tagi_grouped_linear_bwd_param(int E, int S, int R, int K, int N, int has_bia
     a.E = E, a.S = S, a.R = R, a.K = K, a.N = N, a.offsets = offsets, a.token = token, a.var_w = var_w, a.x = mu_a;
     a.var_b = has_bias ? var_b : nullptr, a.a0 = dmu_z, a.a1 = dvar_z, a.o0 = dmu_w, a.o1 = dvar_w, a.ob0 = dmu_b, a.ob1 = dvar_b;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    rc = grouped_tc(PARAM, a, st);
-    if (rc != TAGI_OK || !has_bias) return rc;
+    rc = run(PARAM, a, st);
+    if (rc != TAGI_OK || !has_bias || S <= FEW_PARAM_ROWS) return rc;
     grouped_bias_kernel<<<dim3((N + 31) / 32, E), 256, 0, st>>>(a);
     return launched("grouped_bias_kernel launch");
 }

@@ -98,7 +98,7 @@ __device__ __forceinline__ bool get_item(const GroupedArgs &a, const int *before
     it.c0 = n * it.bn + (PASS == PARAM ? 0 : r0);
     it.p0 = r0;
     it.depth = PASS == FWD ? a.K : PASS == STATE ? a.N : r1 - r0;
-    it.nk = max(1, (it.depth + KC - 1) / KC);
+    it.nk = (it.depth + KC - 1) / KC;
     it.chunks = PASS == FWD && it.kind == VAR ? 2 * it.nk : it.nk;
     return true;
 }
@@ -386,7 +386,8 @@ __global__ void __launch_bounds__(THREADS, 1) grouped_tc_kernel(const GroupedArg
         for (int e0 = 0; e0 < a.E; e0 += 32) {
             int r0 = 0, r1 = 0;
             if (e0 + lane < a.E) expert_rows(a, e0 + lane, r0, r1);
-            const int v = e0 + lane < a.E ? mt * (((PASS == PARAM ? a.N : r1 - r0) + 255) / 256) : 0;
+            // experts with few rows have kernels of their own
+            const int v = r1 - r0 > (PASS == PARAM ? FEW_PARAM_ROWS : FEW_ROWS) ? mt * (((PASS == PARAM ? a.N : r1 - r0) + 255) / 256) : 0;
             int s = v;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -609,7 +610,8 @@ int launch_pass(const GroupedArgs &a, cudaStream_t st) {
                      aligned16(a.x);
     const size_t smem = 2 * SLOT + 1024 + sizeof(Shared) + (a.E + 1) * sizeof(int);
     const long mt = ((PASS == FWD ? a.N : a.K) + 255) / 256;
-    const long most = 2 * mt * (PASS == PARAM ? (long)a.E * ((a.N + 255) / 256) : a.S / 256 + (a.E < a.S ? a.E : a.S));
+    const long experts = a.E < a.S / (few_rows(PASS) + 1) ? a.E : a.S / (few_rows(PASS) + 1);   // at most as many have more rows
+    const long most = 2 * mt * (PASS == PARAM ? experts * ((a.N + 255) / 256) : a.S / 256 + experts);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2 * (unsigned)(most < PAIRS ? most : PAIRS));
     cfg.blockDim = dim3(THREADS);
