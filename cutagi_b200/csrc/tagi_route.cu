@@ -15,8 +15,10 @@
 namespace tagi {
 namespace {
 
-constexpr int THREADS = 256, WARPS = THREADS / 32;
 constexpr int MAX_EXPERTS = 1024, MAX_K = 32;
+// Warps of a block: the more the shorter the chain of tokens that a warp ranks one after the other (a block per SM holds
+// them all), as far as the per-warp counts fit shared memory and a lane's scores its registers.
+__host__ __device__ constexpr int warps_for(int E) { return E <= 256 ? 32 : 8; }
 constexpr int ONE_BLOCK_TOKENS = 32;
 constexpr int MAX_BLOCKS = 148;
 constexpr unsigned FULL = 0xffffffffu;
@@ -88,6 +90,18 @@ __device__ __forceinline__ void rank_token(const RouteArgs &a, long t) {
     }
 }
 
+// Ranks the tokens [t0, t1) of the block and adds their slots to count[e].
+template <int EPL, int WARPS>
+__device__ __forceinline__ void rank_tokens(const RouteArgs &a, long t0, long t1, int *count) {
+    const int lane = threadIdx.x & 31;
+    for (long t = t0 + (threadIdx.x >> 5); t < t1; t += WARPS) {
+        rank_token<EPL>(a, t);
+        __syncwarp();
+        const int e = lane < a.k ? a.expert[t * a.k + lane] : -1;
+        if (e >= 0) atomicAdd(count + e, 1);
+    }
+}
+
 // Exclusive sum over the experts of total[e], in place; total[E] receives the sum. Called by the whole block.
 __device__ __forceinline__ void exclusive_sum(int *total, int E) {
     if (threadIdx.x < 32) {
@@ -110,10 +124,11 @@ __device__ __forceinline__ void exclusive_sum(int *total, int E) {
 
 // Positions of the slots [i0, i1) of this block. base[e] is where the block's first slot of expert e goes. Each warp
 // takes a contiguous segment: it counts, the counts of the warps before it are added, then it ranks 32 slots at a time.
+template <int WARPS>
 __device__ __forceinline__ void place_slots(const RouteArgs &a, long i0, long i1, const int *base, int *warp_count) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int *mine = warp_count + warp * a.E;
-    for (int e = threadIdx.x; e < WARPS * a.E; e += THREADS) warp_count[e] = 0;
+    for (int e = threadIdx.x; e < WARPS * a.E; e += WARPS * 32) warp_count[e] = 0;
     __syncthreads();
     const long seg = ((i1 - i0 + WARPS - 1) / WARPS + 31) / 32 * 32, s0 = min(i1, i0 + warp * seg), s1 = min(i1, s0 + seg);
     for (long i = s0 + lane; i < s1; i += 32) {
@@ -121,7 +136,7 @@ __device__ __forceinline__ void place_slots(const RouteArgs &a, long i0, long i1
         if (e >= 0) atomicAdd(mine + e, 1);
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < a.E; e += THREADS) {
+    for (int e = threadIdx.x; e < a.E; e += WARPS * 32) {
         int s = base[e];
         for (int w = 0; w < WARPS; w++) {
             const int c = warp_count[w * a.E + e];
@@ -150,95 +165,95 @@ __device__ __forceinline__ void clear_tail(const RouteArgs &a, long live, long f
     for (long i = live + first; i < (long)a.T * a.k; i += stride) a.token[i] = -1;
 }
 
-template <int EPL>
-__global__ void __launch_bounds__(THREADS) route_rank_kernel(const RouteArgs a) {
+template <int EPL, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32) route_rank_kernel(const RouteArgs a) {
     extern __shared__ int count[];
     const long t0 = (long)blockIdx.x * a.per_block, t1 = min((long)a.T, t0 + a.per_block);
-    for (int e = threadIdx.x; e < a.E; e += THREADS) count[e] = 0;
+    for (int e = threadIdx.x; e < a.E; e += WARPS * 32) count[e] = 0;
     __syncthreads();
-    for (long t = t0 + (threadIdx.x >> 5); t < t1; t += WARPS) {
-        rank_token<EPL>(a, t);
-        __syncwarp();
-        const int lane = threadIdx.x & 31, e = lane < a.k ? a.expert[t * a.k + lane] : -1;
-        if (e >= 0) atomicAdd(count + e, 1);
-    }
+    rank_tokens<EPL, WARPS>(a, t0, t1, count);
     __syncthreads();
-    for (int e = threadIdx.x; e < a.E; e += THREADS) a.counts[(long)blockIdx.x * a.E + e] = count[e];
+    for (int e = threadIdx.x; e < a.E; e += WARPS * 32) a.counts[(long)blockIdx.x * a.E + e] = count[e];
 }
 
-__global__ void __launch_bounds__(THREADS) route_place_kernel(const RouteArgs a) {
+template <int WARPS>
+__global__ void __launch_bounds__(WARPS * 32) route_place_kernel(const RouteArgs a) {
     extern __shared__ int sh[];  // total [E + 1], before [E], warp counts [WARPS][E]
     int *total = sh, *before = sh + a.E + 1, *warp_count = before + a.E;
-    for (int e = threadIdx.x; e < a.E; e += THREADS) {
+    for (int e = threadIdx.x; e < 2 * a.E + 1; e += WARPS * 32) sh[e] = 0;
+    __syncthreads();
+    // slots of each expert in all blocks and in the blocks before this one: every thread adds up some of the blocks' counts
+    // of one expert
+    const int groups = max(1, WARPS * 32 / a.E);
+    for (int i = threadIdx.x; i < groups * a.E; i += WARPS * 32) {
+        const int e = i % a.E;
         int all = 0, mine = 0;
-        for (int b = 0; b < (int)gridDim.x; b++) {
-            if (b == (int)blockIdx.x) mine = all;
-            all += __ldg(a.counts + (long)b * a.E + e);
+#pragma unroll 4
+        for (int b = i / a.E; b < (int)gridDim.x; b += groups) {
+            const int c = __ldg(a.counts + (long)b * a.E + e);
+            all += c;
+            mine += b < (int)blockIdx.x ? c : 0;
         }
-        total[e] = all;
-        before[e] = mine;
+        atomicAdd(total + e, all);
+        atomicAdd(before + e, mine);
     }
     __syncthreads();
     exclusive_sum(total, a.E);
-    for (int e = threadIdx.x; e < a.E; e += THREADS) before[e] += total[e];
+    for (int e = threadIdx.x; e < a.E; e += WARPS * 32) before[e] += total[e];
     if (blockIdx.x == 0)
-        for (int e = threadIdx.x; e <= a.E; e += THREADS) a.offsets[e] = total[e];
+        for (int e = threadIdx.x; e <= a.E; e += WARPS * 32) a.offsets[e] = total[e];
     __syncthreads();
     const long i0 = (long)blockIdx.x * a.per_block * a.k, i1 = min((long)a.T * a.k, i0 + (long)a.per_block * a.k);
-    place_slots(a, i0, i1, before, warp_count);
-    clear_tail(a, total[a.E], (long)blockIdx.x * THREADS + threadIdx.x, (long)gridDim.x * THREADS);
+    place_slots<WARPS>(a, i0, i1, before, warp_count);
+    clear_tail(a, total[a.E], (long)blockIdx.x * WARPS * 32 + threadIdx.x, (long)gridDim.x * WARPS * 32);
 }
 
-template <int EPL>
-__global__ void __launch_bounds__(THREADS) route_one_block_kernel(const RouteArgs a) {
+template <int EPL, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32) route_one_block_kernel(const RouteArgs a) {
     extern __shared__ int sh[];
     int *total = sh, *warp_count = sh + a.E + 1;
-    for (int e = threadIdx.x; e < a.E; e += THREADS) total[e] = 0;
+    for (int e = threadIdx.x; e < a.E; e += WARPS * 32) total[e] = 0;
     __syncthreads();
-    for (long t = threadIdx.x >> 5; t < a.T; t += WARPS) {
-        rank_token<EPL>(a, t);
-        __syncwarp();
-        const int lane = threadIdx.x & 31, e = lane < a.k ? a.expert[t * a.k + lane] : -1;
-        if (e >= 0) atomicAdd(total + e, 1);
-    }
+    rank_tokens<EPL, WARPS>(a, 0, a.T, total);
     __syncthreads();
     exclusive_sum(total, a.E);
-    for (int e = threadIdx.x; e <= a.E; e += THREADS) a.offsets[e] = total[e];
-    place_slots(a, 0, (long)a.T * a.k, total, warp_count);
-    clear_tail(a, total[a.E], threadIdx.x, THREADS);
+    for (int e = threadIdx.x; e <= a.E; e += WARPS * 32) a.offsets[e] = total[e];
+    place_slots<WARPS>(a, 0, (long)a.T * a.k, total, warp_count);
+    clear_tail(a, total[a.E], threadIdx.x, WARPS * 32);
 }
 
-// dmu_s_j = sum_i J_ij dmu_g_i, dvar_s_j = sum_i J_ij^2 dvar_g_i over the chosen, J_ij = g_i (d_ij - g_j); one warp per token.
-__global__ void __launch_bounds__(THREADS) route_bwd_kernel(int T, int E, int k, const int *__restrict__ expert,
-                                                            const float *__restrict__ mu_g, const float *__restrict__ dmu_g,
-                                                            const float *__restrict__ dvar_g, float *__restrict__ dmu_s,
-                                                            float *__restrict__ dvar_s) {
-    const long t = (long)blockIdx.x * WARPS + (threadIdx.x >> 5);
+// dmu_s_j = sum_i J_ij dmu_g_i, dvar_s_j = sum_i J_ij^2 dvar_g_i over the chosen, J_ij = g_i (d_ij - g_j); one warp per token
+// writes zeros along the whole row, then the chosen experts' entries. VEC: rows of a multiple of four, 16-byte aligned.
+constexpr int BWD_WARPS = 8;
+template <bool VEC>
+__global__ void __launch_bounds__(BWD_WARPS * 32) route_bwd_kernel(int T, int E, int k, const int *__restrict__ expert,
+                                                                   const float *__restrict__ mu_g, const float *__restrict__ dmu_g,
+                                                                   const float *__restrict__ dvar_g, float *dmu_s, float *dvar_s) {
+    const long t = (long)blockIdx.x * BWD_WARPS + (threadIdx.x >> 5);
     if (t >= T) return;
     const int lane = threadIdx.x & 31;
-    const bool slot = lane < k;
-    const int e = slot ? __ldg(expert + t * k + lane) : -1;
+    int e = lane < k ? __ldg(expert + t * k + lane) : -1;
+    if (e >= E) e = -1;
     const bool has = e >= 0;   // a slot without an expert has no part in the sums, whatever its deltas hold
     const float g = has ? __ldg(mu_g + t * k + lane) : 0.f, d = has ? __ldg(dmu_g + t * k + lane) : 0.f,
                 w = has ? __ldg(dvar_g + t * k + lane) : 0.f;
+    if (VEC) {
+        for (int c = lane * 4; c < E; c += 128) {
+            *reinterpret_cast<float4 *>(dmu_s + t * E + c) = make_float4(0.f, 0.f, 0.f, 0.f);
+            *reinterpret_cast<float4 *>(dvar_s + t * E + c) = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+    } else {
+        for (int c = lane; c < E; c += 32) dmu_s[t * E + c] = dvar_s[t * E + c] = 0.f;
+    }
     float rest = 0.f, dm = 0.f, dv = 0.f;
     for (int i = 0; i < k; i++) {
         const float gi = __shfl_sync(FULL, g, i), di = __shfl_sync(FULL, d, i), wi = __shfl_sync(FULL, w, i);
         if (i != lane) rest += gi, dm += gi * (d - di), dv += gi * gi * wi;
     }
-    dm *= g;
-    dv = g * g * (rest * rest * w + dv);
-    for (int c0 = 0; c0 < E; c0 += 32) {
-        float m = 0.f, v = 0.f;
-        for (int i = 0; i < k; i++) {
-            const int ei = __shfl_sync(FULL, e, i);
-            const float mi = __shfl_sync(FULL, dm, i), vi = __shfl_sync(FULL, dv, i);
-            if (ei == c0 + lane) m = mi, v = vi;
-        }
-        if (c0 + lane < E) {
-            dmu_s[t * E + c0 + lane] = m;
-            dvar_s[t * E + c0 + lane] = v;
-        }
+    __syncwarp();   // the zeros lie below
+    if (has) {
+        dmu_s[t * E + e] = g * dm;
+        dvar_s[t * E + e] = g * g * (rest * rest * w + dv);
     }
 }
 
@@ -257,16 +272,17 @@ int blocks_of(int T) { return (T + per_block(T) - 1) / per_block(T); }
 
 template <int EPL>
 int route_launch(const RouteArgs &a, cudaStream_t st) {
+    constexpr int WARPS = warps_for(EPL * 32);
     const size_t ints = sizeof(int);
     if (a.T <= ONE_BLOCK_TOKENS) {
-        route_one_block_kernel<EPL><<<1, THREADS, (a.E + 1 + WARPS * a.E) * ints, st>>>(a);
+        route_one_block_kernel<EPL, WARPS><<<1, WARPS * 32, (a.E + 1 + WARPS * a.E) * ints, st>>>(a);
         return launched("route_one_block_kernel launch");
     }
     const int blocks = blocks_of(a.T);
-    route_rank_kernel<EPL><<<blocks, THREADS, a.E * ints, st>>>(a);
+    route_rank_kernel<EPL, WARPS><<<blocks, WARPS * 32, a.E * ints, st>>>(a);
     int rc = launched("route_rank_kernel launch");
     if (rc != TAGI_OK) return rc;
-    route_place_kernel<<<blocks, THREADS, (2 * a.E + 1 + WARPS * a.E) * ints, st>>>(a);
+    route_place_kernel<WARPS><<<blocks, WARPS * 32, (2 * a.E + 1 + WARPS * a.E) * ints, st>>>(a);
     return launched("route_place_kernel launch");
 }
 
@@ -312,6 +328,7 @@ int tagi_route_fwd(int T, int E, int k, const float *mu_s, const float *var_s, i
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (E <= 32) return route_launch<1>(a, st);
     if (E <= 128) return route_launch<4>(a, st);
+    if (E <= 256) return route_launch<8>(a, st);
     if (E <= 512) return route_launch<16>(a, st);
     return route_launch<32>(a, st);
 }
@@ -326,8 +343,12 @@ int tagi_route_bwd(int T, int E, int k, const int *expert, const float *mu_g, co
     TAGI_PTR(dvar_g);
     TAGI_PTR(dmu_s);
     TAGI_PTR(dvar_s);
-    route_bwd_kernel<<<(T + WARPS - 1) / WARPS, THREADS, 0, static_cast<cudaStream_t>(stream)>>>(T, E, k, expert, mu_g, dmu_g,
-                                                                                               dvar_g, dmu_s, dvar_s);
+    const int blocks = (T + BWD_WARPS - 1) / BWD_WARPS;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (E % 4 == 0 && aligned16(dmu_s) && aligned16(dvar_s))
+        route_bwd_kernel<true><<<blocks, BWD_WARPS * 32, 0, st>>>(T, E, k, expert, mu_g, dmu_g, dvar_g, dmu_s, dvar_s);
+    else
+        route_bwd_kernel<false><<<blocks, BWD_WARPS * 32, 0, st>>>(T, E, k, expert, mu_g, dmu_g, dvar_g, dmu_s, dvar_s);
     return launched("route_bwd_kernel launch");
 }
 

@@ -211,19 +211,21 @@ __global__ void __launch_bounds__(LN_BWD_THREADS) ln_bwd_kernel(const LnBwdArgs 
     }
 }
 
-// Sum of the chunks' partials in a fixed order: 32 columns x 8 groups of chunks per CTA, one of the four sums per blockIdx.y
-__global__ void __launch_bounds__(256) ln_bwd_final_kernel(const LnBwdArgs a, int chunks) {
-    __shared__ float red[8][33];
+// Sum of the chunks' partials in a fixed order: 32 columns x 32 groups of chunks per CTA, one of the four sums per blockIdx.y
+constexpr int FINAL_GROUPS = 32;
+__global__ void __launch_bounds__(FINAL_GROUPS * 32) ln_bwd_final_kernel(const LnBwdArgs a, int chunks) {
+    __shared__ float red[FINAL_GROUPS][33];
     const int c = threadIdx.x & 31, g = threadIdx.x >> 5, i = blockIdx.x * 32 + c, q = blockIdx.y;
     float s = 0.f;
     if (i < a.n)
-        for (int k = g; k < chunks; k += 8) s += __ldg(a.part + ((size_t)k * 4 + q) * a.n + i);
+#pragma unroll 4
+        for (int k = g; k < chunks; k += FINAL_GROUPS) s += __ldg(a.part + ((size_t)k * 4 + q) * a.n + i);
     red[g][c] = s;
     __syncthreads();
     if (g != 0 || i >= a.n) return;
     s = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; k++) s += red[k][c];
+    for (int k = 0; k < FINAL_GROUPS; k++) s += red[k][c];
     const float *f = q < 2 ? a.var_w : a.var_b;
     const float v = __ldg(f + i);
     float *o = q == 0 ? a.dmu_w : q == 1 ? a.dvar_w : q == 2 ? a.dmu_b : a.dvar_b;
@@ -320,36 +322,71 @@ struct CombineBwdArgs {
     float *dmu_x, *dvar_x, *dmu_g, *dvar_g;
 };
 
-// One CTA per token: the deltas of the slots' rows, and for each slot the sums of x dmu_y and x^2 dvar_y over the features.
-template <int W>
+// TPR threads per token: the deltas of the slots' rows, and for each slot the sums of x dmu_y and x^2 dvar_y over the features.
+// Four slots at a time, so that their rows are fetched together and the token's deltas once.
+constexpr int SLOTS = 4;
+template <int W, int TPR>
 __global__ void __launch_bounds__(256) combine_bwd_kernel(const CombineBwdArgs a) {
-    __shared__ float2 red[32];
-    const long t = blockIdx.x;
-    for (int j = 0; j < a.k; j++) {
-        const int p = slot_row(a.pos, t * a.k + j, a.S);
-        float s = 0.f, s2 = 0.f;
-        if (p >= 0) {
-            const float g = __ldg(a.mu_g + t * a.k + j);
-            for (int i = threadIdx.x * W; i < a.N; i += 256 * W) {
-                float x[W], dm[W], dv[W], q[W], o[W], u[W];
-                load<W>(a.mu_x + (long)p * a.N + i, x);
-                load<W>(a.dmu_y + t * a.N + i, dm);
-                load<W>(a.dvar_y + t * a.N + i, dv);
-                if (a.jcb) load<W>(a.jcb + (long)p * a.N + i, q);
+    __shared__ float red[8][2 * SLOTS];
+    const long t = (long)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+    const int u = threadIdx.x % TPR;
+    if (TPR == 32 && t >= a.T) return;   // wider: the grid has one CTA per token
+    for (int j0 = 0; j0 < a.k; j0 += SLOTS) {
+        int p[SLOTS];
+        float g[SLOTS], s[2 * SLOTS];
 #pragma unroll
-                for (int c = 0; c < W; c++) {
-                    const float f = a.jcb ? g * q[c] : g;
-                    s += x[c] * dm[c];
-                    s2 += x[c] * dv[c] * x[c];
-                    o[c] = f * dm[c];
-                    u[c] = f * dv[c] * f;
-                }
-                store<W>(a.dmu_x + (long)p * a.N + i, o);
-                store<W>(a.dvar_x + (long)p * a.N + i, u);
-            }
+        for (int j = 0; j < SLOTS; j++) {
+            p[j] = j0 + j < a.k ? slot_row(a.pos, t * a.k + j0 + j, a.S) : -1;
+            g[j] = p[j] >= 0 ? __ldg(a.mu_g + t * a.k + j0 + j) : 0.f;
+            s[2 * j] = s[2 * j + 1] = 0.f;
         }
-        row_sum2<256>(s, s2, red);
-        if (threadIdx.x == 0) a.dmu_g[t * a.k + j] = s, a.dvar_g[t * a.k + j] = s2;
+        for (int i = u * W; i < a.N; i += TPR * W) {
+            float dm[W], dv[W], x[SLOTS][W], q[SLOTS][W];
+            load<W>(a.dmu_y + t * a.N + i, dm);
+            load<W>(a.dvar_y + t * a.N + i, dv);
+#pragma unroll
+            for (int j = 0; j < SLOTS; j++)
+                if (p[j] >= 0) {
+                    load<W>(a.mu_x + (long)p[j] * a.N + i, x[j]);
+                    if (a.jcb) load<W>(a.jcb + (long)p[j] * a.N + i, q[j]);
+                }
+#pragma unroll
+            for (int j = 0; j < SLOTS; j++)
+                if (p[j] >= 0) {
+                    float o[W], r[W];
+#pragma unroll
+                    for (int c = 0; c < W; c++) {
+                        const float f = a.jcb ? g[j] * q[j][c] : g[j];
+                        s[2 * j] += x[j][c] * dm[c];
+                        s[2 * j + 1] += x[j][c] * dv[c] * x[j][c];
+                        o[c] = f * dm[c];
+                        r[c] = f * dv[c] * f;
+                    }
+                    store<W>(a.dmu_x + (long)p[j] * a.N + i, o);
+                    store<W>(a.dvar_x + (long)p[j] * a.N + i, r);
+                }
+        }
+#pragma unroll
+        for (int q = 0; q < 2 * SLOTS; q++) s[q] = warp_sum(s[q]);
+        if (TPR > 32) {
+            __syncthreads();
+            if ((threadIdx.x & 31) == 0)
+#pragma unroll
+                for (int q = 0; q < 2 * SLOTS; q++) red[threadIdx.x >> 5][q] = s[q];
+            __syncthreads();
+        }
+        if (u < 2 * SLOTS && j0 + u / 2 < a.k) {
+            float v = 0.f;
+            if (TPR > 32) {
+#pragma unroll
+                for (int w = 0; w < 8; w++) v += red[w][u];
+            } else {
+#pragma unroll
+                for (int q = 0; q < 2 * SLOTS; q++)
+                    if (q == u) v = s[q];
+            }
+            ((u & 1) ? a.dvar_g : a.dmu_g)[t * a.k + j0 + u / 2] = v;
+        }
     }
 }
 
@@ -438,7 +475,7 @@ int tagi_ln_bwd(int R, int n, int has_bias, int state_update, float eps, const f
     else ln_bwd_kernel<1><<<grid, LN_BWD_THREADS, 0, st>>>(a);
     int rc = launched("ln_bwd_kernel launch");
     if (rc != TAGI_OK || chunks <= 1) return rc;
-    ln_bwd_final_kernel<<<dim3((n + 31) / 32, has_bias ? 4 : 2), 256, 0, st>>>(a, chunks);
+    ln_bwd_final_kernel<<<dim3((n + 31) / 32, has_bias ? 4 : 2), FINAL_GROUPS * 32, 0, st>>>(a, chunks);
     return launched("ln_bwd_final_kernel launch");
 }
 
@@ -493,10 +530,13 @@ int tagi_combine_bwd(int T, int k, int N, int S, const int *pos, const float *mu
     TAGI_PTR(dvar_g);
     TAGI_REQUIRE(jcb == nullptr || aligned4(jcb), "jcb is not 4-byte aligned");
     const CombineBwdArgs a{T, k, N, S, pos, mu_g, mu_x, jcb, dmu_y, dvar_y, dmu_x, dvar_x, dmu_g, dvar_g};
-    if (N % 4 == 0 && all16({mu_x, jcb, dmu_y, dvar_y, dmu_x, dvar_x}))
-        combine_bwd_kernel<4><<<T, 256, 0, static_cast<cudaStream_t>(stream)>>>(a);
-    else
-        combine_bwd_kernel<1><<<T, 256, 0, static_cast<cudaStream_t>(stream)>>>(a);
+    // a warp per token where a row is at most four of its strides long, else a CTA
+    const bool vec = N % 4 == 0 && all16({mu_x, jcb, dmu_y, dvar_y, dmu_x, dvar_x});
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (vec && N > 512) combine_bwd_kernel<4, 256><<<T, 256, 0, st>>>(a);
+    else if (vec) combine_bwd_kernel<4, 32><<<(T + 7) / 8, 256, 0, st>>>(a);
+    else if (N > 128) combine_bwd_kernel<1, 256><<<T, 256, 0, st>>>(a);
+    else combine_bwd_kernel<1, 32><<<(T + 7) / 8, 256, 0, st>>>(a);
     return launched("combine_bwd_kernel launch");
 }
 
