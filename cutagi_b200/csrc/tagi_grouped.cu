@@ -13,7 +13,7 @@ __global__ void __launch_bounds__(256) grouped_bias_kernel(const GroupedArgs a) 
     const int c = threadIdx.x & 31, g = threadIdx.x >> 5, n = blockIdx.x * 32 + c, e = blockIdx.y;
     int r0, r1;
     expert_rows(a, e, r0, r1);
-    if (r1 - r0 <= FEW_PARAM_ROWS) return;
+    if (r1 - r0 <= FEW_ROWS) return;
     float s = 0.f, v = 0.f;
     if (n < a.N)
         for (int r = r0 + g; r < r1; r += 8) s += __ldg(a.a0 + (size_t)r * a.N + n), v += __ldg(a.a1 + (size_t)r * a.N + n);
@@ -35,7 +35,7 @@ inline int launched(const char *what) {
 
 int run(int pass, const GroupedArgs &a, cudaStream_t st) {
     const int rc = grouped_few(pass, a, st);
-    return rc != TAGI_OK || a.S <= few_rows(pass) ? rc : grouped_tc(pass, a, st);
+    return rc != TAGI_OK || a.S <= FEW_ROWS ? rc : grouped_tc(pass, a, st);
 }
 
 int check_grouped(const char *who, int E, int S, int K, int N, const int *offsets) {
@@ -136,7 +136,7 @@ int tagi_grouped_linear_bwd_param(int E, int S, int R, int K, int N, int has_bia
     a.var_b = has_bias ? var_b : nullptr, a.a0 = dmu_z, a.a1 = dvar_z, a.o0 = dmu_w, a.o1 = dvar_w, a.ob0 = dmu_b, a.ob1 = dvar_b;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     rc = run(PARAM, a, st);
-    if (rc != TAGI_OK || !has_bias || S <= FEW_PARAM_ROWS) return rc;
+    if (rc != TAGI_OK || !has_bias || S <= FEW_ROWS) return rc;
     grouped_bias_kernel<<<dim3((N + 31) / 32, E), 256, 0, st>>>(a);
     return launched("grouped_bias_kernel launch");
 }

@@ -31,8 +31,7 @@ __device__ __forceinline__ int input_row(const GroupedArgs &a, int p) {
 
 // Experts with up to this many rows run on the kernels of tagi_grouped_few.cu (one pass over the weights on the FP32 pipe),
 // those with more on the tensor cores.
-constexpr int FEW_ROWS = 8, FEW_PARAM_ROWS = 16;
-inline int few_rows(int pass) { return pass == PARAM ? FEW_PARAM_ROWS : FEW_ROWS; }
+constexpr int FEW_ROWS = 32;
 
 int grouped_few(int pass, const GroupedArgs &a, cudaStream_t st);
 int grouped_tc(int pass, const GroupedArgs &a, cudaStream_t st);

@@ -1,16 +1,212 @@
 // Linear layers grouped by expert, experts with few rows: every weight is read once and met by all rows of its expert, on
-// the FP32 pipe. These passes are bound by HBM (8, 4 and 12 bytes a weight in the forward, state and parameter pass), as
-// long as the rows' multiplications keep up: 3, 2 and 2 a weight and row. Experts with more rows than the limits below are
-// left to the tensor-core kernel, which in turn leaves these alone; the offsets are device data, so both are launched when
-// the number of rows in all does not rule one out.
+// the FP32 pipe. These passes are bound by HBM (8, 4 and 12 bytes a weight in the forward, state and parameter pass) until
+// the rows' multiplications (3, 2 and 2 a weight and row) take longer, at about 14, 11 and 33 rows. Experts with more than
+// FEW_ROWS are left to the tensor-core kernel, which in turn leaves these alone; the offsets are device data, so both are
+// launched unless the number of rows in all rules one out.
+//
+// Forward and state pass: a CTA computes 64 output columns of all the expert's rows. The weights come in slabs of 32
+// contraction steps through a ring filled with cp.async, so that the bytes in flight cost no registers: four stages where
+// two CTAs share an SM, as many as fit where there are too few CTAs for that. Eight warps share a slab: they cut it along the contraction and, with
+// more than eight rows, among groups of eight; a thread multiplies its two columns with eight rows, whose entries
+// all lanes read at the same address. The warps' sums are added in a fixed order at the end.
 #include "tagi_grouped.h"
 
 namespace tagi {
 namespace {
 
-constexpr unsigned FULL = 0xffffffffu;
+constexpr int OUT = 64, SLAB = 32, WARPS = 8, THREADS = WARPS * 32, GROUP = 8;
+constexpr int PITCH = SLAB + 4;                          // floats of a weight row in shared memory: no bank conflicts
+constexpr int FWD_WEIGHTS = 2 * OUT * PITCH, STATE_WEIGHTS = SLAB * OUT;
 
-// W consecutive floats. Weights pass by once: they are kept out of L1, where the rows are wanted.
+__device__ __forceinline__ uint32_t smem_at(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+// Four floats to shared memory, of which the first `valid` (any number, also none or more than four) exist; zeros else.
+template <bool VEC>
+__device__ __forceinline__ void copy4(float *dst, const float *src, int valid) {
+    const uint32_t d = smem_at(dst);
+    if (VEC) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(valid > 0 ? 16 : 0) : "memory");
+    } else {
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(d + c * 4), "l"(src + (c < valid ? c : 0)), "r"(c < valid ? 4 : 0)
+                         : "memory");
+    }
+}
+__device__ __forceinline__ float4 at4(const float *p) { return *reinterpret_cast<const float4 *>(p); }
+
+// Two contraction steps of a sum in one register pair: two multiply-adds are one instruction.
+typedef unsigned long long Pair;
+__device__ __forceinline__ Pair pair_of(float a, float b) {
+    Pair p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
+    return p;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+    Pair d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float sum_of(Pair p) {
+    float a, b;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+    return a + b;
+}
+
+// GROUPS of eight rows. smem: STAGES stages of weights and rows, used again for the warps' sums.
+template <int PASS, bool VEC, int GROUPS, int STAGES>
+__device__ __forceinline__ void few_rows_pass(const GroupedArgs &a, int e, int r0, int rows, float *smem) {
+    constexpr int ROWS = GROUP * GROUPS, WEIGHTS = PASS == FWD ? FWD_WEIGHTS : STATE_WEIGHTS, STAGE = WEIGHTS + 2 * ROWS * SLAB;
+    constexpr int SPLITS = WARPS / GROUPS;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = warp % GROUPS, split = warp / GROUPS;
+    const int o0 = blockIdx.x * OUT, outs = PASS == FWD ? a.N : a.K, depth = PASS == FWD ? a.K : a.N;
+    const size_t wbase = (size_t)e * a.N * a.K;
+
+    // rows of this thread's copies: copy c = tid + i * 256 is quad c & 7 of row (c >> 3) % ROWS, means first
+    constexpr int COPIES = (2 * ROWS * 8 + THREADS - 1) / THREADS;
+    int row[COPIES];
+#pragma unroll
+    for (int i = 0; i < COPIES; i++) {
+        const int c = tid + i * THREADS, r = (c >> 3) % ROWS;
+        row[i] = c < 2 * ROWS * 8 && r < rows ? (PASS == FWD ? input_row(a, r0 + r) : r0 + r) : -1;
+    }
+    auto fetch = [&](int slab) {
+        const int k0 = slab * SLAB;
+        float *s = smem + (slab % STAGES) * STAGE;
+        if (k0 < depth) {
+            if (PASS == FWD) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int c = tid + (i & 1) * THREADS, n = c >> 3, k = k0 + (c & 7) * 4;
+                    copy4<VEC>(s + (i >> 1) * OUT * PITCH + n * PITCH + (c & 7) * 4,
+                               (i < 2 ? a.mu_w : a.var_w) + (o0 + n < a.N ? wbase + (size_t)(o0 + n) * a.K + (k < a.K ? k : 0) : 0),
+                               o0 + n < a.N ? a.K - k : 0);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const int c = tid + i * THREADS, n = k0 + (c >> 4), k = o0 + (c & 15) * 4;
+                    copy4<VEC>(s + (c >> 4) * OUT + (c & 15) * 4, a.mu_w + (n < a.N ? wbase + (size_t)n * a.K + (k < a.K ? k : 0) : 0),
+                               n < a.N ? a.K - k : 0);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < COPIES; i++) {
+                const int c = tid + i * THREADS;
+                if (c >= 2 * ROWS * 8) break;
+                const int k = k0 + (c & 7) * 4;
+                copy4<VEC>(s + WEIGHTS + c * 4, (c < ROWS * 8 ? a.a0 : a.a1) + (row[i] >= 0 && k < depth ? (size_t)row[i] * depth + k : 0),
+                           row[i] >= 0 ? depth - k : 0);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    const int live = min(GROUP, rows - group * GROUP);
+    Pair z[2][GROUP], vz[2][GROUP];
+#pragma unroll
+    for (int t = 0; t < GROUP; t++) z[0][t] = z[1][t] = vz[0][t] = vz[1][t] = 0;
+    const int slabs = (depth + SLAB - 1) / SLAB;
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; s++) fetch(s);
+    for (int it = 0; it < slabs; it++) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+        __syncthreads();   // slab `it` is there for all, and nobody reads the stage that is filled next any more
+        fetch(it + STAGES - 1);
+        const float *w = smem + (it % STAGES) * STAGE, *x = w + WEIGHTS + group * GROUP * SLAB, *y = x + ROWS * SLAB;
+#pragma unroll
+        for (int q = split; q < SLAB / 4; q += SPLITS) {
+            Pair wm[2][2], wq[2][2], wv[2][2];   // the thread's two columns at four steps: means, their squares, variances
+#pragma unroll
+            for (int f = 0; f < 2; f++) {
+                if (PASS == FWD) {
+                    const float4 m = at4(w + (f * 32 + lane) * PITCH + q * 4), v = at4(w + OUT * PITCH + (f * 32 + lane) * PITCH + q * 4);
+                    wm[f][0] = pair_of(m.x, m.y), wm[f][1] = pair_of(m.z, m.w);
+                    wv[f][0] = pair_of(v.x, v.y), wv[f][1] = pair_of(v.z, v.w);
+                } else {
+                    const float *p = w + q * 4 * OUT + f * 32 + lane;
+                    wm[f][0] = pair_of(p[0], p[OUT]), wm[f][1] = pair_of(p[2 * OUT], p[3 * OUT]);
+                }
+                wq[f][0] = mul2(wm[f][0], wm[f][0]), wq[f][1] = mul2(wm[f][1], wm[f][1]);
+            }
+#pragma unroll
+            for (int t = 0; t < GROUP; t++)
+                if (t < live) {
+                    const float4 xt = at4(x + t * SLAB + q * 4), yt = at4(y + t * SLAB + q * 4);
+                    const Pair xs[2] = {pair_of(xt.x, xt.y), pair_of(xt.z, xt.w)}, ys[2] = {pair_of(yt.x, yt.y), pair_of(yt.z, yt.w)};
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        const Pair second = PASS == FWD ? fma2(xs[c], xs[c], ys[c]) : 0;
+#pragma unroll
+                        for (int f = 0; f < 2; f++) {
+                            z[f][t] = fma2(xs[c], wm[f][c], z[f][t]);
+                            vz[f][t] = fma2(ys[c], wq[f][c], vz[f][t]);
+                            if (PASS == FWD) vz[f][t] = fma2(second, wv[f][c], vz[f][t]);
+                        }
+                    }
+                }
+        }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+    // red[split][row][kind][column]
+    float *red = smem;
+#pragma unroll
+    for (int t = 0; t < GROUP; t++)
+#pragma unroll
+        for (int f = 0; f < 2; f++) {
+            const int at = ((split * ROWS + group * GROUP + t) * 2) * OUT + f * 32 + lane;
+            red[at] = sum_of(z[f][t]);
+            red[at + OUT] = sum_of(vz[f][t]);
+        }
+    __syncthreads();
+    for (int i = tid; i < rows * 2 * OUT; i += THREADS) {
+        float s = 0.f;
+#pragma unroll
+        for (int p = 0; p < SPLITS; p++) s += red[p * ROWS * 2 * OUT + i];
+        const int c = o0 + (i & (OUT - 1)), r = i / (2 * OUT);
+        const bool var = (i / OUT) & 1;
+        if (c >= outs) continue;
+        const size_t o = (size_t)(r0 + r) * outs + c;
+        if (PASS == FWD) {
+            if (a.mu_b) s += __ldg((var ? a.var_b : a.mu_b) + (size_t)e * a.N + c);
+        } else if (a.jcb) {
+            const float j = __ldg(a.jcb + o);
+            s = var ? s * j * j : s * j;
+        }
+        (var ? a.o1 : a.o0)[o] = s;
+    }
+}
+
+template <int PASS>
+constexpr size_t few_smem(int groups, int stages) {
+    const size_t stage = (PASS == FWD ? FWD_WEIGHTS : STATE_WEIGHTS) + 2 * groups * GROUP * SLAB, sums = WARPS * GROUP * 2 * OUT;
+    return (stages * stage > sums ? stages * stage : sums) * sizeof(float);
+}
+
+// MOST: groups of rows that an expert can have, by the rows there are in all
+template <int PASS, bool VEC, int MOST, int STAGES>
+__global__ void __launch_bounds__(THREADS, STAGES == 4 ? 2 : 1) grouped_few_kernel(const GroupedArgs a) {
+    extern __shared__ __align__(16) float smem[];
+    const int e = blockIdx.y;
+    int r0, r1;
+    expert_rows(a, e, r0, r1);
+    const int rows = r1 - r0;
+    if (rows == 0 || rows > FEW_ROWS) return;
+    if (rows <= 8) few_rows_pass<PASS, VEC, 1, STAGES>(a, e, r0, rows, smem);
+    else if (MOST >= 2 && rows <= 16) few_rows_pass<PASS, VEC, 2, STAGES>(a, e, r0, rows, smem);
+    else if (MOST == 4) few_rows_pass<PASS, VEC, 4, STAGES>(a, e, r0, rows, smem);
+}
+
+// -------------------------------------------------------------------------------------------------------- parameters
+// A warp computes PARAM_N output features x 32 lanes of W input features; a CTA stacks 8 warps along the output features. The
+// prior variances are fetched before the rows are added up; the deltas come from shared memory, at one address for all lanes.
+constexpr int PARAM_N = 8, PARAM_OUT = WARPS * PARAM_N;
+
 template <int W>
 __device__ __forceinline__ void load(const float *p, float (&v)[W]) {
     if (W == 4) {
@@ -20,228 +216,60 @@ __device__ __forceinline__ void load(const float *p, float (&v)[W]) {
         v[0] = __ldg(p);
     }
 }
-template <int W>
-__device__ __forceinline__ void load_once(const float *p, float (&v)[W]) {
-    if (W == 4)
-        asm("ld.global.nc.L1::no_allocate.v4.f32 {%0, %1, %2, %3}, [%4];"
-            : "=f"(v[0]), "=f"(v[1 % W]), "=f"(v[2 % W]), "=f"(v[3 % W])
-            : "l"(p));
-    else
-        asm("ld.global.nc.L1::no_allocate.f32 %0, [%1];" : "=f"(v[0]) : "l"(p));
-}
-template <int W>
-__device__ __forceinline__ void zero(float (&v)[W]) {
-#pragma unroll
-    for (int c = 0; c < W; c++) v[c] = 0.f;
-}
-
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
-    return v;
-}
-
-// ---------------------------------------------------------------------------------------------------------- forward
-// A warp computes FEATURES output features of R rows, its lanes along the contraction.
-constexpr int FEATURES = 4, FWD_WARPS = 8;
-
-template <int W, int R>
-__device__ __forceinline__ void forward_rows(const GroupedArgs &a, int e, int r0, int rows, int n0) {
-    const int lane = threadIdx.x & 31;
-    float z[FEATURES][R], vz[FEATURES][R];
-#pragma unroll
-    for (int f = 0; f < FEATURES; f++)
-#pragma unroll
-        for (int r = 0; r < R; r++) z[f][r] = vz[f][r] = 0.f;
-    int row[R];
-#pragma unroll
-    for (int r = 0; r < R; r++) row[r] = r < rows ? input_row(a, r0 + r) : -1;
-    const size_t w0 = ((size_t)e * a.N + n0) * a.K;
-#pragma unroll 1
-    for (int k = lane * W; k < a.K; k += 32 * W) {
-        float w[FEATURES][W], vw[FEATURES][W];
-#pragma unroll
-        for (int f = 0; f < FEATURES; f++) {
-            zero(w[f]), zero(vw[f]);
-            if (n0 + f < a.N) {
-                load_once<W>(a.mu_w + w0 + (size_t)f * a.K + k, w[f]);
-                load_once<W>(a.var_w + w0 + (size_t)f * a.K + k, vw[f]);
-            }
-        }
-#pragma unroll
-        for (int r = 0; r < R; r++) {
-            float x[W], v[W];
-            zero(x), zero(v);
-            if (row[r] >= 0) {
-                load<W>(a.a0 + (size_t)row[r] * a.K + k, x);
-                load<W>(a.a1 + (size_t)row[r] * a.K + k, v);
-            }
-#pragma unroll
-            for (int c = 0; c < W; c++) {
-                const float s = fmaf(x[c], x[c], v[c]);
-#pragma unroll
-                for (int f = 0; f < FEATURES; f++) {
-                    z[f][r] = fmaf(x[c], w[f][c], z[f][r]);
-                    vz[f][r] = fmaf(s, vw[f][c], fmaf(v[c], w[f][c] * w[f][c], vz[f][r]));
-                }
-            }
-        }
-    }
-#pragma unroll
-    for (int f = 0; f < FEATURES; f++)
-#pragma unroll
-        for (int r = 0; r < R; r++) {
-            const float m = warp_sum(z[f][r]), v = warp_sum(vz[f][r]);
-            const int n = n0 + f;
-            if (lane == (f * R + r) % 32 && n < a.N && r < rows) {
-                const size_t o = (size_t)(r0 + r) * a.N + n;
-                a.o0[o] = m + (a.mu_b ? __ldg(a.mu_b + (size_t)e * a.N + n) : 0.f);
-                a.o1[o] = v + (a.mu_b ? __ldg(a.var_b + (size_t)e * a.N + n) : 0.f);
-            }
-        }
-}
 
 template <int W>
-__global__ void __launch_bounds__(FWD_WARPS * 32) grouped_few_fwd_kernel(const GroupedArgs a) {
-    const int e = blockIdx.y, n0 = (blockIdx.x * FWD_WARPS + (threadIdx.x >> 5)) * FEATURES;
-    int r0, r1;
-    expert_rows(a, e, r0, r1);
-    const int rows = r1 - r0;
-    if (rows == 0 || rows > FEW_ROWS || n0 >= a.N) return;
-    if (rows == 1) forward_rows<W, 1>(a, e, r0, rows, n0);
-    else if (rows == 2) forward_rows<W, 2>(a, e, r0, rows, n0);
-    else if (rows <= 4) forward_rows<W, 4>(a, e, r0, rows, n0);
-    else forward_rows<W, 8>(a, e, r0, rows, n0);
-}
-
-// ------------------------------------------------------------------------------------------------------------ state
-// A CTA computes 64 input features of R rows: 16 lanes of four features each, the contraction over the output features cut
-// among the 32 half-warps of 16 warps, whose sums are then added in a fixed order.
-constexpr int STATE_WARPS = 16, STATE_COLS = 64;
-
-template <int W, int R>
-__device__ __forceinline__ void state_rows(const GroupedArgs &a, int e, int r0, int rows, float *red) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp * 2 + (lane >> 4);
-    const int k = blockIdx.x * STATE_COLS + (lane & 15) * 4;
-    float d[R][4], v[R][4];
-#pragma unroll
-    for (int r = 0; r < R; r++) zero(d[r]), zero(v[r]);
-    // W == 4: four output features at a time, k .. k + 3 all inside or all outside
-    for (int n = part * W; n < a.N; n += 2 * STATE_WARPS * W) {
-        float w[W][4];
-#pragma unroll
-        for (int i = 0; i < W; i++) {
-            zero(w[i]);
-            const float *p = a.mu_w + ((size_t)e * a.N + n + i) * a.K + k;
-            if (W == 4) {
-                if (k < a.K) load_once<4>(p, w[i]);
-            } else {
-#pragma unroll
-                for (int c = 0; c < 4; c++)
-                    if (k + c < a.K) w[i][c] = __ldg(p + c);
-            }
-        }
-#pragma unroll
-        for (int r = 0; r < R; r++) {
-            float x[W], y[W];
-            zero(x), zero(y);
-            if (r < rows) {
-                load<W>(a.a0 + (size_t)(r0 + r) * a.N + n, x);
-                load<W>(a.a1 + (size_t)(r0 + r) * a.N + n, y);
-            }
-#pragma unroll
-            for (int i = 0; i < W; i++)
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    d[r][c] = fmaf(x[i], w[i][c], d[r][c]);
-                    v[r][c] = fmaf(y[i], w[i][c] * w[i][c], v[r][c]);
-                }
-        }
-    }
-    // the halves of a warp, then the warps, one row at a time: red holds [STATE_WARPS][2][64]
-#pragma unroll
-    for (int r = 0; r < R; r++) {
-        if (r >= rows) break;
-        __syncthreads();
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-            const float s = d[r][c] + __shfl_xor_sync(FULL, d[r][c], 16), t = v[r][c] + __shfl_xor_sync(FULL, v[r][c], 16);
-            if (lane < 16) {
-                red[warp * 128 + lane * 4 + c] = s;
-                red[warp * 128 + 64 + lane * 4 + c] = t;
-            }
-        }
-        __syncthreads();
-        if (threadIdx.x < 128) {
-            float s = 0.f;
-#pragma unroll
-            for (int w = 0; w < STATE_WARPS; w++) s += red[w * 128 + threadIdx.x];
-            const int col = blockIdx.x * STATE_COLS + (threadIdx.x & 63);
-            if (col < a.K) {
-                const size_t o = (size_t)(r0 + r) * a.K + col;
-                const float j = a.jcb ? __ldg(a.jcb + o) : 1.f;
-                if (threadIdx.x < 64) a.o0[o] = s * j;
-                else a.o1[o] = s * j * j;
-            }
-        }
-    }
-}
-
-template <int W>
-__global__ void __launch_bounds__(STATE_WARPS * 32) grouped_few_state_kernel(const GroupedArgs a) {
-    __shared__ float red[STATE_WARPS * 128];
-    const int e = blockIdx.y;
-    int r0, r1;
-    expert_rows(a, e, r0, r1);
-    const int rows = r1 - r0;
-    if (rows == 0 || rows > FEW_ROWS) return;
-    if (rows == 1) state_rows<W, 1>(a, e, r0, rows, red);
-    else if (rows == 2) state_rows<W, 2>(a, e, r0, rows, red);
-    else if (rows <= 4) state_rows<W, 4>(a, e, r0, rows, red);
-    else state_rows<W, 8>(a, e, r0, rows, red);
-}
-
-// -------------------------------------------------------------------------------------------------------- parameters
-// A warp computes PARAM_N output features x 32 lanes of W input features; a CTA stacks 8 warps along the output features.
-constexpr int PARAM_N = 8, PARAM_WARPS = 8;
-
-template <int W>
-__global__ void __launch_bounds__(PARAM_WARPS * 32) grouped_few_param_kernel(const GroupedArgs a) {
+__global__ void __launch_bounds__(THREADS, 2) grouped_few_param_kernel(const GroupedArgs a) {
+    __shared__ __align__(16) float delta[FEW_ROWS][2][PARAM_OUT];
+    __shared__ int input[FEW_ROWS];
     const int e = blockIdx.z;
     int r0, r1;
     expert_rows(a, e, r0, r1);
-    if (r1 - r0 > FEW_PARAM_ROWS) return;
-    const int lane = threadIdx.x & 31, block_n = blockIdx.y * PARAM_WARPS * PARAM_N, n0 = block_n + (threadIdx.x >> 5) * PARAM_N;
+    const int rows = r1 - r0;
+    if (rows > FEW_ROWS) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, block_n = blockIdx.y * PARAM_OUT, n0 = block_n + warp * PARAM_N;
     const int k = (blockIdx.x * 32 + lane) * W;
-    if (a.var_b && blockIdx.x == 0 && threadIdx.x < PARAM_WARPS * PARAM_N && block_n + threadIdx.x < a.N) {
-        const int n = block_n + threadIdx.x;
-        float s = 0.f, t = 0.f;
-        for (int r = r0; r < r1; r++) s += __ldg(a.a0 + (size_t)r * a.N + n), t += __ldg(a.a1 + (size_t)r * a.N + n);
-        const float vb = __ldg(a.var_b + (size_t)e * a.N + n);
-        a.ob0[(size_t)e * a.N + n] = vb * s;
-        a.ob1[(size_t)e * a.N + n] = vb * vb * t;
-    }
-    if (n0 >= a.N || k >= a.K) return;
+    const bool live = k < a.K;
     float d[PARAM_N][W], v[PARAM_N][W], s[PARAM_N][W];
     const size_t o = ((size_t)e * a.N + n0) * a.K + k;
 #pragma unroll
     for (int i = 0; i < PARAM_N; i++) {
-        zero(d[i]), zero(v[i]), zero(s[i]);
-        if (n0 + i < a.N) load_once<W>(a.var_w + o + (size_t)i * a.K, s[i]);   // on their way while the rows are added up
+#pragma unroll
+        for (int c = 0; c < W; c++) d[i][c] = v[i][c] = s[i][c] = 0.f;
+        if (live && n0 + i < a.N) load<W>(a.var_w + o + (size_t)i * a.K, s[i]);
     }
-    for (int r = r0; r < r1; r++) {
-        const int row = input_row(a, r);
-        if (row < 0) continue;
+    for (int i = threadIdx.x; i < rows * 2 * PARAM_OUT; i += THREADS) {
+        const int n = block_n + i % PARAM_OUT, r = i / (2 * PARAM_OUT);
+        delta[r][(i / PARAM_OUT) & 1][i % PARAM_OUT] = n < a.N ? __ldg(((i / PARAM_OUT) & 1 ? a.a1 : a.a0) + (size_t)(r0 + r) * a.N + n) : 0.f;
+    }
+    for (int r = threadIdx.x; r < rows; r += THREADS) input[r] = input_row(a, r0 + r);
+    __syncthreads();
+    if (a.var_b && blockIdx.x == 0 && threadIdx.x < 2 * PARAM_OUT) {
+        const int kind = threadIdx.x / PARAM_OUT, n = block_n + threadIdx.x % PARAM_OUT;
+        if (n < a.N) {
+            float t = 0.f;
+            for (int r = 0; r < rows; r++) t += delta[r][kind][threadIdx.x % PARAM_OUT];
+            const float vb = __ldg(a.var_b + (size_t)e * a.N + n);
+            (kind ? a.ob1 : a.ob0)[(size_t)e * a.N + n] = kind ? vb * vb * t : vb * t;
+        }
+    }
+    if (!live) return;
+#pragma unroll 2
+    for (int r = 0; r < rows; r++) {
+        const int row = input[r];
         float x[W], q[W];
-        load<W>(a.x + (size_t)row * a.K + k, x);
+#pragma unroll
+        for (int c = 0; c < W; c++) x[c] = 0.f;
+        if (row >= 0) load<W>(a.x + (size_t)row * a.K + k, x);
 #pragma unroll
         for (int c = 0; c < W; c++) q[c] = x[c] * x[c];
 #pragma unroll
-        for (int i = 0; i < PARAM_N; i++) {
-            if (n0 + i >= a.N) break;
-            const float dm = __ldg(a.a0 + (size_t)r * a.N + n0 + i), dv = __ldg(a.a1 + (size_t)r * a.N + n0 + i);
+        for (int h = 0; h < PARAM_N; h += 4) {
+            const float4 m = at4(&delta[r][0][warp * PARAM_N + h]), u = at4(&delta[r][1][warp * PARAM_N + h]);
+            const float dm[4] = {m.x, m.y, m.z, m.w}, dv[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-            for (int c = 0; c < W; c++) d[i][c] = fmaf(dm, x[c], d[i][c]), v[i][c] = fmaf(dv, q[c], v[i][c]);
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int c = 0; c < W; c++) d[h + i][c] = fmaf(dm[i], x[c], d[h + i][c]), v[h + i][c] = fmaf(dv[i], q[c], v[h + i][c]);
         }
     }
 #pragma unroll
@@ -260,28 +288,42 @@ __global__ void __launch_bounds__(PARAM_WARPS * 32) grouped_few_param_kernel(con
     }
 }
 
+template <int PASS, bool VEC, int MOST, int STAGES>
+int launch_few(const GroupedArgs &a, cudaStream_t st) {
+    auto k = grouped_few_kernel<PASS, VEC, MOST, STAGES>;
+    constexpr size_t smem = few_smem<PASS>(MOST, STAGES);
+    static_assert(smem <= 227 * 1024, "more shared memory than an SM has");
+    TAGI_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    k<<<dim3(((PASS == FWD ? a.N : a.K) + OUT - 1) / OUT, a.E), THREADS, smem, st>>>(a);
+    TAGI_CUDA(cudaGetLastError());
+    return TAGI_OK;
+}
+
+template <int PASS, bool VEC>
+int launch_few(const GroupedArgs &a, cudaStream_t st) {
+    // CTAs that have work, at most: with one or none for an SM, each gets a deep ring
+    const long ctas = (((PASS == FWD ? a.N : a.K) + OUT - 1) / OUT) * (long)(a.E < a.S ? a.E : a.S);
+    if (a.S <= 8) return ctas <= 148 ? launch_few<PASS, VEC, 1, 10>(a, st) : launch_few<PASS, VEC, 1, 4>(a, st);
+    return launch_few<PASS, VEC, 4, 4>(a, st);
+}
+
+template <int PASS>
+int launch(const GroupedArgs &a, cudaStream_t st) {
+    const bool vec = a.K % 4 == 0 && (PASS == FWD || a.N % 4 == 0) && aligned16(a.mu_w) && aligned16(a.var_w) && aligned16(a.a0) &&
+                     aligned16(a.a1);
+    return vec ? launch_few<PASS, true>(a, st) : launch_few<PASS, false>(a, st);
+}
+
 }  // namespace
 
 int grouped_few(int pass, const GroupedArgs &a, cudaStream_t st) {
-    const bool k4 = a.K % 4 == 0, n4 = a.N % 4 == 0;
-    if (pass == FWD) {
-        const dim3 grid((a.N + FWD_WARPS * FEATURES - 1) / (FWD_WARPS * FEATURES), a.E);
-        if (k4 && aligned16(a.mu_w) && aligned16(a.var_w) && aligned16(a.a0) && aligned16(a.a1))
-            grouped_few_fwd_kernel<4><<<grid, FWD_WARPS * 32, 0, st>>>(a);
-        else
-            grouped_few_fwd_kernel<1><<<grid, FWD_WARPS * 32, 0, st>>>(a);
-    } else if (pass == STATE) {
-        const dim3 grid((a.K + STATE_COLS - 1) / STATE_COLS, a.E);
-        if (k4 && n4 && aligned16(a.mu_w) && aligned16(a.a0) && aligned16(a.a1))
-            grouped_few_state_kernel<4><<<grid, STATE_WARPS * 32, 0, st>>>(a);
-        else
-            grouped_few_state_kernel<1><<<grid, STATE_WARPS * 32, 0, st>>>(a);
-    } else {
-        const bool vec = k4 && aligned16(a.var_w) && aligned16(a.x) && aligned16(a.o0) && aligned16(a.o1);
-        const dim3 grid((a.K + 32 * (vec ? 4 : 1) - 1) / (32 * (vec ? 4 : 1)), (a.N + PARAM_WARPS * PARAM_N - 1) / (PARAM_WARPS * PARAM_N), a.E);
-        if (vec) grouped_few_param_kernel<4><<<grid, PARAM_WARPS * 32, 0, st>>>(a);
-        else grouped_few_param_kernel<1><<<grid, PARAM_WARPS * 32, 0, st>>>(a);
-    }
+    if (pass == FWD) return launch<FWD>(a, st);
+    if (pass == STATE) return launch<STATE>(a, st);
+    const bool vec = a.K % 4 == 0 && aligned16(a.var_w) && aligned16(a.x) && aligned16(a.o0) && aligned16(a.o1);
+    const int per = 32 * (vec ? 4 : 1);
+    const dim3 grid((a.K + per - 1) / per, (a.N + PARAM_OUT - 1) / PARAM_OUT, a.E);
+    if (vec) grouped_few_param_kernel<4><<<grid, THREADS, 0, st>>>(a);
+    else grouped_few_param_kernel<1><<<grid, THREADS, 0, st>>>(a);
     TAGI_CUDA(cudaGetLastError());
     return TAGI_OK;
 }

@@ -11,9 +11,9 @@
 // Shape of the work. Rows of the tensor-core tile are features (of the weights: always many), columns are the expert's
 // rows (ragged: any width in steps of 32), so a thin expert costs a narrow tile. Two CTAs of a cluster share a tile of
 // 256 features x up to 256 columns (cta_group::2); every accumulator lane is a feature, so stores run along memory.
-// The mean and the variance are two accumulations over different operands (forward: mu_w.mu_a; var_w.(mu_a^2 + var_a)
-// followed by mu_w^2.var_a as one contraction of twice the length), done one after the other by the same pair, which
-// finds the second's operands in L2.
+// The mean and the variance are two accumulations over different operands (forward: mu_w.mu_a; mu_w^2.var_a followed by
+// var_w.(mu_a^2 + var_a) as one contraction of twice the length), which neighbouring pairs do at the same time: mu_w is
+// fetched from HBM for one and found in L2 by the other.
 //
 // Roles. Eight converter warps fetch both operands from global memory into registers (gathered rows, ragged edges and any
 // alignment cost nothing extra there), form squares, split and store the parts to shared memory in the swizzled layouts
@@ -216,7 +216,7 @@ __device__ __forceinline__ void release(Shared &sh, int j, int lane) {
 // What both operands' converters follow: the chunk that is loaded next. It runs ahead of the chunk that is stored.
 struct Cursor {
     int j, c, chunks, kc;
-    bool var, half;   // of a variance; second half of a forward variance (mu_w^2 . var_a)
+    bool var, half;   // of a variance; second half of a forward variance (var_w . (mu_a^2 + var_a))
 };
 
 // A: 128 features of this CTA. A chunk is fetched whole as soon as the registers of the one before have been stored (one
@@ -265,7 +265,7 @@ __device__ __forceinline__ void convert_a(const GroupedArgs &a, Shared &sh, int 
         }
 #pragma unroll
         for (int g = 0; g < 4; g++) {
-            const float *src = PASS == FWD ? (cu.var && !cu.half ? a.var_w : a.mu_w) + base + cu.kc + (size_t)(g * 32) * a.K
+            const float *src = PASS == FWD ? (cu.var && cu.half ? a.var_w : a.mu_w) + base + cu.kc + (size_t)(g * 32) * a.K
                                : PASS == STATE ? a.mu_w + base + (size_t)(cu.kc + g * 16) * a.K : a.x + base;
             int4 r = make_int4(-1, -1, -1, -1);
             if (PASS == PARAM) r = *reinterpret_cast<const int4 *>(&sh.rows[w][g * 4]);
@@ -282,7 +282,7 @@ __device__ __forceinline__ void convert_a(const GroupedArgs &a, Shared &sh, int 
     look_up();
     for (int i = 0; cu.chunks > 0; i++) {
         const int s = i & 1;
-        const bool square = cu.var && (PASS != FWD || cu.half);
+        const bool square = cu.var && !cu.half;
         load();
         advance();   // and looks up what the next load needs
         if (i >= 2 && !mbar_wait(sh.done + s, ((i - 2) >> 1) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_EMPTY)) return;
@@ -328,7 +328,7 @@ __device__ __forceinline__ void convert_b(const GroupedArgs &a, Shared &sh, int 
         else if (PASS == FWD && cu.c == nk) cu.kc = 0, cu.half = true;
     };
     auto load = [&](int g) {
-        const float *src = PASS == FWD ? (!cu.var ? a.a0 : cu.half ? a.a1 : a.second) + (size_t)max(rows[g], 0) * a.K + cu.kc + along
+        const float *src = PASS == FWD ? (!cu.var ? a.a0 : cu.half ? a.second : a.a1) + (size_t)max(rows[g], 0) * a.K + cu.kc + along
                                        : (cu.var ? a.a1 : a.a0) + base + (PASS == STATE ? (size_t)(g * 32) * a.N + cu.kc : (size_t)(cu.kc + g * 16) * a.N);
 #pragma unroll
         for (int s = 0; s < 4; s++) {
@@ -387,7 +387,7 @@ __global__ void __launch_bounds__(THREADS, 1) grouped_tc_kernel(const GroupedArg
             int r0 = 0, r1 = 0;
             if (e0 + lane < a.E) expert_rows(a, e0 + lane, r0, r1);
             // experts with few rows have kernels of their own
-            const int v = r1 - r0 > (PASS == PARAM ? FEW_PARAM_ROWS : FEW_ROWS) ? mt * (((PASS == PARAM ? a.N : r1 - r0) + 255) / 256) : 0;
+            const int v = r1 - r0 > FEW_ROWS ? mt * (((PASS == PARAM ? a.N : r1 - r0) + 255) / 256) : 0;
             int s = v;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -610,7 +610,7 @@ int launch_pass(const GroupedArgs &a, cudaStream_t st) {
                      aligned16(a.x);
     const size_t smem = 2 * SLOT + 1024 + sizeof(Shared) + (a.E + 1) * sizeof(int);
     const long mt = ((PASS == FWD ? a.N : a.K) + 255) / 256;
-    const long experts = a.E < a.S / (few_rows(PASS) + 1) ? a.E : a.S / (few_rows(PASS) + 1);   // at most as many have more rows
+    const long experts = a.E < a.S / (FEW_ROWS + 1) ? a.E : a.S / (FEW_ROWS + 1);   // at most as many have more rows
     const long most = 2 * mt * (PASS == PARAM ? experts * ((a.N + 255) / 256) : a.S / 256 + experts);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2 * (unsigned)(most < PAIRS ? most : PAIRS));
