@@ -13,7 +13,7 @@ __global__ void __launch_bounds__(256) grouped_bias_kernel(const GroupedArgs a) 
     const int c = threadIdx.x & 31, g = threadIdx.x >> 5, n = blockIdx.x * 32 + c, e = blockIdx.y;
     int r0, r1;
     expert_rows(a, e, r0, r1);
-    if (r1 - r0 <= FEW_ROWS) return;
+    if (r1 - r0 <= a.few) return;
     float s = 0.f, v = 0.f;
     if (n < a.N)
         for (int r = r0 + g; r < r1; r += 8) s += __ldg(a.a0 + (size_t)r * a.N + n), v += __ldg(a.a1 + (size_t)r * a.N + n);
@@ -33,9 +33,19 @@ inline int launched(const char *what) {
     return e == cudaSuccess ? TAGI_OK : cuda_fail(e, what);
 }
 
-int run(int pass, const GroupedArgs &a, cudaStream_t st) {
-    const int rc = grouped_few(pass, a, st);
-    return rc != TAGI_OK || a.S <= FEW_ROWS ? rc : grouped_tc(pass, a, st);
+int run(int pass, GroupedArgs &a, cudaStream_t st) {
+    if (pass == PARAM) {
+        a.few = a.thin = FEW_PARAM_ROWS;
+    } else if (a.K % 4 == 0 && (pass == FWD || a.N % 4 == 0) && aligned16(a.mu_w) && aligned16(a.var_w) && aligned16(a.a0) && aligned16(a.a1)) {
+        a.few = FEW_ROWS, a.thin = THIN_ROWS;
+    } else {
+        a.few = a.thin = FEW_UNALIGNED_ROWS;
+    }
+    int rc = grouped_few(pass, a, st);
+    if (rc != TAGI_OK || a.S <= a.few) return rc;
+    if (pass == FWD && (rc = grouped_second_moment(a, st)) != TAGI_OK) return rc;
+    if (a.thin > a.few && ((rc = grouped_thin(pass, a, st)) != TAGI_OK || a.S <= a.thin)) return rc;
+    return grouped_tc(pass, a, st);
 }
 
 int check_grouped(const char *who, int E, int S, int K, int N, const int *offsets) {
@@ -136,7 +146,7 @@ int tagi_grouped_linear_bwd_param(int E, int S, int R, int K, int N, int has_bia
     a.var_b = has_bias ? var_b : nullptr, a.a0 = dmu_z, a.a1 = dvar_z, a.o0 = dmu_w, a.o1 = dvar_w, a.ob0 = dmu_b, a.ob1 = dvar_b;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     rc = run(PARAM, a, st);
-    if (rc != TAGI_OK || !has_bias || S <= FEW_ROWS) return rc;
+    if (rc != TAGI_OK || !has_bias || S <= a.few) return rc;
     grouped_bias_kernel<<<dim3((N + 31) / 32, E), 256, 0, st>>>(a);
     return launched("grouped_bias_kernel launch");
 }

@@ -8,6 +8,7 @@ enum { FWD = 0, STATE = 1, PARAM = 2 };
 
 struct GroupedArgs {
     int E, S, R, K, N;
+    int few, thin;   // most rows of an expert for the kernels of tagi_grouped_few.cu and tagi_grouped_thin.cu
     const int *offsets, *token;
     // a0, a1: activations (forward) or deltas (backward); x: input means of the parameter pass
     const float *mu_w, *var_w, *mu_b, *var_b, *a0, *a1, *jcb, *x;
@@ -29,11 +30,21 @@ __device__ __forceinline__ int input_row(const GroupedArgs &a, int p) {
 }
 #endif
 
-// Experts with up to this many rows run on the kernels of tagi_grouped_few.cu (one pass over the weights on the FP32 pipe),
-// those with more on the tensor cores.
-constexpr int FEW_ROWS = 32;
+// Which kernel an expert's rows run on, decided on the device by their number (few, thin: see GroupedArgs):
+//   up to few    tagi_grouped_few.cu   one pass over the weights on the FP32 pipe
+//   up to thin   tagi_grouped_thin.cu  tensor cores, tiles of 128 features fed by TMA (forward and state pass, aligned rows)
+//   more         tagi_grouped_tc.cu    tensor cores, tiles of 256 features x up to 256 rows
+// Measured on eight experts of 4096 x 4096, forward pass, 4 / 8 / 16 / 32 / 40 rows each: few 223 / 309 / 520 / 936 us; thin
+// 413 to 424 us up to 32 rows, 507 us at 40; the wide kernel 750 us from 9 to 64. Parameter pass: few 462 / 593 / 887 us at
+// 8 / 16 / 32 rows, the wide kernel 700 us at 16. Rows that are not multiples of 16 bytes (2047 x 2047, four experts of 16
+// rows): few 147 us, wide 169 us.
+constexpr int FEW_ROWS = 8, FEW_UNALIGNED_ROWS = 16, FEW_PARAM_ROWS = 20, THIN_ROWS = 48;
 
+// mu_a^2 + var_a of every input row to a.second, for the tensor-core kernels
+int grouped_second_moment(const GroupedArgs &a, cudaStream_t st);
 int grouped_few(int pass, const GroupedArgs &a, cudaStream_t st);
+int grouped_thin(int pass, const GroupedArgs &a, cudaStream_t st);
+int grouped_thin_status(int *out, int reset);
 int grouped_tc(int pass, const GroupedArgs &a, cudaStream_t st);
 
 }  // namespace tagi

@@ -1,7 +1,7 @@
 // Linear layers grouped by expert, experts with few rows: every weight is read once and met by all rows of its expert, on
 // the FP32 pipe. These passes are bound by HBM (8, 4 and 12 bytes a weight in the forward, state and parameter pass) until
 // the rows' multiplications (3, 2 and 2 a weight and row) take longer, at about 14, 11 and 33 rows. Experts with more than
-// FEW_ROWS are left to the tensor-core kernel, which in turn leaves these alone; the offsets are device data, so both are
+// `few` rows are left to the tensor-core kernels, which in turn leave these alone; the offsets are device data, so all are
 // launched unless the number of rows in all rules one out.
 //
 // Forward and state pass: a CTA computes 64 output columns of all the expert's rows. The weights come in slabs of 32
@@ -188,7 +188,7 @@ constexpr size_t few_smem(int groups, int stages) {
     return (stages * stage > sums ? stages * stage : sums) * sizeof(float);
 }
 
-// MOST: groups of rows that an expert can have, by the rows there are in all
+// MOST: groups of rows that an expert can have
 template <int PASS, bool VEC, int MOST, int STAGES>
 __global__ void __launch_bounds__(THREADS, STAGES == 4 ? 2 : 1) grouped_few_kernel(const GroupedArgs a) {
     extern __shared__ __align__(16) float smem[];
@@ -196,10 +196,9 @@ __global__ void __launch_bounds__(THREADS, STAGES == 4 ? 2 : 1) grouped_few_kern
     int r0, r1;
     expert_rows(a, e, r0, r1);
     const int rows = r1 - r0;
-    if (rows == 0 || rows > FEW_ROWS) return;
+    if (rows == 0 || rows > a.few) return;
     if (rows <= 8) few_rows_pass<PASS, VEC, 1, STAGES>(a, e, r0, rows, smem);
-    else if (MOST >= 2 && rows <= 16) few_rows_pass<PASS, VEC, 2, STAGES>(a, e, r0, rows, smem);
-    else if (MOST == 4) few_rows_pass<PASS, VEC, 4, STAGES>(a, e, r0, rows, smem);
+    else if (MOST == 2) few_rows_pass<PASS, VEC, 2, STAGES>(a, e, r0, rows, smem);
 }
 
 // -------------------------------------------------------------------------------------------------------- parameters
@@ -217,15 +216,26 @@ __device__ __forceinline__ void load(const float *p, float (&v)[W]) {
     }
 }
 
+// weights pass by once: they are kept out of L1, where the rows are wanted
+template <int W>
+__device__ __forceinline__ void load_once(const float *p, float (&v)[W]) {
+    if (W == 4)
+        asm volatile("ld.global.nc.L1::no_allocate.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(v[0]), "=f"(v[1 % W]), "=f"(v[2 % W]), "=f"(v[3 % W])
+                     : "l"(p));
+    else
+        asm volatile("ld.global.nc.L1::no_allocate.f32 %0, [%1];" : "=f"(v[0]) : "l"(p));
+}
+
 template <int W>
 __global__ void __launch_bounds__(THREADS, 2) grouped_few_param_kernel(const GroupedArgs a) {
-    __shared__ __align__(16) float delta[FEW_ROWS][2][PARAM_OUT];
-    __shared__ int input[FEW_ROWS];
+    __shared__ __align__(16) float delta[FEW_PARAM_ROWS][2][PARAM_OUT];
+    __shared__ int input[FEW_PARAM_ROWS];
     const int e = blockIdx.z;
     int r0, r1;
     expert_rows(a, e, r0, r1);
     const int rows = r1 - r0;
-    if (rows > FEW_ROWS) return;
+    if (rows > a.few) return;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, block_n = blockIdx.y * PARAM_OUT, n0 = block_n + warp * PARAM_N;
     const int k = (blockIdx.x * 32 + lane) * W;
     const bool live = k < a.K;
@@ -235,7 +245,7 @@ __global__ void __launch_bounds__(THREADS, 2) grouped_few_param_kernel(const Gro
     for (int i = 0; i < PARAM_N; i++) {
 #pragma unroll
         for (int c = 0; c < W; c++) d[i][c] = v[i][c] = s[i][c] = 0.f;
-        if (live && n0 + i < a.N) load<W>(a.var_w + o + (size_t)i * a.K, s[i]);
+        if (live && rows > 0 && n0 + i < a.N) load_once<W>(a.var_w + o + (size_t)i * a.K, s[i]);
     }
     for (int i = threadIdx.x; i < rows * 2 * PARAM_OUT; i += THREADS) {
         const int n = block_n + i % PARAM_OUT, r = i / (2 * PARAM_OUT);
@@ -279,11 +289,11 @@ __global__ void __launch_bounds__(THREADS, 2) grouped_few_param_kernel(const Gro
         for (int c = 0; c < W; c++) d[i][c] *= s[i][c], v[i][c] *= s[i][c] * s[i][c];
         float *p = a.o0 + o + (size_t)i * a.K, *u = a.o1 + o + (size_t)i * a.K;
         if (W == 4) {
-            *reinterpret_cast<float4 *>(p) = make_float4(d[i][0], d[i][1 % W], d[i][2 % W], d[i][3 % W]);
-            *reinterpret_cast<float4 *>(u) = make_float4(v[i][0], v[i][1 % W], v[i][2 % W], v[i][3 % W]);
+            __stcs(reinterpret_cast<float4 *>(p), make_float4(d[i][0], d[i][1 % W], d[i][2 % W], d[i][3 % W]));
+            __stcs(reinterpret_cast<float4 *>(u), make_float4(v[i][0], v[i][1 % W], v[i][2 % W], v[i][3 % W]));
         } else {
-            *p = d[i][0];
-            *u = v[i][0];
+            __stcs(p, d[i][0]);
+            __stcs(u, v[i][0]);
         }
     }
 }
@@ -303,15 +313,14 @@ template <int PASS, bool VEC>
 int launch_few(const GroupedArgs &a, cudaStream_t st) {
     // CTAs that have work, at most: with one or none for an SM, each gets a deep ring
     const long ctas = (((PASS == FWD ? a.N : a.K) + OUT - 1) / OUT) * (long)(a.E < a.S ? a.E : a.S);
-    if (a.S <= 8) return ctas <= 148 ? launch_few<PASS, VEC, 1, 10>(a, st) : launch_few<PASS, VEC, 1, 4>(a, st);
-    return launch_few<PASS, VEC, 4, 4>(a, st);
+    static_assert(FEW_ROWS == GROUP && FEW_UNALIGNED_ROWS == 2 * GROUP, "groups of the instances");
+    if (a.S <= GROUP && ctas <= 148) return launch_few<PASS, VEC, 1, 10>(a, st);
+    return launch_few<PASS, VEC, VEC ? 1 : 2, 4>(a, st);
 }
 
 template <int PASS>
 int launch(const GroupedArgs &a, cudaStream_t st) {
-    const bool vec = a.K % 4 == 0 && (PASS == FWD || a.N % 4 == 0) && aligned16(a.mu_w) && aligned16(a.var_w) && aligned16(a.a0) &&
-                     aligned16(a.a1);
-    return vec ? launch_few<PASS, true>(a, st) : launch_few<PASS, false>(a, st);
+    return a.few == FEW_ROWS ? launch_few<PASS, true>(a, st) : launch_few<PASS, false>(a, st);
 }
 
 }  // namespace

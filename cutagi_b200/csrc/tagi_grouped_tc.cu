@@ -22,16 +22,12 @@
 // operands and two accumulators of 256 columns fill tensor memory; a slot's "full" barrier counts the converters (operands
 // written) and the summing warps (accumulator read), its "done" barrier the MMAs' completion. Nothing stops at a tile's
 // end: the next tile's operands are converted while the last one's chunks multiply and its sums are written.
-#include "tagi_grouped.h"
+#include "tagi_grouped_split.cuh"
 
 #include <cstddef>
 
-#include "tagi_tc_ptx.cuh"
-
 namespace tagi {
 namespace {
-
-using namespace ptx;
 
 constexpr int SUMMERS = 8, CONVERTERS = 8, ISSUER = SUMMERS + CONVERTERS;   // warps 0-7; 8-11 (A), 12-15 (B); 16 (17-19 idle)
 constexpr int THREADS = 32 * (ISSUER + 4);
@@ -73,8 +69,6 @@ struct Shared {                 // behind the slots
 };
 static_assert(offsetof(Shared, rows) % 16 == 0 && sizeof(Shared) % 8 == 0, "rows are read 16 bytes at a time");
 
-__device__ __forceinline__ int round_up(int a, int b) { return (a + b - 1) / b * b; }
-
 // Item j of pair `pair`. The two kinds of a tile are neighbours, so two pairs work on the same weights at the same time, and
 // a pair's kinds alternate from one item to the next (in the forward pass a variance costs twice a mean).
 template <int PASS>
@@ -101,82 +95,6 @@ __device__ __forceinline__ bool get_item(const GroupedArgs &a, const int *before
     it.nk = (it.depth + KC - 1) / KC;
     it.chunks = PASS == FWD && it.kind == VAR ? 2 * it.nk : it.nk;
     return true;
-}
-
-// Four consecutive floats, of which the first `valid` (0..4) exist. VEC: all four or none, 16-byte aligned.
-template <bool VEC>
-__device__ __forceinline__ float4 ld4(const float *p, int valid) {
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (VEC) {
-        if (valid > 0) v = __ldg(reinterpret_cast<const float4 *>(p));
-    } else {
-        if (valid > 0) v.x = __ldg(p);
-        if (valid > 1) v.y = __ldg(p + 1);
-        if (valid > 2) v.z = __ldg(p + 2);
-        if (valid > 3) v.w = __ldg(p + 3);
-    }
-    return v;
-}
-
-__device__ __forceinline__ uint32_t top_halves(float a, float b) {   // a's upper 16 bits below b's
-    uint32_t r;
-    asm("prmt.b32 %0, %1, %2, 0x7632;" : "=r"(r) : "r"(__float_as_uint(a)), "r"(__float_as_uint(b)));
-    return r;
-}
-__device__ __forceinline__ float truncated(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
-// two 32-bit operations as one instruction
-__device__ __forceinline__ void add2(float &a, float &b, float x, float y) {
-    asm("{\n\t.reg .b64 s, t;\n\tmov.b64 s, {%0, %1};\n\tmov.b64 t, {%2, %3};\n\tadd.rn.f32x2 s, s, t;\n\tmov.b64 {%0, %1}, s;\n\t}"
-        : "+f"(a), "+f"(b)
-        : "f"(x), "f"(y));
-}
-__device__ __forceinline__ void subtract_truncated2(float &a, float &b) {
-    const float x = truncated(a), y = truncated(b);
-    asm("{\n\t.reg .b64 s, t;\n\tmov.b64 s, {%0, %1};\n\tmov.b64 t, {%2, %3};\n\tsub.rn.f32x2 s, s, t;\n\tmov.b64 {%0, %1}, s;\n\t}"
-        : "+f"(a), "+f"(b)
-        : "f"(x), "f"(y));
-}
-__device__ __forceinline__ void sts64(uint32_t at, uint32_t a, uint32_t b) {
-    asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(a), "r"(b) : "memory");
-}
-// hi, mid, lo of four values to their part tiles
-__device__ __forceinline__ void store_split(uint32_t at, float4 v) {
-    sts64(at, top_halves(v.x, v.y), top_halves(v.z, v.w));
-    subtract_truncated2(v.x, v.y), subtract_truncated2(v.z, v.w);
-    sts64(at + PART, top_halves(v.x, v.y), top_halves(v.z, v.w));
-    subtract_truncated2(v.x, v.y), subtract_truncated2(v.z, v.w);
-    sts64(at + 2 * PART, top_halves(v.x, v.y), top_halves(v.z, v.w));
-}
-__device__ __forceinline__ float4 squared(float4 v) { return make_float4(v.x * v.x, v.y * v.y, v.z * v.z, v.w * v.w); }
-
-// kind::f16 instruction descriptor: FP32 accumulation, bf16 operands (see make_idesc_tf32 for the fields)
-__host__ __device__ constexpr uint32_t make_idesc_bf16(int M, int N, int a_mn, int b_mn) {
-    return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(N >> 3) << 17) |
-           ((uint32_t)(M >> 4) << 24);
-}
-// The six products of 16 contraction steps of a slot: operand parts lie PART bytes apart, the high descriptor words are the
-// same for all. One asm block each: building descriptors between the instructions costs the issuing thread more than the
-// tensor core needs for a narrow tile.
-#define GROUPED_MMA(AP, BP, P)                                                        \
-    "add.u32 ra, %1, " AP ";\n\tadd.u32 rb, %2, " BP ";\n\t"                          \
-    "mov.b64 da, {ra, %3};\n\tmov.b64 db, {rb, %3};\n\t"                              \
-    "tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %4, " P ";\n\t"
-static_assert((PART >> 4) == 1024, "part distance in the asm blocks");
-// lo hi, hi lo, mid mid, mid hi, hi mid; accumulate == 0: the first overwrites the accumulator
-__device__ __forceinline__ void mma_small_products(uint32_t d, uint32_t x, uint32_t y, uint32_t hi, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p, t;\n\t.reg .b32 ra, rb;\n\t.reg .b64 da, db;\n\t"
-        "setp.ne.b32 p, %5, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
-        GROUPED_MMA("2048", "0", "p") GROUPED_MMA("0", "2048", "t") GROUPED_MMA("1024", "1024", "t")
-        GROUPED_MMA("1024", "0", "t") GROUPED_MMA("0", "1024", "t") "}"
-        ::"r"(d), "r"(x), "r"(y), "r"(hi), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-__device__ __forceinline__ void mma_large_product(uint32_t d, uint32_t x, uint32_t y, uint32_t hi, uint32_t idesc) {
-    asm volatile(
-        "{\n\t.reg .pred t;\n\t.reg .b32 ra, rb;\n\t.reg .b64 da, db;\n\tsetp.eq.b32 t, 0, 0;\n\t" GROUPED_MMA("0", "0", "t") "}"
-        ::"r"(d), "r"(x), "r"(y), "r"(hi), "r"(idesc)
-        : "memory");
 }
 
 // Operands of 128 rows x 64 contraction steps as the tensor core reads them (128-byte swizzle: 16-byte chunk c of line r
@@ -287,7 +205,7 @@ __device__ __forceinline__ void convert_a(const GroupedArgs &a, Shared &sh, int 
         advance();   // and looks up what the next load needs
         if (i >= 2 && !mbar_wait(sh.done + s, ((i - 2) >> 1) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_EMPTY)) return;
 #pragma unroll
-        for (int q = 0; q < TASKS; q++) store_split(P::at(to + s * SLOT, q), square ? squared(v[q]) : v[q]);
+        for (int q = 0; q < TASKS; q++) store_split(P::at(to + s * SLOT, q), PART, square ? squared(v[q]) : v[q]);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(sh.full + s, 0);
@@ -349,7 +267,7 @@ __device__ __forceinline__ void convert_b(const GroupedArgs &a, Shared &sh, int 
             if (MN || g * 32 < lines) {   // narrow tiles have no columns for the later groups
 #pragma unroll
                 for (int q = g * 4; q < g * 4 + 4; q++)
-                    if (MN ? along < round_up(lines, 64) : g * 32 + row < lines) store_split(P::at(to + s * SLOT, q), v[q]);
+                    if (MN ? along < round_up(lines, 64) : g * 32 + row < lines) store_split(P::at(to + s * SLOT, q), PART, v[q]);
             }
         fence_proxy_async_smem();
         __syncwarp();
@@ -367,6 +285,27 @@ __global__ void __launch_bounds__(THREADS, 1) grouped_tc_kernel(const GroupedArg
     Shared &sh = *reinterpret_cast<Shared *>(smem_raw + (smem_base - smem_u32(smem_raw)) + 2 * SLOT);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int cta = (int)cluster_ctarank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    if (warp == 0) {
+        const int mt = ((PASS == FWD ? a.N : a.K) + 255) / 256;
+        int carry = 0;
+        for (int e0 = 0; e0 < a.E; e0 += 32) {
+            int r0 = 0, r1 = 0;
+            if (e0 + lane < a.E) expert_rows(a, e0 + lane, r0, r1);
+            // experts with few rows have kernels of their own
+            const int v = r1 - r0 > a.thin ? mt * (((PASS == PARAM ? a.N : r1 - r0) + 255) / 256) : 0;
+            int s = v;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, s, o);
+                if (lane >= o) s += u;
+            }
+            if (e0 + lane < a.E) sh.before[e0 + lane] = carry + s - v;
+            carry += __shfl_sync(0xffffffffu, s, 31);
+        }
+        if (lane == 0) sh.before[a.E] = carry;
+    }
+    __syncthreads();
+    if (sh.before[a.E] == 0) return;   // no expert of this size; the same in both CTAs
     if (threadIdx.x == 0) {
         for (int s = 0; s < 2; s++) {
             mbar_init(sh.full + s, 2 * (SUMMERS + CONVERTERS));   // counted in CTA 0
@@ -380,25 +319,6 @@ __global__ void __launch_bounds__(THREADS, 1) grouped_tc_kernel(const GroupedArg
         mbar_init_fence();
     }
     if (warp == ISSUER) tmem_alloc_pair(&sh.tmem, 2 * ACC);
-    if (warp == 0) {
-        const int mt = ((PASS == FWD ? a.N : a.K) + 255) / 256;
-        int carry = 0;
-        for (int e0 = 0; e0 < a.E; e0 += 32) {
-            int r0 = 0, r1 = 0;
-            if (e0 + lane < a.E) expert_rows(a, e0 + lane, r0, r1);
-            // experts with few rows have kernels of their own
-            const int v = r1 - r0 > FEW_ROWS ? mt * (((PASS == PARAM ? a.N : r1 - r0) + 255) / 256) : 0;
-            int s = v;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int u = __shfl_up_sync(0xffffffffu, s, o);
-                if (lane >= o) s += u;
-            }
-            if (e0 + lane < a.E) sh.before[e0 + lane] = carry + s - v;
-            carry += __shfl_sync(0xffffffffu, s, 31);
-        }
-        if (lane == 0) sh.before[a.E] = carry;
-    }
     tc_fence_before_sync();
     __syncthreads();
     cluster_sync_all();   // the peer's barriers exist before anyone arrives on them
@@ -431,7 +351,7 @@ __global__ void __launch_bounds__(THREADS, 1) grouped_tc_kernel(const GroupedArg
                     tc_fence_after_sync();
                     const uint32_t al = desc_lo(smem_base + s * SLOT, PA::LBO), bl = desc_lo(smem_base + s * SLOT + 3 * PART, PB::LBO);
                     const uint32_t d = tmem + s * ACC;
-                    for (int k = 0; k < steps; k++) mma_small_products(d, al + k * PA::KSTEP, bl + k * PB::KSTEP, HI, idesc, k);
+                    for (int k = 0; k < steps; k++) mma_small_products<(PART >> 4), (PART >> 4)>(d, al + k * PA::KSTEP, bl + k * PB::KSTEP, HI, idesc, k);
                     for (int k = 0; k < steps; k++) mma_large_product(d, al + k * PA::KSTEP, bl + k * PB::KSTEP, HI, idesc);
                     mma_commit_pair(sh.done + s);
                 }
@@ -598,19 +518,11 @@ __global__ void __launch_bounds__(256) grouped_second_moment_unaligned_kernel(co
 
 template <int PASS>
 int launch_pass(const GroupedArgs &a, cudaStream_t st) {
-    if (PASS == FWD) {
-        const size_t n = (size_t)a.R * a.K;
-        if (aligned16(a.a0) && aligned16(a.a1))
-            grouped_second_moment_kernel<<<(unsigned)((n + 1023) / 1024), 256, 0, st>>>(a.a0, a.a1, n, a.second);
-        else
-            grouped_second_moment_unaligned_kernel<<<(unsigned)((n + 255) / 256), 256, 0, st>>>(a.a0, a.a1, n, a.second);
-        TAGI_CUDA(cudaGetLastError());
-    }
     const bool vec = a.K % 4 == 0 && a.N % 4 == 0 && aligned16(a.mu_w) && aligned16(a.var_w) && aligned16(a.a0) && aligned16(a.a1) &&
                      aligned16(a.x);
     const size_t smem = 2 * SLOT + 1024 + sizeof(Shared) + (a.E + 1) * sizeof(int);
     const long mt = ((PASS == FWD ? a.N : a.K) + 255) / 256;
-    const long experts = a.E < a.S / (FEW_ROWS + 1) ? a.E : a.S / (FEW_ROWS + 1);   // at most as many have more rows
+    const long experts = a.E < a.S / (a.thin + 1) ? a.E : a.S / (a.thin + 1);   // at most as many have more rows
     const long most = 2 * mt * (PASS == PARAM ? experts * ((a.N + 255) / 256) : a.S / 256 + experts);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2 * (unsigned)(most < PAIRS ? most : PAIRS));
@@ -632,6 +544,16 @@ int launch_pass(const GroupedArgs &a, cudaStream_t st) {
 
 }  // namespace
 
+int grouped_second_moment(const GroupedArgs &a, cudaStream_t st) {
+    const size_t n = (size_t)a.R * a.K;
+    if (aligned16(a.a0) && aligned16(a.a1))
+        grouped_second_moment_kernel<<<(unsigned)((n + 1023) / 1024), 256, 0, st>>>(a.a0, a.a1, n, a.second);
+    else
+        grouped_second_moment_unaligned_kernel<<<(unsigned)((n + 255) / 256), 256, 0, st>>>(a.a0, a.a1, n, a.second);
+    TAGI_CUDA(cudaGetLastError());
+    return TAGI_OK;
+}
+
 int grouped_tc(int pass, const GroupedArgs &a, cudaStream_t st) {
     return pass == FWD ? launch_pass<FWD>(a, st) : pass == STATE ? launch_pass<STATE>(a, st) : launch_pass<PARAM>(a, st);
 }
@@ -640,7 +562,10 @@ int grouped_tc_status(int *out, int reset) {
     TAGI_CUDA(cudaMemcpyFromSymbol(out, g_status, sizeof(int)));
     const int zero = 0;
     if (reset && *out) TAGI_CUDA(cudaMemcpyToSymbol(g_status, &zero, sizeof(int)));
-    return TAGI_OK;
+    int thin = 0;
+    const int rc = grouped_thin_status(&thin, reset);
+    if (*out == 0) *out = thin;
+    return rc;
 }
 
 }  // namespace tagi

@@ -1,0 +1,408 @@
+// Linear layers grouped by expert, forward and state pass of experts with few < rows <= thin on the tensor cores:
+// the arithmetic of tagi_grouped_tc.cu for tiles so narrow that the weights' way from HBM, not the multiplication, is what
+// takes the time. Bound: HBM, 8 (forward) or 4 (state) bytes a weight.
+//
+// One CTA computes 128 features x all rows of an expert. The weights come through a ring of eight half-chunks (16 KiB each),
+// so that about 100 KB of each SM are on their way from HBM whatever the converters do: by TMA. Sixteen warps read them, a feature to a lane, and store the values' bf16
+// parts to tensor memory, where the MMAs take that operand from (through shared memory, its parts would be read six times
+// from there). Four more warps fetch and split the rows, which come from L2; eight add up the accumulators of chunks of 64
+// steps; one thread issues the MMAs. Mean and variance of a tile go to neighbouring CTAs at the same time, mu_w first in
+// both, so that it is fetched from HBM once.
+//
+// A thread issues an MMA every 70 cycles at best, and a chunk has to be done in 1380 (32 KiB at an SM's share of HBM), so the
+// six products of 16 steps are three MMAs: the rows' parts lie below each other and count as one operand of up to 3 x 48
+// columns. hi.[hi mid lo] adds to accumulators 0, 1 and 2, mid.[hi mid] to 1 and 2, lo.[hi] to 2: the accumulators hold the
+// terms of one magnitude each and are added up when a chunk is read.
+#include "tagi_grouped_split.cuh"
+#include "tagi_tc_tile.cuh"
+
+namespace tagi {
+namespace {
+namespace thin {
+
+constexpr int SUMMERS = 8, CONVERT_A = 16, CONVERT_B = 4, LOADERS = 1;
+constexpr int FIRST_A = SUMMERS, FIRST_B = FIRST_A + CONVERT_A, FIRST_LOADER = FIRST_B + CONVERT_B, ISSUER = FIRST_LOADER + LOADERS;
+constexpr int THREADS = 32 * (ISSUER + 2);       // the last warp works out the items
+constexpr int ROWS = 128, COLS = 48, KC = 64, HALF = 32, RING = 8, RECORDS = 4, CTAS = 148;
+constexpr uint32_t SLOT = 3 * COLS * KC * 2, RAW = ROWS * HALF * 4;   // the parts of a tile lie bn rows of 128 bytes apart
+// tensor-memory columns: two slots of three accumulators, two slots of A's parts (two bf16 values a column)
+constexpr uint32_t ACC = 3 * COLS, A_PART = KC / 2, A_SLOT = 3 * A_PART, A_COL = 2 * ACC, TMEM_COLS = 512;
+static_assert(SLOT % 1024 == 0, "the swizzle counts lines from multiples of 1024 bytes");
+static_assert(A_COL + 2 * A_SLOT <= TMEM_COLS, "");
+constexpr int MEAN = 0, VAR = 1;
+static_assert(THIN_ROWS <= COLS, "one tile for all rows of an expert");
+
+__device__ int g_status;  // first wait that ran out
+
+struct Item {
+    int chunks;                   // of the item; 0: there are no more items
+    int e, m0, r0, rows, bn;      // expert; first feature; first row and their number; tile width
+    int kind, depth, nk;          // MEAN or VAR; contraction length; chunks of one contraction
+};
+struct Shared {                   // behind the slots and the ring
+    uint64_t full[2], done[2], raw_full[RING], raw_empty[RING], item_full[RECORDS], item_empty[RECORDS];
+    uint32_t tmem;
+    volatile int abort_flag;
+    Item item[RECORDS];
+    int input[RECORDS][COLS];     // forward: input rows of the item's columns, -1 where there is none
+    int before[];                 // tiles of the experts before e, E + 1 entries
+};
+static_assert(sizeof(Shared) % 8 == 0, "");
+
+// Item j of a CTA: kinds of a tile are neighbours, a CTA's kinds alternate (see tagi_grouped_tc.cu).
+template <int PASS>
+__device__ __forceinline__ void get_item(const GroupedArgs &a, const int *before, int j, Item &it) {
+    const int ctas = gridDim.x, i = blockIdx.x + j * ctas, t = i >> 1;
+    it.chunks = 0;
+    if (t >= before[a.E]) return;
+    it.kind = (i + 2 * t / ctas) & 1;
+    int lo = 0, hi = a.E - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (before[mid] <= t) lo = mid; else hi = mid - 1;
+    }
+    it.e = lo;
+    int r1;
+    expert_rows(a, lo, it.r0, r1);
+    it.rows = r1 - it.r0;
+    it.m0 = (t - before[lo]) * ROWS;
+    it.bn = round_up(it.rows, 16);
+    it.depth = PASS == FWD ? a.K : a.N;
+    it.nk = (it.depth + KC - 1) / KC;
+    it.chunks = PASS == FWD && it.kind == VAR ? 2 * it.nk : it.nk;
+}
+
+__device__ __forceinline__ bool take(Shared &sh, int j, Item &t) {
+    t.chunks = 0;
+    if (!mbar_wait(sh.item_full + j % RECORDS, (j / RECORDS) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_RAW)) return false;
+    t = sh.item[j % RECORDS];
+    return true;
+}
+__device__ __forceinline__ void release(Shared &sh, int j, int lane) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(sh.item_empty + j % RECORDS);
+}
+
+__device__ __forceinline__ float4 lds4(uint32_t at) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+    return v;
+}
+
+template <int PASS>
+__global__ void __launch_bounds__(THREADS, 1)
+grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_constant__ CUtensorMap var_map, const GroupedArgs a) {
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u, ring = smem_base + 2 * SLOT;
+    Shared &sh = *reinterpret_cast<Shared *>(smem_raw + (smem_base - smem_u32(smem_raw)) + 2 * SLOT + RING * RAW);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (warp == 0) {
+        const int mt = ((PASS == FWD ? a.N : a.K) + ROWS - 1) / ROWS;
+        int carry = 0;
+        for (int e0 = 0; e0 < a.E; e0 += 32) {
+            int r0 = 0, r1 = 0;
+            if (e0 + lane < a.E) expert_rows(a, e0 + lane, r0, r1);
+            const int v = r1 - r0 > a.few && r1 - r0 <= a.thin ? mt : 0;
+            int s = v;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, s, o);
+                if (lane >= o) s += u;
+            }
+            if (e0 + lane < a.E) sh.before[e0 + lane] = carry + s - v;
+            carry += __shfl_sync(0xffffffffu, s, 31);
+        }
+        if (lane == 0) sh.before[a.E] = carry;
+    }
+    __syncthreads();
+    if (sh.before[a.E] == 0) return;   // no expert of this size
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < 2; s++) {
+            mbar_init(sh.full + s, SUMMERS + CONVERT_A / 2 + CONVERT_B);   // half the converters of A write a slot
+            mbar_init(sh.done + s, 1);
+        }
+        for (int s = 0; s < RING; s++) {
+            mbar_init(sh.raw_full + s, 1);   // the loading thread, and the bytes
+            mbar_init(sh.raw_empty + s, CONVERT_A / 4);   // and a quarter read a half-chunk
+        }
+        for (int s = 0; s < RECORDS; s++) {
+            mbar_init(sh.item_full + s, 1);
+            mbar_init(sh.item_empty + s, SUMMERS + CONVERT_A + CONVERT_B + LOADERS + 1);
+        }
+        sh.abort_flag = 0;
+        mbar_init_fence();
+    }
+    if (warp == ISSUER) tmem_alloc(&sh.tmem, TMEM_COLS);
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem = sh.tmem;
+
+    if (warp < SUMMERS) {
+        // -------------------------------------------------------------------------------------------- sums and output
+        const int quad = warp & 3, group = warp >> 2;
+        const uint32_t lane_addr = tmem + ((uint32_t)(quad * 32) << 16);
+        float acc[COLS / 2];
+#pragma unroll
+        for (int x = 0; x < COLS / 2; x++) acc[x] = 0.f;
+        if (lane == 0) {   // both accumulators are free
+            mbar_arrive(sh.full);
+            mbar_arrive(sh.full + 1);
+        }
+        Item it;
+        bool ok = true;
+        for (int j = 0, i = 0; ok && take(sh, j, it) && it.chunks > 0; j++) {
+            const int per = it.bn >> 1, first = group * per;   // multiples of 8
+            for (int c = 0; c < it.chunks; c++, i++) {
+                const int s = i & 1;
+                ok = mbar_wait(sh.done + s, (i >> 1) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_ACC);
+                if (!ok) break;
+                tc_fence_after_sync();
+#pragma unroll
+                for (int g = 0; g < COLS / 2; g += 8)
+                    if (g < per) {
+                        float v[8], u[8], t[8];
+                        tmem_ld_32x8_async(lane_addr + s * ACC + 2 * it.bn + first + g, v);
+                        tmem_ld_32x8_async(lane_addr + s * ACC + it.bn + first + g, u);
+                        tmem_ld_32x8_async(lane_addr + s * ACC + first + g, t);
+                        tmem_wait_ld(v, u, t);
+#pragma unroll
+                        for (int x = 0; x < 8; x += 2) {
+                            add2(v[x], v[x + 1], u[x], u[x + 1]);
+                            add2(v[x], v[x + 1], t[x], t[x + 1]);
+                            add2(acc[g + x], acc[g + x + 1], v[x], v[x + 1]);
+                        }
+                    }
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(sh.full + s);
+            }
+            if (!ok) break;
+            const int m = it.m0 + quad * 32 + lane, ld = PASS == FWD ? a.N : a.K, n = m < ld ? min(per, it.rows - first) : 0;
+            const size_t base = (size_t)(it.r0 + first) * ld + m;
+            float *out = (it.kind == VAR ? a.o1 : a.o0) + base;
+            float bias = 0.f;
+            if (PASS == FWD && a.mu_b && n > 0) bias = __ldg((it.kind == VAR ? a.var_b : a.mu_b) + (size_t)it.e * a.N + m);
+            const bool scaled = PASS == STATE && a.jcb != nullptr;
+            float f[8];
+#pragma unroll
+            for (int x = 0; x < COLS / 2; x++) {
+                if (x >= n) break;
+                if (PASS == STATE && x % 8 == 0) {
+#pragma unroll
+                    for (int y = 0; y < 8; y++) f[y] = scaled && x + y < n ? __ldg(a.jcb + base + (size_t)(x + y) * ld) : 1.f;
+                }
+                float z = acc[x];
+                if (PASS == FWD) z += bias;
+                else z = it.kind == VAR ? z * f[x % 8] * f[x % 8] : z * f[x % 8];
+                out[(size_t)x * ld] = z;
+            }
+#pragma unroll
+            for (int x = 0; x < COLS / 2; x++) acc[x] = 0.f;
+            release(sh, j, lane);
+        }
+    } else if (warp < FIRST_B) {
+        // ------------------------------------------------------------------------------------------ weights, ring -> parts
+        // h: which half of each chunk; slot: which chunks, the even or the odd
+        const int w = warp - FIRST_A, quad = w & 3, h = (w >> 2) & 1, slot = w >> 3, row = quad * 32 + lane;
+        const uint32_t to = tmem + ((uint32_t)(quad * 32) << 16) + A_COL + slot * A_SLOT + h * (HALF / 2);
+        Item it;
+        bool ok = true;
+        for (int j = 0, i = 0; ok && take(sh, j, it) && it.chunks > 0; j++) {
+            release(sh, j, lane);
+            for (int c = 0; c < it.chunks; c++, i++) {
+                if ((i & 1) != slot) continue;
+                const int r = 2 * i + h;
+                const bool square = it.kind == VAR && (PASS == STATE || c < it.nk);
+                ok = mbar_wait(sh.raw_full + r % RING, (r / RING) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_RAW) &&
+                     (i < 2 || mbar_wait(sh.done + slot, ((i - 2) >> 1) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_EMPTY));
+                if (!ok) break;
+                tc_fence_after_sync();
+                const uint32_t raw = ring + (r % RING) * RAW;
+#pragma unroll
+                for (int b = 0; b < HALF; b += 16) {   // sixteen steps at a time: two bf16 a column, eight columns a part
+                    float v[16];
+                    if (PASS == FWD) {
+#pragma unroll
+                        for (int q = 0; q < 4; q++) {
+                            const float4 x = lds4(raw + row * (HALF * 4) + (((b / 4 + q) ^ (row & 7)) << 4));
+                            v[q * 4] = x.x, v[q * 4 + 1] = x.y, v[q * 4 + 2] = x.z, v[q * 4 + 3] = x.w;
+                        }
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 16; k++)
+                            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v[k]) : "r"(raw + (b + k) * (ROWS * 4) + row * 4) : "memory");
+                    }
+                    if (square) {
+#pragma unroll
+                        for (int k = 0; k < 16; k++) v[k] *= v[k];
+                    }
+#pragma unroll
+                    for (int p = 0; p < 3; p++) {
+                        float word[8];
+#pragma unroll
+                        for (int k = 0; k < 16; k += 2) {
+                            word[k / 2] = __uint_as_float(top_halves(v[k], v[k + 1]));
+                            if (p < 2) subtract_truncated2(v[k], v[k + 1]);
+                        }
+                        tmem_st_32x8(to + p * A_PART + b / 2, word);
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(sh.raw_empty + r % RING);
+                tmem_wait_st();
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(sh.full + slot);
+            }
+        }
+    } else if (warp < FIRST_LOADER) {
+        // ------------------------------------------------------------------------------- rows, global memory -> parts
+        // a warp loads 64 consecutive bytes of eight rows; the next chunk is on its way while this one is split
+        const int w = warp - FIRST_B, row = w * 8 + ((lane >> 2) & 3) * 2 + (lane >> 4), along = (lane & 3) * 4;
+        const uint32_t to = smem_base + row * 128 + ((((lane & 3) >> 1) ^ (row & 7)) << 4) + (lane & 1) * 8;
+        float4 v[8];
+        Item it;
+        int in[2], j = 0, c = 0;
+        bool ok = true;
+        auto seek = [&]() {
+            take(sh, j, it);
+#pragma unroll
+            for (int g = 0; g < 2; g++) {
+                const int p = g * 32 + row;
+                in[g] = it.chunks == 0 || p >= it.rows ? -1 : PASS == FWD ? sh.input[j % RECORDS][p] : it.r0 + p;
+            }
+            release(sh, j, lane);
+        };
+        auto load = [&]() {
+            const bool second = PASS == FWD && c >= it.nk;
+            const int kc = (second ? c - it.nk : c) * KC;
+            const float *src = it.kind == MEAN ? a.a0 : second ? a.second : a.a1;
+#pragma unroll
+            for (int q = 0; q < 8; q++)
+                v[q] = ld4<true>(src + (size_t)max(in[q >> 2], 0) * it.depth + kc + along + (q & 3) * 16,
+                                in[q >> 2] >= 0 ? it.depth - kc - along - (q & 3) * 16 : 0);
+        };
+        seek();
+        for (int i = 0; it.chunks > 0; i++) {
+            const int s = i & 1, cols = it.bn;
+            load();
+            if (++c == it.chunks) c = 0, j++, seek();
+            if (i >= 2) ok = mbar_wait(sh.done + s, ((i - 2) >> 1) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_EMPTY);
+            if (!ok) break;
+#pragma unroll
+            for (int q = 0; q < 8; q++)
+                if ((q >> 2) * 32 + row < cols) store_split(((to + s * SLOT) ^ ((q & 3) << 5)) + (q >> 2) * 4096, cols * 128, v[q]);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(sh.full + s);
+        }
+    } else if (warp < ISSUER) {
+        // --------------------------------------------------------------------------------------- weights, HBM -> ring
+        // Forward: lines of 32 steps of a feature, 16-byte chunk c of line l at c ^ (l & 7), which is what TMA's 128-byte
+        // swizzle makes and what lets eight lanes read eight lines at once. State: lines of 128 features of a step.
+        if (lane == 0) {
+            Item it;
+            bool ok = true;
+            int r = 0;
+            for (int j = 0; ok && take(sh, j, it) && it.chunks > 0; j++) {
+                mbar_arrive(sh.item_empty + j % RECORDS);
+                for (int c = 0; ok && c < it.chunks; c++) {
+                    const bool second = PASS == FWD && c >= it.nk;
+                    const int kc = (second ? c - it.nk : c) * KC;
+                    for (int h = 0; h < 2; h++, r++) {
+                        if (r >= RING) ok = mbar_wait(sh.raw_empty + r % RING, (r / RING - 1) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_EMPTY);
+                        if (!ok) break;
+                        mbar_arrive_expect_tx(sh.raw_full + r % RING, RAW);
+                        tma_load_3d(ring + (r % RING) * RAW, second ? &var_map : &mean_map, PASS == FWD ? kc + h * HALF : it.m0,
+                                    PASS == FWD ? it.m0 : kc + h * HALF, it.e, sh.raw_full + r % RING);
+                    }
+                }
+            }
+        }
+    } else if (warp == ISSUER) {
+        // ------------------------------------------------------------------------------------------------------- MMA
+        if (lane == 0) {
+            constexpr uint32_t HI = desc_hi(1024, SWZ_128B);
+            Item it;
+            bool ok = true;
+            for (int j = 0, i = 0; ok && take(sh, j, it) && it.chunks > 0; j++) {
+                mbar_arrive(sh.item_empty + j % RECORDS);
+                const uint32_t one = make_idesc_bf16(ROWS, it.bn, 0, 0), two = make_idesc_bf16(ROWS, 2 * it.bn, 0, 0),
+                               three = make_idesc_bf16(ROWS, 3 * it.bn, 0, 0);
+                for (int c = 0; c < it.chunks; c++, i++) {
+                    const int s = i & 1, left = it.depth - (c >= it.nk ? c - it.nk : c) * KC, steps = min(KC / 16, (left + 15) / 16);
+                    ok = mbar_wait(sh.full + s, (i >> 1) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_CONV);
+                    if (!ok) break;
+                    tc_fence_after_sync();
+                    const uint32_t x = tmem + A_COL + s * A_SLOT, y = desc_lo(smem_base + s * SLOT, 16), d = tmem + s * ACC;
+                    for (int k = 0; k < steps; k++)
+                        mma_stacked_ts<A_PART>(d, d + it.bn, d + 2 * it.bn, x + k * 8, y + k * 2, HI, three, two, one, k);
+                    mma_commit(sh.done + s);
+                }
+            }
+        }
+    } else {
+        // ----------------------------------------------------------------------------------------------------- items
+        bool more = true;
+        for (int j = 0; more; j++) {
+            if (j >= RECORDS && !mbar_wait(sh.item_empty + j % RECORDS, (j / RECORDS - 1) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_EMPTY)) break;
+            Item t;
+            get_item<PASS>(a, sh.before, j, t);
+            more = t.chunks > 0;
+            if (lane == 0) sh.item[j % RECORDS] = t;
+            if (PASS == FWD && more)
+                for (int l = lane; l < t.rows; l += 32) sh.input[j % RECORDS][l] = input_row(a, t.r0 + l);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(sh.item_full + j % RECORDS);
+        }
+    }
+    __syncwarp();
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    if (warp == ISSUER) tmem_dealloc(tmem, TMEM_COLS);
+}
+
+// The weights [E][N][K] as boxes of one expert: 32 steps of 128 features (forward, swizzled) or 128 features of 32 steps
+int make_map(int pass, const GroupedArgs &a, const float *w, CUtensorMap *map) {
+    static EncodeTiledFn encode = tc_encode_fn();
+    if (!encode) return fail(TAGI_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+    const cuuint64_t dims[3] = {(cuuint64_t)a.K, (cuuint64_t)a.N, (cuuint64_t)a.E}, strides[2] = {(cuuint64_t)a.K * 4, (cuuint64_t)a.K * a.N * 4};
+    const cuuint32_t box[3] = {pass == FWD ? (cuuint32_t)HALF : (cuuint32_t)ROWS, pass == FWD ? (cuuint32_t)ROWS : (cuuint32_t)HALF, 1};
+    const cuuint32_t step[3] = {1, 1, 1};
+    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<float *>(w), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              pass == FWD ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? TAGI_OK : fail(TAGI_ERR_CUDA, "cuTensorMapEncodeTiled failed with code " + std::to_string((int)r));
+}
+
+template <int PASS>
+int launch_thin(const GroupedArgs &a, cudaStream_t st) {
+    const size_t smem = 2 * SLOT + RING * RAW + 1024 + sizeof(Shared) + (a.E + 1) * sizeof(int);
+    const long mt = ((PASS == FWD ? a.N : a.K) + ROWS - 1) / ROWS, experts = a.E < a.S / (a.few + 1) ? a.E : a.S / (a.few + 1);
+    const long most = 2 * mt * experts;   // experts with more than `few` rows, at most; both kinds
+    CUtensorMap mean = {}, var = {};
+    int rc;
+    if ((rc = make_map(PASS, a, a.mu_w, &mean)) != TAGI_OK) return rc;
+    if (PASS == FWD && (rc = make_map(PASS, a, a.var_w, &var)) != TAGI_OK) return rc;
+    auto k = grouped_thin_kernel<PASS>;
+    TAGI_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    k<<<(unsigned)(most < CTAS ? most : CTAS), THREADS, smem, st>>>(mean, var, a);
+    TAGI_CUDA(cudaGetLastError());
+    return TAGI_OK;
+}
+
+}  // namespace thin
+}  // namespace
+
+int grouped_thin(int pass, const GroupedArgs &a, cudaStream_t st) { return pass == FWD ? thin::launch_thin<FWD>(a, st) : thin::launch_thin<STATE>(a, st); }
+
+int grouped_thin_status(int *out, int reset) {
+    TAGI_CUDA(cudaMemcpyFromSymbol(out, thin::g_status, sizeof(int)));
+    const int zero = 0;
+    if (reset && *out) TAGI_CUDA(cudaMemcpyToSymbol(thin::g_status, &zero, sizeof(int)));
+    return TAGI_OK;
+}
+
+}  // namespace tagi
