@@ -34,17 +34,12 @@ inline int launched(const char *what) {
 }
 
 int run(int pass, GroupedArgs &a, cudaStream_t st) {
-    if (pass == PARAM) {
-        a.few = a.thin = FEW_PARAM_ROWS;
-    } else if (a.K % 4 == 0 && (pass == FWD || a.N % 4 == 0) && aligned16(a.mu_w) && aligned16(a.var_w) && aligned16(a.a0) && aligned16(a.a1)) {
-        a.few = FEW_ROWS, a.thin = THIN_ROWS;
-    } else {
-        a.few = a.thin = FEW_UNALIGNED_ROWS;
-    }
+    a.few = pass == PARAM ? FEW_PARAM_ROWS : FEW_ROWS;
+    a.thin = pass == PARAM ? FEW_PARAM_ROWS : THIN_ROWS;
     int rc = grouped_few(pass, a, st);
     if (rc != TAGI_OK || a.S <= a.few) return rc;
     if (pass == FWD && (rc = grouped_second_moment(a, st)) != TAGI_OK) return rc;
-    if (a.thin > a.few && ((rc = grouped_thin(pass, a, st)) != TAGI_OK || a.S <= a.thin)) return rc;
+    if (pass != PARAM && ((rc = grouped_thin(pass, a, st)) != TAGI_OK || a.S <= a.thin)) return rc;
     return grouped_tc(pass, a, st);
 }
 

@@ -34,11 +34,15 @@ __device__ __forceinline__ int input_row(const GroupedArgs &a, int p) {
 //   up to few    tagi_grouped_few.cu   one pass over the weights on the FP32 pipe
 //   up to thin   tagi_grouped_thin.cu  tensor cores, tiles of 128 features fed by TMA (forward and state pass, aligned rows)
 //   more         tagi_grouped_tc.cu    tensor cores, tiles of 256 features x up to 256 rows
-// Measured on eight experts of 4096 x 4096, forward pass, 4 / 8 / 16 / 32 / 40 rows each: few 223 / 309 / 520 / 936 us; thin
-// 413 to 424 us up to 32 rows, 507 us at 40; the wide kernel 750 us from 9 to 64. Parameter pass: few 462 / 593 / 887 us at
-// 8 / 16 / 32 rows, the wide kernel 700 us at 16. Rows that are not multiples of 16 bytes (2047 x 2047, four experts of 16
-// rows): few 147 us, wide 169 us.
-constexpr int FEW_ROWS = 8, FEW_UNALIGNED_ROWS = 16, FEW_PARAM_ROWS = 20, THIN_ROWS = 48;
+// Measured on eight experts of 4096 x 4096, forward pass, 4 / 8 / 16 / 32 rows each: few 222 / 307 / 522 / 936 us; thin 402 to
+// 413 us up to 32 rows, 506 us at 40; the wide kernel 750 us from 9 to 64. Parameter pass at 8 / 16 / 32 rows: few 380 / 501 /
+// 747 us, the wide kernel 600 us at 16.
+constexpr int FEW_ROWS = 8, FEW_PARAM_ROWS = 20, THIN_ROWS = 48;
+
+// forward and state pass: rows of weights, activations and deltas are whole 16-byte groups
+inline bool grouped_aligned(int pass, const GroupedArgs &a) {
+    return a.K % 4 == 0 && (pass == FWD || a.N % 4 == 0) && aligned16(a.mu_w) && aligned16(a.var_w) && aligned16(a.a0) && aligned16(a.a1);
+}
 
 // mu_a^2 + var_a of every input row to a.second, for the tensor-core kernels
 int grouped_second_moment(const GroupedArgs &a, cudaStream_t st);

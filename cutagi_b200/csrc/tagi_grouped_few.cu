@@ -5,18 +5,21 @@
 // launched unless the number of rows in all rules one out.
 //
 // Forward and state pass: a CTA computes 64 output columns of all the expert's rows. The weights come in slabs of 32
-// contraction steps through a ring filled with cp.async, so that the bytes in flight cost no registers: four stages where
-// two CTAs share an SM, as many as fit where there are too few CTAs for that. Eight warps share a slab: they cut it along the contraction and, with
-// more than eight rows, among groups of eight; a thread multiplies its two columns with eight rows, whose entries
-// all lanes read at the same address. The warps' sums are added in a fixed order at the end.
+// contraction steps through a ring of stages filled with cp.async, so that the bytes in flight cost no registers (two CTAs of
+// an SM keep about 100 KB on their way). Where there are too few tiles for that, a cluster of up to eight CTAs cuts the
+// contraction of a tile, and their sums are added through distributed shared memory in the order of the CTAs. Eight warps share a slab, four steps each; a
+// thread multiplies its two columns with all rows, whose entries all lanes read at the same address. The warps' sums are
+// added in a fixed order at the end.
 #include "tagi_grouped.h"
 
 namespace tagi {
 namespace {
 
-constexpr int OUT = 64, SLAB = 32, WARPS = 8, THREADS = WARPS * 32, GROUP = 8;
+constexpr int OUT = 64, SLAB = 32, WARPS = 8, THREADS = WARPS * 32, ROWS = FEW_ROWS;
+static_assert(SLAB == 4 * WARPS, "a warp takes four steps of a slab");
 constexpr int PITCH = SLAB + 4;                          // floats of a weight row in shared memory: no bank conflicts
 constexpr int FWD_WEIGHTS = 2 * OUT * PITCH, STATE_WEIGHTS = SLAB * OUT;
+__host__ __device__ constexpr int stages(int pass) { return pass == FWD ? 4 : 8; }   // a slab of both is 18 KiB, of means 8
 
 __device__ __forceinline__ uint32_t smem_at(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
@@ -52,33 +55,37 @@ __device__ __forceinline__ Pair mul2(Pair a, Pair b) {
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
+// float at the same place in the shared memory of CTA `cta` of the cluster
+__device__ __forceinline__ float remote(const float *p, int cta) {
+    float v;
+    asm volatile("{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %1, %2;\n\tld.shared::cluster.f32 %0, [r];\n\t}" : "=f"(v) : "r"(smem_at(p)), "r"(cta) : "memory");
+    return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 __device__ __forceinline__ float sum_of(Pair p) {
     float a, b;
     asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
     return a + b;
 }
 
-// GROUPS of eight rows. smem: STAGES stages of weights and rows, used again for the warps' sums.
-template <int PASS, bool VEC, int GROUPS, int STAGES>
+// smem: a ring of stages of weights and rows, used again for the warps' sums.
+template <int PASS, bool VEC>
 __device__ __forceinline__ void few_rows_pass(const GroupedArgs &a, int e, int r0, int rows, float *smem) {
-    constexpr int ROWS = GROUP * GROUPS, WEIGHTS = PASS == FWD ? FWD_WEIGHTS : STATE_WEIGHTS, STAGE = WEIGHTS + 2 * ROWS * SLAB;
-    constexpr int SPLITS = WARPS / GROUPS;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = warp % GROUPS, split = warp / GROUPS;
+    constexpr int WEIGHTS = PASS == FWD ? FWD_WEIGHTS : STATE_WEIGHTS, STAGE = WEIGHTS + 2 * ROWS * SLAB, STAGES = stages(PASS);
+    const int tid = threadIdx.x, lane = tid & 31, q = tid >> 5;   // q: the warp, and its four steps of a slab
     const int o0 = blockIdx.x * OUT, outs = PASS == FWD ? a.N : a.K, depth = PASS == FWD ? a.K : a.N;
     const size_t wbase = (size_t)e * a.N * a.K;
 
-    // rows of this thread's copies: copy c = tid + i * 256 is quad c & 7 of row (c >> 3) % ROWS, means first
-    constexpr int COPIES = (2 * ROWS * 8 + THREADS - 1) / THREADS;
-    int row[COPIES];
-#pragma unroll
-    for (int i = 0; i < COPIES; i++) {
-        const int c = tid + i * THREADS, r = (c >> 3) % ROWS;
-        row[i] = c < 2 * ROWS * 8 && r < rows ? (PASS == FWD ? input_row(a, r0 + r) : r0 + r) : -1;
-    }
-    auto fetch = [&](int slab) {
+    // this thread's copy of the rows: quad tid & 7 of row (tid >> 3) % ROWS, means first
+    static_assert(2 * ROWS * 8 <= THREADS, "one copy a thread");
+    const int mine = tid < 2 * ROWS * 8 && (tid >> 3) % ROWS < rows ? r0 + (tid >> 3) % ROWS : -1;
+    const int row = mine < 0 ? -1 : PASS == FWD ? input_row(a, mine) : mine;
+    auto fetch = [&](int slab, int last) {
         const int k0 = slab * SLAB;
         float *s = smem + (slab % STAGES) * STAGE;
-        if (k0 < depth) {
+        if (slab < last) {
             if (PASS == FWD) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
@@ -95,31 +102,28 @@ __device__ __forceinline__ void few_rows_pass(const GroupedArgs &a, int e, int r
                                n < a.N ? a.K - k : 0);
                 }
             }
-#pragma unroll
-            for (int i = 0; i < COPIES; i++) {
-                const int c = tid + i * THREADS;
-                if (c >= 2 * ROWS * 8) break;
-                const int k = k0 + (c & 7) * 4;
-                copy4<VEC>(s + WEIGHTS + c * 4, (c < ROWS * 8 ? a.a0 : a.a1) + (row[i] >= 0 && k < depth ? (size_t)row[i] * depth + k : 0),
-                           row[i] >= 0 ? depth - k : 0);
+            if (tid < 2 * ROWS * 8) {
+                const int k = k0 + (tid & 7) * 4;
+                copy4<VEC>(s + WEIGHTS + tid * 4, (tid < ROWS * 8 ? a.a0 : a.a1) + (row >= 0 && k < depth ? (size_t)row * depth + k : 0),
+                           row >= 0 ? depth - k : 0);
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    const int live = min(GROUP, rows - group * GROUP);
-    Pair z[2][GROUP], vz[2][GROUP];
+    Pair z[2][ROWS], vz[2][ROWS];
 #pragma unroll
-    for (int t = 0; t < GROUP; t++) z[0][t] = z[1][t] = vz[0][t] = vz[1][t] = 0;
-    const int slabs = (depth + SLAB - 1) / SLAB;
+    for (int t = 0; t < ROWS; t++) z[0][t] = z[1][t] = vz[0][t] = vz[1][t] = 0;
+    // this CTA's slabs of the cluster's
+    const int parts = gridDim.z, all = (depth + SLAB - 1) / SLAB, first = (int)((long)all * blockIdx.z / parts),
+              last = (int)((long)all * (blockIdx.z + 1) / parts);
 #pragma unroll
-    for (int s = 0; s < STAGES - 1; s++) fetch(s);
-    for (int it = 0; it < slabs; it++) {
+    for (int s = 0; s < STAGES - 1; s++) fetch(first + s, last);
+    for (int it = first; it < last; it++) {
         asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
         __syncthreads();   // slab `it` is there for all, and nobody reads the stage that is filled next any more
-        fetch(it + STAGES - 1);
-        const float *w = smem + (it % STAGES) * STAGE, *x = w + WEIGHTS + group * GROUP * SLAB, *y = x + ROWS * SLAB;
-#pragma unroll
-        for (int q = split; q < SLAB / 4; q += SPLITS) {
+        fetch(it + STAGES - 1, last);
+        const float *w = smem + (it % STAGES) * STAGE, *x = w + WEIGHTS, *y = x + ROWS * SLAB;
+        {
             Pair wm[2][2], wq[2][2], wv[2][2];   // the thread's two columns at four steps: means, their squares, variances
 #pragma unroll
             for (int f = 0; f < 2; f++) {
@@ -134,8 +138,8 @@ __device__ __forceinline__ void few_rows_pass(const GroupedArgs &a, int e, int r
                 wq[f][0] = mul2(wm[f][0], wm[f][0]), wq[f][1] = mul2(wm[f][1], wm[f][1]);
             }
 #pragma unroll
-            for (int t = 0; t < GROUP; t++)
-                if (t < live) {
+            for (int t = 0; t < ROWS; t++)
+                if (t < rows) {
                     const float4 xt = at4(x + t * SLAB + q * 4), yt = at4(y + t * SLAB + q * 4);
                     const Pair xs[2] = {pair_of(xt.x, xt.y), pair_of(xt.z, xt.w)}, ys[2] = {pair_of(yt.x, yt.y), pair_of(yt.z, yt.w)};
 #pragma unroll
@@ -153,21 +157,23 @@ __device__ __forceinline__ void few_rows_pass(const GroupedArgs &a, int e, int r
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
-    // red[split][row][kind][column]
+    // red[warp][row][kind][column]
     float *red = smem;
 #pragma unroll
-    for (int t = 0; t < GROUP; t++)
+    for (int t = 0; t < ROWS; t++)
 #pragma unroll
         for (int f = 0; f < 2; f++) {
-            const int at = ((split * ROWS + group * GROUP + t) * 2) * OUT + f * 32 + lane;
+            const int at = ((q * ROWS + t) * 2) * OUT + f * 32 + lane;
             red[at] = sum_of(z[f][t]);
             red[at + OUT] = sum_of(vz[f][t]);
         }
-    __syncthreads();
-    for (int i = tid; i < rows * 2 * OUT; i += THREADS) {
+    if (parts > 1) cluster_sync();
+    else __syncthreads();
+    for (int i = blockIdx.z * THREADS + tid; i < rows * 2 * OUT; i += parts * THREADS) {
         float s = 0.f;
+        for (int c = 0; c < parts; c++)
 #pragma unroll
-        for (int p = 0; p < SPLITS; p++) s += red[p * ROWS * 2 * OUT + i];
+            for (int p = 0; p < WARPS; p++) s += parts > 1 ? remote(red + p * ROWS * 2 * OUT + i, c) : red[p * ROWS * 2 * OUT + i];
         const int c = o0 + (i & (OUT - 1)), r = i / (2 * OUT);
         const bool var = (i / OUT) & 1;
         if (c >= outs) continue;
@@ -180,25 +186,15 @@ __device__ __forceinline__ void few_rows_pass(const GroupedArgs &a, int e, int r
         }
         (var ? a.o1 : a.o0)[o] = s;
     }
+    if (parts > 1) cluster_sync();   // nobody leaves while its sums are read
 }
 
-template <int PASS>
-constexpr size_t few_smem(int groups, int stages) {
-    const size_t stage = (PASS == FWD ? FWD_WEIGHTS : STATE_WEIGHTS) + 2 * groups * GROUP * SLAB, sums = WARPS * GROUP * 2 * OUT;
-    return (stages * stage > sums ? stages * stage : sums) * sizeof(float);
-}
-
-// MOST: groups of rows that an expert can have
-template <int PASS, bool VEC, int MOST, int STAGES>
-__global__ void __launch_bounds__(THREADS, STAGES == 4 ? 2 : 1) grouped_few_kernel(const GroupedArgs a) {
+template <int PASS, bool VEC>
+__global__ void __launch_bounds__(THREADS, 2) grouped_few_kernel(const GroupedArgs a) {
     extern __shared__ __align__(16) float smem[];
-    const int e = blockIdx.y;
     int r0, r1;
-    expert_rows(a, e, r0, r1);
-    const int rows = r1 - r0;
-    if (rows == 0 || rows > a.few) return;
-    if (rows <= 8) few_rows_pass<PASS, VEC, 1, STAGES>(a, e, r0, rows, smem);
-    else if (MOST == 2) few_rows_pass<PASS, VEC, 2, STAGES>(a, e, r0, rows, smem);
+    expert_rows(a, blockIdx.y, r0, r1);
+    if (r1 > r0 && r1 - r0 <= a.few) few_rows_pass<PASS, VEC>(a, blockIdx.y, r0, r1 - r0, smem);   // the same in the whole cluster
 }
 
 // -------------------------------------------------------------------------------------------------------- parameters
@@ -298,29 +294,35 @@ __global__ void __launch_bounds__(THREADS, 2) grouped_few_param_kernel(const Gro
     }
 }
 
-template <int PASS, bool VEC, int MOST, int STAGES>
-int launch_few(const GroupedArgs &a, cudaStream_t st) {
-    auto k = grouped_few_kernel<PASS, VEC, MOST, STAGES>;
-    constexpr size_t smem = few_smem<PASS>(MOST, STAGES);
-    static_assert(smem <= 227 * 1024, "more shared memory than an SM has");
-    TAGI_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    k<<<dim3(((PASS == FWD ? a.N : a.K) + OUT - 1) / OUT, a.E), THREADS, smem, st>>>(a);
-    TAGI_CUDA(cudaGetLastError());
-    return TAGI_OK;
-}
-
 template <int PASS, bool VEC>
 int launch_few(const GroupedArgs &a, cudaStream_t st) {
-    // CTAs that have work, at most: with one or none for an SM, each gets a deep ring
-    const long ctas = (((PASS == FWD ? a.N : a.K) + OUT - 1) / OUT) * (long)(a.E < a.S ? a.E : a.S);
-    static_assert(FEW_ROWS == GROUP && FEW_UNALIGNED_ROWS == 2 * GROUP, "groups of the instances");
-    if (a.S <= GROUP && ctas <= 148) return launch_few<PASS, VEC, 1, 10>(a, st);
-    return launch_few<PASS, VEC, VEC ? 1 : 2, 4>(a, st);
+    constexpr size_t ring = stages(PASS) * ((PASS == FWD ? FWD_WEIGHTS : STATE_WEIGHTS) + 2 * ROWS * SLAB), sums = WARPS * ROWS * 2 * OUT;
+    constexpr size_t smem = (ring > sums ? ring : sums) * sizeof(float);
+    // CTAs that have work, at most: with fewer than two for an SM, clusters cut the contraction, into no less than 256 steps
+    const int tiles = ((PASS == FWD ? a.N : a.K) + OUT - 1) / OUT, depth = PASS == FWD ? a.K : a.N;
+    const long ctas = (long)tiles * (a.E < a.S ? a.E : a.S);
+    int parts = 1;
+    while (parts < 8 && ctas * parts < 2 * 148 && depth >= 512 * parts) parts *= 2;
+    auto k = grouped_few_kernel<PASS, VEC>;
+    TAGI_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(tiles, a.E, parts);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = parts;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    TAGI_CUDA(cudaLaunchKernelEx(&cfg, k, a));
+    return TAGI_OK;
 }
 
 template <int PASS>
 int launch(const GroupedArgs &a, cudaStream_t st) {
-    return a.few == FEW_ROWS ? launch_few<PASS, true>(a, st) : launch_few<PASS, false>(a, st);
+    return grouped_aligned(PASS, a) ? launch_few<PASS, true>(a, st) : launch_few<PASS, false>(a, st);
 }
 
 }  // namespace

@@ -11,19 +11,29 @@ using namespace ptx;
 
 __device__ __forceinline__ int round_up(int a, int b) { return (a + b - 1) / b * b; }
 
-// Four consecutive floats, of which the first `valid` (0..4) exist. VEC: all four or none, 16-byte aligned.
-template <bool VEC>
+// Four floats, STRIDE apart, of which those at offsets below `valid` exist; the others are zero. VEC (STRIDE 1): all four or
+// none, 16-byte aligned.
+template <bool VEC, int STRIDE = 1>
 __device__ __forceinline__ float4 ld4(const float *p, int valid) {
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     if (VEC) {
         if (valid > 0) v = __ldg(reinterpret_cast<const float4 *>(p));
     } else {
         if (valid > 0) v.x = __ldg(p);
-        if (valid > 1) v.y = __ldg(p + 1);
-        if (valid > 2) v.z = __ldg(p + 2);
-        if (valid > 3) v.w = __ldg(p + 3);
+        if (valid > STRIDE) v.y = __ldg(p + STRIDE);
+        if (valid > 2 * STRIDE) v.z = __ldg(p + 2 * STRIDE);
+        if (valid > 3 * STRIDE) v.w = __ldg(p + 3 * STRIDE);
     }
     return v;
+}
+
+// Which of 16 contraction steps lies at place j of an operand whose steps run along memory. Rows that are not aligned to 16
+// bytes are read a float at a time; four lanes then take neighbouring steps (half the sectors of taking every fourth), which
+// leaves a lane with steps 4 apart in four neighbouring places. The order of the steps does not matter to a sum as long as
+// both operands have the same.
+template <bool VEC>
+__device__ __forceinline__ int step_at(int j) {
+    return VEC ? j : (j & ~15) | ((j & 3) << 2) | ((j >> 2) & 3);
 }
 
 __device__ __forceinline__ uint32_t top_halves(float a, float b) {   // a's upper 16 bits below b's

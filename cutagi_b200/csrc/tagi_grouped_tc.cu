@@ -108,7 +108,9 @@ struct Place {
     static constexpr uint32_t KSTEP = (MN ? 16 * 128 : 32) >> 4;             // 16 contraction steps, in 16-byte units
     static constexpr uint32_t LBO = MN ? 64 * 128 : 16, SBO = 1024;
     __device__ static int row(int warp, int lane) { return MN ? warp : warp * 8 + ((lane >> 2) & 3) * 2 + (lane >> 4); }
-    __device__ static int along(int lane) { return MN ? lane * 4 : (lane & 3) * 4; }
+    // first of a thread's four values along memory, and their distance: K-major without alignment, see step_at()
+    template <bool VEC>
+    __device__ static int along(int lane) { return MN ? lane * 4 : VEC ? (lane & 3) * 4 : lane & 3; }
     __device__ static uint32_t base(int warp, int lane) {
         const uint32_t r = row(warp, lane), c = MN ? (lane & 15) >> 1 : (lane & 3) >> 1;
         return (MN ? (lane >> 4) * 8192u : 0u) + r * 128 + ((c ^ (r & 7)) << 4) + (lane & 1) * 8;
@@ -143,7 +145,7 @@ template <int PASS, bool VEC>
 __device__ __forceinline__ void convert_a(const GroupedArgs &a, Shared &sh, int cta, int w, int lane, uint32_t smem_base) {
     constexpr bool MN = PASS != FWD;
     using P = Place<MN>;
-    const int row = P::row(w, lane), along = P::along(lane);
+    const int row = P::row(w, lane), along = P::template along<VEC>(lane);
     const uint32_t to = smem_base + P::base(w, lane);
     float4 v[TASKS];
     Cursor cu;
@@ -164,7 +166,7 @@ __device__ __forceinline__ void convert_a(const GroupedArgs &a, Shared &sh, int 
         left = depth = 0;
         if (t.chunks == 0) return;
         const int m = t.m0 + cta * 128 + (MN ? along : row);
-        base = PASS == FWD ? ((size_t)t.e * a.N + m) * a.K + along : PASS == STATE ? ((size_t)t.e * a.N + row) * a.K + m : m;
+        base = PASS == FWD ? ((size_t)t.e * a.N + m) * a.K + along : PASS == STATE ? (size_t)t.e * a.N * a.K + m : m;
         left = (PASS == FWD ? a.N : a.K) - m;
         cu.var = t.kind == VAR, cu.half = false;
         nk = t.nk, depth = t.depth, p0 = t.p0;
@@ -190,8 +192,8 @@ __device__ __forceinline__ void convert_a(const GroupedArgs &a, Shared &sh, int 
 #pragma unroll
             for (int s = 0; s < 4; s++) {
                 const int rs = s == 0 ? r.x : s == 1 ? r.y : s == 2 ? r.z : r.w;
-                if (PASS == FWD) v[g * 4 + s] = ld4<VEC>(src + s * 16, g * 32 < left ? a.K - cu.kc - along - s * 16 : 0);
-                else if (PASS == STATE) v[g * 4 + s] = ld4<VEC>(src + (size_t)(s * 4) * a.K, cu.kc + (g * 4 + s) * 4 + row < a.N ? left : 0);
+                if (PASS == FWD) v[g * 4 + s] = ld4<VEC, VEC ? 1 : 4>(src + s * 16, g * 32 < left ? a.K - cu.kc - along - s * 16 : 0);
+                else if (PASS == STATE) v[g * 4 + s] = ld4<VEC>(src + (size_t)step_at<VEC>(s * 4 + row) * a.K, cu.kc + g * 16 + step_at<VEC>(s * 4 + row) < a.N ? left : 0);
                 else v[g * 4 + s] = ld4<VEC>(src + (size_t)max(rs, 0) * a.K, rs >= 0 ? left : 0);
             }
         }
@@ -217,7 +219,7 @@ template <int PASS, bool VEC>
 __device__ __forceinline__ void convert_b(const GroupedArgs &a, Shared &sh, int cta, int w, int lane, uint32_t smem_base) {
     constexpr bool MN = PASS == PARAM;
     using P = Place<MN>;
-    const int row = P::row(w, lane), along = P::along(lane);
+    const int row = P::row(w, lane), along = P::template along<VEC>(lane);
     const uint32_t to = smem_base + 3 * PART + P::base(w, lane);
     float4 v[TASKS];
     Cursor cu;
@@ -250,8 +252,8 @@ __device__ __forceinline__ void convert_b(const GroupedArgs &a, Shared &sh, int 
                                        : (cu.var ? a.a1 : a.a0) + base + (PASS == STATE ? (size_t)(g * 32) * a.N + cu.kc : (size_t)(cu.kc + g * 16) * a.N);
 #pragma unroll
         for (int s = 0; s < 4; s++) {
-            if (PASS == FWD) v[g * 4 + s] = ld4<VEC>(src + s * 16, rows[g] >= 0 ? a.K - cu.kc - along - s * 16 : 0);
-            else if (PASS == STATE) v[g * 4 + s] = ld4<VEC>(src + s * 16, g * 32 < left ? a.N - cu.kc - along - s * 16 : 0);
+            if (PASS == FWD) v[g * 4 + s] = ld4<VEC, VEC ? 1 : 4>(src + s * 16, rows[g] >= 0 ? a.K - cu.kc - along - s * 16 : 0);
+            else if (PASS == STATE) v[g * 4 + s] = ld4<VEC, VEC ? 1 : 4>(src + s * 16, g * 32 < left ? a.N - cu.kc - along - s * 16 : 0);
             else v[g * 4 + s] = ld4<VEC>(src + (size_t)(s * 4) * a.N, cu.kc + (g * 4 + s) * 4 + row < depth ? left : 0);
         }
     };

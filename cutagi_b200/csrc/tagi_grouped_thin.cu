@@ -3,7 +3,8 @@
 // takes the time. Bound: HBM, 8 (forward) or 4 (state) bytes a weight.
 //
 // One CTA computes 128 features x all rows of an expert. The weights come through a ring of eight half-chunks (16 KiB each),
-// so that about 100 KB of each SM are on their way from HBM whatever the converters do: by TMA. Sixteen warps read them, a feature to a lane, and store the values' bf16
+// so that about 100 KB of each SM are on their way from HBM whatever the converters do: by TMA, or 4 bytes at a time with
+// cp.async where rows are not multiples of 16 bytes. Sixteen warps read them, a feature to a lane, and store the values' bf16
 // parts to tensor memory, where the MMAs take that operand from (through shared memory, its parts would be read six times
 // from there). Four more warps fetch and split the rows, which come from L2; eight add up the accumulators of chunks of 64
 // steps; one thread issues the MMAs. Mean and variance of a tile go to neighbouring CTAs at the same time, mu_w first in
@@ -20,7 +21,7 @@ namespace tagi {
 namespace {
 namespace thin {
 
-constexpr int SUMMERS = 8, CONVERT_A = 16, CONVERT_B = 4, LOADERS = 1;
+constexpr int SUMMERS = 8, CONVERT_A = 16, CONVERT_B = 4, LOADERS = 2;
 constexpr int FIRST_A = SUMMERS, FIRST_B = FIRST_A + CONVERT_A, FIRST_LOADER = FIRST_B + CONVERT_B, ISSUER = FIRST_LOADER + LOADERS;
 constexpr int THREADS = 32 * (ISSUER + 2);       // the last warp works out the items
 constexpr int ROWS = 128, COLS = 48, KC = 64, HALF = 32, RING = 8, RECORDS = 4, CTAS = 148;
@@ -89,7 +90,7 @@ __device__ __forceinline__ float4 lds4(uint32_t at) {
     return v;
 }
 
-template <int PASS>
+template <int PASS, bool VEC>
 __global__ void __launch_bounds__(THREADS, 1)
 grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_constant__ CUtensorMap var_map, const GroupedArgs a) {
     extern __shared__ uint8_t smem_raw[];
@@ -122,7 +123,7 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
             mbar_init(sh.done + s, 1);
         }
         for (int s = 0; s < RING; s++) {
-            mbar_init(sh.raw_full + s, 1);   // the loading thread, and the bytes
+            mbar_init(sh.raw_full + s, VEC ? 1 : LOADERS * 32);   // the thread that starts TMA, or every loading thread's copies
             mbar_init(sh.raw_empty + s, CONVERT_A / 4);   // and a quarter read a half-chunk
         }
         for (int s = 0; s < RECORDS; s++) {
@@ -226,12 +227,13 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
 #pragma unroll
                         for (int q = 0; q < 4; q++) {
                             const float4 x = lds4(raw + row * (HALF * 4) + (((b / 4 + q) ^ (row & 7)) << 4));
-                            v[q * 4] = x.x, v[q * 4 + 1] = x.y, v[q * 4 + 2] = x.z, v[q * 4 + 3] = x.w;
+                            // places of steps 4 q .. 4 q + 3 (step_at is its own inverse)
+                            v[step_at<VEC>(q * 4)] = x.x, v[step_at<VEC>(q * 4 + 1)] = x.y, v[step_at<VEC>(q * 4 + 2)] = x.z, v[step_at<VEC>(q * 4 + 3)] = x.w;
                         }
                     } else {
 #pragma unroll
                         for (int k = 0; k < 16; k++)
-                            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v[k]) : "r"(raw + (b + k) * (ROWS * 4) + row * 4) : "memory");
+                            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v[step_at<VEC>(k)]) : "r"(raw + (b + k) * (ROWS * 4) + row * 4) : "memory");
                     }
                     if (square) {
 #pragma unroll
@@ -259,7 +261,7 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
     } else if (warp < FIRST_LOADER) {
         // ------------------------------------------------------------------------------- rows, global memory -> parts
         // a warp loads 64 consecutive bytes of eight rows; the next chunk is on its way while this one is split
-        const int w = warp - FIRST_B, row = w * 8 + ((lane >> 2) & 3) * 2 + (lane >> 4), along = (lane & 3) * 4;
+        const int w = warp - FIRST_B, row = w * 8 + ((lane >> 2) & 3) * 2 + (lane >> 4), along = VEC ? (lane & 3) * 4 : lane & 3;
         const uint32_t to = smem_base + row * 128 + ((((lane & 3) >> 1) ^ (row & 7)) << 4) + (lane & 1) * 8;
         float4 v[8];
         Item it;
@@ -280,7 +282,7 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
             const float *src = it.kind == MEAN ? a.a0 : second ? a.second : a.a1;
 #pragma unroll
             for (int q = 0; q < 8; q++)
-                v[q] = ld4<true>(src + (size_t)max(in[q >> 2], 0) * it.depth + kc + along + (q & 3) * 16,
+                v[q] = ld4<VEC, VEC ? 1 : 4>(src + (size_t)max(in[q >> 2], 0) * it.depth + kc + along + (q & 3) * 16,
                                 in[q >> 2] >= 0 ? it.depth - kc - along - (q & 3) * 16 : 0);
         };
         seek();
@@ -301,25 +303,48 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
         // --------------------------------------------------------------------------------------- weights, HBM -> ring
         // Forward: lines of 32 steps of a feature, 16-byte chunk c of line l at c ^ (l & 7), which is what TMA's 128-byte
         // swizzle makes and what lets eight lanes read eight lines at once. State: lines of 128 features of a step.
-        if (lane == 0) {
-            Item it;
-            bool ok = true;
-            int r = 0;
-            for (int j = 0; ok && take(sh, j, it) && it.chunks > 0; j++) {
-                mbar_arrive(sh.item_empty + j % RECORDS);
-                for (int c = 0; ok && c < it.chunks; c++) {
-                    const bool second = PASS == FWD && c >= it.nk;
-                    const int kc = (second ? c - it.nk : c) * KC;
-                    for (int h = 0; h < 2; h++, r++) {
-                        if (r >= RING) ok = mbar_wait(sh.raw_empty + r % RING, (r / RING - 1) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_EMPTY);
-                        if (!ok) break;
+        const int w = warp - FIRST_LOADER;
+        Item it;
+        bool ok = true;
+        int r = 0;
+        for (int j = 0; ok && take(sh, j, it) && it.chunks > 0; j++) {
+            release(sh, j, lane);
+            for (int c = 0; ok && c < it.chunks; c++) {
+                const bool second = PASS == FWD && c >= it.nk;
+                const int kc = (second ? c - it.nk : c) * KC;
+                for (int h = 0; h < 2; h++, r++) {
+                    if (VEC && (w != 0 || lane != 0)) continue;
+                    if (r >= RING) ok = mbar_wait(sh.raw_empty + r % RING, (r / RING - 1) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_EMPTY);
+                    if (!ok) break;
+                    const uint32_t dst = ring + (r % RING) * RAW;
+                    const int k0 = kc + h * HALF;
+                    if (VEC) {
                         mbar_arrive_expect_tx(sh.raw_full + r % RING, RAW);
-                        tma_load_3d(ring + (r % RING) * RAW, second ? &var_map : &mean_map, PASS == FWD ? kc + h * HALF : it.m0,
-                                    PASS == FWD ? it.m0 : kc + h * HALF, it.e, sh.raw_full + r % RING);
+                        tma_load_3d(dst, second ? &var_map : &mean_map, PASS == FWD ? k0 : it.m0, PASS == FWD ? it.m0 : k0, it.e, sh.raw_full + r % RING);
+                        continue;
                     }
+                    // a warp copies every other line (forward: 32 steps of a feature; state: 128 features of a step)
+                    const float *src = (second ? a.var_w : a.mu_w) + (size_t)it.e * a.N * a.K;
+                    const int n0 = PASS == FWD ? it.m0 : k0, k = (PASS == FWD ? k0 : it.m0) + lane, lines = min(PASS == FWD ? ROWS : HALF, a.N - n0);
+                    const float *p = src + (size_t)(n0 + w) * a.K + k;
+#pragma unroll 8
+                    for (int l = w; l < (PASS == FWD ? ROWS : HALF); l += 2, p += 2 * (size_t)a.K) {
+                        if (PASS == FWD) {
+                            const bool in = l < lines && k < a.K;
+                            cp_async_f32(dst + l * 128 + (((lane >> 2) ^ (l & 7)) << 4) + (lane & 3) * 4, in ? p : src, in);
+                        } else {
+#pragma unroll
+                            for (int q = 0; q < 4; q++) {
+                                const bool in = l < lines && k + q * 32 < a.K;
+                                cp_async_f32(dst + l * 512 + (q * 32 + lane) * 4, in ? p + q * 32 : src, in);
+                            }
+                        }
+                    }
+                    cp_async_arrive(sh.raw_full + r % RING);
                 }
             }
         }
+        if (!VEC) cp_async_wait_all();
     } else if (warp == ISSUER) {
         // ------------------------------------------------------------------------------------------------------- MMA
         if (lane == 0) {
@@ -382,11 +407,12 @@ int launch_thin(const GroupedArgs &a, cudaStream_t st) {
     const size_t smem = 2 * SLOT + RING * RAW + 1024 + sizeof(Shared) + (a.E + 1) * sizeof(int);
     const long mt = ((PASS == FWD ? a.N : a.K) + ROWS - 1) / ROWS, experts = a.E < a.S / (a.few + 1) ? a.E : a.S / (a.few + 1);
     const long most = 2 * mt * experts;   // experts with more than `few` rows, at most; both kinds
+    const bool vec = grouped_aligned(PASS, a);
     CUtensorMap mean = {}, var = {};
     int rc;
-    if ((rc = make_map(PASS, a, a.mu_w, &mean)) != TAGI_OK) return rc;
-    if (PASS == FWD && (rc = make_map(PASS, a, a.var_w, &var)) != TAGI_OK) return rc;
-    auto k = grouped_thin_kernel<PASS>;
+    if (vec && (rc = make_map(PASS, a, a.mu_w, &mean)) != TAGI_OK) return rc;
+    if (vec && PASS == FWD && (rc = make_map(PASS, a, a.var_w, &var)) != TAGI_OK) return rc;
+    auto k = vec ? grouped_thin_kernel<PASS, true> : grouped_thin_kernel<PASS, false>;
     TAGI_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     k<<<(unsigned)(most < CTAS ? most : CTAS), THREADS, smem, st>>>(mean, var, a);
     TAGI_CUDA(cudaGetLastError());

@@ -40,16 +40,21 @@ __device__ __forceinline__ unsigned score_key(float s) {
 }
 __device__ __forceinline__ float key_score(unsigned k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k); }
 
-// The whole warp ranks token t and writes its slots' experts and gates. EPL = scores a lane keeps.
+// The warp's scores of token t, EPL to a lane
 template <int EPL>
-__device__ __forceinline__ void rank_token(const RouteArgs &a, long t) {
+__device__ __forceinline__ void load_scores(const RouteArgs &a, long t, float (&score)[EPL]) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int q = 0; q < EPL; q++) score[q] = q * 32 + lane < a.E ? __ldg(a.mu_s + t * a.E + q * 32 + lane) : -INFINITY;
+}
+
+// The whole warp ranks token t and writes its slots' experts and gates. Returns the expert of the lane's slot, or -1.
+template <int EPL>
+__device__ __forceinline__ int rank_token(const RouteArgs &a, long t, const float (&scores)[EPL]) {
     const int lane = threadIdx.x & 31;
     unsigned key[EPL];
 #pragma unroll
-    for (int q = 0; q < EPL; q++) {
-        const int e = q * 32 + lane;
-        key[q] = e < a.E ? score_key(__ldg(a.mu_s + t * a.E + e)) : 0u;
-    }
+    for (int q = 0; q < EPL; q++) key[q] = score_key(scores[q]);
     int mine = -1;        // slot `lane`: its expert and score
     float score = -INFINITY;
     for (int j = 0; j < a.k; j++) {
@@ -88,17 +93,21 @@ __device__ __forceinline__ void rank_token(const RouteArgs &a, long t) {
         a.mu_g[i] = g;
         a.var_g[i] = g * g * (rest * rest * v + others);
     }
+    return mine;
 }
 
-// Ranks the tokens [t0, t1) of the block and adds their slots to count[e].
+// Ranks the tokens [t0, t1) of the block and adds their slots to count[e]. The next token's scores are on their way meanwhile.
 template <int EPL, int WARPS>
 __device__ __forceinline__ void rank_tokens(const RouteArgs &a, long t0, long t1, int *count) {
-    const int lane = threadIdx.x & 31;
-    for (long t = t0 + (threadIdx.x >> 5); t < t1; t += WARPS) {
-        rank_token<EPL>(a, t);
-        __syncwarp();
-        const int e = lane < a.k ? a.expert[t * a.k + lane] : -1;
+    long t = t0 + (threadIdx.x >> 5);
+    float now[EPL], next[EPL];
+    if (t < t1) load_scores<EPL>(a, t, now);
+    for (; t < t1; t += WARPS) {
+        if (t + WARPS < t1) load_scores<EPL>(a, t + WARPS, next);
+        const int e = rank_token<EPL>(a, t, now);
         if (e >= 0) atomicAdd(count + e, 1);
+#pragma unroll
+        for (int q = 0; q < EPL; q++) now[q] = next[q];
     }
 }
 

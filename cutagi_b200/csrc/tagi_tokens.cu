@@ -280,39 +280,55 @@ __device__ __forceinline__ int slot_row(const int *pos, long i, int S) {
 }
 
 // GATED: mu = sum g x, var = sum var_g (x^2 + var_x) + g^2 var_x. Otherwise mu = J sum x, var = J^2 sum var_x.
-template <int W, bool GATED>
+// TPR threads share a token, four features each at a time: consecutive ones (W = 4), or TPR apart (W = 1: rows of an odd
+// length start anywhere, but four loads are on their way all the same).
+template <int W, int TPR, bool GATED>
 __global__ void __launch_bounds__(256) combine_fwd_kernel(const CombineArgs a) {
-    const long tiles = (a.N + 256 * W - 1) / (256 * W);
-    const long t = blockIdx.x / tiles;
-    const int i = (int)((blockIdx.x % tiles) * 256 + threadIdx.x) * W;
-    if (i >= a.N) return;
-    float m[W], s[W];
+    constexpr int U = 4 / W;
+    const int tiles = (a.N + 4 * TPR - 1) / (4 * TPR);   // one, unless TPR is 256
+    const long t = (long)blockIdx.x / tiles * (256 / TPR) + threadIdx.x / TPR;
+    if (t >= a.T) return;
+    const int i0 = (int)(blockIdx.x % tiles) * 4 * TPR + threadIdx.x % TPR * W;
+    float m[U][W], s[U][W];
 #pragma unroll
-    for (int c = 0; c < W; c++) m[c] = s[c] = 0.f;
-#pragma unroll 4
+    for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int c = 0; c < W; c++) m[u][c] = s[u][c] = 0.f;
+#pragma unroll(W)
     for (int j = 0; j < a.k; j++) {
         const int p = slot_row(a.pos, t * a.k + j, a.S);
         if (p < 0) continue;
-        float x[W], v[W];
-        load<W>(a.mu_x + (long)p * a.N + i, x);
-        load<W>(a.var_x + (long)p * a.N + i, v);
-        if (GATED) {
-            const float g = __ldg(a.mu_g + t * a.k + j), vg = __ldg(a.var_g + t * a.k + j);
+        const float g = GATED ? __ldg(a.mu_g + t * a.k + j) : 1.f, vg = GATED ? __ldg(a.var_g + t * a.k + j) : 0.f;
+        float x[U][W], v[U][W];
 #pragma unroll
-            for (int c = 0; c < W; c++) m[c] += g * x[c], s[c] += vg * (x[c] * x[c] + v[c]) + g * g * v[c];
-        } else {
+        for (int u = 0; u < U; u++)
+            if (i0 + u * TPR < a.N) {
+                load<W>(a.mu_x + (long)p * a.N + i0 + u * TPR, x[u]);
+                load<W>(a.var_x + (long)p * a.N + i0 + u * TPR, v[u]);
+            }
 #pragma unroll
-            for (int c = 0; c < W; c++) m[c] += x[c], s[c] += v[c];
+        for (int u = 0; u < U; u++)
+            if (i0 + u * TPR < a.N) {
+#pragma unroll
+                for (int c = 0; c < W; c++) {
+                    if (GATED) m[u][c] += g * x[u][c], s[u][c] += vg * (x[u][c] * x[u][c] + v[u][c]) + g * g * v[u][c];
+                    else m[u][c] += x[u][c], s[u][c] += v[u][c];
+                }
+            }
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int i = i0 + u * TPR;
+        if (i >= a.N) break;
+        if (!GATED && a.jcb) {
+            float q[W];
+            load<W>(a.jcb + t * a.N + i, q);
+#pragma unroll
+            for (int c = 0; c < W; c++) m[u][c] *= q[c], s[u][c] *= q[c] * q[c];
         }
+        store<W>(a.mu_y + t * a.N + i, m[u]);
+        store<W>(a.var_y + t * a.N + i, s[u]);
     }
-    if (!GATED && a.jcb) {
-        float q[W];
-        load<W>(a.jcb + t * a.N + i, q);
-#pragma unroll
-        for (int c = 0; c < W; c++) m[c] *= q[c], s[c] *= q[c] * q[c];
-    }
-    store<W>(a.mu_y + t * a.N + i, m);
-    store<W>(a.var_y + t * a.N + i, s);
 }
 
 struct CombineBwdArgs {
@@ -340,31 +356,43 @@ __global__ void __launch_bounds__(256) combine_bwd_kernel(const CombineBwdArgs a
             g[j] = p[j] >= 0 ? __ldg(a.mu_g + t * a.k + j0 + j) : 0.f;
             s[2 * j] = s[2 * j + 1] = 0.f;
         }
-        for (int i = u * W; i < a.N; i += TPR * W) {
-            float dm[W], dv[W], x[SLOTS][W], q[SLOTS][W];
-            load<W>(a.dmu_y + t * a.N + i, dm);
-            load<W>(a.dvar_y + t * a.N + i, dv);
+        // W = 1: two features at a time, TPR apart
+        constexpr int U = W == 4 ? 1 : 2;
+        for (int i0 = u * W; i0 < a.N; i0 += TPR * W * U) {
+            float dm[U][W], dv[U][W], x[U][SLOTS][W], q[U][SLOTS][W];
 #pragma unroll
-            for (int j = 0; j < SLOTS; j++)
-                if (p[j] >= 0) {
-                    load<W>(a.mu_x + (long)p[j] * a.N + i, x[j]);
-                    if (a.jcb) load<W>(a.jcb + (long)p[j] * a.N + i, q[j]);
-                }
+            for (int h = 0; h < U; h++) {
+                const int i = i0 + h * TPR;
+                if (i >= a.N) break;
+                load<W>(a.dmu_y + t * a.N + i, dm[h]);
+                load<W>(a.dvar_y + t * a.N + i, dv[h]);
 #pragma unroll
-            for (int j = 0; j < SLOTS; j++)
-                if (p[j] >= 0) {
-                    float o[W], r[W];
-#pragma unroll
-                    for (int c = 0; c < W; c++) {
-                        const float f = a.jcb ? g[j] * q[j][c] : g[j];
-                        s[2 * j] += x[j][c] * dm[c];
-                        s[2 * j + 1] += x[j][c] * dv[c] * x[j][c];
-                        o[c] = f * dm[c];
-                        r[c] = f * dv[c] * f;
+                for (int j = 0; j < SLOTS; j++)
+                    if (p[j] >= 0) {
+                        load<W>(a.mu_x + (long)p[j] * a.N + i, x[h][j]);
+                        if (a.jcb) load<W>(a.jcb + (long)p[j] * a.N + i, q[h][j]);
                     }
-                    store<W>(a.dmu_x + (long)p[j] * a.N + i, o);
-                    store<W>(a.dvar_x + (long)p[j] * a.N + i, r);
-                }
+            }
+#pragma unroll
+            for (int h = 0; h < U; h++) {
+                const int i = i0 + h * TPR;
+                if (i >= a.N) break;
+#pragma unroll
+                for (int j = 0; j < SLOTS; j++)
+                    if (p[j] >= 0) {
+                        float o[W], r[W];
+#pragma unroll
+                        for (int c = 0; c < W; c++) {
+                            const float f = a.jcb ? g[j] * q[h][j][c] : g[j];
+                            s[2 * j] += x[h][j][c] * dm[h][c];
+                            s[2 * j + 1] += x[h][j][c] * dv[h][c] * x[h][j][c];
+                            o[c] = f * dm[h][c];
+                            r[c] = f * dv[h][c] * f;
+                        }
+                        store<W>(a.dmu_x + (long)p[j] * a.N + i, o);
+                        store<W>(a.dvar_x + (long)p[j] * a.N + i, r);
+                    }
+            }
         }
 #pragma unroll
         for (int q = 0; q < 2 * SLOTS; q++) s[q] = warp_sum(s[q]);
@@ -390,15 +418,26 @@ __global__ void __launch_bounds__(256) combine_bwd_kernel(const CombineBwdArgs a
     }
 }
 
+template <int W, bool GATED>
+int combine_fwd_launch(const CombineArgs &a, cudaStream_t st) {
+    if (a.N > 512) {
+        const long tiles = (a.N + 1023) / 1024;
+        if (tiles * a.T >= (1L << 31)) return fail(TAGI_ERR_INVALID_ARGUMENT, "combine: too many tokens times features for one launch");
+        combine_fwd_kernel<W, 256, GATED><<<(unsigned)(tiles * a.T), 256, 0, st>>>(a);
+    } else if (a.N > 128) {
+        combine_fwd_kernel<W, 128, GATED><<<(a.T + 1) / 2, 256, 0, st>>>(a);
+    } else if (a.N > 32) {
+        combine_fwd_kernel<W, 32, GATED><<<(a.T + 7) / 8, 256, 0, st>>>(a);
+    } else {
+        combine_fwd_kernel<W, 8, GATED><<<(a.T + 31) / 32, 256, 0, st>>>(a);
+    }
+    return launched("combine_fwd_kernel launch");
+}
 template <bool GATED>
 int combine_fwd(const CombineArgs &a, cudaStream_t st) {
     if (a.T == 0) return TAGI_OK;
     const bool vec = a.N % 4 == 0 && all16({a.mu_x, a.var_x, a.jcb, a.mu_y, a.var_y});
-    const long tiles = (a.N + 256L * (vec ? 4 : 1) - 1) / (256 * (vec ? 4 : 1));
-    if (tiles * a.T >= (1L << 31)) return fail(TAGI_ERR_INVALID_ARGUMENT, "combine: too many tokens times features for one launch");
-    if (vec) combine_fwd_kernel<4, GATED><<<(unsigned)(tiles * a.T), 256, 0, st>>>(a);
-    else combine_fwd_kernel<1, GATED><<<(unsigned)(tiles * a.T), 256, 0, st>>>(a);
-    return launched("combine_fwd_kernel launch");
+    return vec ? combine_fwd_launch<4, GATED>(a, st) : combine_fwd_launch<1, GATED>(a, st);
 }
 
 }  // namespace
@@ -530,12 +569,12 @@ int tagi_combine_bwd(int T, int k, int N, int S, const int *pos, const float *mu
     TAGI_PTR(dvar_g);
     TAGI_REQUIRE(jcb == nullptr || aligned4(jcb), "jcb is not 4-byte aligned");
     const CombineBwdArgs a{T, k, N, S, pos, mu_g, mu_x, jcb, dmu_y, dvar_y, dmu_x, dvar_x, dmu_g, dvar_g};
-    // a warp per token where a row is at most four of its strides long, else a CTA
+    // a warp per token while a row is at most eight of its strides long, else a CTA
     const bool vec = N % 4 == 0 && all16({mu_x, jcb, dmu_y, dvar_y, dmu_x, dvar_x});
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (vec && N > 512) combine_bwd_kernel<4, 256><<<T, 256, 0, st>>>(a);
+    if (vec && N > 1024) combine_bwd_kernel<4, 256><<<T, 256, 0, st>>>(a);
     else if (vec) combine_bwd_kernel<4, 32><<<(T + 7) / 8, 256, 0, st>>>(a);
-    else if (N > 128) combine_bwd_kernel<1, 256><<<T, 256, 0, st>>>(a);
+    else if (N > 512) combine_bwd_kernel<1, 256><<<T, 256, 0, st>>>(a);
     else combine_bwd_kernel<1, 32><<<(T + 7) / 8, 256, 0, st>>>(a);
     return launched("combine_bwd_kernel launch");
 }
