@@ -279,26 +279,28 @@ __device__ __forceinline__ int slot_row(const int *pos, long i, int S) {
     return (unsigned)p < (unsigned)S ? p : -1;
 }
 
+constexpr int SLOTS = 4;   // of a token that are worked on together
+
 // GATED: mu = sum g x, var = sum var_g (x^2 + var_x) + g^2 var_x. Otherwise mu = J sum x, var = J^2 sum var_x.
 // TPR threads share a token, four features each at a time: consecutive ones (W = 4), or TPR apart (W = 1: rows of an odd
 // length start anywhere, but four loads are on their way all the same).
 template <int W, int TPR, bool GATED>
-__global__ void __launch_bounds__(256) combine_fwd_kernel(const CombineArgs a) {
+__global__ void __launch_bounds__(256, W == 4 || !GATED ? 8 : 6) combine_fwd_kernel(const CombineArgs a) {
     constexpr int U = 4 / W;
-    const int tiles = (a.N + 4 * TPR - 1) / (4 * TPR);   // one, unless TPR is 256
-    const long t = (long)blockIdx.x / tiles * (256 / TPR) + threadIdx.x / TPR;
-    if (t >= a.T) return;
+    const unsigned tiles = (a.N + 4 * TPR - 1) / (4 * TPR);   // one, unless TPR is 256
+    const long t = (long)(blockIdx.x / tiles) * (256 / TPR) + threadIdx.x / TPR;
     const int i0 = (int)(blockIdx.x % tiles) * 4 * TPR + threadIdx.x % TPR * W;
+    if (t >= a.T || i0 >= a.N) return;
     float m[U][W], s[U][W];
 #pragma unroll
     for (int u = 0; u < U; u++)
 #pragma unroll
         for (int c = 0; c < W; c++) m[u][c] = s[u][c] = 0.f;
-#pragma unroll(W)
+    // few registers and many threads: fetching the rows of four slots before the first is used was slower (141 against 123 us)
+#pragma unroll(W == 4 ? 4 : 2)
     for (int j = 0; j < a.k; j++) {
         const int p = slot_row(a.pos, t * a.k + j, a.S);
         if (p < 0) continue;
-        const float g = GATED ? __ldg(a.mu_g + t * a.k + j) : 1.f, vg = GATED ? __ldg(a.var_g + t * a.k + j) : 0.f;
         float x[U][W], v[U][W];
 #pragma unroll
         for (int u = 0; u < U; u++)
@@ -306,6 +308,7 @@ __global__ void __launch_bounds__(256) combine_fwd_kernel(const CombineArgs a) {
                 load<W>(a.mu_x + (long)p * a.N + i0 + u * TPR, x[u]);
                 load<W>(a.var_x + (long)p * a.N + i0 + u * TPR, v[u]);
             }
+        const float g = GATED ? __ldg(a.mu_g + t * a.k + j) : 1.f, vg = GATED ? __ldg(a.var_g + t * a.k + j) : 0.f;
 #pragma unroll
         for (int u = 0; u < U; u++)
             if (i0 + u * TPR < a.N) {
@@ -340,7 +343,6 @@ struct CombineBwdArgs {
 
 // TPR threads per token: the deltas of the slots' rows, and for each slot the sums of x dmu_y and x^2 dvar_y over the features.
 // Four slots at a time, so that their rows are fetched together and the token's deltas once.
-constexpr int SLOTS = 4;
 template <int W, int TPR>
 __global__ void __launch_bounds__(256) combine_bwd_kernel(const CombineBwdArgs a) {
     __shared__ float red[8][2 * SLOTS];
