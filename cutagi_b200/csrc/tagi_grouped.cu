@@ -6,33 +6,6 @@
 namespace tagi {
 namespace {
 
-// dmu_b = var_b sum dmu_z, dvar_b = var_b^2 sum dvar_z over the rows of the experts that run on the tensor cores: 32 features
-// x 8 groups of rows per CTA.
-__global__ void __launch_bounds__(256) grouped_bias_kernel(const GroupedArgs a) {
-    __shared__ float2 red[8][32];
-    const int c = threadIdx.x & 31, g = threadIdx.x >> 5, n = blockIdx.x * 32 + c, e = blockIdx.y;
-    int r0, r1;
-    expert_rows(a, e, r0, r1);
-    if (r1 - r0 <= a.few) return;
-    float s = 0.f, v = 0.f;
-    if (n < a.N)
-        for (int r = r0 + g; r < r1; r += 8) s += __ldg(a.a0 + (size_t)r * a.N + n), v += __ldg(a.a1 + (size_t)r * a.N + n);
-    red[g][c] = make_float2(s, v);
-    __syncthreads();
-    if (g != 0 || n >= a.N) return;
-    s = v = 0.f;
-#pragma unroll
-    for (int k = 0; k < 8; k++) s += red[k][c].x, v += red[k][c].y;
-    const float vb = __ldg(a.var_b + (size_t)e * a.N + n);
-    a.ob0[(size_t)e * a.N + n] = vb * s;
-    a.ob1[(size_t)e * a.N + n] = vb * vb * v;
-}
-
-inline int launched(const char *what) {
-    cudaError_t e = cudaGetLastError();
-    return e == cudaSuccess ? TAGI_OK : cuda_fail(e, what);
-}
-
 int run(int pass, GroupedArgs &a, cudaStream_t st) {
     a.few = pass == PARAM ? FEW_PARAM_ROWS : FEW_ROWS;
     a.thin = pass == PARAM ? FEW_PARAM_ROWS : THIN_ROWS;
@@ -140,10 +113,7 @@ int tagi_grouped_linear_bwd_param(int E, int S, int R, int K, int N, int has_bia
     a.E = E, a.S = S, a.R = R, a.K = K, a.N = N, a.offsets = offsets, a.token = token, a.var_w = var_w, a.x = mu_a;
     a.var_b = has_bias ? var_b : nullptr, a.a0 = dmu_z, a.a1 = dvar_z, a.o0 = dmu_w, a.o1 = dvar_w, a.ob0 = dmu_b, a.ob1 = dvar_b;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    rc = run(PARAM, a, st);
-    if (rc != TAGI_OK || !has_bias || S <= a.few) return rc;
-    grouped_bias_kernel<<<dim3((N + 31) / 32, E), 256, 0, st>>>(a);
-    return launched("grouped_bias_kernel launch");
+    return run(PARAM, a, st);
 }
 
 }  // extern "C"

@@ -27,13 +27,13 @@ __device__ __forceinline__ float4 ld4(const float *p, int valid) {
     return v;
 }
 
-// Which of 16 contraction steps lies at place j of an operand whose steps run along memory. Rows that are not aligned to 16
-// bytes are read a float at a time; four lanes then take neighbouring steps (half the sectors of taking every fourth), which
-// leaves a lane with steps 4 apart in four neighbouring places. The order of the steps does not matter to a sum as long as
-// both operands have the same.
-template <bool VEC>
+// Which of 16 contraction steps lies at place j of an operand whose steps run along memory. SPREAD: rows that are not aligned
+// to 16 bytes are read a float at a time; four lanes then take neighbouring steps (half the sectors of taking every fourth),
+// which leaves a lane with steps 4 apart in four neighbouring places. The order of the steps does not matter to a sum as
+// long as both operands have the same.
+template <bool SPREAD>
 __device__ __forceinline__ int step_at(int j) {
-    return VEC ? j : (j & ~15) | ((j & 3) << 2) | ((j >> 2) & 3);
+    return SPREAD ? (j & ~15) | ((j & 3) << 2) | ((j >> 2) & 3) : j;
 }
 
 __device__ __forceinline__ uint32_t top_halves(float a, float b) {   // a's upper 16 bits below b's

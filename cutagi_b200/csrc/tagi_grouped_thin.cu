@@ -228,12 +228,12 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
                         for (int q = 0; q < 4; q++) {
                             const float4 x = lds4(raw + row * (HALF * 4) + (((b / 4 + q) ^ (row & 7)) << 4));
                             // places of steps 4 q .. 4 q + 3 (step_at is its own inverse)
-                            v[step_at<VEC>(q * 4)] = x.x, v[step_at<VEC>(q * 4 + 1)] = x.y, v[step_at<VEC>(q * 4 + 2)] = x.z, v[step_at<VEC>(q * 4 + 3)] = x.w;
+                            v[step_at<!VEC>(q * 4)] = x.x, v[step_at<!VEC>(q * 4 + 1)] = x.y, v[step_at<!VEC>(q * 4 + 2)] = x.z, v[step_at<!VEC>(q * 4 + 3)] = x.w;
                         }
                     } else {
 #pragma unroll
                         for (int k = 0; k < 16; k++)
-                            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v[step_at<VEC>(k)]) : "r"(raw + (b + k) * (ROWS * 4) + row * 4) : "memory");
+                            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v[step_at<!VEC>(k)]) : "r"(raw + (b + k) * (ROWS * 4) + row * 4) : "memory");
                     }
                     if (square) {
 #pragma unroll
