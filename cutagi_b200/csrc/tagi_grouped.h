@@ -39,9 +39,10 @@ __device__ __forceinline__ int input_row(const GroupedArgs &a, int p) {
 // 747 us, the wide kernel 600 us at 16.
 constexpr int FEW_ROWS = 8, FEW_PARAM_ROWS = 20, THIN_ROWS = 48;
 
-// forward and state pass: rows of weights, activations and deltas are whole 16-byte groups
+// the rows that a pass reads (of weights, activations and deltas) are whole 16-byte groups
 inline bool grouped_aligned(int pass, const GroupedArgs &a) {
-    return a.K % 4 == 0 && (pass == FWD || a.N % 4 == 0) && aligned16(a.mu_w) && aligned16(a.var_w) && aligned16(a.a0) && aligned16(a.a1);
+    return a.K % 4 == 0 && (pass == FWD || a.N % 4 == 0) && (pass == PARAM || (aligned16(a.mu_w) && aligned16(a.var_w))) && aligned16(a.a0) &&
+           aligned16(a.a1) && aligned16(a.x);
 }
 
 // mu_a^2 + var_a of every input row to a.second, for the tensor-core kernels

@@ -565,8 +565,7 @@ __global__ void __launch_bounds__(256) grouped_second_moment_unaligned_kernel(co
 
 template <int PASS>
 int launch_pass(const GroupedArgs &a, cudaStream_t st) {
-    const bool vec = a.K % 4 == 0 && a.N % 4 == 0 && aligned16(a.mu_w) && aligned16(a.var_w) && aligned16(a.a0) && aligned16(a.a1) &&
-                     aligned16(a.x);
+    const bool vec = grouped_aligned(PASS, a);
     const size_t smem = 2 * SLOT + 1024 + sizeof(Shared) + (a.E + 1) * sizeof(int);
     const long mt = ((PASS == FWD ? a.N : a.K) + 255) / 256;
     const long experts = a.E < a.S / (a.thin + 1) ? a.E : a.S / (a.thin + 1);   // at most as many have more rows

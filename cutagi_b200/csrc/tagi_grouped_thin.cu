@@ -344,7 +344,11 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
                 }
             }
         }
+        // all copies have landed, unless the CTA gives up: then they are waited for here, again not for ever
         if (!VEC) cp_async_wait_all();
+        else if (!ok || sh.abort_flag)
+            for (int q = max(0, r - RING); w == 0 && lane == 0 && q < r; q++)
+                for (int spin = 0; spin < 100000 && !mbar_try_wait(sh.raw_full + q % RING, (q / RING) & 1); spin++) {}
     } else if (warp == ISSUER) {
         // ------------------------------------------------------------------------------------------------------- MMA
         if (lane == 0) {

@@ -17,7 +17,7 @@
 namespace tagi {
 namespace {
 
-constexpr int MAX_EXPERTS = 1024, MAX_K = 32;
+constexpr int MAX_EXPERTS = 1024, MAX_K = 32, MAX_TOKENS = 1 << 30;
 // Warps of a block: the more the shorter the chain of tokens that a warp ranks one after the other (a block per SM holds
 // them all), as far as the per-warp counts fit shared memory and a lane's scores its registers.
 __host__ __device__ constexpr int warps_for(int E) { return E <= 256 ? 32 : 8; }
@@ -331,6 +331,7 @@ int route_launch(const RouteArgs &a, cudaStream_t st) {
 int check_route(const char *who, int T, int E, int k) {
     if (T < 0 || E < 1 || E > MAX_EXPERTS) return fail(TAGI_ERR_INVALID_ARGUMENT, std::string(who) + ": 1 to 1024 experts, tokens must not be negative");
     if (k < 1 || k > E || k > MAX_K) return fail(TAGI_ERR_INVALID_ARGUMENT, std::string(who) + ": k must be 1 to 32 and at most the number of experts");
+    if (T > MAX_TOKENS) return fail(TAGI_ERR_INVALID_ARGUMENT, std::string(who) + ": more than 2^30 tokens");
     if ((long)T * k >= (1L << 31)) return fail(TAGI_ERR_INVALID_ARGUMENT, std::string(who) + ": more than 2^31 slots");
     return TAGI_OK;
 }
@@ -345,7 +346,7 @@ using namespace tagi;
 extern "C" {
 
 size_t tagi_route_workspace_bytes(int T, int E, int k) {
-    if (T <= ONE_BLOCK_TOKENS || E < 1 || E > MAX_EXPERTS || k < 1 || k > E || k > MAX_K) return 0;
+    if (T <= ONE_BLOCK_TOKENS || T > MAX_TOKENS || E < 1 || E > MAX_EXPERTS || k < 1 || k > E || k > MAX_K) return 0;
     return (size_t)blocks_of(T) * E * sizeof(int);
 }
 

@@ -6,6 +6,8 @@
 namespace tagi {
 namespace {
 
+constexpr int MAX_ROWS = 1 << 30, MAX_FEATURES = 1 << 24;   // what the kernels' and launches' 32-bit counts hold
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -456,6 +458,7 @@ int tagi_ln_fwd(int R, int n, int has_bias, float eps, const float *mu_w, const 
                 const float *var_b, const float *mu_a, const float *var_a, float *mu_row, float *var_row, float *mu_z,
                 float *var_z, void *stream) {
     TAGI_REQUIRE(R >= 0 && n >= 2, "rows must not be negative, features must be at least 2 (the variance divides by n - 1)");
+    TAGI_REQUIRE(R <= MAX_ROWS && n <= MAX_FEATURES, "more than 2^30 rows or 2^24 features");
     TAGI_REQUIRE(eps >= 0.f, "eps must not be negative");
     TAGI_PTR(mu_w);
     TAGI_PTR(var_w);
@@ -475,7 +478,7 @@ int tagi_ln_fwd(int R, int n, int has_bias, float eps, const float *mu_w, const 
 }
 
 size_t tagi_ln_bwd_workspace_bytes(int R, int n) {
-    if (R < 0 || n < 2) return 0;
+    if (R < 0 || n < 2 || R > MAX_ROWS || n > MAX_FEATURES) return 0;
     const int chunks = ln_bwd_chunks(R, n);
     return chunks <= 1 ? 0 : (size_t)chunks * 4 * n * sizeof(float);
 }
@@ -485,6 +488,7 @@ int tagi_ln_bwd(int R, int n, int has_bias, int state_update, float eps, const f
                 const float *dmu_o, const float *dvar_o, float *dmu, float *dvar, float *dmu_w, float *dvar_w, float *dmu_b,
                 float *dvar_b, void *workspace, size_t workspace_bytes, void *stream) {
     TAGI_REQUIRE(R >= 0 && n >= 2, "rows must not be negative, features must be at least 2");
+    TAGI_REQUIRE(R <= MAX_ROWS && n <= MAX_FEATURES, "more than 2^30 rows or 2^24 features");
     TAGI_REQUIRE(eps >= 0.f, "eps must not be negative");
     TAGI_PTR(mu_w);
     TAGI_PTR(var_w);
@@ -523,6 +527,7 @@ int tagi_ln_bwd(int R, int n, int has_bias, int state_update, float eps, const f
 static int check_slots(const char *who, int T, int k, int N, int S, const int *pos) {
     if (T < 0 || S < 0 || k < 1 || N < 1)
         return fail(TAGI_ERR_INVALID_ARGUMENT, std::string(who) + ": sizes must be positive (tokens and rows may be zero)");
+    if (T > MAX_ROWS || N > MAX_FEATURES) return fail(TAGI_ERR_INVALID_ARGUMENT, std::string(who) + ": more than 2^30 tokens or 2^24 features");
     if ((long)T * k >= (1L << 31)) return fail(TAGI_ERR_INVALID_ARGUMENT, std::string(who) + ": more than 2^31 slots");
     if (T > 0 && (pos == nullptr || !aligned4(pos)))
         return fail(TAGI_ERR_INVALID_ARGUMENT, std::string(who) + ": pos is null or not 4-byte aligned");

@@ -10,6 +10,7 @@ import torch
 from . import capi
 
 _F, _I = torch.float32, torch.int32
+_MOST = 2 ** 31 - 1   # the entry points' sizes are 32-bit integers, which ctypes would cut without a word
 _stream = torch._C._cuda_getCurrentRawStream   # of a device; torch.cuda.current_stream makes an object of it first
 
 
@@ -31,7 +32,15 @@ def _index(name, t, dim=2):
     index = t.get_device()
     if index < 0:
         raise ValueError(f"{name}: expected a tensor on a CUDA device, got {t.device}")
+    if t.numel() > _MOST and max(t.shape) > _MOST:
+        raise ValueError(f"{name}: more than 2^31 - 1 entries along a dimension: {tuple(t.shape)}")
     return index
+
+
+def _rows(name, n):
+    if n > _MOST:
+        raise ValueError(f"{name}: more than 2^31 - 1 rows: {n}")
+    return n
 
 
 def _p(name, t, shape, index, dtype=_F):
@@ -138,8 +147,8 @@ def route_backward(r: Routing, dmu_g, dvar_g):
 def grouped_linear(mu_w, var_w, mu_b, var_b, mu_a, var_a, offsets, token=None):
     """tagi_grouped_linear_fwd: (mu_z, var_z) [S][N] in dispatch order. `token` (int32 [S]): the row of mu_a that each row
     reads; without it row p reads row p. Rows that no expert owns are not written."""
-    i, (E, N, K), R = _index("mu_w", mu_w, 3), mu_w.shape, mu_a.shape[0]
-    S = R if token is None else token.numel()
+    i, (E, N, K), R = _index("mu_w", mu_w, 3), mu_w.shape, _rows("mu_a", mu_a.shape[0])
+    S = R if token is None else _rows("token", token.numel())
     bias, w, b = _pair("mu_b / var_b", mu_b, var_b), mu_w.shape, (E, N)
     inputs = (_p("offsets", offsets, (E + 1,), i, _I), _p("token", token, (S,), i, _I), _p("mu_w", mu_w, w, i), _p("var_w", var_w, w, i),
               _p("mu_b", mu_b, b, i), _p("var_b", var_b, b, i), _p("mu_a", mu_a, (R, K), i), _p("var_a", var_a, (R, K), i))
@@ -152,7 +161,7 @@ def grouped_linear(mu_w, var_w, mu_b, var_b, mu_a, var_a, offsets, token=None):
 
 def grouped_linear_state(mu_w, jcb, dmu_z, dvar_z, offsets):
     """tagi_grouped_linear_bwd_state: (dmu_a, dvar_a) [S][K] in dispatch order."""
-    i, (E, N, K), S = _index("mu_w", mu_w, 3), mu_w.shape, dmu_z.shape[0]
+    i, (E, N, K), S = _index("mu_w", mu_w, 3), mu_w.shape, _rows("dmu_z", dmu_z.shape[0])
     inputs = (_p("offsets", offsets, (E + 1,), i, _I), _p("mu_w", mu_w, mu_w.shape, i), _p("jcb", jcb, (S, K), i),
               _p("dmu_z", dmu_z, (S, N), i), _p("dvar_z", dvar_z, (S, N), i))
     dmu_a, dvar_a = _two(mu_w, S, K)
@@ -164,7 +173,7 @@ def grouped_linear_param(var_w, var_b, mu_a, dmu_z, dvar_z, offsets, token=None,
     """tagi_grouped_linear_bwd_param: (dmu_w, dvar_w, dmu_b, dvar_b), the bias deltas None without var_b. `out`: the four
     tensors that receive them."""
     i, w = _index("var_w", var_w, 3), var_w.shape
-    (E, N, K), R, S = w, mu_a.shape[0], dmu_z.shape[0]
+    (E, N, K), R, S = w, _rows("mu_a", mu_a.shape[0]), _rows("dmu_z", dmu_z.shape[0])
     bias, b = var_b is not None, (E, N)
     inputs = (_p("offsets", offsets, (E + 1,), i, _I), _p("token", token, (S,), i, _I), _p("var_w", var_w, w, i), _p("var_b", var_b, b, i),
               _p("mu_a", mu_a, (R, K), i), _p("dmu_z", dmu_z, (S, N), i), _p("dvar_z", dvar_z, (S, N), i))

@@ -319,7 +319,10 @@ int tagi_add_shortcut(const float *mu_s, const float *var_s, const float *jcb, s
  * and calls that may overlap on the GPU need one each), so calls on several streams and CUDA graphs replayed at the same
  * time do not meet. No call waits for the host, allocates, or uses floating-point atomics: results repeat bit for bit.
  * Row counts may be zero (pointers to empty tensors may then be NULL). Any alignment of 4 bytes is accepted; tensors that
- * are 16-byte aligned with rows of a multiple of four floats are faster. */
+ * are 16-byte aligned with rows of a multiple of four floats are faster. Outputs must not overlap inputs. Sizes: up to 2^30
+ * rows (tokens), 2^31 - 1 slots (T * k) and 2^24 features; the grouped Linear layers up to 2^28 rows and 2^20 features. NaN
+ * and infinities stay in the rows, experts and features that they belong to (a sum over an infinite entry may be NaN where
+ * a sum of 32-bit products is infinite). tagi_tc_status covers the tensor-core kernels of the grouped Linear layers too. */
 
 /* LayerNorm of every row over its n >= 2 features: mean = sum mu_a / n, var = (sum (mu_a - mean)^2 + sum var_a) / (n - 1),
  * written to mu_row / var_row [R]; inv = 1 / sqrt(var + eps); mu_z = inv * (mu_a - mean) * mu_w + mu_b;
@@ -361,11 +364,12 @@ int tagi_route_bwd(int T, int E, int k, const int *expert, const float *mu_g, co
  * rows from offsets[E] on and rows before offsets[0] are left as they were. token (device, S entries) names the row of
  * mu_a / var_a [R][K] that each output row reads, so the tokens need no copy in dispatch order; NULL: row p reads row p
  * (then R == S). Bad device data does no harm: offsets are clamped into range, a token outside [0, R) reads as a row of
- * zeros. */
+ * zeros. Sums have the accuracy of 32-bit products. workspace: tagi_grouped_linear_workspace_bytes(S, R, K) bytes (host
+ * helper; 0 = NULL is fine). */
+size_t tagi_grouped_linear_workspace_bytes(int S, int R, int K);
 int tagi_grouped_linear_fwd(int E, int S, int R, int K, int N, int has_bias, const int *offsets, const int *token,
                             const float *mu_w, const float *var_w, const float *mu_b, const float *var_b, const float *mu_a,
                             const float *var_a, float *mu_z, float *var_z, void *workspace, size_t workspace_bytes, void *stream);
-size_t tagi_grouped_linear_workspace_bytes(int S, int R, int K); /* of the forward pass; host helper */
 /* tagi_linear_bwd_state per expert: deltas dmu_z / dvar_z [S][N] and outputs dmu_a / dvar_a [S][K] in dispatch order, jcb
  * [S][K] the Jacobian of the same rows (NULL = 1; where the input was gathered by token, tagi_dispatch_bwd applies it). */
 int tagi_grouped_linear_bwd_state(int E, int S, int K, int N, const int *offsets, const float *mu_w, const float *jcb,

@@ -31,6 +31,8 @@ def test_layer_norm_refusals():
     refused("tagi_ln_fwd", *ln_args(n=1))
     refused("tagi_ln_fwd", *ln_args(eps=-1.0))
     refused("tagi_ln_fwd", *ln_args(eps=float("nan")))
+    refused("tagi_ln_fwd", *ln_args(R=(1 << 30) + 1))
+    refused("tagi_ln_fwd", *ln_args(n=(1 << 24) + 1))
     for i in range(10):
         for bad in (None, P + 2):
             refused("tagi_ln_fwd", *ln_args(p=[bad if j == i else P for j in range(10)]))
@@ -42,6 +44,9 @@ def test_layer_norm_backward_refusals():
         return (R_, n, bias, su, f(1e-5), *p, ws, size, None)
     refused("tagi_ln_bwd", *args(R_=-1))
     refused("tagi_ln_bwd", *args(n=1))
+    refused("tagi_ln_bwd", *args(R_=2 ** 31 - 1))
+    refused("tagi_ln_bwd", *args(n=2 ** 31 - 1))
+    assert lib.tagi_ln_bwd_workspace_bytes(2 ** 31 - 1, 8) == lib.tagi_ln_bwd_workspace_bytes(8, 2 ** 31 - 1) == 0
     for i in range(15):
         if i != 4:      # the Jacobian may be NULL
             refused("tagi_ln_bwd", *args(p=[None if j == i else P for j in range(15)]))
@@ -57,7 +62,7 @@ def test_layer_norm_backward_refusals():
 def test_route_refusals():
     def args(T=100, E=8, k=2, p=None, ws=P, size=1 << 30):
         return (T, E, k, *(p or [P] * 8), ws, size, None)
-    for kw in (dict(T=-1), dict(E=0), dict(E=1025), dict(k=0), dict(k=9), dict(E=64, k=33), dict(T=1 << 30, k=4)):
+    for kw in (dict(T=-1), dict(E=0), dict(E=1025), dict(k=0), dict(k=9), dict(E=64, k=33), dict(T=1 << 30, k=4), dict(T=2 ** 31 - 1, k=1)):
         refused("tagi_route_fwd", *args(**kw))
     for i in range(8):
         if i != 1:      # the variances may be NULL
@@ -113,7 +118,8 @@ def test_grouped_linear_refusals():
 @pytest.mark.parametrize("name, ptrs, optional", [("tagi_combine_fwd", 7, ()), ("tagi_combine_bwd", 10, (3,)),
                                                   ("tagi_dispatch_bwd", 6, (1,))])
 def test_combine_refusals(name, ptrs, optional):
-    for T, k, N, S in ((-1, 2, 8, 8), (4, 0, 8, 8), (4, 2, 0, 8), (4, 2, 8, -1), (1 << 30, 4, 8, 8)):
+    for T, k, N, S in ((-1, 2, 8, 8), (4, 0, 8, 8), (4, 2, 0, 8), (4, 2, 8, -1), (1 << 30, 4, 8, 8), (2 ** 31 - 1, 1, 8, 8),
+                       (4, 2, 2 ** 31 - 1, 8)):
         refused(name, T, k, N, S, *[P] * ptrs, None)
     for i in range(ptrs):
         if i not in optional:
@@ -137,6 +143,35 @@ def test_tensor_functions_refuse_what_the_kernels_cannot_read():
         ops.grouped_linear(z(8, 8), z(8, 8), None, None, z(4, 8), z(4, 8), z(3, dtype=torch.int32))
     with pytest.raises(ValueError):
         ops.combine(z(4, 2, dtype=torch.int32), z(4, 2), z(4, 2), z(8, 8), z(8, 8))
+
+
+def test_tensor_functions_refuse_sizes_that_32_bits_do_not_hold():
+    class Long:       # what the checks look at of a tensor that no test could allocate
+        def __init__(self, *shape):
+            self.shape = shape
+
+        def dim(self):
+            return len(self.shape)
+
+        def get_device(self):
+            return 0
+
+        def numel(self):
+            n = 1
+            for s in self.shape:
+                n *= s
+            return n
+    z, long = torch.zeros, 2 ** 32 + 4
+    for call in (lambda: ops.layer_norm(z(8), z(8), None, None, Long(long, 8), None),
+                 lambda: ops.route(Long(long, 8), None, 2),
+                 lambda: ops.grouped_linear(Long(2, 8, 8), None, None, None, Long(long, 8), None, None),
+                 lambda: ops.grouped_linear(Long(2, 8, 8), None, None, None, z(4, 8), None, None, Long(long)),
+                 lambda: ops.grouped_linear_state(Long(2, 8, 8), None, Long(long, 8), None, None),
+                 lambda: ops.grouped_linear_param(Long(2, 8, 8), None, z(4, 8), Long(long, 8), None, None),
+                 lambda: ops.combine(Long(4, 2), None, None, Long(long, 8), None),
+                 lambda: ops.dispatch_backward(Long(long, 1), None, Long(4, 8), None)):
+        with pytest.raises(ValueError, match="2\\^31"):
+            call()
 
 
 def test_empty_calls_touch_nothing():

@@ -20,6 +20,14 @@ def lib():
     return lib
 
 
+@pytest.fixture(autouse=True)
+def no_wait_ran_out(lib):
+    """The tensor-core kernels give a wait up after a second and leave a word about it: none may have."""
+    from cutagi_b200 import capi
+    yield
+    assert capi.tc_status() == 0
+
+
 class Guard:
     """An output with sentinels around it (and in it, until it is written)."""
 
@@ -182,10 +190,22 @@ def check_route(lib, ms, vs, k):
 
 
 @pytest.mark.parametrize("T", [1, 31, 32, 33, 300, 5001])
-@pytest.mark.parametrize("E, k", [(1, 1), (2, 2), (8, 2), (32, 4), (33, 1), (128, 8), (129, 5), (512, 3), (513, 2), (1000, 32), (1024, 1)])
+@pytest.mark.parametrize("E, k", [(1, 1), (2, 2), (8, 2), (32, 4), (33, 1), (128, 8), (129, 5), (512, 3), (513, 2), (1000, 32), (1024, 1),
+                                  (64, 8), (60, 16), (100, 9), (250, 12), (128, 17), (256, 20), (400, 8)])
 def test_route(lib, T, E, k):
     g = Gen(T * 1000 + E)
     check_route(lib, g.n(T, E, scale=2.0), g.u(T, E), k)
+
+
+def test_route_of_unaligned_scores(lib):
+    g = Gen(8, misalign=1)
+    check_route(lib, g.n(500, 64), g.u(500, 64), 4)
+
+
+@pytest.mark.parametrize("E, k", [(16, 3), (128, 8), (130, 12), (64, 20), (600, 5)])
+def test_route_ties(lib, E, k):
+    g = Gen(E)
+    check_route(lib, torch.round(g.n(301, E)), g.u(301, E), k)
 
 
 @pytest.mark.parametrize("T", [20, 700])
@@ -276,6 +296,128 @@ def test_grouped_linear(lib, counts, K, N, bias, gather, misalign, lead, tail):
             R.check(name, o[i].get(), ref[i], R.sum_tol(max(counts)))
         else:
             assert bool((o[i].get(whole=False) == SENT).all())
+
+
+# experts on both sides of every border between the kernels (8, 20 and 48 rows) and of the widest tile (256), with rows that
+# are aligned to 16 bytes in both, one or none of the two directions
+@pytest.mark.parametrize("counts", [[8, 9, 20, 21, 48, 49, 0, 16, 17], [255, 256, 257, 512, 513, 3], [64, 65, 96, 33, 32, 31]])
+@pytest.mark.parametrize("K, N", [(260, 132), (130, 67), (516, 1031), (129, 300)])
+@pytest.mark.parametrize("bias, gather, misalign, lead, tail", [(True, True, 0, 1, 2), (True, False, 0, 0, 0)])
+def test_grouped_linear_at_the_kernels_borders(lib, counts, K, N, bias, gather, misalign, lead, tail):
+    test_grouped_linear(lib, counts, K, N, bias, gather, misalign, lead, tail)
+
+
+@pytest.mark.parametrize("few, some", [(1, 64), (9, 30), (0, 70)])
+def test_grouped_linear_of_1024_experts(lib, few, some):
+    counts = [few] * 1024
+    for e in (0, 31, 32, 500, 1023):
+        counts[e] = some
+    test_grouped_linear(lib, counts, 68, 40, True, True, 0, 0, 3)
+
+
+def test_grouped_linear_of_many_tiles(lib):
+    """More tiles than CTA pairs, so that each takes several in a row: of both kinds, many widths, all the experts' biases."""
+    test_grouped_linear(lib, [1500, 0, 333, 2100, 7, 30, 900], 1100, 1030, True, True, 0, 0, 0)
+    test_grouped_linear(lib, [40] * 30, 700, 2060, True, False, 0, 0, 0)
+
+
+def big(*shape):
+    if torch.cuda.mem_get_info()[0] < 64 << 30:
+        pytest.skip("needs 64 GB of device memory")
+    return torch.zeros(*shape, device="cuda")
+
+
+@pytest.mark.parametrize("K, N", [(64, 4096), (4096, 64)])
+def test_grouped_linear_row_offsets_past_32_bits(lib, K, N):
+    g, counts = Gen(K), [7, 40, 250]
+    S = 2 ** 19 + 300
+    offsets, S = spread(counts, S - sum(counts))
+    r0 = S - sum(counts)
+    s = K ** -0.5
+    mw, vw, vb = g.n(3, N, K, scale=s), g.u(3, N, K, hi=s * s), g.u(3, N)
+    a, va, dm, dv = (big(S, n) for n in (K, K, N, N))
+    for t in (a, va, dm, dv):
+        t[r0:] = g.u(S - r0, t.shape[1])
+    from cutagi_b200 import ops
+    live = (offsets - r0).to(i32)
+    z, vz = ops.grouped_linear(mw, vw, None, None, a, va, offsets)
+    ref = R.grouped_fwd(mw, vw, None, None, a[r0:], va[r0:], live, None)
+    R.check("mu_z", z[r0:], ref[0], R.sum_tol(K))
+    R.check("var_z", vz[r0:], ref[1], R.sum_tol(2 * K))
+    del z, vz, va
+    da, dva = ops.grouped_linear_state(mw, None, dm, dv, offsets)
+    ref = R.grouped_state(mw, None, dm[r0:], dv[r0:], live)
+    R.check("dmu_a", da[r0:], ref[0], R.sum_tol(N))
+    R.check("dvar_a", dva[r0:], ref[1], R.sum_tol(N))
+    del da, dva
+    got = ops.grouped_linear_param(vw, vb, a, dm, dv, offsets)
+    for name, x, pair in zip(("dmu_w", "dvar_w", "dmu_b", "dvar_b"), got, R.grouped_param(vw, vb, a[r0:], dm[r0:], dv[r0:], live, None)):
+        R.check(name, x, pair, R.sum_tol(max(counts)))
+    del a, dm, dv
+    torch.cuda.empty_cache()
+
+
+def test_grouped_linear_weight_offsets_past_32_bits(lib):
+    from cutagi_b200 import ops
+    E, K, N = 516, 2048, 2048
+    g, counts = Gen(2), [0] * (E - 3) + [5, 40, 60]
+    offsets, S = spread(counts)
+    mw, vw = big(E, N, K), big(E, N, K)
+    s = K ** -0.5
+    mw[-3:], vw[-3:] = g.n(3, N, K, scale=s), g.u(3, N, K, hi=s * s)
+    a, va, dm, dv = g.n(S, K), g.u(S, K), g.n(S, N), g.u(S, N)
+    z, vz = ops.grouped_linear(mw, vw, None, None, a, va, offsets)
+    da, dva = ops.grouped_linear_state(mw, None, dm, dv, offsets)
+    last = offsets[-4:]
+    ref = (*R.grouped_fwd(mw[-3:], vw[-3:], None, None, a, va, last, None), *R.grouped_state(mw[-3:], None, dm, dv, last))
+    for name, x, pair, L in zip(("mu_z", "var_z", "dmu_a", "dvar_a"), (z, vz, da, dva), ref, (K, 2 * K, N, N)):
+        R.check(name, x, pair, R.sum_tol(L))
+    del mw
+    got = ops.grouped_linear_param(vw, None, a, dm, dv, offsets)
+    for name, x, pair in zip(("dmu_w", "dvar_w"), got, R.grouped_param(vw[-3:], None, a, dm, dv, last, None)):
+        R.check(name, x[-3:], pair, R.sum_tol(max(counts)))
+        assert not bool(x[:-3].any())
+    del got, vw
+    torch.cuda.empty_cache()
+
+
+def test_row_offsets_past_32_bits(lib):
+    """LayerNorm and the combination with rows that begin behind 2^31 floats."""
+    from cutagi_b200 import ops
+    g, n, live = Gen(4), 4096, 40
+    rows = 2 ** 19 + live
+    a, va = big(rows, n), big(rows, n)
+    a[-live:], va[-live:] = g.n(live, n), g.u(live, n)
+    mw, vw, mb, vb = ln_params(g, n, True)
+    z, vz, m, v = ops.layer_norm(mw, vw, mb, vb, a, va, EPS)
+    for name, x, pair in zip(("mu_z", "var_z", "mu_row", "var_row"), (z, vz, m, v), R.ln_fwd(mw, vw, mb, vb, a[-live:], va[-live:], C.c_float(EPS).value)):
+        R.check(name, x[-live:], pair, R.U)
+    z.zero_(), vz.zero_()
+    z[-live:], vz[-live:] = g.n(live, n), g.u(live, n)
+    got = ops.layer_norm_backward(mw, vw, vb, a, None, m, v, z, vz, EPS)
+    ref = R.ln_bwd(mw, vw, vb, a[-live:], None, m[-live:], v[-live:], z[-live:], vz[-live:], C.c_float(EPS).value)
+    for i, name in enumerate(("dmu", "dvar", "dmu_w", "dvar_w", "dmu_b", "dvar_b")):   # the other rows' deltas are zero
+        R.check(name, got[i][-live:] if i < 2 else got[i], ref[i], R.sum_tol(live if i >= 2 else 1))
+    del got, z, vz
+    torch.cuda.empty_cache()
+    pos = torch.tensor([[rows - 1, 3], [rows - 2, rows - 30]], dtype=i32, device="cuda")
+    mg, vg, dm, dv = g.u(2, 2), g.u(2, 2), g.n(2, n), g.u(2, n)
+    few = torch.where(pos >= live, pos - (rows - live), -1)
+    y = ops.combine(pos, mg, vg, a, va)
+    for x, pair in zip(y, R.combine_fwd(few, mg, vg, a[-live:], va[-live:])):
+        R.check("combine", x, pair, 12 * R.U)
+    d = ops.dispatch_backward(pos, None, a, va)
+    for x, pair in zip(d, R.dispatch_bwd(few, None, a[-live:], va[-live:])):
+        R.check("dispatch", x, pair, 12 * R.U)
+    got = ops.combine_backward(pos, mg, a, None, dm, dv)
+    ref = R.combine_bwd(few, mg, a[-live:], None, dm, dv)
+    for x, (want, M) in zip(got[:2], ref[:2]):
+        named = ~torch.isnan(want[:, 0])
+        R.check("rows", x[-live:][named], (want[named], M[named]), 8 * R.U)
+    for x, (want, M) in zip(got[2:], ref[2:]):      # slot (0, 1) names row 3, which is zero
+        R.check("gates", x, (want, M), R.sum_tol(n))
+    del a, va, got
+    torch.cuda.empty_cache()
 
 
 def test_grouped_linear_without_rows(lib):
