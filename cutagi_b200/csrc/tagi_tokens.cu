@@ -3,6 +3,8 @@
 // HBM-bound: every tensor is read or written once.
 #include "tagi_common.h"
 
+#include <type_traits>
+
 namespace tagi {
 namespace {
 
@@ -345,10 +347,11 @@ struct CombineBwdArgs {
 
 // TPR threads per token: the deltas of the slots' rows, and for each slot the sums of x dmu_y and x^2 dvar_y over the features.
 // Four slots at a time, so that their rows are fetched together and the token's deltas once.
-template <int W, int TPR>
-__global__ void __launch_bounds__(256) combine_bwd_kernel(const CombineBwdArgs a) {
-    __shared__ float red[8][2 * SLOTS];
-    const long t = (long)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+template <int W, int TPR, bool JCB>
+__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) combine_bwd_kernel(const CombineBwdArgs a) {
+    constexpr int THREADS = TPR == 32 ? 256 : TPR;
+    __shared__ float red[TPR / 32][2 * SLOTS];
+    const long t = (long)blockIdx.x * (THREADS / TPR) + threadIdx.x / TPR;
     const int u = threadIdx.x % TPR;
     if (TPR == 32 && t >= a.T) return;   // wider: the grid has one CTA per token
     for (int j0 = 0; j0 < a.k; j0 += SLOTS) {
@@ -374,7 +377,7 @@ __global__ void __launch_bounds__(256) combine_bwd_kernel(const CombineBwdArgs a
                 for (int j = 0; j < SLOTS; j++)
                     if (p[j] >= 0) {
                         load<W>(a.mu_x + (long)p[j] * a.N + i, x[h][j]);
-                        if (a.jcb) load<W>(a.jcb + (long)p[j] * a.N + i, q[h][j]);
+                        if (JCB) load<W>(a.jcb + (long)p[j] * a.N + i, q[h][j]);
                     }
             }
 #pragma unroll
@@ -387,7 +390,7 @@ __global__ void __launch_bounds__(256) combine_bwd_kernel(const CombineBwdArgs a
                         float o[W], r[W];
 #pragma unroll
                         for (int c = 0; c < W; c++) {
-                            const float f = a.jcb ? g[j] * q[h][j][c] : g[j];
+                            const float f = JCB ? g[j] * q[h][j][c] : g[j];
                             s[2 * j] += x[h][j][c] * dm[h][c];
                             s[2 * j + 1] += x[h][j][c] * dv[h][c] * x[h][j][c];
                             o[c] = f * dm[h][c];
@@ -411,7 +414,7 @@ __global__ void __launch_bounds__(256) combine_bwd_kernel(const CombineBwdArgs a
             float v = 0.f;
             if (TPR > 32) {
 #pragma unroll
-                for (int w = 0; w < 8; w++) v += red[w][u];
+                for (int w = 0; w < TPR / 32; w++) v += red[w][u];
             } else {
 #pragma unroll
                 for (int q = 0; q < 2 * SLOTS; q++)
@@ -576,13 +579,19 @@ int tagi_combine_bwd(int T, int k, int N, int S, const int *pos, const float *mu
     TAGI_PTR(dvar_g);
     TAGI_REQUIRE(jcb == nullptr || aligned4(jcb), "jcb is not 4-byte aligned");
     const CombineBwdArgs a{T, k, N, S, pos, mu_g, mu_x, jcb, dmu_y, dvar_y, dmu_x, dvar_x, dmu_g, dvar_g};
-    // a warp per token while a row is at most eight of its strides long, else a CTA
+    // A warp per token up to two of its strides, else a CTA of 128: 8192 tokens, four rows of 1024: 79 us (a warp 85 us, a CTA
+    // of 256 threads 85 us); 16384 tokens, two rows of 2048: 184 us (197 and 195 us).
     const bool vec = N % 4 == 0 && all16({mu_x, jcb, dmu_y, dvar_y, dmu_x, dvar_x});
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (vec && N > 1024) combine_bwd_kernel<4, 256><<<T, 256, 0, st>>>(a);
-    else if (vec) combine_bwd_kernel<4, 32><<<(T + 7) / 8, 256, 0, st>>>(a);
-    else if (N > 512) combine_bwd_kernel<1, 256><<<T, 256, 0, st>>>(a);
-    else combine_bwd_kernel<1, 32><<<(T + 7) / 8, 256, 0, st>>>(a);
+    auto start = [&](auto with) {
+        constexpr bool J = decltype(with)::value;
+        if (vec && N > 256) combine_bwd_kernel<4, 128, J><<<T, 128, 0, st>>>(a);
+        else if (vec) combine_bwd_kernel<4, 32, J><<<(T + 7) / 8, 256, 0, st>>>(a);
+        else if (N > 128) combine_bwd_kernel<1, 128, J><<<T, 128, 0, st>>>(a);
+        else combine_bwd_kernel<1, 32, J><<<(T + 7) / 8, 256, 0, st>>>(a);
+    };
+    if (jcb) start(std::true_type());
+    else start(std::false_type());
     return launched("combine_bwd_kernel launch");
 }
 

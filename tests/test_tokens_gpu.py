@@ -553,6 +553,13 @@ def _expert_inputs(seed, T=200, E=6, K=96, N=128):
                 a=g.n(T, K), va=g.u(T, K), g=g.n(N), vg=g.u(N), dm=g.n(T, N), dv=g.u(T, N, lo=-1.0, hi=0.0))
 
 
+def test_no_tokens_at_all(lib):
+    from cutagi_b200 import ops
+    out = _expert_layer(ops, _expert_inputs(1, T=0))
+    assert [tuple(t.shape) for t in out[:6]] == [(0, 128), (0, 128), (128,), (128,), (0, 6), (0, 6)]
+    assert all(not bool(t.any()) for t in out)      # parameter deltas of no tokens are zero
+
+
 def test_results_repeat_bit_for_bit(lib):
     from cutagi_b200 import ops
     x = _expert_inputs(1)
