@@ -18,25 +18,41 @@ namespace {
 constexpr int OUT = 64, SLAB = 32, WARPS = 8, THREADS = WARPS * 32, ROWS = FEW_ROWS;
 static_assert(SLAB == 4 * WARPS, "a warp takes four steps of a slab");
 constexpr int PITCH = SLAB + 4;                          // floats of a weight row in shared memory: no bank conflicts
-constexpr int FWD_WEIGHTS = 2 * OUT * PITCH, STATE_WEIGHTS = SLAB * OUT;
+constexpr int FWD_WEIGHTS = 2 * OUT * PITCH;
+// Rows that do not begin at multiples of 16 bytes are copied in the 16-byte groups of memory all the same, one more of them,
+// and begin up to three floats behind their place in shared memory. One row of two experts of 4095 x 4095, forward: 74 us,
+// with 4-byte copies 94 us; of 4096 x 4096 55 us.
+__host__ __device__ constexpr int state_pitch(bool vec) { return vec ? OUT : OUT + 4; }
+__host__ __device__ constexpr int weights(int pass, bool vec) { return pass == FWD ? FWD_WEIGHTS : SLAB * state_pitch(vec); }
 __host__ __device__ constexpr int stages(int pass) { return pass == FWD ? 4 : 8; }   // a slab of both is 18 KiB, of means 8
 
 __device__ __forceinline__ uint32_t smem_at(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
-// Four floats to shared memory, of which the first `valid` (any number, also none or more than four) exist; zeros else.
-template <bool VEC>
-__device__ __forceinline__ void copy4(float *dst, const float *src, int valid) {
-    const uint32_t d = smem_at(dst);
-    if (VEC) {
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(valid > 0 ? 16 : 0) : "memory");
-    } else {
-#pragma unroll
-        for (int c = 0; c < 4; c++)
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(d + c * 4), "l"(src + (c < valid ? c : 0)), "r"(c < valid ? 4 : 0)
-                         : "memory");
-    }
+// floats of p's 16-byte group of memory before p
+__device__ __forceinline__ int shift_of(const float *p) { return (int)((unsigned long long)p >> 2) & 3; }
+// The 16-byte group of memory at src, of whose floats `left` lie before the row's end; zeros behind it.
+__device__ __forceinline__ void copy_group(float *dst, const float *src, int left) {
+    if (left > 0)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_at(dst)), "l"(src), "r"(left < 4 ? left * 4 : 16) : "memory");
+    else
+        *reinterpret_cast<float4 *>(dst) = make_float4(0.f, 0.f, 0.f, 0.f);
+}
+__device__ __forceinline__ void copy_float(float *dst, const float *src, bool in) {
+    if (in) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_at(dst)), "l"(src) : "memory");
+    else *dst = 0.f;
+}
+// A group that begins before its tensor does, `before` floats: only the floats of the tensor.
+__device__ __forceinline__ void copy_first_group(float *dst, const float *src, int before, int left) {
+    for (int c = before; c < 4; c++) copy_float(dst + c, src + c, c < left);
 }
 __device__ __forceinline__ float4 at4(const float *p) { return *reinterpret_cast<const float4 *>(p); }
+// four floats from p + shift on, p aligned
+__device__ __forceinline__ float4 at4(const float *p, int shift) {
+    const float4 a = at4(p), b = at4(p + 4);
+    const bool one = shift & 1, two = shift & 2;
+    const float x = one ? a.y : a.x, y = one ? a.z : a.y, z = one ? a.w : a.z, w = one ? b.x : a.w, u = one ? b.y : b.x, v = one ? b.z : b.y;
+    return make_float4(two ? z : x, two ? w : y, two ? u : z, two ? v : w);
+}
 
 // Two contraction steps of a sum in one register pair: two multiply-adds are one instruction.
 typedef unsigned long long Pair;
@@ -73,67 +89,130 @@ __device__ __forceinline__ float sum_of(Pair p) {
 // smem: a ring of stages of weights and rows, used again for the warps' sums.
 template <int PASS, bool VEC>
 __device__ __forceinline__ void few_rows_pass(const GroupedArgs &a, int e, int r0, int rows, float *smem) {
-    constexpr int WEIGHTS = PASS == FWD ? FWD_WEIGHTS : STATE_WEIGHTS, STAGE = WEIGHTS + 2 * ROWS * SLAB, STAGES = stages(PASS);
+    constexpr int WEIGHTS = weights(PASS, VEC), SP = state_pitch(VEC), STAGE = WEIGHTS + 2 * ROWS * SLAB, STAGES = stages(PASS);
     const int tid = threadIdx.x, lane = tid & 31, q = tid >> 5;   // q: the warp, and its four steps of a slab
     const int o0 = blockIdx.x * OUT, outs = PASS == FWD ? a.N : a.K, depth = PASS == FWD ? a.K : a.N;
     const size_t wbase = (size_t)e * a.N * a.K;
 
-    // this thread's copy of the rows: quad tid & 7 of row (tid >> 3) % ROWS, means first
-    static_assert(2 * ROWS * 8 <= THREADS, "one copy a thread");
-    const int mine = tid < 2 * ROWS * 8 && (tid >> 3) % ROWS < rows ? r0 + (tid >> 3) % ROWS : -1;
-    const int row = mine < 0 ? -1 : PASS == FWD ? input_row(a, mine) : mine;
-    auto fetch = [&](int slab, int last) {
+    // this CTA's slabs of the cluster's
+    const int parts = gridDim.z, all = (depth + SLAB - 1) / SLAB, first = (int)((long)all * blockIdx.z / parts),
+              last = (int)((long)all * (blockIdx.z + 1) / parts);
+
+    // What this thread copies of a slab, as addresses that move on by a slab each time (working them out anew took more
+    // instructions than all else). Weights: forward, group tid & 7 of lines n and n + 32 of both tensors; state, group tid & 15
+    // of lines n and n + 16. Lines that are so far apart begin equally far from a multiple of 16 bytes. Where that is not zero
+    // a line has one more group, `more`.
+    constexpr int FAR = PASS == FWD ? 32 : 16, GROUPS = PASS == FWD ? 8 : 16;
+    const int n = tid / GROUPS, g = (tid % GROUPS) * 4;
+    const size_t far = (size_t)FAR * a.K, move = PASS == FWD ? SLAB : (size_t)SLAB * a.K;
+    const float *pm = a.mu_w + wbase + (PASS == FWD ? (size_t)(o0 + n) * a.K + first * SLAB : (size_t)(first * SLAB + n) * a.K + o0), *pv = nullptr;
+    int at = PASS == FWD ? first * SLAB : o0;   // place of the slab's first column in its line
+    const int sm = VEC ? 0 : shift_of(pm);
+    int sv = 0;
+    pm += g - sm;
+    if (PASS == FWD) {
+        pv = a.var_w + wbase + (size_t)(o0 + n) * a.K + first * SLAB;
+        sv = VEC ? 0 : shift_of(pv);
+        pv += g - sv;
+    }
+    const int extra = PASS == FWD ? tid & (OUT - 1) : tid;   // the line whose last group this thread copies: forward, of means, then of variances
+    const bool has_extra = !VEC && (PASS == FWD ? tid < 2 * OUT && o0 + extra < a.N : tid < SLAB);
+    const float *more = nullptr;
+    int se = 0;
+    if (!VEC) {
+        more = (PASS == FWD && tid >= OUT ? a.var_w : a.mu_w) + wbase +
+               (PASS == FWD ? (size_t)(o0 + extra) * a.K + first * SLAB : (size_t)(first * SLAB + extra) * a.K + o0);
+        se = shift_of(more);
+        more += GROUPS * 4 - se;
+    }
+    const bool tensor_begins = !VEC && blockIdx.y == 0 && n == 0 && g == 0 && o0 == 0 && first == 0;   // its first group may begin before it
+
+    // and of the rows: four entries (VEC: threads of means, then of variances), or one of both
+    const int t = VEC ? (tid >> 3) % ROWS : tid >> 5, tk = VEC ? (tid & 7) * 4 : lane;
+    const bool mine = t < rows && (!VEC || tid < 2 * ROWS * 8);
+    const int row = !mine ? -1 : PASS == FWD ? input_row(a, r0 + t) : r0 + t;
+    const size_t row_at = (size_t)max(row, 0) * depth + first * SLAB + tk;
+    const float *px = (VEC && tid >= ROWS * 8 ? a.a1 : a.a0) + row_at, *py = a.a1 + row_at;
+    auto fetch = [&](int slab) {
         const int k0 = slab * SLAB;
         float *s = smem + (slab % STAGES) * STAGE;
         if (slab < last) {
             if (PASS == FWD) {
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int c = tid + (i & 1) * THREADS, n = c >> 3, k = k0 + (c & 7) * 4;
-                    copy4<VEC>(s + (i >> 1) * OUT * PITCH + n * PITCH + (c & 7) * 4,
-                               (i < 2 ? a.mu_w : a.var_w) + (o0 + n < a.N ? wbase + (size_t)(o0 + n) * a.K + (k < a.K ? k : 0) : 0),
-                               o0 + n < a.N ? a.K - k : 0);
+                const bool in = o0 + n < a.N, in_far = o0 + n + FAR < a.N;
+                const int lm = a.K - at + sm - g, lv = a.K - at + sv - g;
+                float *d = s + n * PITCH + g;
+                if (in) {
+                    if (tensor_begins && slab == 0 && (sm | sv) != 0) {
+                        copy_first_group(d, pm, sm, lm);
+                        copy_first_group(d + OUT * PITCH, pv, sv, lv);
+                    } else {
+                        copy_group(d, pm, lm);
+                        copy_group(d + OUT * PITCH, pv, lv);
+                    }
                 }
+                if (in_far) {
+                    copy_group(d + FAR * PITCH, pm + far, lm);
+                    copy_group(d + (OUT + FAR) * PITCH, pv + far, lv);
+                }
+                if (has_extra) copy_group(s + (tid >> 6) * OUT * PITCH + extra * PITCH + GROUPS * 4, more, a.K - at + se - GROUPS * 4);
+                at += SLAB, pv += move;
             } else {
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const int c = tid + i * THREADS, n = k0 + (c >> 4), k = o0 + (c & 15) * 4;
-                    copy4<VEC>(s + (c >> 4) * OUT + (c & 15) * 4, a.mu_w + (n < a.N ? wbase + (size_t)n * a.K + (k < a.K ? k : 0) : 0),
-                               n < a.N ? a.K - k : 0);
-                }
+                const int lm = a.K - at + sm - g, le = a.K - at + se - GROUPS * 4;   // a column behind the end: whatever, but for zeros in lines behind the last
+                float *d = s + n * SP + g;
+                if (tensor_begins && slab == 0 && sm != 0) copy_first_group(d, pm, sm, lm);
+                else copy_group(d, pm, k0 + n < a.N ? lm : 0);
+                copy_group(d + FAR * SP, pm + far, k0 + n + FAR < a.N ? lm : 0);
+                if (has_extra) copy_group(s + extra * SP + GROUPS * 4, more, k0 + extra < a.N ? le : 0);
             }
-            if (tid < 2 * ROWS * 8) {
-                const int k = k0 + (tid & 7) * 4;
-                copy4<VEC>(s + WEIGHTS + tid * 4, (tid < ROWS * 8 ? a.a0 : a.a1) + (row >= 0 && k < depth ? (size_t)row * depth + k : 0),
-                           row >= 0 ? depth - k : 0);
+            pm += move;
+            if (!VEC) more += move;
+            if (mine) {
+                const bool in = row >= 0 && k0 + tk < depth;
+                if (VEC) {
+                    copy_group(s + WEIGHTS + tid * 4, px, in ? 4 : 0);
+                } else {
+                    copy_float(s + WEIGHTS + t * SLAB + lane, px, in);
+                    copy_float(s + WEIGHTS + (ROWS + t) * SLAB + lane, py, in);
+                    py += SLAB;
+                }
+                px += SLAB;
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
+    // shifts of what this thread reads, the same in all slabs (32 floats apart, or 32 rows): forward pass, its two columns' means
+    // and variances; state pass, its four steps
+    int shift[2][2] = {};
+    if (!VEC) {
+#pragma unroll
+        for (int f = 0; f < 2; f++)
+#pragma unroll
+            for (int v = 0; v < 2; v++)
+                shift[f][v] = PASS == FWD ? shift_of((v ? a.var_w : a.mu_w) + wbase + (size_t)(o0 + f * 32 + lane) * a.K)
+                                          : shift_of(a.mu_w + wbase + (size_t)(q * 4 + f * 2 + v) * a.K);
+    }
     Pair z[2][ROWS], vz[2][ROWS];
 #pragma unroll
     for (int t = 0; t < ROWS; t++) z[0][t] = z[1][t] = vz[0][t] = vz[1][t] = 0;
-    // this CTA's slabs of the cluster's
-    const int parts = gridDim.z, all = (depth + SLAB - 1) / SLAB, first = (int)((long)all * blockIdx.z / parts),
-              last = (int)((long)all * (blockIdx.z + 1) / parts);
 #pragma unroll
-    for (int s = 0; s < STAGES - 1; s++) fetch(first + s, last);
+    for (int s = 0; s < STAGES - 1; s++) fetch(first + s);
     for (int it = first; it < last; it++) {
         asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
         __syncthreads();   // slab `it` is there for all, and nobody reads the stage that is filled next any more
-        fetch(it + STAGES - 1, last);
+        fetch(it + STAGES - 1);
         const float *w = smem + (it % STAGES) * STAGE, *x = w + WEIGHTS, *y = x + ROWS * SLAB;
         {
             Pair wm[2][2], wq[2][2], wv[2][2];   // the thread's two columns at four steps: means, their squares, variances
 #pragma unroll
             for (int f = 0; f < 2; f++) {
                 if (PASS == FWD) {
-                    const float4 m = at4(w + (f * 32 + lane) * PITCH + q * 4), v = at4(w + OUT * PITCH + (f * 32 + lane) * PITCH + q * 4);
+                    const float *p = w + (f * 32 + lane) * PITCH + q * 4;
+                    const float4 m = VEC ? at4(p) : at4(p, shift[f][0]), v = VEC ? at4(p + OUT * PITCH) : at4(p + OUT * PITCH, shift[f][1]);
                     wm[f][0] = pair_of(m.x, m.y), wm[f][1] = pair_of(m.z, m.w);
                     wv[f][0] = pair_of(v.x, v.y), wv[f][1] = pair_of(v.z, v.w);
                 } else {
-                    const float *p = w + q * 4 * OUT + f * 32 + lane;
-                    wm[f][0] = pair_of(p[0], p[OUT]), wm[f][1] = pair_of(p[2 * OUT], p[3 * OUT]);
+                    const float *p = w + q * 4 * SP + f * 32 + lane;
+                    wm[f][0] = pair_of(p[shift[0][0]], p[SP + shift[0][1]]), wm[f][1] = pair_of(p[2 * SP + shift[1][0]], p[3 * SP + shift[1][1]]);
                 }
                 wq[f][0] = mul2(wm[f][0], wm[f][0]), wq[f][1] = mul2(wm[f][1], wm[f][1]);
             }
@@ -198,32 +277,35 @@ __global__ void __launch_bounds__(THREADS, 2) grouped_few_kernel(const GroupedAr
 }
 
 // -------------------------------------------------------------------------------------------------------- parameters
-// A warp computes PARAM_N output features x 32 lanes of W input features; a CTA stacks 8 warps along the output features. The
+// A warp computes PARAM_N output features x 32 lanes of four input features (neighbours, or 32 apart where rows are not aligned: two a lane were slower from eight rows on); a CTA stacks 8 warps along the output features. The
 // prior variances are fetched before the rows are added up; the deltas come from shared memory, at one address for all lanes.
 constexpr int PARAM_N = 8, PARAM_OUT = WARPS * PARAM_N;
 
-template <int W>
-__device__ __forceinline__ void load(const float *p, float (&v)[W]) {
-    if (W == 4) {
+// Four entries of a row, of which `left` follow from p on: neighbours (VEC: at least one is left), or 32 apart.
+template <bool VEC>
+__device__ __forceinline__ void load(const float *p, int left, float (&v)[4]) {
+    if (VEC) {
         const float4 t = __ldg(reinterpret_cast<const float4 *>(p));
-        v[0] = t.x, v[1 % W] = t.y, v[2 % W] = t.z, v[3 % W] = t.w;
+        v[0] = t.x, v[1] = t.y, v[2] = t.z, v[3] = t.w;
     } else {
-        v[0] = __ldg(p);
+#pragma unroll
+        for (int c = 0; c < 4; c++) v[c] = c * 32 < left ? __ldg(p + c * 32) : 0.f;
     }
 }
 
 // weights pass by once: they are kept out of L1, where the rows are wanted
-template <int W>
-__device__ __forceinline__ void load_once(const float *p, float (&v)[W]) {
-    if (W == 4)
-        asm volatile("ld.global.nc.L1::no_allocate.v4.f32 {%0, %1, %2, %3}, [%4];"
-                     : "=f"(v[0]), "=f"(v[1 % W]), "=f"(v[2 % W]), "=f"(v[3 % W])
-                     : "l"(p));
-    else
-        asm volatile("ld.global.nc.L1::no_allocate.f32 %0, [%1];" : "=f"(v[0]) : "l"(p));
+template <bool VEC>
+__device__ __forceinline__ void load_once(const float *p, int left, float (&v)[4]) {
+    if (VEC) {
+        asm volatile("ld.global.nc.L1::no_allocate.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "l"(p));
+    } else {
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+            if (c * 32 < left) asm volatile("ld.global.nc.L1::no_allocate.f32 %0, [%1];" : "=f"(v[c]) : "l"(p + c * 32));
+    }
 }
 
-template <int W>
+template <bool VEC>
 __global__ void __launch_bounds__(THREADS, 2) grouped_few_param_kernel(const GroupedArgs a) {
     __shared__ __align__(16) float delta[FEW_PARAM_ROWS][2][PARAM_OUT];
     __shared__ int input[FEW_PARAM_ROWS];
@@ -233,15 +315,15 @@ __global__ void __launch_bounds__(THREADS, 2) grouped_few_param_kernel(const Gro
     const int rows = r1 - r0;
     if (rows > a.few) return;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, block_n = blockIdx.y * PARAM_OUT, n0 = block_n + warp * PARAM_N;
-    const int k = (blockIdx.x * 32 + lane) * W;
-    const bool live = k < a.K;
+    constexpr int W = 4;
+    const int k = blockIdx.x * 32 * W + (VEC ? lane * 4 : lane), left = a.K - k;
     float d[PARAM_N][W], v[PARAM_N][W], s[PARAM_N][W];
     const size_t o = ((size_t)e * a.N + n0) * a.K + k;
 #pragma unroll
     for (int i = 0; i < PARAM_N; i++) {
 #pragma unroll
         for (int c = 0; c < W; c++) d[i][c] = v[i][c] = s[i][c] = 0.f;
-        if (live && rows > 0 && n0 + i < a.N) load_once<W>(a.var_w + o + (size_t)i * a.K, s[i]);
+        if ((!VEC || left > 0) && rows > 0 && n0 + i < a.N) load_once<VEC>(a.var_w + o + (size_t)i * a.K, left, s[i]);
     }
     for (int i = threadIdx.x; i < rows * 2 * PARAM_OUT; i += THREADS) {
         const int n = block_n + i % PARAM_OUT, r = i / (2 * PARAM_OUT);
@@ -258,14 +340,14 @@ __global__ void __launch_bounds__(THREADS, 2) grouped_few_param_kernel(const Gro
             (kind ? a.ob1 : a.ob0)[(size_t)e * a.N + n] = kind ? vb * vb * t : vb * t;
         }
     }
-    if (!live) return;
+    if (left <= 0) return;
 #pragma unroll 2
     for (int r = 0; r < rows; r++) {
         const int row = input[r];
         float x[W], q[W];
 #pragma unroll
         for (int c = 0; c < W; c++) x[c] = 0.f;
-        if (row >= 0) load<W>(a.x + (size_t)row * a.K + k, x);
+        if (row >= 0) load<VEC>(a.x + (size_t)row * a.K + k, left, x);
 #pragma unroll
         for (int c = 0; c < W; c++) q[c] = x[c] * x[c];
 #pragma unroll
@@ -284,19 +366,20 @@ __global__ void __launch_bounds__(THREADS, 2) grouped_few_param_kernel(const Gro
 #pragma unroll
         for (int c = 0; c < W; c++) d[i][c] *= s[i][c], v[i][c] *= s[i][c] * s[i][c];
         float *p = a.o0 + o + (size_t)i * a.K, *u = a.o1 + o + (size_t)i * a.K;
-        if (W == 4) {
-            __stcs(reinterpret_cast<float4 *>(p), make_float4(d[i][0], d[i][1 % W], d[i][2 % W], d[i][3 % W]));
-            __stcs(reinterpret_cast<float4 *>(u), make_float4(v[i][0], v[i][1 % W], v[i][2 % W], v[i][3 % W]));
+        if (VEC) {
+            __stcs(reinterpret_cast<float4 *>(p), make_float4(d[i][0], d[i][1], d[i][2], d[i][3]));
+            __stcs(reinterpret_cast<float4 *>(u), make_float4(v[i][0], v[i][1], v[i][2], v[i][3]));
         } else {
-            __stcs(p, d[i][0]);
-            __stcs(u, v[i][0]);
+#pragma unroll
+            for (int c = 0; c < W; c++)
+                if (c * 32 < left) p[c * 32] = d[i][c], u[c * 32] = v[i][c];
         }
     }
 }
 
 template <int PASS, bool VEC>
 int launch_few(const GroupedArgs &a, cudaStream_t st) {
-    constexpr size_t ring = stages(PASS) * ((PASS == FWD ? FWD_WEIGHTS : STATE_WEIGHTS) + 2 * ROWS * SLAB), sums = WARPS * ROWS * 2 * OUT;
+    constexpr size_t ring = stages(PASS) * (weights(PASS, VEC) + 2 * ROWS * SLAB), sums = WARPS * ROWS * 2 * OUT;
     constexpr size_t smem = (ring > sums ? ring : sums) * sizeof(float);
     // CTAs that have work, at most: with fewer than two for an SM, clusters cut the contraction, into no less than 256 steps
     const int tiles = ((PASS == FWD ? a.N : a.K) + OUT - 1) / OUT, depth = PASS == FWD ? a.K : a.N;
@@ -331,10 +414,9 @@ int grouped_few(int pass, const GroupedArgs &a, cudaStream_t st) {
     if (pass == FWD) return launch<FWD>(a, st);
     if (pass == STATE) return launch<STATE>(a, st);
     const bool vec = a.K % 4 == 0 && aligned16(a.var_w) && aligned16(a.x) && aligned16(a.o0) && aligned16(a.o1);
-    const int per = 32 * (vec ? 4 : 1);
-    const dim3 grid((a.K + per - 1) / per, (a.N + PARAM_OUT - 1) / PARAM_OUT, a.E);
-    if (vec) grouped_few_param_kernel<4><<<grid, THREADS, 0, st>>>(a);
-    else grouped_few_param_kernel<1><<<grid, THREADS, 0, st>>>(a);
+    const dim3 grid((a.K + 127) / 128, (a.N + PARAM_OUT - 1) / PARAM_OUT, a.E);
+    if (vec) grouped_few_param_kernel<true><<<grid, THREADS, 0, st>>>(a);
+    else grouped_few_param_kernel<false><<<grid, THREADS, 0, st>>>(a);
     TAGI_CUDA(cudaGetLastError());
     return TAGI_OK;
 }

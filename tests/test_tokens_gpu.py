@@ -298,6 +298,29 @@ def test_grouped_linear(lib, counts, K, N, bias, gather, misalign, lead, tail):
             assert bool((o[i].get(whole=False) == SENT).all())
 
 
+@pytest.mark.parametrize("counts", [[1, 3], [20, 9], [70, 130]])
+@pytest.mark.parametrize("K, N", [(37, 70), (64, 64)])
+def test_grouped_linear_of_tensors_aligned_differently(lib, counts, K, N):
+    """Each tensor begins at its own distance from a multiple of 16 bytes, behind a NaN."""
+    from cutagi_b200 import ops
+
+    def at(t, off):
+        b = torch.full((t.numel() + 8,), torch.nan, device="cuda")
+        b[off:off + t.numel()] = t.reshape(-1)
+        return b[off:off + t.numel()].reshape(t.shape)
+    g, E = Gen(K), len(counts)
+    offsets, S = spread(counts)
+    for d in range(4):
+        mw, vw, a, va = at(g.n(E, N, K), 1 + d), at(g.u(E, N, K), 1 + (d + 1) % 4), at(g.n(S, K), 1 + (d + 2) % 4), at(g.u(S, K), 2)
+        dm, dv = at(g.n(S, N), 1 + (d + 3) % 4), at(g.u(S, N), 3)
+        got = (*ops.grouped_linear(mw, vw, None, None, a, va, offsets), *ops.grouped_linear_state(mw, None, dm, dv, offsets),
+               *ops.grouped_linear_param(vw, None, a, dm, dv, offsets)[:2])
+        ref = (*R.grouped_fwd(mw, vw, None, None, a, va, offsets, None), *R.grouped_state(mw, None, dm, dv, offsets),
+               *R.grouped_param(vw, None, a, dm, dv, offsets, None))
+        for x, pair, L in zip(got, ref, (K, 2 * K, N, N, max(counts), max(counts))):
+            R.check(f"offset {d}", x, pair, R.sum_tol(L))
+
+
 # experts on both sides of every border between the kernels (8, 20 and 48 rows) and of the widest tile (256), with rows that
 # are aligned to 16 bytes in both, one or none of the two directions
 @pytest.mark.parametrize("counts", [[8, 9, 20, 21, 48, 49, 0, 16, 17], [255, 256, 257, 512, 513, 3], [64, 65, 96, 33, 32, 31]])
@@ -450,10 +473,11 @@ def test_grouped_linear_bad_device_data_stays_in_range(lib, rows):
     R.check("dvar_w", o[1].get(), ref[1], R.sum_tol(rows))
 
 
-@pytest.mark.parametrize("counts", [[2, 3, 1], [40, 170, 90]])
-def test_grouped_linear_rows_of_other_experts_do_not_leak(lib, counts):
+@pytest.mark.parametrize("counts", [[2, 3, 1], [40, 170, 90], [16, 30, 48]])
+@pytest.mark.parametrize("K, N", [(200, 96), (199, 97)])
+def test_grouped_linear_rows_of_other_experts_do_not_leak(lib, counts, K, N):
     """NaN and infinities in one expert's rows, weights and deltas, and in rows that no expert owns, stay there."""
-    g, K, N, E = Gen(9), 200, 96, len(counts)
+    g, E = Gen(9), len(counts)
     offsets, S = spread(counts, 3, 4)
     mw, vw, ma, va = g.n(E, N, K, scale=K ** -0.5), g.u(E, N, K, hi=1.0 / K), g.n(S, K), g.u(S, K)
     dm, dv = g.n(S, N), g.n(S, N)
