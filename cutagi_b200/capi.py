@@ -65,9 +65,9 @@ _SIGNATURES = {
     "tagi_route_fwd": [_i, _i, _i] + [_p] * 9 + [C.c_size_t, _p],
     "tagi_route_bwd": [_i, _i, _i] + [_p] * 7,
     "tagi_grouped_linear_fwd": [_i] * 6 + [_p] * 11 + [C.c_size_t, _p],
-    "tagi_grouped_linear_workspace_bytes": [_i, _i, _i],
-    "tagi_grouped_linear_bwd_state": [_i] * 4 + [_p] * 8,
-    "tagi_grouped_linear_bwd_param": [_i] * 6 + [_p] * 12,
+    "tagi_grouped_linear_workspace_bytes": [_i] * 6,
+    "tagi_grouped_linear_bwd_state": [_i] * 4 + [_p] * 8 + [C.c_size_t, _p],
+    "tagi_grouped_linear_bwd_param": [_i] * 6 + [_p] * 12 + [C.c_size_t, _p],
     "tagi_combine_fwd": [_i] * 4 + [_p] * 8,
     "tagi_combine_bwd": [_i] * 4 + [_p] * 11,
     "tagi_dispatch_bwd": [_i] * 4 + [_p] * 7,

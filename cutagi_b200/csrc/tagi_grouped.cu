@@ -16,14 +16,31 @@ int run(int pass, GroupedArgs &a, cudaStream_t st) {
     return grouped_tc(pass, a, st);
 }
 
+bool sizes_fit(int E, int S, int K, int N) {
+    return E >= 1 && E <= 1024 && S >= 0 && S <= (1 << 28) && K >= 1 && K <= (1 << 20) && N >= 1 && N <= (1 << 20);
+}
+// Workspace: partial sums of the tensor-core kernel, then, forward, mu_a^2 + var_a; nothing where the number of rows in all
+// rules these kernels out.
+size_t parts_bytes(int pass, int E, int S, int K, int N) {
+    return S <= (pass == PARAM ? FEW_PARAM_ROWS : THIN_ROWS) ? 0 : grouped_tc_parts_bytes(pass, E, S, K, N);
+}
+size_t second_bytes(int S, int R, int K) { return S <= FEW_ROWS ? 0 : (size_t)R * K * sizeof(float); }
+
+int check_workspace(const char *who, int pass, const GroupedArgs &a, const void *workspace, size_t bytes) {
+    const size_t need = tagi_grouped_linear_workspace_bytes(pass, a.E, a.S, a.R, a.K, a.N);
+    if (need > 0 && (workspace == nullptr || !aligned16(workspace) || bytes < need))
+        return fail(TAGI_ERR_INVALID_ARGUMENT,
+                    std::string(who) + ": workspace is null, not 16-byte aligned or smaller than tagi_grouped_linear_workspace_bytes");
+    return TAGI_OK;
+}
+
 int check_grouped(const char *who, int E, int S, int K, int N, const int *offsets) {
+    if (sizes_fit(E, S, K, N) && offsets != nullptr && aligned4(offsets)) return TAGI_OK;
     if (E < 1 || E > 1024 || S < 0 || K < 1 || N < 1)
         return fail(TAGI_ERR_INVALID_ARGUMENT, std::string(who) + ": 1 to 1024 experts, positive feature counts, rows must not be negative");
     if (K > (1 << 20) || N > (1 << 20) || S > (1 << 28))
         return fail(TAGI_ERR_INVALID_ARGUMENT, std::string(who) + ": more than 2^20 features or 2^28 rows");
-    if (offsets == nullptr || !aligned4(offsets))
-        return fail(TAGI_ERR_INVALID_ARGUMENT, std::string(who) + ": offsets is null or not 4-byte aligned");
-    return TAGI_OK;
+    return fail(TAGI_ERR_INVALID_ARGUMENT, std::string(who) + ": offsets is null or not 4-byte aligned");
 }
 
 }  // namespace
@@ -35,9 +52,9 @@ using namespace tagi;
 
 extern "C" {
 
-size_t tagi_grouped_linear_workspace_bytes(int S, int R, int K) {
-    if (S <= FEW_ROWS || R <= 0 || K <= 0) return 0;
-    return (size_t)R * K * sizeof(float);
+size_t tagi_grouped_linear_workspace_bytes(int pass, int E, int S, int R, int K, int N) {
+    if (pass < FWD || pass > PARAM || !sizes_fit(E, S, K, N) || R < 0) return 0;
+    return parts_bytes(pass, E, S, K, N) + (pass == FWD ? second_bytes(S, R, K) : 0);
 }
 
 int tagi_grouped_linear_fwd(int E, int S, int R, int K, int N, int has_bias, const int *offsets, const int *token,
@@ -60,18 +77,18 @@ int tagi_grouped_linear_fwd(int E, int S, int R, int K, int N, int has_bias, con
     TAGI_PTR(var_a);
     TAGI_PTR(mu_z);
     TAGI_PTR(var_z);
-    const size_t need = tagi_grouped_linear_workspace_bytes(S, R, K);
-    TAGI_REQUIRE(need == 0 || (workspace != nullptr && aligned16(workspace) && workspace_bytes >= need),
-                 "workspace is null, not 16-byte aligned or smaller than tagi_grouped_linear_workspace_bytes");
     GroupedArgs a{};
     a.E = E, a.S = S, a.R = R, a.K = K, a.N = N, a.offsets = offsets, a.token = token, a.mu_w = mu_w, a.var_w = var_w;
     a.mu_b = has_bias ? mu_b : nullptr, a.var_b = has_bias ? var_b : nullptr, a.a0 = mu_a, a.a1 = var_a, a.o0 = mu_z, a.o1 = var_z;
-    a.second = static_cast<float *>(workspace);
+    if ((rc = check_workspace(__func__, FWD, a, workspace, workspace_bytes)) != TAGI_OK) return rc;
+    a.parts = static_cast<float *>(workspace);
+    a.second = a.parts + parts_bytes(FWD, E, S, K, N) / sizeof(float);
     return run(FWD, a, static_cast<cudaStream_t>(stream));
 }
 
 int tagi_grouped_linear_bwd_state(int E, int S, int K, int N, const int *offsets, const float *mu_w, const float *jcb,
-                                  const float *dmu_z, const float *dvar_z, float *dmu_a, float *dvar_a, void *stream) {
+                                  const float *dmu_z, const float *dvar_z, float *dmu_a, float *dvar_a, void *workspace,
+                                  size_t workspace_bytes, void *stream) {
     int rc = check_grouped(__func__, E, S, K, N, offsets);
     if (rc != TAGI_OK) return rc;
     TAGI_PTR(mu_w);
@@ -84,12 +101,15 @@ int tagi_grouped_linear_bwd_state(int E, int S, int K, int N, const int *offsets
     GroupedArgs a{};
     a.E = E, a.S = S, a.R = S, a.K = K, a.N = N, a.offsets = offsets, a.mu_w = mu_w, a.jcb = jcb, a.a0 = dmu_z, a.a1 = dvar_z;
     a.o0 = dmu_a, a.o1 = dvar_a;
+    if ((rc = check_workspace(__func__, STATE, a, workspace, workspace_bytes)) != TAGI_OK) return rc;
+    a.parts = static_cast<float *>(workspace);
     return run(STATE, a, static_cast<cudaStream_t>(stream));
 }
 
 int tagi_grouped_linear_bwd_param(int E, int S, int R, int K, int N, int has_bias, const int *offsets, const int *token,
                                   const float *var_w, const float *var_b, const float *mu_a, const float *dmu_z,
-                                  const float *dvar_z, float *dmu_w, float *dvar_w, float *dmu_b, float *dvar_b, void *stream) {
+                                  const float *dvar_z, float *dmu_w, float *dvar_w, float *dmu_b, float *dvar_b, void *workspace,
+                                  size_t workspace_bytes, void *stream) {
     int rc = check_grouped(__func__, E, S, K, N, offsets);
     if (rc != TAGI_OK) return rc;
     TAGI_PTR(var_w);
@@ -112,8 +132,9 @@ int tagi_grouped_linear_bwd_param(int E, int S, int R, int K, int N, int has_bia
     GroupedArgs a{};
     a.E = E, a.S = S, a.R = R, a.K = K, a.N = N, a.offsets = offsets, a.token = token, a.var_w = var_w, a.x = mu_a;
     a.var_b = has_bias ? var_b : nullptr, a.a0 = dmu_z, a.a1 = dvar_z, a.o0 = dmu_w, a.o1 = dvar_w, a.ob0 = dmu_b, a.ob1 = dvar_b;
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return run(PARAM, a, st);
+    if ((rc = check_workspace(__func__, PARAM, a, workspace, workspace_bytes)) != TAGI_OK) return rc;
+    a.parts = static_cast<float *>(workspace);
+    return run(PARAM, a, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

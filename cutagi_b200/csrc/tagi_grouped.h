@@ -12,7 +12,8 @@ struct GroupedArgs {
     const int *offsets, *token;
     // a0, a1: activations (forward) or deltas (backward); x: input means of the parameter pass
     const float *mu_w, *var_w, *mu_b, *var_b, *a0, *a1, *jcb, *x;
-    float *second;   // forward: workspace for mu_a^2 + var_a, [R][K], 16-byte aligned
+    // workspaces, 16-byte aligned: partial sums of the tiles that tagi_grouped_tc.cu cuts; forward, mu_a^2 + var_a [R][K]
+    float *parts, *second;
     float *o0, *o1, *ob0, *ob1;
 };
 
@@ -51,5 +52,7 @@ int grouped_few(int pass, const GroupedArgs &a, cudaStream_t st);
 int grouped_thin(int pass, const GroupedArgs &a, cudaStream_t st);
 int grouped_thin_status(int *out, int reset);
 int grouped_tc(int pass, const GroupedArgs &a, cudaStream_t st);
+int grouped_tc_pairs(int pass, int E, int S, int K, int N);
+size_t grouped_tc_parts_bytes(int pass, int E, int S, int K, int N);
 
 }  // namespace tagi

@@ -49,14 +49,19 @@ struct Item {
     int chunks;                 // of the item; 0: there are no more items
     int e, m0, c0, cols, bn;    // expert; first feature; first column (output row, or feature in the parameter pass); live columns; width
     int kind, depth, p0, nk;    // MEAN or VAR; contraction length; first contraction row (parameter pass); chunks of one contraction
+    int from, part;             // first chunk; WHOLE, or which of the pair's two partial sums the item goes to
 };
 // A warp of each CTA works out the items ahead of the others and hands them over through shared memory.
 struct Record {
     Item item;
-    int pad[2];
     int rows[128];              // forward pass: input rows of this CTA's columns, -1 where there is none
 };
 constexpr int RECORDS = 8;
+constexpr int WHOLE = -1, LATER = 0, BEGIN = 1;
+#ifndef CUTS
+#define CUTS 8
+#endif
+constexpr int CUT_SAVES = CUTS;
 
 struct Shared {                 // behind the slots
     uint64_t full[2], done[2], item_full[RECORDS], item_empty[RECORDS], turn;
@@ -66,17 +71,16 @@ struct Shared {                 // behind the slots
     alignas(16) int rows[4][16];      // parameter pass: input rows of a chunk's steps, per warp of A
     float aux[8][3][8][32];     // scale entries on their way to the summing warps: three groups of eight columns each
     float bias[128];            // parameter pass: sums of the deltas of this CTA's columns
+    int start[2 * PAIRS + 2];   // of the tiles that are cut: chunks of those before each
     int before[];               // tiles of the experts before e, E + 1 entries
 };
 static_assert(offsetof(Shared, rows) % 16 == 0 && sizeof(Shared) % 8 == 0, "rows are read 16 bytes at a time");
 
-// Item j of pair `pair`. The two kinds of a tile are neighbours, so two pairs work on the same weights at the same time, and
-// a pair's kinds alternate from one item to the next (in the forward pass a variance costs twice a mean).
+// Work list: the two kinds of every tile are neighbours, so two pairs work on the same weights at the same time, and a pair's
+// kinds alternate from one item to the next (in the forward pass a variance costs twice a mean).
 template <int PASS>
-__device__ __forceinline__ bool get_item(const GroupedArgs &a, const int *before, int pair, int pairs, int j, Item &it) {
-    const int i = pair + j * pairs, t = i >> 1;
-    if (t >= before[a.E]) return false;
-    it.kind = (i + 2 * t / pairs) & 1;
+__device__ __forceinline__ void tile_item(const GroupedArgs &a, const int *before, int t, int kind, Item &it) {
+    it.kind = kind;
     int lo = 0, hi = a.E - 1;   // the last expert whose tiles begin at or before t
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
@@ -94,7 +98,73 @@ __device__ __forceinline__ bool get_item(const GroupedArgs &a, const int *before
     it.p0 = r0;
     it.depth = PASS == FWD ? a.K : PASS == STATE ? a.N : r1 - r0;
     it.nk = (it.depth + KC - 1) / KC;
-    it.chunks = PASS == FWD && it.kind == VAR ? 2 * it.nk : it.nk;
+    it.chunks = PASS == FWD && kind == VAR ? 2 * it.nk : it.nk;
+    it.from = 0;
+    it.part = WHOLE;
+}
+
+// The items go round the pairs; what is left when the rounds no longer fill the GPU is cut along the contraction, so that
+// all pairs get the same number of chunks: each pair has at most the end of one tile (LATER) and the beginning of another
+// (BEGIN), whose sums go to the workspace, and grouped_join_kernel adds up and writes out the tiles that were cut.
+// JOINFIG
+struct Plan {
+    int items, whole;   // all items; those that go round
+    int chunks;         // of the items that are cut; -1: not looked at yet
+};
+__device__ __forceinline__ int kind_of(int i, int pairs) { return (i + 2 * (i >> 1) / pairs) & 1; }
+
+// Whether the rest is cut. Called by one whole warp, when the whole rounds have been handed out.
+template <int PASS>
+__device__ __forceinline__ void look_at_rest(const GroupedArgs &a, Shared &sh, int pairs, Plan &p) {
+    const int lane = threadIdx.x & 31;
+    int carry = 0, longest = 0;
+    for (int j0 = 0; j0 < p.items - p.whole; j0 += 32) {
+        const int j = j0 + lane, i = p.whole + j;
+        Item it;
+        it.chunks = 0;
+        if (i < p.items) tile_item<PASS>(a, sh.before, i >> 1, kind_of(i, pairs), it);
+        int sum = it.chunks;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += u;
+        }
+        if (i < p.items) sh.start[j] = carry + sum - it.chunks;
+        longest = max(longest, __reduce_max_sync(0xffffffffu, it.chunks));
+        carry += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    if (lane == 0) sh.start[p.items - p.whole] = carry;
+    __syncwarp();
+    // cutting costs about 10 us, the time of four chunks; uncut, the last round takes as long as its longest item
+    const bool cut = longest - (carry + pairs - 1) / pairs >= CUT_SAVES;
+    p.chunks = cut ? carry : 0;
+    if (!cut) p.whole = p.items;
+}
+
+// Item j of pair `pair`.
+template <int PASS>
+__device__ __forceinline__ bool get_item(const GroupedArgs &a, Shared &sh, Plan &p, int pair, int pairs, int j, Item &it) {
+    const int i = pair + j * pairs;
+    if (i >= p.whole && p.chunks < 0) look_at_rest<PASS>(a, sh, pairs, p);
+    if (i < p.whole) {
+        tile_item<PASS>(a, sh.before, i >> 1, kind_of(i, pairs), it);
+        return true;
+    }
+    // this pair's chunks of the tiles that are cut, one tile after the other
+    const int begin = (int)((long)p.chunks * pair / pairs), end = (int)((long)p.chunks * (pair + 1) / pairs), rest = p.items - p.whole;
+    if (begin == end) return false;
+    int lo = 0, hi = rest - 1;   // the tile of the first of them
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (sh.start[mid] <= begin) lo = mid; else hi = mid - 1;
+    }
+    lo += j - p.whole / pairs;
+    if (lo >= rest || sh.start[lo] >= end) return false;
+    tile_item<PASS>(a, sh.before, (p.whole + lo) >> 1, kind_of(p.whole + lo, pairs), it);
+    const int last = sh.start[lo + 1], c0 = max(begin, sh.start[lo]), c1 = min(end, last);
+    it.from = c0 - sh.start[lo];
+    it.chunks = c1 - c0;
+    it.part = it.from > 0 ? LATER : c1 < last ? BEGIN : WHOLE;
     return true;
 }
 
@@ -136,9 +206,27 @@ __device__ __forceinline__ void release(Shared &sh, int j, int lane) {
 
 // What both operands' converters follow: the chunk that is loaded next. It runs ahead of the chunk that is stored.
 struct Cursor {
-    int j, c, chunks, kc;
+    int j, c, end, kc;   // item; chunk, and the one behind the item's last (0: there are no more items); contraction step
     bool var, half;   // of a variance; second half of a forward variance (var_w . (mu_a^2 + var_a))
+    __device__ void set(const Item &t, int item) {
+        j = item, c = kc = end = 0, var = half = false;
+        if (t.chunks == 0) return;   // the rest of such an item means nothing
+        c = t.from, end = t.from + t.chunks;
+        var = t.kind == VAR, half = t.from >= t.nk;   // only a forward variance has more than nk chunks
+        kc = (half ? c - t.nk : c) * KC;
+    }
 };
+
+// A pair's partial sums of a tile: [columns][256 features], then the sums of the deltas of its columns (parameter pass).
+constexpr int PART_FLOATS = 256 * 256, PART_PITCH = PART_FLOATS + 256;
+__device__ __forceinline__ float *part_of(const GroupedArgs &a, int pair, int part) { return a.parts + (size_t)(pair * 2 + part) * PART_PITCH; }
+// What a partial sum belongs to, for the kernel that joins them; `ends`: it holds the tile's last chunk.
+struct Piece {
+    int used, ends, e, m0, c0, cols, bn, kind;
+};
+__device__ __forceinline__ Piece *piece_of(const GroupedArgs &a, int pairs, int pair, int part) {
+    return reinterpret_cast<Piece *>(a.parts + (size_t)pairs * 2 * PART_PITCH) + pair * 2 + part;
+}
 
 // A: 128 features of this CTA. A chunk is fetched whole as soon as the registers of the one before have been stored (one
 // latency a chunk: loads that are waited for in turn would cost one each).
@@ -164,18 +252,17 @@ __device__ __forceinline__ void convert_a(const GroupedArgs &a, Shared &sh, int 
         Item t;
         take(sh, j, t);
         release(sh, j, lane);
-        cu.j = j, cu.c = cu.kc = 0, cu.chunks = t.chunks;
+        cu.set(t, j);
         left = depth = 0;
         if (t.chunks == 0) return;
         const int m = t.m0 + cta * 128 + (MN ? along : row);
         base = PASS == FWD ? ((size_t)t.e * a.N + m) * a.K + along : PASS == STATE ? (size_t)t.e * a.N * a.K + m : m;
         left = (PASS == FWD ? a.N : a.K) - m;
-        cu.var = t.kind == VAR, cu.half = false;
         nk = t.nk, depth = t.depth, p0 = t.p0;
     };
     auto advance = [&]() {
         cu.kc += KC;
-        if (++cu.c == cu.chunks) seek(cu.j + 1);
+        if (++cu.c == cu.end) seek(cu.j + 1);
         else if (PASS == FWD && cu.c == nk) cu.kc = 0, cu.half = true;
         look_up();
     };
@@ -202,7 +289,7 @@ __device__ __forceinline__ void convert_a(const GroupedArgs &a, Shared &sh, int 
     };
     seek(0);
     look_up();
-    for (int i = 0; cu.chunks > 0; i++) {
+    for (int i = 0; cu.end > 0; i++) {
         const int s = i & 1;
         const bool square = cu.var && !cu.half;
         load();
@@ -241,7 +328,7 @@ __device__ __forceinline__ void convert_b(const GroupedArgs &a, Shared &sh, int 
     auto seek = [&](int j) {
         Item t;
         take(sh, j, t);
-        cu.j = j, cu.c = cu.kc = 0, cu.chunks = t.chunks, cu.var = t.kind == VAR, cu.half = false;
+        cu.set(t, j);
         half_bn = t.chunks ? t.bn >> 1 : 0;
         const int n = cta * half_bn + (MN ? along : row);
         left = t.chunks == 0 ? 0 : MN ? (along < half_bn ? t.cols - n : 0) : min(half_bn - row, t.cols - n);
@@ -257,7 +344,7 @@ __device__ __forceinline__ void convert_b(const GroupedArgs &a, Shared &sh, int 
     };
     auto advance = [&]() {
         cu.kc += KC;
-        if (++cu.c == cu.chunks) seek(cu.j + 1);
+        if (++cu.c == cu.end) seek(cu.j + 1);
         else if (PASS == FWD && cu.c == nk) cu.kc = 0, cu.half = true;
     };
     auto load = [&](int g) {
@@ -271,12 +358,12 @@ __device__ __forceinline__ void convert_b(const GroupedArgs &a, Shared &sh, int 
         }
     };
     seek(0);
-    for (int i = 0; cu.chunks > 0; i++) {
+    for (int i = 0; cu.end > 0; i++) {
         const int s = i & 1, lines = half_bn;
 #pragma unroll
         for (int g = 0; g < 4; g++) load(g);
         const bool sums = PASS == PARAM && sum;
-        const int ended = PASS == PARAM && cu.c + 1 == cu.chunks ? cu.j : -1;   // the item that ends with this chunk
+        const int ended = PASS == PARAM && cu.c + 1 == cu.end ? cu.j : -1;   // the item that ends with this chunk
         advance();
         if (i >= 2 && !mbar_wait(sh.done + s, ((i - 2) >> 1) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_EMPTY)) return;
 #pragma unroll
@@ -309,7 +396,9 @@ __device__ __forceinline__ void convert_b(const GroupedArgs &a, Shared &sh, int 
                 }
                 total = make_float4(0.f, 0.f, 0.f, 0.f);
                 const int c = w * 32 + lane, n = cta * (t.bn >> 1) + c;
-                if (c < t.bn >> 1 && n < t.cols) {
+                if (c < t.bn >> 1 && t.part != WHOLE) {
+                    part_of(a, blockIdx.x >> 1, t.part)[PART_FLOATS + n] = sh.bias[c];
+                } else if (c < t.bn >> 1 && n < t.cols) {
                     const size_t o = (size_t)t.e * a.N + t.c0 + n;
                     const float vb = __ldg(a.var_b + o);
                     (t.kind == VAR ? a.ob1 : a.ob0)[o] = t.kind == VAR ? vb * vb * sh.bias[c] : vb * sh.bias[c];
@@ -351,6 +440,7 @@ __global__ void __launch_bounds__(THREADS, 1) grouped_tc_kernel(const GroupedArg
         if (lane == 0) sh.before[a.E] = carry;
     }
     __syncthreads();
+    if (cta == 0 && threadIdx.x < 2) piece_of(a, pairs, pair, threadIdx.x)->used = 0;
     if (sh.before[a.E] == 0) return;   // no expert of this size; the same in both CTAs
     if (threadIdx.x == 0) {
         for (int s = 0; s < 2; s++) {
@@ -390,7 +480,7 @@ __global__ void __launch_bounds__(THREADS, 1) grouped_tc_kernel(const GroupedArg
             for (int j = 0; ok && take(sh, j, it) && it.chunks > 0; j++) {
                 mbar_arrive(sh.item_empty + j % RECORDS);
                 const uint32_t idesc = make_idesc_bf16(256, it.bn, A_MN, B_MN);
-                for (int c = 0; c < it.chunks; c++, i++) {
+                for (int c = it.from; c < it.from + it.chunks; c++, i++) {
                     const int s = i & 1, left = it.depth - (c >= it.nk ? c - it.nk : c) * KC;
                     const int steps = max(1, min(KC / 16, (left + 15) / 16));
                     ok = mbar_wait_cluster(sh.full + s, (i >> 1) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_CONV);
@@ -406,14 +496,19 @@ __global__ void __launch_bounds__(THREADS, 1) grouped_tc_kernel(const GroupedArg
         }
         if (warp == ISSUER + 1) {
             // ------------------------------------------------------------------------------------------------- items
+            Plan plan{2 * sh.before[a.E], 0, -1};
+            // the forward pass's rounds come in twos, as many means as variances for each pair
+            plan.whole = PASS == FWD ? plan.items / (2 * pairs) * (2 * pairs) : plan.items / pairs * pairs;
             bool more = true;
             for (int j = 0; more; j++) {
                 Record &r = sh.record[j % RECORDS];
                 if (j >= RECORDS && !mbar_wait(sh.item_empty + j % RECORDS, (j / RECORDS - 1) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_EMPTY))
                     break;
                 Item t;
-                more = get_item<PASS>(a, sh.before, pair, pairs, j, t);
+                more = get_item<PASS>(a, sh, plan, pair, pairs, j, t);
                 if (!more) t.chunks = 0;
+                if (more && t.part != WHOLE && cta == 0 && lane == 0)
+                    *piece_of(a, pairs, pair, t.part) = Piece{1, t.from + t.chunks == (PASS == FWD && t.kind == VAR ? 2 : 1) * t.nk, t.e, t.m0, t.c0, t.cols, t.bn, t.kind};
                 if (lane == 0) r.item = t;
                 if (PASS == FWD && more)
                     for (int l = lane; l < t.bn >> 1; l += 32) {
@@ -446,6 +541,7 @@ __global__ void __launch_bounds__(THREADS, 1) grouped_tc_kernel(const GroupedArg
         struct Output {
             size_t base;   // first entry of the thread's column `first`
             int n, m, ld, kind, e;   // live columns of the warp's part; feature; pitch
+            bool whole;
         };
         auto locate = [&](int j) {
             const volatile Item &t = sh.record[j % RECORDS].item;
@@ -456,13 +552,19 @@ __global__ void __launch_bounds__(THREADS, 1) grouped_tc_kernel(const GroupedArg
             o.ld = PASS == FWD ? a.N : a.K;
             o.kind = t.kind, o.e = t.e;
             if (o.m >= o.ld) o.n = 0;
+            o.whole = t.part == WHOLE;
+            if (!o.whole) {   // a partial sum
+                o.ld = 256;
+                o.base = (size_t)(pair * 2 + t.part) * PART_PITCH + first * 256 + cta * 128 + quad * 32 + lane;
+                return o;
+            }
             o.base = ((PASS == PARAM ? (size_t)o.e * a.N : 0) + t.c0 + first) * o.ld + o.m;
             return o;
         };
         // Scale entries (Jacobian, prior variances) come from HBM and there are no registers to wait for them in either: a
         // lane copies its own to shared memory, 24 columns ahead, the first before the last chunk is done.
         auto fetch = [&](const Output &o, int g) {   // columns g .. g + 7
-            if (scaled) {
+            if (scaled && o.whole) {
                 const float *aux = (PASS == PARAM ? a.var_w : a.jcb) + o.base + (size_t)g * o.ld;
 #pragma unroll
                 for (int x = 0; x < 8; x++)
@@ -502,9 +604,9 @@ __global__ void __launch_bounds__(THREADS, 1) grouped_tc_kernel(const GroupedArg
             if (!ok) break;
             const Output o = locate(j);
             release(sh, j, lane);
-            float *out = (o.kind == VAR ? a.o1 : a.o0) + o.base;
+            float *out = (!o.whole ? a.parts : o.kind == VAR ? a.o1 : a.o0) + o.base;
             float bias = 0.f;
-            if (PASS == FWD && a.mu_b && o.n > 0) bias = __ldg((o.kind == VAR ? a.var_b : a.mu_b) + (size_t)o.e * a.N + o.m);
+            if (PASS == FWD && a.mu_b && o.whole && o.n > 0) bias = __ldg((o.kind == VAR ? a.var_b : a.mu_b) + (size_t)o.e * a.N + o.m);
 #pragma unroll
             for (int g = 0; g < 128; g += 8) {
                 if (g >= o.n) break;
@@ -515,7 +617,7 @@ __global__ void __launch_bounds__(THREADS, 1) grouped_tc_kernel(const GroupedArg
                         float z = acc[g + x];
                         if (PASS == FWD) {
                             z += bias;
-                        } else if (scaled) {
+                        } else if (scaled && o.whole) {
                             float f;
                             asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f) : "r"(aux_at + ((g / 8 % 3) * 8 + x) * 128));
                             z = o.kind == VAR ? z * f * f : z * f;
@@ -545,6 +647,54 @@ __global__ void __launch_bounds__(THREADS, 1) grouped_tc_kernel(const GroupedArg
     }
 }
 
+// Adds up the partial sums of the tiles that were cut, in the order of the contraction, and writes them out. blockIdx.x: a
+// pair's partial sum that begins a tile, the others do nothing; blockIdx.y: eight columns of it. A thread has a feature.
+constexpr int JOIN_COLUMNS = 8;
+template <int PASS>
+__global__ void __launch_bounds__(256) grouped_join_kernel(const GroupedArgs a, int pairs) {
+    const int pair = blockIdx.x, x0 = blockIdx.y * JOIN_COLUMNS;
+    const Piece t = *piece_of(a, pairs, pair, BEGIN);
+    if (!t.used || x0 >= t.cols) return;
+    float acc[JOIN_COLUMNS], bias = 0.f;
+    const bool sum = PASS == PARAM && a.var_b && t.m0 == 0 && blockIdx.y == 0;
+#pragma unroll
+    for (int x = 0; x < JOIN_COLUMNS; x++) acc[x] = 0.f;
+    bool ends = false;
+    for (int q = pair; q < pairs && !ends; q++) {   // a tile that begins here goes on with the next pairs
+        const int part = q == pair ? BEGIN : LATER;
+        const Piece *piece = piece_of(a, pairs, q, part);
+        if (!piece->used) continue;   // a pair without a chunk
+        const float *p = part_of(a, q, part);
+#pragma unroll
+        for (int x = 0; x < JOIN_COLUMNS; x++)
+            if (x0 + x < t.cols) acc[x] += p[(x0 + x) * 256 + threadIdx.x];
+        if (sum && (int)threadIdx.x < t.cols) bias += p[PART_FLOATS + threadIdx.x];
+        ends = piece->ends;
+    }
+    if (sum && (int)threadIdx.x < t.cols) {
+        const size_t o = (size_t)t.e * a.N + t.c0 + threadIdx.x;
+        const float vb = __ldg(a.var_b + o);
+        (t.kind == VAR ? a.ob1 : a.ob0)[o] = t.kind == VAR ? vb * vb * bias : vb * bias;
+    }
+    const int m = t.m0 + threadIdx.x, ld = PASS == FWD ? a.N : a.K;
+    if (m >= ld) return;
+    const size_t base = ((PASS == PARAM ? (size_t)t.e * a.N : 0) + t.c0 + x0) * ld + m;
+    const float *scale = PASS == PARAM ? a.var_w : a.jcb;
+    float add = 0.f;
+    if (PASS == FWD && a.mu_b) add = __ldg((t.kind == VAR ? a.var_b : a.mu_b) + (size_t)t.e * a.N + m);
+#pragma unroll
+    for (int x = 0; x < JOIN_COLUMNS; x++) {
+        if (x0 + x >= t.cols) break;
+        const size_t o = base + (size_t)x * ld;
+        float z = acc[x] + add;
+        if (PASS != FWD && scale) {
+            const float f = __ldg(scale + o);
+            z = t.kind == VAR ? z * f * f : z * f;
+        }
+        (t.kind == VAR ? a.o1 : a.o0)[o] = z;
+    }
+}
+
 // mu_a^2 + var_a, the forward variance's operand
 __global__ void __launch_bounds__(256) grouped_second_moment_kernel(const float *__restrict__ mu, const float *__restrict__ var,
                                                                     size_t n, float *__restrict__ out) {
@@ -567,11 +717,9 @@ template <int PASS>
 int launch_pass(const GroupedArgs &a, cudaStream_t st) {
     const bool vec = grouped_aligned(PASS, a);
     const size_t smem = 2 * SLOT + 1024 + sizeof(Shared) + (a.E + 1) * sizeof(int);
-    const long mt = ((PASS == FWD ? a.N : a.K) + 255) / 256;
-    const long experts = a.E < a.S / (a.thin + 1) ? a.E : a.S / (a.thin + 1);   // at most as many have more rows
-    const long most = 2 * mt * (PASS == PARAM ? experts * ((a.N + 255) / 256) : a.S / 256 + experts);
+    const int pairs = grouped_tc_pairs(PASS, a.E, a.S, a.K, a.N);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(2 * (unsigned)(most < PAIRS ? most : PAIRS));
+    cfg.gridDim = dim3(2 * pairs);
     cfg.blockDim = dim3(THREADS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
@@ -585,10 +733,25 @@ int launch_pass(const GroupedArgs &a, cudaStream_t st) {
     auto k = vec ? grouped_tc_kernel<PASS, true> : grouped_tc_kernel<PASS, false>;
     TAGI_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     TAGI_CUDA(cudaLaunchKernelEx(&cfg, k, a));
+    grouped_join_kernel<PASS><<<dim3(pairs, 256 / JOIN_COLUMNS), 256, 0, st>>>(a, pairs);
+    TAGI_CUDA(cudaGetLastError());
     return TAGI_OK;
 }
 
 }  // namespace
+
+// CTA pairs that may find work: one per SM pair, or as many as there can be chunks
+int grouped_tc_pairs(int pass, int E, int S, int K, int N) {
+    const int thin = pass == PARAM ? FEW_PARAM_ROWS : THIN_ROWS;
+    const long mt = ((pass == FWD ? N : K) + 255) / 256, experts = E < S / (thin + 1) ? E : S / (thin + 1);   // at most as many have more rows
+    const long tiles = mt * (pass == PARAM ? experts * ((N + 255) / 256) : S / 256 + experts);
+    const long chunks = ((pass == FWD ? K : pass == STATE ? N : S) + KC - 1) / KC;
+    const long most = tiles * chunks * (pass == FWD ? 3 : 2);
+    return (int)(most < 1 ? 1 : most < PAIRS ? most : PAIRS);
+}
+size_t grouped_tc_parts_bytes(int pass, int E, int S, int K, int N) {
+    return (size_t)grouped_tc_pairs(pass, E, S, K, N) * 2 * (PART_PITCH * sizeof(float) + sizeof(Piece));
+}
 
 int grouped_second_moment(const GroupedArgs &a, cudaStream_t st) {
     const size_t n = (size_t)a.R * a.K;

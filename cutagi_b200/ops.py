@@ -153,7 +153,7 @@ def grouped_linear(mu_w, var_w, mu_b, var_b, mu_a, var_a, offsets, token=None):
     inputs = (_p("offsets", offsets, (E + 1,), i, _I), _p("token", token, (S,), i, _I), _p("mu_w", mu_w, w, i), _p("var_w", var_w, w, i),
               _p("mu_b", mu_b, b, i), _p("var_b", var_b, b, i), _p("mu_a", mu_a, (R, K), i), _p("var_a", var_a, (R, K), i))
     mu_z, var_z = _two(mu_w, S, N)
-    nbytes = capi.load().tagi_grouped_linear_workspace_bytes(S, R, K)
+    nbytes = capi.load().tagi_grouped_linear_workspace_bytes(0, E, S, R, K, N)
     keep, ws = _workspace(nbytes, mu_w)
     _run("tagi_grouped_linear_fwd", i, E, S, R, K, N, bias, *inputs, mu_z.data_ptr(), var_z.data_ptr(), ws, nbytes)
     return mu_z, var_z
@@ -165,7 +165,9 @@ def grouped_linear_state(mu_w, jcb, dmu_z, dvar_z, offsets):
     inputs = (_p("offsets", offsets, (E + 1,), i, _I), _p("mu_w", mu_w, mu_w.shape, i), _p("jcb", jcb, (S, K), i),
               _p("dmu_z", dmu_z, (S, N), i), _p("dvar_z", dvar_z, (S, N), i))
     dmu_a, dvar_a = _two(mu_w, S, K)
-    _run("tagi_grouped_linear_bwd_state", i, E, S, K, N, *inputs, dmu_a.data_ptr(), dvar_a.data_ptr())
+    nbytes = capi.load().tagi_grouped_linear_workspace_bytes(1, E, S, S, K, N)
+    keep, ws = _workspace(nbytes, mu_w)
+    _run("tagi_grouped_linear_bwd_state", i, E, S, K, N, *inputs, dmu_a.data_ptr(), dvar_a.data_ptr(), ws, nbytes)
     return dmu_a, dvar_a
 
 
@@ -179,8 +181,10 @@ def grouped_linear_param(var_w, var_b, mu_a, dmu_z, dvar_z, offsets, token=None,
               _p("mu_a", mu_a, (R, K), i), _p("dmu_z", dmu_z, (S, N), i), _p("dvar_z", dvar_z, (S, N), i))
     if out is None:
         out = (*_two(var_w), *(_two(var_b) if bias else (None, None)))
+    nbytes = capi.load().tagi_grouped_linear_workspace_bytes(2, E, S, R, K, N)
+    keep, ws = _workspace(nbytes, var_w)
     _run("tagi_grouped_linear_bwd_param", i, E, S, R, K, N, int(bias), *inputs, _p("out[0]", out[0], w, i), _p("out[1]", out[1], w, i),
-         _p("out[2]", out[2], b, i), _p("out[3]", out[3], b, i))
+         _p("out[2]", out[2], b, i), _p("out[3]", out[3], b, i), ws, nbytes)
     return tuple(out)
 
 

@@ -364,21 +364,23 @@ int tagi_route_bwd(int T, int E, int k, const int *expert, const float *mu_g, co
  * rows from offsets[E] on and rows before offsets[0] are left as they were. token (device, S entries) names the row of
  * mu_a / var_a [R][K] that each output row reads, so the tokens need no copy in dispatch order; NULL: row p reads row p
  * (then R == S). Bad device data does no harm: offsets are clamped into range, a token outside [0, R) reads as a row of
- * zeros. Sums have the accuracy of 32-bit products. workspace: tagi_grouped_linear_workspace_bytes(S, R, K) bytes (host
- * helper; 0 = NULL is fine). */
-size_t tagi_grouped_linear_workspace_bytes(int S, int R, int K);
+ * zeros. Sums have the accuracy of 32-bit products. workspace, of this and the backward passes: tagi_grouped_linear_workspace_bytes
+ * bytes (host helper; pass: 0 forward, 1 state, 2 parameters, with R == S for the state pass; 0 = NULL is fine). */
+size_t tagi_grouped_linear_workspace_bytes(int pass, int E, int S, int R, int K, int N);
 int tagi_grouped_linear_fwd(int E, int S, int R, int K, int N, int has_bias, const int *offsets, const int *token,
                             const float *mu_w, const float *var_w, const float *mu_b, const float *var_b, const float *mu_a,
                             const float *var_a, float *mu_z, float *var_z, void *workspace, size_t workspace_bytes, void *stream);
 /* tagi_linear_bwd_state per expert: deltas dmu_z / dvar_z [S][N] and outputs dmu_a / dvar_a [S][K] in dispatch order, jcb
  * [S][K] the Jacobian of the same rows (NULL = 1; where the input was gathered by token, tagi_dispatch_bwd applies it). */
 int tagi_grouped_linear_bwd_state(int E, int S, int K, int N, const int *offsets, const float *mu_w, const float *jcb,
-                                  const float *dmu_z, const float *dvar_z, float *dmu_a, float *dvar_a, void *stream);
+                                  const float *dmu_z, const float *dvar_z, float *dmu_a, float *dvar_a, void *workspace,
+                                  size_t workspace_bytes, void *stream);
 /* tagi_linear_bwd_param per expert: dmu_w / dvar_w [E][N][K] and, when has_bias, dmu_b / dvar_b [E][N] are written for
  * every expert, zeros for one without rows. token / R as for the forward pass: the rows of mu_a [R][K] that were read. */
 int tagi_grouped_linear_bwd_param(int E, int S, int R, int K, int N, int has_bias, const int *offsets, const int *token,
                                   const float *var_w, const float *var_b, const float *mu_a, const float *dmu_z,
-                                  const float *dvar_z, float *dmu_w, float *dvar_w, float *dmu_b, float *dvar_b, void *stream);
+                                  const float *dvar_z, float *dmu_w, float *dvar_w, float *dmu_b, float *dvar_b, void *workspace,
+                                  size_t workspace_bytes, void *stream);
 
 /* A token's expert rows joined with its gates, as products of independent Gaussians: over the token's slots with a row
  * p = pos[t][j] in [0, S): mu_y = sum mu_g * mu_x[p]; var_y = sum var_g * (mu_x[p]^2 + var_x[p]) + mu_g^2 * var_x[p].

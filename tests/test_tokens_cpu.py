@@ -90,14 +90,15 @@ def test_grouped_linear_refusals():
         if i != 1:      # the gather index may be NULL
             refused("tagi_grouped_linear_fwd", *fwd(p=[None if j == i else P for j in range(10)]))
         refused("tagi_grouped_linear_fwd", *fwd(p=[P + 2 if j == i else P for j in range(10)]))
-    need = lib.tagi_grouped_linear_workspace_bytes(1000, 500, 64)
-    assert need >= 500 * 64 * 4 and lib.tagi_grouped_linear_workspace_bytes(0, 500, 64) == 0
+    need = lib.tagi_grouped_linear_workspace_bytes(0, 4, 1000, 500, 64, 16)
+    assert need >= 500 * 64 * 4 and lib.tagi_grouped_linear_workspace_bytes(0, 4, 0, 500, 64, 16) == 0
+    assert lib.tagi_grouped_linear_workspace_bytes(0, 4, 1 << 30, 500, 64, 16) == lib.tagi_grouped_linear_workspace_bytes(3, 4, 8, 8, 64, 16) == 0
     for kw in (dict(ws=None), dict(ws=P + 4), dict(size=need - 1)):
         refused("tagi_grouped_linear_fwd", *fwd(S=1000, R_=500, K=64, **kw))
     refused("tagi_grouped_linear_fwd", *fwd(R_=7, p=[P, None] + [P] * 8))     # no gather index: R must equal S
 
-    def state(E=4, S=8, K=16, N=16, p=None):
-        return (E, S, K, N, *(p or [P] * 7), None)
+    def state(E=4, S=8, K=16, N=16, p=None, ws=P, size=1 << 40):
+        return (E, S, K, N, *(p or [P] * 7), ws, size, None)
     for kw in (dict(E=0), dict(S=-1), dict(K=0), dict(N=0)):
         refused("tagi_grouped_linear_bwd_state", *state(**kw))
     for i in range(7):
@@ -105,8 +106,13 @@ def test_grouped_linear_refusals():
             refused("tagi_grouped_linear_bwd_state", *state(p=[None if j == i else P for j in range(7)]))
         refused("tagi_grouped_linear_bwd_state", *state(p=[P + 2 if j == i else P for j in range(7)]))
 
-    def param(E=4, S=8, R_=8, K=16, N=16, bias=1, p=None):
-        return (E, S, R_, K, N, bias, *(p or [P] * 11), None)
+    def param(E=4, S=8, R_=8, K=16, N=16, bias=1, p=None, ws=P, size=1 << 40):
+        return (E, S, R_, K, N, bias, *(p or [P] * 11), ws, size, None)
+    for which, name, args in ((1, "tagi_grouped_linear_bwd_state", state), (2, "tagi_grouped_linear_bwd_param", lambda **kw: param(R_=1000, **kw))):
+        need = lib.tagi_grouped_linear_workspace_bytes(which, 4, 1000, 1000, 16, 16)
+        assert need > 0 and lib.tagi_grouped_linear_workspace_bytes(which, 4, 8, 8, 16, 16) == 0
+        for kw in (dict(ws=None), dict(ws=P + 4), dict(size=need - 1)):
+            refused(name, *args(S=1000, **kw))
     for kw in (dict(E=0), dict(S=-1), dict(K=0), dict(N=0), dict(R_=0)):
         refused("tagi_grouped_linear_bwd_param", *param(**kw))
     for i in range(11):
@@ -177,7 +183,7 @@ def test_tensor_functions_refuse_sizes_that_32_bits_do_not_hold():
 def test_empty_calls_touch_nothing():
     assert lib.tagi_ln_fwd(*ln_args(R=0, p=[P] * 4 + [None] * 6)) == 0
     assert lib.tagi_grouped_linear_fwd(4, 0, 0, 16, 16, 1, P, None, P, P, P, P, None, None, None, None, None, 0, None) == 0
-    assert lib.tagi_grouped_linear_bwd_state(4, 0, 16, 16, P, P, None, None, None, None, None, None) == 0
+    assert lib.tagi_grouped_linear_bwd_state(4, 0, 16, 16, P, P, None, None, None, None, None, None, 0, None) == 0
     assert lib.tagi_combine_fwd(0, 2, 8, 0, *[None] * 8) == 0
     assert lib.tagi_combine_bwd(0, 2, 8, 0, *[None] * 11) == 0
     assert lib.tagi_dispatch_bwd(0, 2, 8, 0, *[None] * 7) == 0

@@ -103,12 +103,25 @@ def test_layer_norm_forward(lib, rows, n, bias, misalign):
         R.check(name, got.get(), pair, R.U)
 
 
-def grouped_fwd(lib, E, S, rows, K, N, *args):
-    """tagi_grouped_linear_fwd with a guarded workspace."""
-    size = lib.tagi_grouped_linear_workspace_bytes(S, rows, K)
-    ws = torch.full((size // 4 + 32,), SENT, device="cuda")
-    lib.tagi_grouped_linear_fwd(E, S, rows, K, N, *args, p(ws), size, st())
+def with_workspace(lib, name, which, E, S, rows, K, N, *args):
+    """A pass of the grouped Linear layers with a guarded workspace full of NaN."""
+    size = lib.tagi_grouped_linear_workspace_bytes(which, E, S, rows, K, N)
+    ws = torch.full((size // 4 + 32,), torch.nan, device="cuda")
+    ws[size // 4:] = SENT
+    getattr(lib, name)(*args, p(ws), size, st())
     assert bool((ws[size // 4:] == SENT).all())
+
+
+def grouped_fwd(lib, E, S, rows, K, N, *args):
+    with_workspace(lib, "tagi_grouped_linear_fwd", 0, E, S, rows, K, N, E, S, rows, K, N, *args)
+
+
+def grouped_state(lib, E, S, K, N, *args):
+    with_workspace(lib, "tagi_grouped_linear_bwd_state", 1, E, S, S, K, N, E, S, K, N, *args)
+
+
+def grouped_param(lib, E, S, rows, K, N, *args):
+    with_workspace(lib, "tagi_grouped_linear_bwd_param", 2, E, S, rows, K, N, E, S, rows, K, N, *args)
 
 
 def test_layer_norm_forward_of_a_constant_row(lib):
@@ -282,14 +295,14 @@ def test_grouped_linear(lib, counts, K, N, bias, gather, misalign, lead, tail):
 
     dm, dv, jcb = g.n(S, N, scale=0.1), g.u(S, N, lo=-0.2, hi=0.0), (g.u(S, K) if bias else None)
     da, dva = Guard(S, K, misalign=misalign), Guard(S, K, misalign=misalign)
-    lib.tagi_grouped_linear_bwd_state(E, S, K, N, p(offsets), p(mw), p(jcb), p(dm), p(dv), da.ptr(), dva.ptr(), st())
+    grouped_state(lib, E, S, K, N, p(offsets), p(mw), p(jcb), p(dm), p(dv), da.ptr(), dva.ptr())
     ref = R.grouped_state(mw, jcb, dm, dv, offsets)
     R.check("dmu_a", guard_rows(da, r0, r1), sub(ref[0], r0, r1), R.sum_tol(N))
     R.check("dvar_a", guard_rows(dva, r0, r1), sub(ref[1], r0, r1), R.sum_tol(N))
 
     o = [Guard(E, N, K, misalign=misalign) for _ in range(2)] + [Guard(E, N) for _ in range(2)]
-    lib.tagi_grouped_linear_bwd_param(E, S, rows, K, N, int(bias), p(offsets), p(token), p(vw), p(vb), p(ma), p(dm), p(dv),
-                                      *[x.ptr() for x in o], st())
+    grouped_param(lib, E, S, rows, K, N, int(bias), p(offsets), p(token), p(vw), p(vb), p(ma), p(dm), p(dv),
+                                      *[x.ptr() for x in o])
     ref = R.grouped_param(vw, vb, ma, dm, dv, offsets, token)
     for i, name in enumerate(("dmu_w", "dvar_w", "dmu_b", "dvar_b")):
         if i < 2 or bias:
@@ -342,6 +355,14 @@ def test_grouped_linear_of_many_tiles(lib):
     """More tiles than CTA pairs, so that each takes several in a row: of both kinds, many widths, all the experts' biases."""
     test_grouped_linear(lib, [1500, 0, 333, 2100, 7, 30, 900], 1100, 1030, True, True, 0, 0, 0)
     test_grouped_linear(lib, [40] * 30, 700, 2060, True, False, 0, 0, 0)
+
+
+@pytest.mark.parametrize("counts, K, N", [([300], 3000, 100), ([60, 50], 100, 3000), ([5000, 30, 800], 24, 40), ([520, 0, 70], 1536, 1403),
+                                          ([100] * 11, 2050, 513), ([49], 4100, 16), ([2000], 16, 300)])
+@pytest.mark.parametrize("bias, gather", [(True, True), (False, False)])
+def test_grouped_linear_of_few_tiles_and_long_contractions(lib, counts, K, N, bias, gather):
+    """Tiles that are cut along the contraction, because whole ones would leave most of the GPU idle."""
+    test_grouped_linear(lib, counts, K, N, bias, gather, 0, 1, 1)
 
 
 def big(*shape):
@@ -447,7 +468,7 @@ def test_grouped_linear_without_rows(lib):
     E, K, N = 3, 20, 24
     offsets = torch.zeros(E + 1, dtype=i32, device="cuda")
     v, o = torch.ones(E, N, K, device="cuda"), [Guard(E, N, K), Guard(E, N, K), Guard(E, N), Guard(E, N)]
-    lib.tagi_grouped_linear_bwd_param(E, 0, 0, K, N, 1, p(offsets), None, p(v), p(v), None, None, None, *[x.ptr() for x in o], st())
+    grouped_param(lib, E, 0, 0, K, N, 1, p(offsets), None, p(v), p(v), None, None, None, *[x.ptr() for x in o])
     assert all(bool((x.get() == 0).all()) for x in o)
 
 
@@ -466,8 +487,8 @@ def test_grouped_linear_bad_device_data_stays_in_range(lib, rows):
     R.check("mu_z", z.get(), ref[0], R.sum_tol(K))
     R.check("var_z", vz.get(), ref[1], R.sum_tol(2 * K))
     o, dm = [Guard(2, N, K) for _ in range(2)], g.n(rows, N)
-    lib.tagi_grouped_linear_bwd_param(2, rows, rows, K, N, 0, p(offsets), p(token), p(vw), None, p(ma), p(dm), p(dm),
-                                      o[0].ptr(), o[1].ptr(), None, None, st())
+    grouped_param(lib, 2, rows, rows, K, N, 0, p(offsets), p(token), p(vw), None, p(ma), p(dm), p(dm),
+                                      o[0].ptr(), o[1].ptr(), None, None)
     ref = R.grouped_param(vw, None, ma, dm, dm, offsets, token)
     R.check("dmu_w", o[0].get(), ref[0], R.sum_tol(rows))
     R.check("dvar_w", o[1].get(), ref[1], R.sum_tol(rows))
@@ -490,8 +511,8 @@ def test_grouped_linear_rows_of_other_experts_do_not_leak(lib, counts, K, N):
     o = [Guard(E, N, K) for _ in range(2)] + [Guard(E, N) for _ in range(2)]
     vb = g.u(E, N)
     grouped_fwd(lib, E, S, S, K, N, 0, p(offsets), None, p(mw), p(vw), None, None, p(ma), p(va), z.ptr(), vz.ptr())
-    lib.tagi_grouped_linear_bwd_state(E, S, K, N, p(offsets), p(mw), None, p(dm), p(dv), da.ptr(), dva.ptr(), st())
-    lib.tagi_grouped_linear_bwd_param(E, S, S, K, N, 1, p(offsets), None, p(vw), p(vb), p(ma), p(dm), p(dv), *[x.ptr() for x in o], st())
+    grouped_state(lib, E, S, K, N, p(offsets), p(mw), None, p(dm), p(dv), da.ptr(), dva.ptr())
+    grouped_param(lib, E, S, S, K, N, 1, p(offsets), None, p(vw), p(vb), p(ma), p(dm), p(dv), *[x.ptr() for x in o])
     rows = torch.cat([torch.arange(lo, a), torch.arange(b, hi)]).cuda()
     for pair, got, L in zip((*R.grouped_fwd(mw, vw, None, None, ma, va, offsets, None), *R.grouped_state(mw, None, dm, dv, offsets)),
                             (z, vz, da, dva), (K, 2 * K, N, N)):
