@@ -36,9 +36,9 @@ __device__ __forceinline__ int input_row(const GroupedArgs &a, int p) {
 //   up to thin   tagi_grouped_thin.cu  tensor cores, tiles of 128 features fed by TMA (forward and state pass, aligned rows)
 //   more         tagi_grouped_tc.cu    tensor cores, tiles of 256 features x up to 256 rows
 // Measured on eight experts of 4096 x 4096, forward pass, 4 / 8 / 16 / 32 rows each: few 222 / 307 / 522 / 936 us; thin 402 to
-// 413 us up to 32 rows, 506 us at 40; the wide kernel 750 us from 9 to 64. Parameter pass at 8 / 16 / 32 rows: few 380 / 501 /
-// 747 us, the wide kernel 600 us at 16.
-constexpr int FEW_ROWS = 8, FEW_PARAM_ROWS = 20, THIN_ROWS = 48;
+// 425 us up to 32 rows, 506 us at 40; the wide kernel 780 us from 9 to 64. Parameter pass at 7 / 10 / 14 / 20 rows: few 377 /
+// 419 / 486 / 595 us, the wide kernel 503 to 507 us.
+constexpr int FEW_ROWS = 8, FEW_PARAM_ROWS = 14, THIN_ROWS = 48;
 
 // the rows that a pass reads (of weights, activations and deltas) are whole 16-byte groups
 inline bool grouped_aligned(int pass, const GroupedArgs &a) {

@@ -334,9 +334,9 @@ def test_grouped_linear_of_tensors_aligned_differently(lib, counts, K, N):
             R.check(f"offset {d}", x, pair, R.sum_tol(L))
 
 
-# experts on both sides of every border between the kernels (8, 20 and 48 rows) and of the widest tile (256), with rows that
+# experts on both sides of every border between the kernels (8, 14 and 48 rows) and of the widest tile (256), with rows that
 # are aligned to 16 bytes in both, one or none of the two directions
-@pytest.mark.parametrize("counts", [[8, 9, 20, 21, 48, 49, 0, 16, 17], [255, 256, 257, 512, 513, 3], [64, 65, 96, 33, 32, 31]])
+@pytest.mark.parametrize("counts", [[8, 9, 14, 15, 48, 49, 0, 16, 17], [255, 256, 257, 512, 513, 3], [64, 65, 96, 33, 32, 31]])
 @pytest.mark.parametrize("K, N", [(260, 132), (130, 67), (516, 1031), (129, 300)])
 @pytest.mark.parametrize("bias, gather, misalign, lead, tail", [(True, True, 0, 1, 2), (True, False, 0, 0, 0)])
 def test_grouped_linear_at_the_kernels_borders(lib, counts, K, N, bias, gather, misalign, lead, tail):
