@@ -29,6 +29,25 @@ __device__ __forceinline__ int input_row(const GroupedArgs &a, int p) {
     const int r = a.token ? __ldg(a.token + p) : p;
     return (unsigned)r < (unsigned)a.R ? r : -1;
 }
+
+__device__ __forceinline__ uint32_t smem_at(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+// floats of p's 16-byte group of memory before p
+__device__ __forceinline__ int shift_of(const float *p) { return (int)((unsigned long long)p >> 2) & 3; }
+// The 16-byte group of memory at src, of whose floats `left` lie before the row's end; zeros behind it.
+__device__ __forceinline__ void copy_group(float *dst, const float *src, int left) {
+    if (left > 0)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_at(dst)), "l"(src), "r"(left < 4 ? left * 4 : 16) : "memory");
+    else
+        *reinterpret_cast<float4 *>(dst) = make_float4(0.f, 0.f, 0.f, 0.f);
+}
+__device__ __forceinline__ void copy_float(float *dst, const float *src, bool in) {
+    if (in) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_at(dst)), "l"(src) : "memory");
+    else *dst = 0.f;
+}
+// A group that begins before its tensor does, `before` floats: only the floats of the tensor.
+__device__ __forceinline__ void copy_first_group(float *dst, const float *src, int before, int left) {
+    for (int c = before; c < 4; c++) copy_float(dst + c, src + c, c < left);
+}
 #endif
 
 // Which kernel an expert's rows run on, decided on the device by their number (few, thin: see GroupedArgs):

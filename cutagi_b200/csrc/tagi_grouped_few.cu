@@ -26,25 +26,6 @@ __host__ __device__ constexpr int state_pitch(bool vec) { return vec ? OUT : OUT
 __host__ __device__ constexpr int weights(int pass, bool vec) { return pass == FWD ? FWD_WEIGHTS : SLAB * state_pitch(vec); }
 __host__ __device__ constexpr int stages(int pass) { return pass == FWD ? 4 : 8; }   // a slab of both is 18 KiB, of means 8
 
-__device__ __forceinline__ uint32_t smem_at(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-// floats of p's 16-byte group of memory before p
-__device__ __forceinline__ int shift_of(const float *p) { return (int)((unsigned long long)p >> 2) & 3; }
-// The 16-byte group of memory at src, of whose floats `left` lie before the row's end; zeros behind it.
-__device__ __forceinline__ void copy_group(float *dst, const float *src, int left) {
-    if (left > 0)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_at(dst)), "l"(src), "r"(left < 4 ? left * 4 : 16) : "memory");
-    else
-        *reinterpret_cast<float4 *>(dst) = make_float4(0.f, 0.f, 0.f, 0.f);
-}
-__device__ __forceinline__ void copy_float(float *dst, const float *src, bool in) {
-    if (in) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_at(dst)), "l"(src) : "memory");
-    else *dst = 0.f;
-}
-// A group that begins before its tensor does, `before` floats: only the floats of the tensor.
-__device__ __forceinline__ void copy_first_group(float *dst, const float *src, int before, int left) {
-    for (int c = before; c < 4; c++) copy_float(dst + c, src + c, c < left);
-}
 __device__ __forceinline__ float4 at4(const float *p) { return *reinterpret_cast<const float4 *>(p); }
 // four floats from p + shift on, p aligned
 __device__ __forceinline__ float4 at4(const float *p, int shift) {

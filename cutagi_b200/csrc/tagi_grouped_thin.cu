@@ -3,8 +3,9 @@
 // takes the time. Bound: HBM, 8 (forward) or 4 (state) bytes a weight.
 //
 // One CTA computes 128 features x all rows of an expert. The weights come through a ring of eight half-chunks (16 KiB each),
-// so that about 100 KB of each SM are on their way from HBM whatever the converters do: by TMA, or 4 bytes at a time with
-// cp.async where rows are not multiples of 16 bytes. Sixteen warps read them, a feature to a lane, and store the values' bf16
+// so that about 100 KB of each SM are on their way from HBM whatever the converters do: by TMA, or with cp.async, by the 16-byte
+// groups of memory that they lie in, where rows are not multiples of 16 bytes (30 rows of 4 experts of 2047 x 2047, forward: 122
+// us; 4 bytes at a time 140 us; of 2048 x 2048 82 us). Sixteen warps read them, a feature to a lane, and store the values' bf16
 // parts to tensor memory, where the MMAs take that operand from (through shared memory, its parts would be read six times
 // from there). Four more warps fetch and split the rows, which come from L2; eight add up the accumulators of chunks of 64
 // steps; one thread issues the MMAs. Mean and variance of a tile go to neighbouring CTAs at the same time, mu_w first in
@@ -25,7 +26,12 @@ constexpr int SUMMERS = 8, CONVERT_A = 16, CONVERT_B = 4, LOADERS = 2;
 constexpr int FIRST_A = SUMMERS, FIRST_B = FIRST_A + CONVERT_A, FIRST_LOADER = FIRST_B + CONVERT_B, ISSUER = FIRST_LOADER + LOADERS;
 constexpr int THREADS = 32 * (ISSUER + 2);       // the last warp works out the items
 constexpr int ROWS = 128, COLS = 48, KC = 64, HALF = 32, RING = 8, RECORDS = 4, CTAS = 148;
-constexpr uint32_t SLOT = 3 * COLS * KC * 2, RAW = ROWS * HALF * 4;   // the parts of a tile lie bn rows of 128 bytes apart
+constexpr uint32_t SLOT = 3 * COLS * KC * 2;   // the parts of a tile lie bn rows of 128 bytes apart
+// A half-chunk of weights. Lines that do not begin at multiples of 16 bytes take one 16-byte group more, begin up to three floats
+// behind their place, and are not swizzled: a pitch of 36 floats keeps eight lines off each other's banks as well.
+constexpr int FWD_PITCH = HALF + 4, STATE_PITCH = ROWS + 4;   // floats
+__host__ __device__ constexpr uint32_t raw_bytes(bool vec) { return vec ? ROWS * HALF * 4 : ROWS * FWD_PITCH * 4; }
+static_assert(HALF * STATE_PITCH * 4 <= raw_bytes(false), "");
 // tensor-memory columns: two slots of three accumulators, two slots of A's parts (two bf16 values a column)
 constexpr uint32_t ACC = 3 * COLS, A_PART = KC / 2, A_SLOT = 3 * A_PART, A_COL = 2 * ACC, TMEM_COLS = 512;
 static_assert(SLOT % 1024 == 0, "the swizzle counts lines from multiples of 1024 bytes");
@@ -90,9 +96,19 @@ __device__ __forceinline__ float4 lds4(uint32_t at) {
     return v;
 }
 
+// 16 bytes to shared memory, the last 16 - `bytes` of them zero, if `on`: no branch.
+__device__ __forceinline__ void copy16(uint32_t dst, const float *src, int bytes, bool on) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.s32 p, %3, 0;\n\t@p cp.async.cg.shared.global [%0], [%1], 16, %2;\n\t}" ::"r"(dst), "l"(src),
+                 "r"(bytes), "r"((int)on)
+                 : "memory");
+}
+// of a 16-byte group before whose end lie `floats` of a line's floats (any number)
+__device__ __forceinline__ int bytes_of(int floats) { return min(max(floats, 0), 4) * 4; }
+
 template <int PASS, bool VEC>
 __global__ void __launch_bounds__(THREADS, 1)
 grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_constant__ CUtensorMap var_map, const GroupedArgs a) {
+    constexpr uint32_t RAW = raw_bytes(VEC);
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u, ring = smem_base + 2 * SLOT;
     Shared &sh = *reinterpret_cast<Shared *>(smem_raw + (smem_base - smem_u32(smem_raw)) + 2 * SLOT + RING * RAW);
@@ -211,6 +227,14 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
         bool ok = true;
         for (int j = 0, i = 0; ok && take(sh, j, it) && it.chunks > 0; j++) {
             release(sh, j, lane);
+            int shift[4] = {};   // not aligned: of this lane's line (forward), of every fourth line (state)
+            if (!VEC) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const size_t line = (size_t)it.e * a.N * a.K + (PASS == FWD ? (size_t)(it.m0 + row) * a.K : (size_t)k * a.K + it.m0);
+                    shift[k] = PASS == FWD && k > 0 ? shift_of(a.var_w + line) : shift_of(a.mu_w + line);
+                }
+            }
             for (int c = 0; c < it.chunks; c++, i++) {
                 if ((i & 1) != slot) continue;
                 const int r = 2 * i + h;
@@ -223,17 +247,32 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
 #pragma unroll
                 for (int b = 0; b < HALF; b += 16) {   // sixteen steps at a time: two bf16 a column, eight columns a part
                     float v[16];
-                    if (PASS == FWD) {
+                    if (PASS == FWD && !VEC) {
+                        const int s4 = c >= it.nk ? shift[1] : shift[0];
+                        const bool one = s4 & 1, two = s4 & 2;
+                        float u[20];
+#pragma unroll
+                        for (int q = 0; q < 5; q++) {
+                            const float4 x = lds4(raw + row * (FWD_PITCH * 4) + (b + q * 4) * 4);
+                            u[q * 4] = x.x, u[q * 4 + 1] = x.y, u[q * 4 + 2] = x.z, u[q * 4 + 3] = x.w;
+                        }
+#pragma unroll
+                        for (int k = 0; k < 18; k++) u[k] = one ? u[k + 1] : u[k];
+#pragma unroll
+                        for (int k = 0; k < 16; k++) v[step_at<true>(k)] = two ? u[k + 2] : u[k];
+                    } else if (PASS == FWD) {
 #pragma unroll
                         for (int q = 0; q < 4; q++) {
                             const float4 x = lds4(raw + row * (HALF * 4) + (((b / 4 + q) ^ (row & 7)) << 4));
-                            // places of steps 4 q .. 4 q + 3 (step_at is its own inverse)
-                            v[step_at<!VEC>(q * 4)] = x.x, v[step_at<!VEC>(q * 4 + 1)] = x.y, v[step_at<!VEC>(q * 4 + 2)] = x.z, v[step_at<!VEC>(q * 4 + 3)] = x.w;
+                            v[q * 4] = x.x, v[q * 4 + 1] = x.y, v[q * 4 + 2] = x.z, v[q * 4 + 3] = x.w;
                         }
                     } else {
 #pragma unroll
                         for (int k = 0; k < 16; k++)
-                            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v[step_at<!VEC>(k)]) : "r"(raw + (b + k) * (ROWS * 4) + row * 4) : "memory");
+                            asm volatile("ld.shared.f32 %0, [%1];"
+                                         : "=f"(v[step_at<!VEC>(k)])   // its place (step_at is its own inverse)
+                                         : "r"(raw + (b + k) * ((VEC ? ROWS : STATE_PITCH) * 4) + (row + shift[k & 3]) * 4)
+                                         : "memory");
                     }
                     if (square) {
 #pragma unroll
@@ -323,21 +362,47 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
                         tma_load_3d(dst, second ? &var_map : &mean_map, PASS == FWD ? k0 : it.m0, PASS == FWD ? it.m0 : k0, it.e, sh.raw_full + r % RING);
                         continue;
                     }
-                    // a warp copies every other line (forward: 32 steps of a feature; state: 128 features of a step)
-                    const float *src = (second ? a.var_w : a.mu_w) + (size_t)it.e * a.N * a.K;
-                    const int n0 = PASS == FWD ? it.m0 : k0, k = (PASS == FWD ? k0 : it.m0) + lane, lines = min(PASS == FWD ? ROWS : HALF, a.N - n0);
-                    const float *p = src + (size_t)(n0 + w) * a.K + k;
-#pragma unroll 8
-                    for (int l = w; l < (PASS == FWD ? ROWS : HALF); l += 2, p += 2 * (size_t)a.K) {
-                        if (PASS == FWD) {
-                            const bool in = l < lines && k < a.K;
-                            cp_async_f32(dst + l * 128 + (((lane >> 2) ^ (l & 7)) << 4) + (lane & 3) * 4, in ? p : src, in);
-                        } else {
+                    // 16-byte groups of lines: forward, 32 steps of a feature, by eight lanes; state, 128 features of a step, by a
+                    // warp; then the lines' last groups. Lines eight (four) apart begin equally far from a multiple of 16 bytes.
+                    const float *w0 = second ? a.var_w : a.mu_w, *safe = w0 - shift_of(w0);   // an address for copies of nothing
+                    const float *src = w0 + (size_t)it.e * a.N * a.K + (size_t)(PASS == FWD ? it.m0 : k0) * a.K + (PASS == FWD ? k0 : it.m0);
+                    const int lines = a.N - (PASS == FWD ? it.m0 : k0), live = a.K - (PASS == FWD ? k0 : it.m0), x = w * 32 + lane;
+                    if (PASS == FWD) {
+                        const int l = x >> 3, g = (x & 7) * 4;
+                        const float *p = src + (size_t)l * a.K;
+                        const int shift = shift_of(p), bytes = bytes_of(live + shift - g);
+                        p += g - shift;
+                        const uint32_t d = dst + (l * FWD_PITCH + g) * 4;
+                        const bool begins = p < w0;   // the tensor begins within the group
+                        if (begins)
+                            for (int y = 1; y < 4; y++) cp_async_f32(d + y * 4, y >= shift ? p + y : w0, y >= shift && y < live + shift);
+                        copy16(d, bytes ? p : safe, bytes, l < lines && !begins);
 #pragma unroll
-                            for (int q = 0; q < 4; q++) {
-                                const bool in = l < lines && k + q * 32 < a.K;
-                                cp_async_f32(dst + l * 512 + (q * 32 + lane) * 4, in ? p + q * 32 : src, in);
-                            }
+                        for (int i = 1; i < 16; i++) copy16(d + i * 8 * FWD_PITCH * 4, (bytes ? p : safe) + (bytes ? (size_t)i * 8 * a.K : 0), bytes, l + i * 8 < lines);
+#pragma unroll
+                        for (int i = 0; i < 2; i++) {
+                            const float *q = src + (size_t)(x + i * 64) * a.K;
+                            const int n = bytes_of(live + shift_of(q) - HALF);
+                            copy16(dst + ((x + i * 64) * FWD_PITCH + HALF) * 4, n ? q - shift_of(q) + HALF : safe, n, x + i * 64 < lines);
+                        }
+                    } else {
+                        const int g = lane * 4;
+                        const float *p = src + (size_t)w * a.K, *p2 = p + 2 * (size_t)a.K;
+                        const int shift = shift_of(p), shift2 = shift_of(p2), bytes = bytes_of(live + shift - g), bytes2 = bytes_of(live + shift2 - g);
+                        p += g - shift, p2 += g - shift2;
+                        const uint32_t d = dst + (w * STATE_PITCH + g) * 4;
+                        const bool begins = p < w0;
+                        if (begins)
+                            for (int y = 1; y < 4; y++) cp_async_f32(d + y * 4, y >= shift ? p + y : w0, y >= shift && y < live + shift);
+#pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            const int n = w + i * 2 < lines ? (i & 1 ? bytes2 : bytes) : 0;   // zeros for steps behind the last
+                            copy16(d + i * 2 * STATE_PITCH * 4, n ? (i & 1 ? p2 : p) + (size_t)(i / 2 * 4) * a.K : safe, n, i > 0 || !begins);
+                        }
+                        if (w == 0) {
+                            const float *q = src + (size_t)lane * a.K;
+                            const int n = lane < lines ? bytes_of(live + shift_of(q) - ROWS) : 0;
+                            copy16(dst + (lane * STATE_PITCH + ROWS) * 4, n ? q - shift_of(q) + ROWS : safe, n, true);
                         }
                     }
                     cp_async_arrive(sh.raw_full + r % RING);
@@ -408,10 +473,10 @@ int make_map(int pass, const GroupedArgs &a, const float *w, CUtensorMap *map) {
 
 template <int PASS>
 int launch_thin(const GroupedArgs &a, cudaStream_t st) {
-    const size_t smem = 2 * SLOT + RING * RAW + 1024 + sizeof(Shared) + (a.E + 1) * sizeof(int);
+    const bool vec = grouped_aligned(PASS, a);
+    const size_t smem = 2 * SLOT + RING * raw_bytes(vec) + 1024 + sizeof(Shared) + (a.E + 1) * sizeof(int);
     const long mt = ((PASS == FWD ? a.N : a.K) + ROWS - 1) / ROWS, experts = a.E < a.S / (a.few + 1) ? a.E : a.S / (a.few + 1);
     const long most = 2 * mt * experts;   // experts with more than `few` rows, at most; both kinds
-    const bool vec = grouped_aligned(PASS, a);
     CUtensorMap mean = {}, var = {};
     int rc;
     if (vec && (rc = make_map(PASS, a, a.mu_w, &mean)) != TAGI_OK) return rc;
