@@ -643,6 +643,45 @@ def test_captured_calls_replay_on_new_inputs(lib, T):
             assert all(torch.equal(a, b) for a, b in zip(got, ref))
 
 
+def test_cut_tiles_repeat_in_graphs_and_beside_each_other(lib):
+    """Tiles that are cut along the contraction: the same bits in a graph whose row counts change, twice at the same time."""
+    from cutagi_b200 import ops
+
+    def call(x):
+        return [*ops.grouped_linear(x["w"], x["vw"], x["b"], x["vb"], x["a"], x["va"], x["o"]),
+                *ops.grouped_linear_state(x["w"], None, x["dm"], x["dv"], x["o"]),
+                *ops.grouped_linear_param(x["vw"], x["vb"], x["a"], x["dm"], x["dv"], x["o"])]
+
+    def inputs(seed, counts, K=2000, N=1900):
+        g = Gen(seed)
+        o, S = spread(counts)
+        return dict(w=g.n(2, N, K, scale=0.02), vw=g.u(2, N, K, hi=1e-3), b=g.n(2, N), vb=g.u(2, N), a=g.n(S, K), va=g.u(S, K),
+                    dm=g.n(S, N), dv=g.u(S, N), o=o)
+    xs = [inputs(1, [300, 500]), inputs(2, [700, 100])]
+    graphs, outs = [], []
+    call(xs[0])
+    torch.cuda.synchronize()
+    for x in xs:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs.append(call(x))
+        graphs.append(gr)
+    for counts in ([60, 740], [0, 800], [400, 400]):
+        want = []
+        for i, x in enumerate(xs):
+            new = inputs(i + 7, counts)
+            for name, t in new.items():
+                x[name].copy_(t)
+            want.append([t.clone() for t in call(new)])
+        torch.cuda.synchronize()
+        for gr in graphs:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                gr.replay()
+        torch.cuda.synchronize()
+        for got, ref in zip(outs, want):
+            assert all(torch.equal(a, b) for a, b in zip(got, ref))
+
+
 def test_calls_follow_the_current_stream(lib):
     """Inputs that are written late on a side stream are seen by calls on that stream, with other calls on a second stream."""
     from cutagi_b200 import ops
