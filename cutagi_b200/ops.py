@@ -11,12 +11,13 @@ from . import capi
 
 _F, _I = torch.float32, torch.int32
 _MOST = 2 ** 31 - 1   # the entry points' sizes are 32-bit integers, which ctypes would cut without a word
-_stream = torch._C._cuda_getCurrentRawStream   # of a device; torch.cuda.current_stream makes an object of it first
+# what torch.cuda.current_stream and current_device come down to
+_stream, _device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
 def _run(name, index, *args):
     """Calls the entry point with device `index` current, on its current stream; raises TagiError on a bad status."""
-    if index != torch.cuda.current_device():
+    if index != _device():
         with torch.cuda.device(index):
             return _run(name, index, *args)
     lib = capi.load()
@@ -97,12 +98,16 @@ def layer_norm_backward(mu_w, var_w, var_b, mu_a, jcb, mu_row, var_row, dmu_o, d
               _p("jcb", jcb, s, i), _p("mu_row", mu_row, (R,), i), _p("var_row", var_row, (R,), i), _p("dmu_o", dmu_o, s, i),
               _p("dvar_o", dvar_o, s, i))
     if out is None:
-        out = (*_two(mu_w), *(_two(mu_w) if bias else (None, None)))
+        out = mu_w.new_empty(4 if bias else 2, n).unbind(0)
+        outputs = [t.data_ptr() for t in out] if bias else (out[0].data_ptr(), out[1].data_ptr(), None, None)
+        out = out if bias else (*out, None, None)
+    else:
+        outputs = [_p(f"out[{k}]", t, f, i) for k, t in enumerate(out)]
     dmu, dvar = _two(mu_a) if state_update else (None, None)
+    state = (dmu.data_ptr(), dvar.data_ptr()) if state_update else (None, None)
     nbytes = capi.load().tagi_ln_bwd_workspace_bytes(R, n)
     keep, ws = _workspace(nbytes, mu_a)
-    _run("tagi_ln_bwd", i, R, n, int(bias), int(state_update), eps, *inputs, _p("dmu", dmu, s, i), _p("dvar", dvar, s, i),
-         _p("out[0]", out[0], f, i), _p("out[1]", out[1], f, i), _p("out[2]", out[2], f, i), _p("out[3]", out[3], f, i), ws, nbytes)
+    _run("tagi_ln_bwd", i, R, n, int(bias), int(state_update), eps, *inputs, *state, *outputs, ws, nbytes)
     return (dmu, dvar, *out)
 
 
@@ -181,10 +186,12 @@ def grouped_linear_param(var_w, var_b, mu_a, dmu_z, dvar_z, offsets, token=None,
               _p("mu_a", mu_a, (R, K), i), _p("dmu_z", dmu_z, (S, N), i), _p("dvar_z", dvar_z, (S, N), i))
     if out is None:
         out = (*_two(var_w), *(_two(var_b) if bias else (None, None)))
+        outputs = [None if t is None else t.data_ptr() for t in out]
+    else:
+        outputs = [_p(f"out[{k}]", t, w if k < 2 else b, i) for k, t in enumerate(out)]
     nbytes = capi.load().tagi_grouped_linear_workspace_bytes(2, E, S, R, K, N)
     keep, ws = _workspace(nbytes, var_w)
-    _run("tagi_grouped_linear_bwd_param", i, E, S, R, K, N, int(bias), *inputs, _p("out[0]", out[0], w, i), _p("out[1]", out[1], w, i),
-         _p("out[2]", out[2], b, i), _p("out[3]", out[3], b, i), ws, nbytes)
+    _run("tagi_grouped_linear_bwd_param", i, E, S, R, K, N, int(bias), *inputs, *outputs, ws, nbytes)
     return tuple(out)
 
 
