@@ -15,13 +15,17 @@
 // var_w.(mu_a^2 + var_a) as one contraction of twice the length), which neighbouring pairs do at the same time: mu_w is
 // fetched from HBM for one and found in L2 by the other.
 //
-// Roles. Eight converter warps fetch both operands from global memory into registers (gathered rows, ragged edges and any
-// alignment cost nothing extra there), form squares, split and store the parts to shared memory in the swizzled layouts
-// the tensor core reads; half a chunk ahead is in flight. Eight summing warps add each chunk's accumulator to their
-// registers and write finished tiles out. One thread issues the MMAs. Two slots of 64 contraction steps hold 2 x 96 KiB of
-// operands and two accumulators of 256 columns fill tensor memory; a slot's "full" barrier counts the converters (operands
-// written) and the summing warps (accumulator read), its "done" barrier the MMAs' completion. Nothing stops at a tile's
-// end: the next tile's operands are converted while the last one's chunks multiply and its sums are written.
+// Roles. Four warps fetch A from global memory into registers, four B (gathered rows, ragged edges and any alignment cost
+// nothing extra there), a chunk at a time; they form squares, split, and store the parts to shared memory in the swizzled layouts
+// the tensor core reads. Eight summing warps add each chunk's accumulator to their registers and write finished tiles out. One
+// thread issues the MMAs, and a warp works out the items ahead of the others. Two slots of 64 contraction steps hold 2 x 96
+// KiB of operands and two accumulators of 256 columns fill tensor memory; a slot's "full" barrier counts the converters
+// (operands written) and the summing warps (accumulator read), its "done" barrier the MMAs' completion. Nothing stops at a
+// tile's end: the next tile's operands are converted while the last one's chunks multiply and its sums are written.
+//
+// Bound by the tensor cores (and the power cap) from about 250 rows an expert on; by the converters with fewer (100 rows: 5000
+// cycles a chunk, 1200 to issue its loads, 1500 until the values are there, 1200 to split and store them); by the output of
+// the tiles in the parameter pass of few rows (12 bytes a weight).
 #include "tagi_grouped_split.cuh"
 
 #include <cstddef>
@@ -172,23 +176,38 @@ __device__ __forceinline__ bool get_item(const GroupedArgs &a, Shared &sh, Plan 
 //  loads 64 consecutive bytes of eight rows and stores to all banks.
 //  MN-major: line = 64 rows of one step; the 64 lines of rows 0..63 come before those of rows 64..127. Task t: step
 //  4 t + row(), rows along() + 0..3; a warp loads 512 consecutive bytes.
-template <bool MN>
+// Rows that are not aligned to 16 bytes are read a float at a time, and a warp's loads have to be neighbours all the same (the
+// load unit takes a line of memory at a time). Neither the order of the steps nor that of the features matters to a sum:
+//  forward pass, both operands: the order of step_at(); four lanes read neighbours.
+//  state pass (WIDE), B: place 4 i + c of a line holds step i + 16 c, so that sixteen lanes read neighbours. Task t: row 8 t +
+//  row(). A: its steps lie in the same order, and place 4 i + c of the CTA's 128 features holds feature i + 32 c. 3000 rows of 5
+//  experts, 1001 to 1515 features: 168 us; 185 us without. In the other passes this was slower (forward: a thread then has
+//  sixteen gathered rows; parameters: their output is scattered).
+template <bool MN, bool SPREAD, bool WIDE>
 struct Place {
     static constexpr uint32_t KSTEP = (MN ? 16 * 128 : 32) >> 4;             // 16 contraction steps, in 16-byte units
-    static constexpr uint32_t LBO = MN ? 64 * 128 : 16, SBO = 1024;
-    __device__ static int row(int warp, int lane) { return MN ? warp : warp * 8 + ((lane >> 2) & 3) * 2 + (lane >> 4); }
-    // first of a thread's four values along memory; SPREAD: see step_at()
-    template <bool SPREAD>
-    __device__ static int along(int lane) { return MN ? lane * 4 : SPREAD ? lane & 3 : (lane & 3) * 4; }
+    static constexpr uint32_t LBO = MN ? 64 * 128 : 16;
+    static constexpr bool LINE = !MN && WIDE;
+    static constexpr int STRIDE = MN ? WIDE ? 32 : 1 : WIDE ? 16 : SPREAD ? 4 : 1;   // of a thread's four values along memory
+    __device__ static int row(int warp, int lane) { return MN ? warp : LINE ? warp * 2 + (lane >> 4) : warp * 8 + ((lane >> 2) & 3) * 2 + (lane >> 4); }
+    __device__ static int along(int lane) { return MN ? WIDE ? lane : lane * 4 : LINE ? lane & 15 : SPREAD ? lane & 3 : (lane & 3) * 4; }
     __device__ static uint32_t base(int warp, int lane) {
-        const uint32_t r = row(warp, lane), c = MN ? (lane & 15) >> 1 : (lane & 3) >> 1;
+        const uint32_t r = row(warp, lane), c = (MN || LINE ? lane & 15 : lane & 3) >> 1;
         return (MN ? (lane >> 4) * 8192u : 0u) + r * 128 + ((c ^ (r & 7)) << 4) + (lane & 1) * 8;
     }
     // where task t goes, from base(): the swizzle's exclusive or with the bits of t that change the chunk or the line
     __device__ static uint32_t at(uint32_t base, int t) {
-        return MN ? (base ^ ((t & 1) << 6)) + t * 512 : (base ^ ((t & 3) << 5)) + (t >> 2) * 4096;
+        return LINE ? base + t * 1024 : MN ? (base ^ ((t & 1) << 6)) + t * 512 : (base ^ ((t & 3) << 5)) + (t >> 2) * 4096;
     }
 };
+template <int PASS, bool VEC>
+constexpr bool wide = !VEC && PASS == STATE;
+template <int PASS, bool VEC>
+using PlaceA = Place<PASS != FWD, !VEC && PASS == FWD, wide<PASS, VEC>>;
+template <int PASS, bool VEC>
+using PlaceB = Place<PASS == PARAM, !VEC && PASS == FWD, wide<PASS, VEC>>;
+// Feature (of the CTA's 128) at place p.
+__device__ __forceinline__ int feature_at(bool mix, int p) { return mix ? (p & 3) * 32 + (p >> 2) : p; }
 
 // Item j, as it was handed over; false when the CTA is aborting. release(): this warp needs the record no longer.
 __device__ __forceinline__ bool take(Shared &sh, int j, Item &t) {
@@ -230,10 +249,9 @@ __device__ __forceinline__ Piece *piece_of(const GroupedArgs &a, int pairs, int 
 // latency a chunk: loads that are waited for in turn would cost one each).
 template <int PASS, bool VEC>
 __device__ __forceinline__ void convert_a(const GroupedArgs &a, Shared &sh, int cta, int w, int lane, uint32_t smem_base) {
-    constexpr bool MN = PASS != FWD;
-    constexpr bool SPREAD = !VEC && PASS != PARAM;   // state pass, experts of 2048 rows of 2046: 456 us; without 557 us
-    using P = Place<MN>;
-    const int row = P::row(w, lane), along = P::template along<SPREAD>(lane);
+    constexpr bool MN = PASS != FWD, WIDE = wide<PASS, VEC>;
+    using P = PlaceA<PASS, VEC>;
+    const int row = P::row(w, lane), along = P::along(lane);
     const uint32_t to = smem_base + P::base(w, lane);
     float4 v[TASKS];
     Cursor cu;
@@ -273,15 +291,20 @@ __device__ __forceinline__ void convert_a(const GroupedArgs &a, Shared &sh, int 
 #pragma unroll
         for (int g = 0; g < 4; g++) {
             const float *src = PASS == FWD ? (cu.var && cu.half ? a.var_w : a.mu_w) + base + cu.kc + (size_t)(g * 32) * a.K
-                               : PASS == STATE ? a.mu_w + base + (size_t)(cu.kc + g * 16) * a.K : a.x + base;
+                               : PASS == STATE ? a.mu_w + base + (size_t)cu.kc * a.K : a.x + base;
             int4 r = make_int4(-1, -1, -1, -1);
             if (PASS == PARAM) r = *reinterpret_cast<const int4 *>(&sh.rows[w][g * 4]);
 #pragma unroll
             for (int s = 0; s < 4; s++) {
                 const int rs = s == 0 ? r.x : s == 1 ? r.y : s == 2 ? r.z : r.w;
-                if (PASS == FWD) v[g * 4 + s] = ld4<VEC, SPREAD ? 4 : 1>(src + s * 16, g * 32 < left ? a.K - cu.kc - along - s * 16 : 0);
-                else if (PASS == STATE) v[g * 4 + s] = ld4<VEC>(src + (size_t)step_at<SPREAD>(s * 4 + row) * a.K, cu.kc + g * 16 + step_at<SPREAD>(s * 4 + row) < a.N ? left : 0);
-                else v[g * 4 + s] = ld4<VEC>(src + (size_t)max(rs, 0) * a.K, rs >= 0 ? left : 0);
+                if (PASS == FWD) {
+                    v[g * 4 + s] = ld4<VEC, P::STRIDE>(src + s * 16, g * 32 < left ? a.K - cu.kc - along - s * 16 : 0);
+                } else if (PASS == STATE) {
+                    const int k = WIDE ? row * 16 + g * 4 + s : g * 16 + s * 4 + row;
+                    v[g * 4 + s] = ld4<VEC, P::STRIDE>(src + (size_t)k * a.K, cu.kc + k < a.N ? left : 0);
+                } else {
+                    v[g * 4 + s] = ld4<VEC>(src + (size_t)max(rs, 0) * a.K, rs >= 0 ? left : 0);
+                }
             }
         }
     };
@@ -306,9 +329,8 @@ __device__ __forceinline__ void convert_a(const GroupedArgs &a, Shared &sh, int 
 template <int PASS, bool VEC>
 __device__ __forceinline__ void convert_b(const GroupedArgs &a, Shared &sh, int cta, int w, int lane, uint32_t smem_base) {
     constexpr bool MN = PASS == PARAM;
-    constexpr bool SPREAD = !VEC && PASS != PARAM;
-    using P = Place<MN>;
-    const int row = P::row(w, lane), along = P::template along<SPREAD>(lane);
+    using P = PlaceB<PASS, VEC>;
+    const int row = P::row(w, lane), along = P::along(lane);
     const uint32_t to = smem_base + 3 * PART + P::base(w, lane);
     float4 v[TASKS];
     Cursor cu;
@@ -350,9 +372,15 @@ __device__ __forceinline__ void convert_b(const GroupedArgs &a, Shared &sh, int 
                                        : (cu.var ? a.a1 : a.a0) + base + (PASS == STATE ? (size_t)(g * 32) * a.N + cu.kc : (size_t)(cu.kc + g * 16) * a.N);
 #pragma unroll
         for (int s = 0; s < 4; s++) {
-            if (PASS == FWD) v[g * 4 + s] = ld4<VEC, SPREAD ? 4 : 1>(src + s * 16, rows[g] >= 0 ? a.K - cu.kc - along - s * 16 : 0);
-            else if (PASS == STATE) v[g * 4 + s] = ld4<VEC, SPREAD ? 4 : 1>(src + s * 16, g * 32 < left ? a.N - cu.kc - along - s * 16 : 0);
-            else v[g * 4 + s] = ld4<VEC>(src + (size_t)(s * 4) * a.N, cu.kc + (g * 4 + s) * 4 + row < depth ? left : 0);
+            if (P::LINE) {
+                v[g * 4 + s] = ld4<VEC, P::STRIDE>(src + (size_t)(s * 8) * a.N, g * 32 + s * 8 < left ? a.N - cu.kc - along : 0);
+            } else if (PASS == FWD) {
+                v[g * 4 + s] = ld4<VEC, P::STRIDE>(src + s * 16, rows[g] >= 0 ? a.K - cu.kc - along - s * 16 : 0);
+            } else if (PASS == STATE) {
+                v[g * 4 + s] = ld4<VEC>(src + s * 16, g * 32 < left ? a.N - cu.kc - along - s * 16 : 0);
+            } else {
+                v[g * 4 + s] = ld4<VEC>(src + (size_t)(s * 4) * a.N, cu.kc + (g * 4 + s) * 4 + row < depth ? left : 0);
+            }
         }
     };
     seek(0);
@@ -369,7 +397,7 @@ __device__ __forceinline__ void convert_b(const GroupedArgs &a, Shared &sh, int 
             if (MN || g * 32 < lines) {   // narrow tiles have no columns for the later groups
 #pragma unroll
                 for (int q = g * 4; q < g * 4 + 4; q++)
-                    if (MN ? along < round_up(lines, 64) : g * 32 + row < lines) store_split(P::at(to + s * SLOT, q), PART, v[q]);
+                    if (MN ? along < round_up(lines, 64) : P::LINE ? q * 8 < lines : g * 32 + row < lines) store_split(P::at(to + s * SLOT, q), PART, v[q]);
             }
         fence_proxy_async_smem();
         __syncwarp();
@@ -411,8 +439,8 @@ __device__ __forceinline__ void convert_b(const GroupedArgs &a, Shared &sh, int 
 template <int PASS, bool VEC>
 __global__ void __launch_bounds__(THREADS, 1) grouped_tc_kernel(const GroupedArgs a) {
     constexpr bool A_MN = PASS != FWD, B_MN = PASS == PARAM;
-    using PA = Place<A_MN>;   // layouts of the operands
-    using PB = Place<B_MN>;
+    using PA = PlaceA<PASS, VEC>;   // layouts of the operands
+    using PB = PlaceB<PASS, VEC>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     Shared &sh = *reinterpret_cast<Shared *>(smem_raw + (smem_base - smem_u32(smem_raw)) + 2 * SLOT);
@@ -480,7 +508,7 @@ __global__ void __launch_bounds__(THREADS, 1) grouped_tc_kernel(const GroupedArg
                 const uint32_t idesc = make_idesc_bf16(256, it.bn, A_MN, B_MN);
                 for (int c = it.from; c < it.from + it.chunks; c++, i++) {
                     const int s = i & 1, left = it.depth - (c >= it.nk ? c - it.nk : c) * KC;
-                    const int steps = max(1, min(KC / 16, (left + 15) / 16));
+                    const int steps = wide<PASS, VEC> ? KC / 16 : max(1, min(KC / 16, (left + 15) / 16));
                     ok = mbar_wait_cluster(sh.full + s, (i >> 1) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_CONV);
                     if (!ok) break;
                     tc_fence_after_sync();
@@ -546,7 +574,7 @@ __global__ void __launch_bounds__(THREADS, 1) grouped_tc_kernel(const GroupedArg
             Output o;
             const int per = t.bn >> 1, first = group * per;
             o.n = min(per, t.cols - first);
-            o.m = t.m0 + cta * 128 + quad * 32 + lane;
+            o.m = t.m0 + cta * 128 + feature_at(wide<PASS, VEC>, quad * 32 + lane);
             o.ld = PASS == FWD ? a.N : a.K;
             o.kind = t.kind, o.e = t.e;
             if (o.m >= o.ld) o.n = 0;
@@ -647,7 +675,7 @@ __global__ void __launch_bounds__(THREADS, 1) grouped_tc_kernel(const GroupedArg
 // pair's partial sum that begins a tile, the others do nothing; blockIdx.y: eight columns of it. A thread has a feature.
 constexpr int JOIN_COLUMNS = 8;
 template <int PASS>
-__global__ void __launch_bounds__(256) grouped_join_kernel(const GroupedArgs a, int pairs) {
+__global__ void __launch_bounds__(256) grouped_join_kernel(const GroupedArgs a, int pairs, bool mix) {
     const int pair = blockIdx.x, x0 = blockIdx.y * JOIN_COLUMNS;
     const Piece t = *piece_of(a, pairs, pair, BEGIN);
     if (!t.used || x0 >= t.cols) return;
@@ -672,7 +700,7 @@ __global__ void __launch_bounds__(256) grouped_join_kernel(const GroupedArgs a, 
         const float vb = __ldg(a.var_b + o);
         (t.kind == VAR ? a.ob1 : a.ob0)[o] = t.kind == VAR ? vb * vb * bias : vb * bias;
     }
-    const int m = t.m0 + threadIdx.x, ld = PASS == FWD ? a.N : a.K;
+    const int m = t.m0 + (threadIdx.x & 128) + feature_at(mix, threadIdx.x & 127), ld = PASS == FWD ? a.N : a.K;
     if (m >= ld) return;
     const size_t base = ((PASS == PARAM ? (size_t)t.e * a.N : 0) + t.c0 + x0) * ld + m;
     const float *scale = PASS == PARAM ? a.var_w : a.jcb;
@@ -729,7 +757,7 @@ int launch_pass(const GroupedArgs &a, cudaStream_t st) {
     auto k = vec ? grouped_tc_kernel<PASS, true> : grouped_tc_kernel<PASS, false>;
     TAGI_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     TAGI_CUDA(cudaLaunchKernelEx(&cfg, k, a));
-    grouped_join_kernel<PASS><<<dim3(pairs, 256 / JOIN_COLUMNS), 256, 0, st>>>(a, pairs);
+    grouped_join_kernel<PASS><<<dim3(pairs, 256 / JOIN_COLUMNS), 256, 0, st>>>(a, pairs, vec ? wide<PASS, true> : wide<PASS, false>);
     TAGI_CUDA(cudaGetLastError());
     return TAGI_OK;
 }
