@@ -781,12 +781,12 @@ int launch_pass(const GroupedArgs &a, int above, int upto, cudaStream_t st) {
     TAGI_CUDA(cudaGetLastError());
     return TAGI_OK;
 }
-// Narrow tiles for experts of up to 128 rows, if most are so small on the average: a kernel that finds nothing to do takes 7 us
-// with its join. The kernels follow one another and use the same workspace. Eight experts of 4096 x 4096, forward pass, 56 /
+// Narrow tiles for experts of up to 128 rows, where the average expert makes some likely: a kernel that finds nothing to do takes
+// 7 us with its join. The kernels follow one another and use the same workspace. Eight experts of 4096 x 4096, forward pass, 56 /
 // 100 / 128 rows each: 546 / 653 / 697 us, with wide tiles 813 / 843 / 862 us; state pass 352 / 421 / 454 and 477 / 516 / 529.
 template <int PASS>
 int launch_rows(const GroupedArgs &a, cudaStream_t st) {
-    if (a.S > (NARROW_ROWS + 32) * a.E) return launch_pass<PASS, false>(a, a.thin, a.S, st);
+    if (a.S <= THIN_ROWS / 2 * a.E || a.S > (NARROW_ROWS + 32) * a.E) return launch_pass<PASS, false>(a, a.thin, a.S, st);
     int rc = launch_pass<PASS, true>(a, a.thin, NARROW_ROWS, st);
     if (rc != TAGI_OK || a.S <= NARROW_ROWS) return rc;
     return launch_pass<PASS, false>(a, NARROW_ROWS, a.S, st);
