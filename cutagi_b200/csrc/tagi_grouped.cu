@@ -19,10 +19,12 @@ int run(int pass, GroupedArgs &a, cudaStream_t st) {
 bool sizes_fit(int E, int S, int K, int N) {
     return E >= 1 && E <= 1024 && S >= 0 && S <= (1 << 28) && K >= 1 && K <= (1 << 20) && N >= 1 && N <= (1 << 20);
 }
-// Workspace: partial sums of the tensor-core kernel, then, forward, mu_a^2 + var_a; nothing where the number of rows in all
-// rules these kernels out.
+// Workspace: partial sums of the tensor-core kernels, which use it one after the other, then, forward, mu_a^2 + var_a; nothing
+// where the number of rows in all rules these kernels out.
 size_t parts_bytes(int pass, int E, int S, int K, int N) {
-    return S <= (pass == PARAM ? FEW_PARAM_ROWS : THIN_ROWS) ? 0 : grouped_tc_parts_bytes(pass, E, S, K, N);
+    const size_t thin = pass == PARAM || S <= FEW_ROWS ? 0 : grouped_thin_parts_bytes(pass, E, S, K, N);
+    const size_t tc = S <= (pass == PARAM ? FEW_PARAM_ROWS : THIN_ROWS) ? 0 : grouped_tc_parts_bytes(pass, E, S, K, N);
+    return thin > tc ? thin : tc;
 }
 size_t second_bytes(int S, int R, int K) { return S <= FEW_ROWS ? 0 : (size_t)R * K * sizeof(float); }
 

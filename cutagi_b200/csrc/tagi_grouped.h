@@ -12,7 +12,7 @@ struct GroupedArgs {
     const int *offsets, *token;
     // a0, a1: activations (forward) or deltas (backward); x: input means of the parameter pass
     const float *mu_w, *var_w, *mu_b, *var_b, *a0, *a1, *jcb, *x;
-    // workspaces, 16-byte aligned: partial sums of the tiles that tagi_grouped_tc.cu cuts; forward, mu_a^2 + var_a [R][K]
+    // workspaces, 16-byte aligned: partial sums of the tiles that are cut; forward, mu_a^2 + var_a [R][K]
     float *parts, *second;
     float *o0, *o1, *ob0, *ob1;
 };
@@ -70,6 +70,7 @@ inline bool grouped_aligned(int pass, const GroupedArgs &a) {
 int grouped_second_moment(const GroupedArgs &a, cudaStream_t st);
 int grouped_few(int pass, const GroupedArgs &a, cudaStream_t st);
 int grouped_thin(int pass, const GroupedArgs &a, cudaStream_t st);
+size_t grouped_thin_parts_bytes(int pass, int E, int S, int K, int N);   // forward and state pass
 int grouped_thin_status(int *out, int reset);
 int grouped_tc(int pass, const GroupedArgs &a, cudaStream_t st);
 int grouped_tc_pairs(int pass, int E, int S, int K, int N);

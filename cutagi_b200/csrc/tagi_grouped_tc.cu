@@ -27,6 +27,7 @@
 // Bound by the tensor cores (and the power cap) from about 250 rows an expert on; by the converters with fewer (wide tiles, 100
 // rows: 5000 cycles a chunk, 1200 to issue its loads, 1500 until the values are there, 1200 to split and store them); by the output of
 // the tiles in the parameter pass of few rows (12 bytes a weight).
+#include "tagi_grouped_plan.cuh"
 #include "tagi_grouped_split.cuh"
 
 #include <cstddef>
@@ -54,7 +55,6 @@ constexpr int KC = 64;                          // contraction steps of a chunk
 constexpr uint32_t PART = 128 * KC * 2;         // one bf16 part of 128 rows (or columns) of a chunk: 16 KiB
 constexpr uint32_t SLOT = 6 * PART;             // hi, mid, lo of A, then of B
 constexpr uint32_t ACC = 256;                   // tensor-memory columns of a slot's accumulator
-constexpr int MEAN = 0, VAR = 1;
 constexpr int PAIRS = 74;
 
 __device__ int g_status;  // first wait that ran out, read and cleared by grouped_tc_status
@@ -71,8 +71,7 @@ struct Record {
     int rows[128];              // forward pass: input rows of this CTA's columns, -1 where there is none
 };
 constexpr int RECORDS = 8;
-constexpr int WHOLE = -1, LATER = 0, BEGIN = 1;
-constexpr int CUT_SAVES = 8;
+constexpr int CUT_SAVES = 8;    // chunks that cutting has to save (see tagi_grouped_plan.cuh): it costs about 10 us, the time of four
 
 struct Shared {                 // behind the slots
     uint64_t full[2], done[2], item_full[RECORDS], item_empty[RECORDS], turn;
@@ -87,8 +86,7 @@ struct Shared {                 // behind the slots
 };
 static_assert(offsetof(Shared, rows) % 16 == 0 && sizeof(Shared) % 8 == 0, "rows are read 16 bytes at a time");
 
-// Work list: the two kinds of every tile are neighbours, so two pairs work on the same weights at the same time, and a pair's
-// kinds alternate from one item to the next (in the forward pass a variance costs twice a mean).
+// The mean or the variance of tile t.
 template <int PASS, bool NARROW>
 __device__ __forceinline__ void tile_item(const GroupedArgs &a, const int *before, int t, int kind, Item &it) {
     it.kind = kind;
@@ -114,69 +112,19 @@ __device__ __forceinline__ void tile_item(const GroupedArgs &a, const int *befor
     it.part = WHOLE;
 }
 
-// The items go round the pairs; what is left when the rounds no longer fill the GPU is cut along the contraction, so that
-// all pairs get the same number of chunks: each pair has at most the end of one tile (LATER) and the beginning of another
-// (BEGIN), whose sums go to the workspace, and grouped_join_kernel adds up and writes out the tiles that were cut.
-// 3000 rows of 5 experts, 1001 to 1515 features, forward: 267 us whole, 216 us cut; 7288 rows of 2 experts, 16 to 75 features,
-// parameter pass: 174 and 47 us.
-struct Plan {
-    int items, whole;   // all items; those that go round
-    int chunks;         // of the items that are cut; -1: not looked at yet
-};
-__device__ __forceinline__ int kind_of(int i, int pairs) { return (i + 2 * (i >> 1) / pairs) & 1; }
-
-// Whether the rest is cut. Called by one whole warp, when the whole rounds have been handed out.
-template <int PASS, bool NARROW>
-__device__ __forceinline__ void look_at_rest(const GroupedArgs &a, Shared &sh, int pairs, Plan &p) {
-    const int lane = threadIdx.x & 31;
-    int carry = 0, longest = 0;
-    for (int j0 = 0; j0 < p.items - p.whole; j0 += 32) {
-        const int j = j0 + lane, i = p.whole + j;
-        Item it;
-        it.chunks = 0;
-        if (i < p.items) tile_item<PASS, NARROW>(a, sh.before, i >> 1, kind_of(i, pairs), it);
-        int sum = it.chunks;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int u = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += u;
-        }
-        if (i < p.items) sh.start[j] = carry + sum - it.chunks;
-        longest = max(longest, __reduce_max_sync(0xffffffffu, it.chunks));
-        carry += __shfl_sync(0xffffffffu, sum, 31);
-    }
-    if (lane == 0) sh.start[p.items - p.whole] = carry;
-    __syncwarp();
-    // cutting costs about 10 us, the time of four chunks; uncut, the last round takes as long as its longest item
-    const bool cut = longest - (carry + pairs - 1) / pairs >= CUT_SAVES;
-    p.chunks = cut ? carry : 0;
-    if (!cut) p.whole = p.items;
-}
-
-// Item j of pair `pair`.
+// Item j of pair `pair`. Cut tiles: 3000 rows of 5 experts, 1001 to 1515 features, forward: 267 us whole, 216 us cut; 7288 rows of
+// 2 experts, 16 to 75 features, parameter pass: 174 and 47 us.
 template <int PASS, bool NARROW>
 __device__ __forceinline__ bool get_item(const GroupedArgs &a, Shared &sh, Plan &p, int pair, int pairs, int j, Item &it) {
-    const int i = pair + j * pairs;
-    if (i >= p.whole && p.chunks < 0) look_at_rest<PASS, NARROW>(a, sh, pairs, p);
-    if (i < p.whole) {
-        tile_item<PASS, NARROW>(a, sh.before, i >> 1, kind_of(i, pairs), it);
-        return true;
-    }
-    // this pair's chunks of the tiles that are cut, one tile after the other
-    const int begin = (int)((long)p.chunks * pair / pairs), end = (int)((long)p.chunks * (pair + 1) / pairs), rest = p.items - p.whole;
-    if (begin == end) return false;
-    int lo = 0, hi = rest - 1;   // the tile of the first of them
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (sh.start[mid] <= begin) lo = mid; else hi = mid - 1;
-    }
-    lo += j - p.whole / pairs;
-    if (lo >= rest || sh.start[lo] >= end) return false;
-    tile_item<PASS, NARROW>(a, sh.before, (p.whole + lo) >> 1, kind_of(p.whole + lo, pairs), it);
-    const int last = sh.start[lo + 1], c0 = max(begin, sh.start[lo]), c1 = min(end, last);
-    it.from = c0 - sh.start[lo];
-    it.chunks = c1 - c0;
-    it.part = it.from > 0 ? LATER : c1 < last ? BEGIN : WHOLE;
+    Share s;
+    auto chunks_of = [&](int i) {
+        Item t;
+        tile_item<PASS, NARROW>(a, sh.before, i >> 1, kind_of(i, pairs), t);
+        return t.chunks;
+    };
+    if (!share_of(sh.start, p, pair, pairs, CUT_SAVES, j, chunks_of, s)) return false;
+    tile_item<PASS, NARROW>(a, sh.before, s.i >> 1, kind_of(s.i, pairs), it);
+    if (s.chunks) it.from = s.from, it.chunks = s.chunks, it.part = s.part;
     return true;
 }
 
@@ -219,9 +167,6 @@ template <int PASS, bool VEC, bool NARROW>
 using PlaceA = Place<PASS != FWD, !VEC && PASS == FWD, wide<PASS, VEC>, Shape<NARROW>::CONVERTERS>;
 template <int PASS, bool VEC, bool NARROW>
 using PlaceB = Place<PASS == PARAM, !VEC && PASS == FWD, wide<PASS, VEC>, Shape<NARROW>::CONVERTERS>;
-// Feature (of the CTA's 128) at place p.
-__device__ __forceinline__ int feature_at(bool mix, int p) { return mix ? (p & 3) * 32 + (p >> 2) : p; }
-
 // Item j, as it was handed over; false when the CTA is aborting. release(): this warp needs the record no longer.
 __device__ __forceinline__ bool take(Shared &sh, int j, Item &t) {
     t.chunks = 0;
@@ -247,16 +192,7 @@ struct Cursor {
     }
 };
 
-// A pair's partial sums of a tile: [columns][256 features], then the sums of the deltas of its columns (parameter pass).
-constexpr int PART_FLOATS = 256 * 256, PART_PITCH = PART_FLOATS + 256;
-__device__ __forceinline__ float *part_of(const GroupedArgs &a, int pair, int part) { return a.parts + (size_t)(pair * 2 + part) * PART_PITCH; }
-// What a partial sum belongs to, for the kernel that joins them; `ends`: it holds the tile's last chunk.
-struct Piece {
-    int used, ends, e, m0, c0, cols, bn, kind;
-};
-__device__ __forceinline__ Piece *piece_of(const GroupedArgs &a, int pairs, int pair, int part) {
-    return reinterpret_cast<Piece *>(a.parts + (size_t)pairs * 2 * PART_PITCH) + pair * 2 + part;
-}
+using TcParts = Parts<256, 256>;
 
 // A: 128 features of this CTA. A chunk is fetched whole as soon as the registers of the one before have been stored (one
 // latency a chunk: loads that are waited for in turn would cost one each).
@@ -440,7 +376,7 @@ __device__ __forceinline__ void convert_b(const GroupedArgs &a, Shared &sh, int 
                 total = make_float4(0.f, 0.f, 0.f, 0.f);
                 const int c = w * 32 + lane, n = cta * (t.bn >> 1) + c;
                 if (c < t.bn >> 1 && t.part != WHOLE) {
-                    part_of(a, blockIdx.x >> 1, t.part)[PART_FLOATS + n] = sh.bias[c];
+                    TcParts::of(a, blockIdx.x >> 1, t.part)[TcParts::FLOATS + n] = sh.bias[c];
                 } else if (c < t.bn >> 1 && n < t.cols) {
                     const size_t o = (size_t)t.e * a.N + t.c0 + n;
                     const float vb = __ldg(a.var_b + o);
@@ -485,7 +421,7 @@ __global__ void __launch_bounds__(Shape<NARROW>::THREADS, 1) grouped_tc_kernel(c
         if (lane == 0) sh.before[a.E] = carry;
     }
     __syncthreads();
-    if (cta == 0 && threadIdx.x < 2) piece_of(a, pairs, pair, threadIdx.x)->used = 0;
+    if (cta == 0 && threadIdx.x < 2) TcParts::piece(a, pairs, pair, threadIdx.x)->used = 0;
     if (sh.before[a.E] == 0) return;   // no expert of this size; the same in both CTAs
     if (threadIdx.x == 0) {
         for (int s = 0; s < 2; s++) {
@@ -541,9 +477,7 @@ __global__ void __launch_bounds__(Shape<NARROW>::THREADS, 1) grouped_tc_kernel(c
         }
         if (warp == ISSUER + 1) {
             // ------------------------------------------------------------------------------------------------- items
-            Plan plan{2 * sh.before[a.E], 0, -1};
-            // the forward pass's rounds come in twos, as many means as variances for each pair
-            plan.whole = PASS == FWD ? plan.items / (2 * pairs) * (2 * pairs) : plan.items / pairs * pairs;
+            Plan plan = make_plan(PASS == FWD, 2 * sh.before[a.E], pairs, true);
             bool more = true;
             for (int j = 0; more; j++) {
                 Record &r = sh.record[j % RECORDS];
@@ -553,7 +487,7 @@ __global__ void __launch_bounds__(Shape<NARROW>::THREADS, 1) grouped_tc_kernel(c
                 more = get_item<PASS, NARROW>(a, sh, plan, pair, pairs, j, t);
                 if (!more) t.chunks = 0;
                 if (more && t.part != WHOLE && cta == 0 && lane == 0)
-                    *piece_of(a, pairs, pair, t.part) = Piece{1, t.from + t.chunks == (PASS == FWD && t.kind == VAR ? 2 : 1) * t.nk, t.e, t.m0, t.c0, t.cols, t.bn, t.kind};
+                    *TcParts::piece(a, pairs, pair, t.part) = Piece{1, t.from + t.chunks == (PASS == FWD && t.kind == VAR ? 2 : 1) * t.nk, t.e, t.m0, t.c0, t.cols, t.bn, t.kind};
                 if (lane == 0) r.item = t;
                 if (PASS == FWD && more)
                     for (int l = lane; l < t.bn >> 1; l += 32) {
@@ -600,7 +534,7 @@ __global__ void __launch_bounds__(Shape<NARROW>::THREADS, 1) grouped_tc_kernel(c
             o.whole = t.part == WHOLE;
             if (!o.whole) {   // a partial sum
                 o.ld = 256;
-                o.base = (size_t)(pair * 2 + t.part) * PART_PITCH + first * 256 + cta * 128 + quad * 32 + lane;
+                o.base = (size_t)(pair * 2 + t.part) * TcParts::PITCH + first * 256 + cta * 128 + quad * 32 + lane;
                 return o;
             }
             o.base = ((PASS == PARAM ? (size_t)o.e * a.N : 0) + t.c0 + first) * o.ld + o.m;
@@ -690,54 +624,6 @@ __global__ void __launch_bounds__(Shape<NARROW>::THREADS, 1) grouped_tc_kernel(c
     }
 }
 
-// Adds up the partial sums of the tiles that were cut, in the order of the contraction, and writes them out. blockIdx.x: a
-// pair's partial sum that begins a tile, the others do nothing; blockIdx.y: eight columns of it. A thread has a feature.
-constexpr int JOIN_COLUMNS = 8;
-template <int PASS>
-__global__ void __launch_bounds__(256) grouped_join_kernel(const GroupedArgs a, int pairs, bool mix) {
-    const int pair = blockIdx.x, x0 = blockIdx.y * JOIN_COLUMNS;
-    const Piece t = *piece_of(a, pairs, pair, BEGIN);
-    if (!t.used || x0 >= t.cols) return;
-    float acc[JOIN_COLUMNS], bias = 0.f;
-    const bool sum = PASS == PARAM && a.var_b && t.m0 == 0 && blockIdx.y == 0;
-#pragma unroll
-    for (int x = 0; x < JOIN_COLUMNS; x++) acc[x] = 0.f;
-    bool ends = false;
-    for (int q = pair; q < pairs && !ends; q++) {   // a tile that begins here goes on with the next pairs
-        const int part = q == pair ? BEGIN : LATER;
-        const Piece *piece = piece_of(a, pairs, q, part);
-        if (!piece->used) continue;   // a pair without a chunk
-        const float *p = part_of(a, q, part);
-#pragma unroll
-        for (int x = 0; x < JOIN_COLUMNS; x++)
-            if (x0 + x < t.cols) acc[x] += p[(x0 + x) * 256 + threadIdx.x];
-        if (sum && (int)threadIdx.x < t.cols) bias += p[PART_FLOATS + threadIdx.x];
-        ends = piece->ends;
-    }
-    if (sum && (int)threadIdx.x < t.cols) {
-        const size_t o = (size_t)t.e * a.N + t.c0 + threadIdx.x;
-        const float vb = __ldg(a.var_b + o);
-        (t.kind == VAR ? a.ob1 : a.ob0)[o] = t.kind == VAR ? vb * vb * bias : vb * bias;
-    }
-    const int m = t.m0 + (threadIdx.x & 128) + feature_at(mix, threadIdx.x & 127), ld = PASS == FWD ? a.N : a.K;
-    if (m >= ld) return;
-    const size_t base = ((PASS == PARAM ? (size_t)t.e * a.N : 0) + t.c0 + x0) * ld + m;
-    const float *scale = PASS == PARAM ? a.var_w : a.jcb;
-    float add = 0.f;
-    if (PASS == FWD && a.mu_b) add = __ldg((t.kind == VAR ? a.var_b : a.mu_b) + (size_t)t.e * a.N + m);
-#pragma unroll
-    for (int x = 0; x < JOIN_COLUMNS; x++) {
-        if (x0 + x >= t.cols) break;
-        const size_t o = base + (size_t)x * ld;
-        float z = acc[x] + add;
-        if (PASS != FWD && scale) {
-            const float f = __ldg(scale + o);
-            z = t.kind == VAR ? z * f * f : z * f;
-        }
-        (t.kind == VAR ? a.o1 : a.o0)[o] = z;
-    }
-}
-
 // mu_a^2 + var_a, the forward variance's operand
 __global__ void __launch_bounds__(256) grouped_second_moment_kernel(const float *__restrict__ mu, const float *__restrict__ var,
                                                                     size_t n, float *__restrict__ out) {
@@ -777,7 +663,7 @@ int launch_pass(const GroupedArgs &a, int above, int upto, cudaStream_t st) {
     auto k = vec ? grouped_tc_kernel<PASS, true, NARROW> : grouped_tc_kernel<PASS, false, NARROW>;
     TAGI_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     TAGI_CUDA(cudaLaunchKernelEx(&cfg, k, a, above, upto));
-    grouped_join_kernel<PASS><<<dim3(pairs, Sh::WIDTH / JOIN_COLUMNS), 256, 0, st>>>(a, pairs, vec ? wide<PASS, true> : wide<PASS, false>);
+    grouped_join_kernel<PASS, 256, 256><<<dim3(pairs, Sh::WIDTH / JOIN_COLUMNS), 256, 0, st>>>(a, pairs, vec ? wide<PASS, true> : wide<PASS, false>);
     TAGI_CUDA(cudaGetLastError());
     return TAGI_OK;
 }
@@ -804,7 +690,7 @@ int grouped_tc_pairs(int pass, int E, int S, int K, int N) {
     return (int)(most < 1 ? 1 : most < PAIRS ? most : PAIRS);
 }
 size_t grouped_tc_parts_bytes(int pass, int E, int S, int K, int N) {
-    return (size_t)grouped_tc_pairs(pass, E, S, K, N) * 2 * (PART_PITCH * sizeof(float) + sizeof(Piece));
+    return TcParts::bytes(grouped_tc_pairs(pass, E, S, K, N));
 }
 
 int grouped_second_moment(const GroupedArgs &a, cudaStream_t st) {

@@ -15,6 +15,7 @@
 // six products of 16 steps are three MMAs: the rows' parts lie below each other and count as one operand of up to 3 x 48
 // columns. hi.[hi mid lo] adds to accumulators 0, 1 and 2, mid.[hi mid] to 1 and 2, lo.[hi] to 2: the accumulators hold the
 // terms of one magnitude each and are added up when a chunk is read.
+#include "tagi_grouped_plan.cuh"
 #include "tagi_grouped_split.cuh"
 #include "tagi_tc_tile.cuh"
 
@@ -36,7 +37,8 @@ static_assert(HALF * STATE_PITCH * 4 <= raw_bytes(false), "");
 constexpr uint32_t ACC = 3 * COLS, A_PART = KC / 2, A_SLOT = 3 * A_PART, A_COL = 2 * ACC, TMEM_COLS = 512;
 static_assert(SLOT % 1024 == 0, "the swizzle counts lines from multiples of 1024 bytes");
 static_assert(A_COL + 2 * A_SLOT <= TMEM_COLS, "");
-constexpr int MEAN = 0, VAR = 1;
+constexpr int CUT_SAVES = 12;   // chunks that cutting has to save (see tagi_grouped_plan.cuh): a chunk takes 1 us, cutting about 10
+using ThinParts = Parts<ROWS, COLS>;
 static_assert(THIN_ROWS <= COLS, "one tile for all rows of an expert");
 
 __device__ int g_status;  // first wait that ran out
@@ -45,6 +47,7 @@ struct Item {
     int chunks;                   // of the item; 0: there are no more items
     int e, m0, r0, rows, bn;      // expert; first feature; first row and their number; tile width
     int kind, depth, nk;          // MEAN or VAR; contraction length; chunks of one contraction
+    int from, part;               // first chunk; WHOLE, or which of the CTA's two partial sums the item goes to
 };
 struct Shared {                   // behind the slots and the ring
     uint64_t full[2], done[2], raw_full[RING], raw_empty[RING], item_full[RECORDS], item_empty[RECORDS];
@@ -52,17 +55,23 @@ struct Shared {                   // behind the slots and the ring
     volatile int abort_flag;
     Item item[RECORDS];
     int input[RECORDS][COLS];     // forward: input rows of the item's columns, -1 where there is none
+    int start[2 * CTAS + 2];      // of the tiles that are cut: chunks of those before each
     int before[];                 // tiles of the experts before e, E + 1 entries
 };
 static_assert(sizeof(Shared) % 8 == 0, "");
 
-// Item j of a CTA: kinds of a tile are neighbours, a CTA's kinds alternate (see tagi_grouped_tc.cu).
+// Item j of a CTA; chunks == 0: there is none.
 template <int PASS>
-__device__ __forceinline__ void get_item(const GroupedArgs &a, const int *before, int j, Item &it) {
-    const int ctas = gridDim.x, i = blockIdx.x + j * ctas, t = i >> 1;
+__device__ __forceinline__ void get_item(const GroupedArgs &a, Shared &sh, Plan &p, int j, Item &it) {
+    const int ctas = gridDim.x, *before = sh.before;
+    it.depth = PASS == FWD ? a.K : a.N;
+    it.nk = (it.depth + KC - 1) / KC;
     it.chunks = 0;
-    if (t >= before[a.E]) return;
-    it.kind = (i + 2 * t / ctas) & 1;
+    Share s;
+    auto chunks_of = [&](int i) { return PASS == FWD && kind_of(i, ctas) == VAR ? 2 * it.nk : it.nk; };
+    if (!share_of(sh.start, p, blockIdx.x, ctas, CUT_SAVES, j, chunks_of, s)) return;
+    const int t = s.i >> 1;
+    it.kind = kind_of(s.i, ctas);
     int lo = 0, hi = a.E - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
@@ -74,9 +83,8 @@ __device__ __forceinline__ void get_item(const GroupedArgs &a, const int *before
     it.rows = r1 - it.r0;
     it.m0 = (t - before[lo]) * ROWS;
     it.bn = round_up(it.rows, 16);
-    it.depth = PASS == FWD ? a.K : a.N;
-    it.nk = (it.depth + KC - 1) / KC;
-    it.chunks = PASS == FWD && it.kind == VAR ? 2 * it.nk : it.nk;
+    it.from = s.from, it.part = s.part;
+    it.chunks = s.chunks ? s.chunks : chunks_of(s.i);
 }
 
 __device__ __forceinline__ bool take(Shared &sh, int j, Item &t) {
@@ -107,7 +115,7 @@ __device__ __forceinline__ int bytes_of(int floats) { return min(max(floats, 0),
 
 template <int PASS, bool VEC>
 __global__ void __launch_bounds__(THREADS, 1)
-grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_constant__ CUtensorMap var_map, const GroupedArgs a) {
+grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_constant__ CUtensorMap var_map, const GroupedArgs a, bool may_cut) {
     constexpr uint32_t RAW = raw_bytes(VEC);
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u, ring = smem_base + 2 * SLOT;
@@ -132,6 +140,7 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
         if (lane == 0) sh.before[a.E] = carry;
     }
     __syncthreads();
+    if (may_cut && threadIdx.x < 2) ThinParts::piece(a, gridDim.x, blockIdx.x, threadIdx.x)->used = 0;
     if (sh.before[a.E] == 0) return;   // no expert of this size
     if (threadIdx.x == 0) {
         for (int s = 0; s < 2; s++) {
@@ -195,12 +204,14 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
                 if (lane == 0) mbar_arrive(sh.full + s);
             }
             if (!ok) break;
-            const int m = it.m0 + quad * 32 + lane, ld = PASS == FWD ? a.N : a.K, n = m < ld ? min(per, it.rows - first) : 0;
-            const size_t base = (size_t)(it.r0 + first) * ld + m;
-            float *out = (it.kind == VAR ? a.o1 : a.o0) + base;
+            const bool whole = it.part == WHOLE;
+            const int m = it.m0 + quad * 32 + lane, features = PASS == FWD ? a.N : a.K, n = m < features ? min(per, it.rows - first) : 0,
+                      ld = whole ? features : ROWS;
+            const size_t base = (size_t)(it.r0 + first) * features + m;
+            float *out = whole ? (it.kind == VAR ? a.o1 : a.o0) + base : ThinParts::of(a, blockIdx.x, it.part) + first * ROWS + quad * 32 + lane;
             float bias = 0.f;
-            if (PASS == FWD && a.mu_b && n > 0) bias = __ldg((it.kind == VAR ? a.var_b : a.mu_b) + (size_t)it.e * a.N + m);
-            const bool scaled = PASS == STATE && a.jcb != nullptr;
+            if (PASS == FWD && a.mu_b && whole && n > 0) bias = __ldg((it.kind == VAR ? a.var_b : a.mu_b) + (size_t)it.e * a.N + m);
+            const bool scaled = PASS == STATE && a.jcb != nullptr && whole;
             float f[8];
 #pragma unroll
             for (int x = 0; x < COLS / 2; x++) {
@@ -235,7 +246,7 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
                     shift[k] = PASS == FWD && k > 0 ? shift_of(a.var_w + line) : shift_of(a.mu_w + line);
                 }
             }
-            for (int c = 0; c < it.chunks; c++, i++) {
+            for (int c = it.from; c < it.from + it.chunks; c++, i++) {
                 if ((i & 1) != slot) continue;
                 const int r = 2 * i + h;
                 const bool square = it.kind == VAR && (PASS == STATE || c < it.nk);
@@ -304,7 +315,7 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
         const uint32_t to = smem_base + row * 128 + ((((lane & 3) >> 1) ^ (row & 7)) << 4) + (lane & 1) * 8;
         float4 v[8];
         Item it;
-        int in[2], j = 0, c = 0;
+        int in[2], j = 0, c = 0;   // c: the chunk that is loaded next
         bool ok = true;
         auto seek = [&]() {
             take(sh, j, it);
@@ -313,6 +324,7 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
                 const int p = g * 32 + row;
                 in[g] = it.chunks == 0 || p >= it.rows ? -1 : PASS == FWD ? sh.input[j % RECORDS][p] : it.r0 + p;
             }
+            c = it.from;
             release(sh, j, lane);
         };
         auto load = [&]() {
@@ -328,7 +340,7 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
         for (int i = 0; it.chunks > 0; i++) {
             const int s = i & 1, cols = it.bn;
             load();
-            if (++c == it.chunks) c = 0, j++, seek();
+            if (++c == it.from + it.chunks) j++, seek();
             if (i >= 2) ok = mbar_wait(sh.done + s, ((i - 2) >> 1) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_EMPTY);
             if (!ok) break;
 #pragma unroll
@@ -348,7 +360,7 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
         int r = 0;
         for (int j = 0; ok && take(sh, j, it) && it.chunks > 0; j++) {
             release(sh, j, lane);
-            for (int c = 0; ok && c < it.chunks; c++) {
+            for (int c = it.from; ok && c < it.from + it.chunks; c++) {
                 const bool second = PASS == FWD && c >= it.nk;
                 const int kc = (second ? c - it.nk : c) * KC;
                 for (int h = 0; h < 2; h++, r++) {
@@ -424,7 +436,7 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
                 mbar_arrive(sh.item_empty + j % RECORDS);
                 const uint32_t one = make_idesc_bf16(ROWS, it.bn, 0, 0), two = make_idesc_bf16(ROWS, 2 * it.bn, 0, 0),
                                three = make_idesc_bf16(ROWS, 3 * it.bn, 0, 0);
-                for (int c = 0; c < it.chunks; c++, i++) {
+                for (int c = it.from; c < it.from + it.chunks; c++, i++) {
                     const int s = i & 1, left = it.depth - (c >= it.nk ? c - it.nk : c) * KC, steps = min(KC / 16, (left + 15) / 16);
                     ok = mbar_wait(sh.full + s, (i >> 1) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_CONV);
                     if (!ok) break;
@@ -438,12 +450,16 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
         }
     } else {
         // ----------------------------------------------------------------------------------------------------- items
+        Plan plan = make_plan(PASS == FWD, 2 * sh.before[a.E], gridDim.x, may_cut);
         bool more = true;
         for (int j = 0; more; j++) {
             if (j >= RECORDS && !mbar_wait(sh.item_empty + j % RECORDS, (j / RECORDS - 1) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_EMPTY)) break;
             Item t;
-            get_item<PASS>(a, sh.before, j, t);
+            get_item<PASS>(a, sh, plan, j, t);
             more = t.chunks > 0;
+            if (more && t.part != WHOLE && lane == 0)
+                *ThinParts::piece(a, gridDim.x, blockIdx.x, t.part) =
+                    Piece{1, t.from + t.chunks == (PASS == FWD && t.kind == VAR ? 2 : 1) * t.nk, t.e, t.m0, t.r0, t.rows, t.bn, t.kind};
             if (lane == 0) sh.item[j % RECORDS] = t;
             if (PASS == FWD && more)
                 for (int l = lane; l < t.rows; l += 32) sh.input[j % RECORDS][l] = input_row(a, t.r0 + l);
@@ -471,20 +487,39 @@ int make_map(int pass, const GroupedArgs &a, const float *w, CUtensorMap *map) {
     return r == CUDA_SUCCESS ? TAGI_OK : fail(TAGI_ERR_CUDA, "cuTensorMapEncodeTiled failed with code " + std::to_string((int)r));
 }
 
+// CTAs, and whether tiles may be cut (which takes a second kernel, 5 us even if it finds nothing to do): where the items do not
+// go once round the CTAs, if sharing them out saves 16 chunks; else if items are long and rounds few. 20 rows of one expert, 4096
+// to 1000 features, forward: 122 us whole, 38 us cut.
+struct Grid {
+    int ctas;
+    bool may_cut;
+};
+Grid grid_of(int pass, int E, int S, int K, int N) {
+    const long mt = ((pass == FWD ? N : K) + ROWS - 1) / ROWS, experts = E < S / (FEW_ROWS + 1) ? E : S / (FEW_ROWS + 1);
+    const long items = 2 * mt * experts, nk = ((pass == FWD ? K : N) + KC - 1) / KC;   // experts with more than `few` rows, at most
+    const long longest = pass == FWD ? 2 * nk : nk, chunks = pass == FWD ? items / 2 * 3 * nk : items * nk;
+    const bool may_cut = items <= CTAS ? longest - chunks / CTAS >= 16 : items < 4 * CTAS && longest >= 48;
+    const long most = may_cut ? chunks : items;
+    return Grid{(int)(most < 1 ? 1 : most < CTAS ? most : CTAS), may_cut};
+}
+
 template <int PASS>
 int launch_thin(const GroupedArgs &a, cudaStream_t st) {
     const bool vec = grouped_aligned(PASS, a);
     const size_t smem = 2 * SLOT + RING * raw_bytes(vec) + 1024 + sizeof(Shared) + (a.E + 1) * sizeof(int);
-    const long mt = ((PASS == FWD ? a.N : a.K) + ROWS - 1) / ROWS, experts = a.E < a.S / (a.few + 1) ? a.E : a.S / (a.few + 1);
-    const long most = 2 * mt * experts;   // experts with more than `few` rows, at most; both kinds
+    const Grid g = grid_of(PASS, a.E, a.S, a.K, a.N);
     CUtensorMap mean = {}, var = {};
     int rc;
     if (vec && (rc = make_map(PASS, a, a.mu_w, &mean)) != TAGI_OK) return rc;
     if (vec && PASS == FWD && (rc = make_map(PASS, a, a.var_w, &var)) != TAGI_OK) return rc;
     auto k = vec ? grouped_thin_kernel<PASS, true> : grouped_thin_kernel<PASS, false>;
     TAGI_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    k<<<(unsigned)(most < CTAS ? most : CTAS), THREADS, smem, st>>>(mean, var, a);
+    k<<<g.ctas, THREADS, smem, st>>>(mean, var, a, g.may_cut);
     TAGI_CUDA(cudaGetLastError());
+    if (g.may_cut) {
+        grouped_join_kernel<PASS, ROWS, COLS><<<dim3(g.ctas, COLS / JOIN_COLUMNS), ROWS, 0, st>>>(a, g.ctas, false);
+        TAGI_CUDA(cudaGetLastError());
+    }
     return TAGI_OK;
 }
 
@@ -492,6 +527,11 @@ int launch_thin(const GroupedArgs &a, cudaStream_t st) {
 }  // namespace
 
 int grouped_thin(int pass, const GroupedArgs &a, cudaStream_t st) { return pass == FWD ? thin::launch_thin<FWD>(a, st) : thin::launch_thin<STATE>(a, st); }
+
+size_t grouped_thin_parts_bytes(int pass, int E, int S, int K, int N) {
+    const thin::Grid g = thin::grid_of(pass, E, S, K, N);
+    return g.may_cut ? thin::ThinParts::bytes(g.ctas) : 0;
+}
 
 int grouped_thin_status(int *out, int reset) {
     TAGI_CUDA(cudaMemcpyFromSymbol(out, thin::g_status, sizeof(int)));

@@ -358,7 +358,8 @@ def test_grouped_linear_of_many_tiles(lib):
 
 
 @pytest.mark.parametrize("counts, K, N", [([300], 3000, 100), ([60, 50], 100, 3000), ([5000, 30, 800], 24, 40), ([520, 0, 70], 1536, 1403),
-                                          ([100] * 11, 2050, 513), ([49], 4100, 16), ([2000], 16, 300)])
+                                          ([100] * 11, 2050, 513), ([49], 4100, 16), ([2000], 16, 300), ([9], 4100, 20), ([30, 0, 48], 2047, 300),
+                                          ([20, 5, 40, 130], 1300, 1290)])
 @pytest.mark.parametrize("bias, gather", [(True, True), (False, False)])
 def test_grouped_linear_of_few_tiles_and_long_contractions(lib, counts, K, N, bias, gather):
     """Tiles that are cut along the contraction, because whole ones would leave most of the GPU idle."""
