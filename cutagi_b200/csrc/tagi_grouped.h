@@ -55,8 +55,8 @@ __device__ __forceinline__ void copy_first_group(float *dst, const float *src, i
 //   up to thin   tagi_grouped_thin.cu  tensor cores, tiles of 128 features (forward and state pass)
 //   more         tagi_grouped_tc.cu    tensor cores, tiles of 256 features x up to 128 rows (up to NARROW_ROWS; forward and state
 //                                      pass) or 256 rows
-// Measured on eight experts of 4096 x 4096, forward pass, 4 / 8 / 16 / 32 rows each: few 222 / 307 / 522 / 936 us; thin 402 to
-// 425 us up to 32 rows, 506 us at 40; the kernel after it 546 us at 56. Parameter pass at 7 / 10 / 14 / 20 rows: few 377 /
+// Measured on eight experts of 4096 x 4096, forward pass, 4 / 8 / 16 / 32 rows each: few 220 / 307 / 522 / 936 us; thin 371 to
+// 392 us up to 32 rows, 465 us at 40; the kernel after it 546 us at 56. Parameter pass at 7 / 10 / 14 / 20 rows: few 377 /
 // 419 / 486 / 595 us, the wide kernel 503 to 507 us.
 constexpr int FEW_ROWS = 8, FEW_PARAM_ROWS = 14, THIN_ROWS = 48, NARROW_ROWS = 128;
 
