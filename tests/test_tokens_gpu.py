@@ -524,6 +524,26 @@ def test_grouped_linear_rows_of_other_experts_do_not_leak(lib, counts, K, N):
         assert not bool(torch.isfinite(got.get(whole=False)[1]).any())
 
 
+@pytest.mark.parametrize("counts", [[5, 7], [30, 12], [100, 64], [300, 140]])
+@pytest.mark.parametrize("K, N", [(200, 132), (199, 131)])
+def test_grouped_linear_a_row_that_is_not_finite_stays_alone(lib, counts, K, N):
+    """One row of each expert holds NaN and infinities: the expert's other rows are what they would be without it."""
+    from cutagi_b200 import ops
+    g, E = Gen(sum(counts)), len(counts)
+    offsets, S = spread(counts)
+    mw, vw = g.n(E, N, K, scale=K ** -0.5), g.u(E, N, K, hi=1.0 / K)
+    a, va, dm, dv = g.n(S, K), g.u(S, K), g.n(S, N), g.u(S, N)
+    clean = (*ops.grouped_linear(mw, vw, None, None, a, va, offsets), *ops.grouped_linear_state(mw, None, dm, dv, offsets))
+    bad = offsets[:-1].long() + 3
+    for t, x in ((a, torch.nan), (va, torch.inf), (dm, -torch.inf), (dv, torch.nan)):
+        t[bad] = x
+    rest = torch.ones(S, dtype=torch.bool, device="cuda")
+    rest[bad] = False
+    dirty = (*ops.grouped_linear(mw, vw, None, None, a, va, offsets), *ops.grouped_linear_state(mw, None, dm, dv, offsets))
+    for x, y in zip(clean, dirty):
+        assert torch.equal(x[rest], y[rest]) and not bool(torch.isfinite(y[bad]).any())
+
+
 @pytest.mark.parametrize("rows", [4, 200])
 def test_grouped_linear_wide_range_of_values(lib, rows):
     """Entries of one contraction that differ by many powers of two keep the accuracy of 32-bit products: large inputs
