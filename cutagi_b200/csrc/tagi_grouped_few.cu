@@ -362,11 +362,13 @@ template <int PASS, bool VEC>
 int launch_few(const GroupedArgs &a, cudaStream_t st) {
     constexpr size_t ring = stages(PASS) * (weights(PASS, VEC) + 2 * ROWS * SLAB), sums = WARPS * ROWS * 2 * OUT;
     constexpr size_t smem = (ring > sums ? ring : sums) * sizeof(float);
-    // CTAs that have work, at most: with fewer than two for an SM, clusters cut the contraction, into no less than 256 steps
+    // CTAs that have work, at most: as long as twice as many still run at the same time (two an SM), clusters cut the contraction,
+    // into no less than 256 steps; the forward pass also beyond that, into no less than 2048. One row of one expert of 4096 x
+    // 4096, forward, in 1 / 2 / 4 / 8 parts: 60 / 45 / 33 / 40 us; of two experts 78 / 56 / 56 / 69 us; of four 108 / 99 / 106 us.
     const int tiles = ((PASS == FWD ? a.N : a.K) + OUT - 1) / OUT, depth = PASS == FWD ? a.K : a.N;
     const long ctas = (long)tiles * (a.E < a.S ? a.E : a.S);
     int parts = 1;
-    while (parts < 8 && ctas * parts < 2 * 148 && depth >= 512 * parts) parts *= 2;
+    while (parts < 8 && depth >= 512 * parts && (ctas * parts <= 148 || (PASS == FWD && ctas * parts < 2 * 148 && depth >= 4096 * parts))) parts *= 2;
     auto k = grouped_few_kernel<PASS, VEC>;
     TAGI_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     cudaLaunchConfig_t cfg = {};
