@@ -109,19 +109,29 @@ __device__ __forceinline__ void mma_small_products(uint32_t d, uint32_t x, uint3
 }
 __device__ __forceinline__ void mma_large_product(uint32_t d, uint32_t x, uint32_t y, uint32_t hi, uint32_t idesc) { GROUPED_LARGE("2"); }
 
+// The lane that issues for a warp whose lanes all run the same code: with values that are the same in all lanes, instructions
+// take them from uniform registers. From a branch that only one lane takes, each MMA cost 104 cycles: its operands are moved there
+// one by one.
+__device__ __forceinline__ bool elected() {
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+    return e != 0;
+}
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+
 // 16 contraction steps for one CTA with A in tensor memory, its parts AP columns apart, and B's parts below each other as one
 // operand (idesc3: of three parts' columns, and so on): hi.[hi mid lo] to accumulators d0.., mid.[hi mid] to d1.., lo.[hi]
-// to d2. accumulate == 0: the first overwrites all three.
+// to d2. accumulate == 0: the first overwrites all three. Called by the whole warp, `lead`: elected().
 template <uint32_t AP>
 __device__ __forceinline__ void mma_stacked_ts(uint32_t d0, uint32_t d1, uint32_t d2, uint32_t x, uint32_t y, uint32_t hi, uint32_t idesc3,
-                                               uint32_t idesc2, uint32_t idesc1, uint32_t accumulate) {
+                                               uint32_t idesc2, uint32_t idesc1, uint32_t accumulate, uint32_t lead) {
     asm volatile(
-        "{\n\t.reg .pred p, t;\n\t.reg .b32 r, s;\n\t.reg .b64 db;\n\t"
+        "{\n\t.reg .pred p, t, q;\n\t.reg .b32 r, s;\n\t.reg .b64 db;\n\tsetp.ne.b32 q, %12, 0;\n\t"
         "setp.ne.b32 p, %9, 0;\n\tsetp.eq.b32 t, 0, 0;\n\tmov.b64 db, {%4, %5};\n\tadd.u32 r, %3, %10;\n\tadd.u32 s, %3, %11;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%3], db, %6, p;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%1], [r], db, %7, t;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%2], [s], db, %8, t;\n\t}"
-        ::"r"(d0), "r"(d1), "r"(d2), "r"(x), "r"(y), "r"(hi), "r"(idesc3), "r"(idesc2), "r"(idesc1), "r"(accumulate), "n"(AP), "n"(2 * AP)
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%3], db, %6, p;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%1], [r], db, %7, t;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%2], [s], db, %8, t;\n\t}"
+        ::"r"(d0), "r"(d1), "r"(d2), "r"(x), "r"(y), "r"(hi), "r"(idesc3), "r"(idesc2), "r"(idesc1), "r"(accumulate), "n"(AP), "n"(2 * AP), "r"(lead)
         : "memory");
 }
 

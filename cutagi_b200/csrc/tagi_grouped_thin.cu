@@ -428,24 +428,26 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
                 for (int spin = 0; spin < 100000 && !mbar_try_wait(sh.raw_full + q % RING, (q / RING) & 1); spin++) {}
     } else if (warp == ISSUER) {
         // ------------------------------------------------------------------------------------------------------- MMA
-        if (lane == 0) {
-            constexpr uint32_t HI = desc_hi(1024, SWZ_128B);
-            Item it;
-            bool ok = true;
-            for (int j = 0, i = 0; ok && take(sh, j, it) && it.chunks > 0; j++) {
-                mbar_arrive(sh.item_empty + j % RECORDS);
-                const uint32_t one = make_idesc_bf16(ROWS, it.bn, 0, 0), two = make_idesc_bf16(ROWS, 2 * it.bn, 0, 0),
-                               three = make_idesc_bf16(ROWS, 3 * it.bn, 0, 0);
-                for (int c = it.from; c < it.from + it.chunks; c++, i++) {
-                    const int s = i & 1, left = it.depth - (c >= it.nk ? c - it.nk : c) * KC, steps = min(KC / 16, (left + 15) / 16);
-                    ok = mbar_wait(sh.full + s, (i >> 1) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_CONV);
-                    if (!ok) break;
-                    tc_fence_after_sync();
-                    const uint32_t x = tmem + A_COL + s * A_SLOT, y = desc_lo(smem_base + s * SLOT, 16), d = tmem + s * ACC;
-                    for (int k = 0; k < steps; k++)
-                        mma_stacked_ts<A_PART>(d, d + it.bn, d + 2 * it.bn, x + k * 8, y + k * 2, HI, three, two, one, k);
-                    mma_commit(sh.done + s);
-                }
+        // the whole warp, with values that are the same in all lanes
+        constexpr uint32_t HI = desc_hi(1024, SWZ_128B);
+        const bool lead = elected();
+        const uint32_t tm = uniform(tmem), base = uniform(smem_base);
+        Item it;
+        bool ok = true;
+        for (int j = 0, i = 0; ok && take(sh, j, it) && it.chunks > 0; j++) {
+            release(sh, j, lane);
+            const int bn = uniform(it.bn), nk = uniform(it.nk), depth = uniform(it.depth), from = uniform(it.from), end = from + uniform(it.chunks);
+            const uint32_t one = make_idesc_bf16(ROWS, bn, 0, 0), two = make_idesc_bf16(ROWS, 2 * bn, 0, 0), three = make_idesc_bf16(ROWS, 3 * bn, 0, 0);
+            for (int c = from; c < end; c++, i++) {
+                const int s = i & 1, left = depth - (c >= nk ? c - nk : c) * KC, steps = min(KC / 16, (left + 15) / 16);
+                ok = mbar_wait(sh.full + s, (i >> 1) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_CONV);
+                if (!ok) break;
+                tc_fence_after_sync();
+                const uint32_t x = tm + A_COL + s * A_SLOT, y = desc_lo(base + s * SLOT, 16), d = tm + s * ACC;
+                for (int k = 0; k < steps; k++)
+                    mma_stacked_ts<A_PART>(d, d + bn, d + 2 * bn, x + k * 8, y + k * 2, HI, three, two, one, k, lead);
+                if (lead) mma_commit(sh.done + s);
+                __syncwarp();
             }
         }
     } else {
