@@ -23,7 +23,7 @@ namespace tagi {
 namespace {
 namespace thin {
 
-constexpr int SUMMERS = 8, CONVERT_A = 16, CONVERT_B = 4, LOADERS = 2;
+constexpr int SUMMERS = 8, CONVERT_A = 8, CONVERT_B = 8, LOADERS = 2;
 constexpr int FIRST_A = SUMMERS, FIRST_B = FIRST_A + CONVERT_A, FIRST_LOADER = FIRST_B + CONVERT_B, ISSUER = FIRST_LOADER + LOADERS;
 constexpr int THREADS = 32 * (ISSUER + 2);       // the last warp works out the items
 constexpr int ROWS = 128, COLS = 48, KC = 64, HALF = 32, RING = 8, RECORDS = 4, CTAS = 148;
@@ -144,12 +144,12 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
     if (sh.before[a.E] == 0) return;   // no expert of this size
     if (threadIdx.x == 0) {
         for (int s = 0; s < 2; s++) {
-            mbar_init(sh.full + s, SUMMERS + CONVERT_A / 2 + CONVERT_B);   // half the converters of A write a slot
+            mbar_init(sh.full + s, SUMMERS + CONVERT_A + CONVERT_B / 2);   // half the converters of B write a slot
             mbar_init(sh.done + s, 1);
         }
         for (int s = 0; s < RING; s++) {
             mbar_init(sh.raw_full + s, VEC ? 1 : LOADERS * 32);   // the thread that starts TMA, or every loading thread's copies
-            mbar_init(sh.raw_empty + s, CONVERT_A / 4);   // and a quarter read a half-chunk
+            mbar_init(sh.raw_empty + s, CONVERT_A / 2);   // and half of A's read a half-chunk
         }
         for (int s = 0; s < RECORDS; s++) {
             mbar_init(sh.item_full + s, 1);
@@ -231,9 +231,8 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
         }
     } else if (warp < FIRST_B) {
         // ------------------------------------------------------------------------------------------ weights, ring -> parts
-        // h: which half of each chunk; slot: which chunks, the even or the odd
-        const int w = warp - FIRST_A, quad = w & 3, h = (w >> 2) & 1, slot = w >> 3, row = quad * 32 + lane;
-        const uint32_t to = tmem + ((uint32_t)(quad * 32) << 16) + A_COL + slot * A_SLOT + h * (HALF / 2);
+        // h: which half of each chunk
+        const int w = warp - FIRST_A, quad = w & 3, h = w >> 2, row = quad * 32 + lane;
         Item it;
         bool ok = true;
         for (int j = 0, i = 0; ok && take(sh, j, it) && it.chunks > 0; j++) {
@@ -247,8 +246,8 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
                 }
             }
             for (int c = it.from; c < it.from + it.chunks; c++, i++) {
-                if ((i & 1) != slot) continue;
-                const int r = 2 * i + h;
+                const int r = 2 * i + h, slot = i & 1;
+                const uint32_t to = tmem + ((uint32_t)(quad * 32) << 16) + A_COL + slot * A_SLOT + h * (HALF / 2);
                 const bool square = it.kind == VAR && (PASS == STATE || c < it.nk);
                 ok = mbar_wait(sh.raw_full + r % RING, (r / RING) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_RAW) &&
                      (i < 2 || mbar_wait(sh.done + slot, ((i - 2) >> 1) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_EMPTY));
@@ -310,8 +309,8 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
         }
     } else if (warp < FIRST_LOADER) {
         // ------------------------------------------------------------------------------- rows, global memory -> parts
-        // a warp loads 64 consecutive bytes of eight rows; the next chunk is on its way while this one is split
-        const int w = warp - FIRST_B, row = w * 8 + ((lane >> 2) & 3) * 2 + (lane >> 4), along = VEC ? (lane & 3) * 4 : lane & 3;
+        // a warp loads 64 consecutive bytes of eight rows; two groups of four warps take turns at the chunks
+        const int w = (warp - FIRST_B) & 3, turn = (warp - FIRST_B) >> 2, row = w * 8 + ((lane >> 2) & 3) * 2 + (lane >> 4), along = VEC ? (lane & 3) * 4 : lane & 3;
         const uint32_t to = smem_base + row * 128 + ((((lane & 3) >> 1) ^ (row & 7)) << 4) + (lane & 1) * 8;
         float4 v[8];
         Item it;
@@ -336,11 +335,16 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
                 v[q] = ld4<VEC, VEC ? 1 : 4>(src + (size_t)max(in[q >> 2], 0) * it.depth + kc + along + (q & 3) * 16,
                                 in[q >> 2] >= 0 ? it.depth - kc - along - (q & 3) * 16 : 0);
         };
+        auto step = [&]() {
+            if (it.chunks > 0 && ++c == it.from + it.chunks) j++, seek();
+        };
         seek();
-        for (int i = 0; it.chunks > 0; i++) {
-            const int s = i & 1, cols = it.bn;
+        if (turn == 1) step();
+        for (int i = turn; it.chunks > 0; i += 2) {
+            const int s = turn, cols = it.bn;
             load();
-            if (++c == it.from + it.chunks) j++, seek();
+            step();
+            step();
             if (i >= 2) ok = mbar_wait(sh.done + s, ((i - 2) >> 1) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_EMPTY);
             if (!ok) break;
 #pragma unroll
