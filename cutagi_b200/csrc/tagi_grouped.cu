@@ -8,12 +8,11 @@ namespace {
 
 int run(int pass, GroupedArgs &a, cudaStream_t st) {
     a.few = pass == PARAM ? FEW_PARAM_ROWS : FEW_ROWS;
-    a.thin = pass == PARAM ? FEW_PARAM_ROWS : THIN_ROWS;
     int rc = grouped_few(pass, a, st);
     if (rc != TAGI_OK || a.S <= a.few) return rc;
     if (pass == FWD && (rc = grouped_second_moment(a, st)) != TAGI_OK) return rc;
-    if (pass != PARAM && ((rc = grouped_thin(pass, a, st)) != TAGI_OK || a.S <= a.thin)) return rc;
-    return grouped_tc(pass, a, st);
+    if (pass != PARAM && (rc = grouped_thin(pass, a, st)) != TAGI_OK) return rc;
+    return pass != PARAM && a.S <= THIN_ROWS ? TAGI_OK : grouped_tc(pass, a, st);
 }
 
 bool sizes_fit(int E, int S, int K, int N) {

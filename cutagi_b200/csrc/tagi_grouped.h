@@ -8,7 +8,7 @@ enum { FWD = 0, STATE = 1, PARAM = 2 };
 
 struct GroupedArgs {
     int E, S, R, K, N;
-    int few, thin;   // most rows of an expert for the kernels of tagi_grouped_few.cu and tagi_grouped_thin.cu
+    int few;   // most rows of an expert for the kernels of tagi_grouped_few.cu
     const int *offsets, *token;
     // a0, a1: activations (forward) or deltas (backward); x: input means of the parameter pass
     const float *mu_w, *var_w, *mu_b, *var_b, *a0, *a1, *jcb, *x;
@@ -50,15 +50,18 @@ __device__ __forceinline__ void copy_first_group(float *dst, const float *src, i
 }
 #endif
 
-// Which kernel an expert's rows run on, decided on the device by their number (few, thin: see GroupedArgs):
-//   up to few    tagi_grouped_few.cu   one pass over the weights on the FP32 pipe
-//   up to thin   tagi_grouped_thin.cu  tensor cores, tiles of 128 features (forward and state pass)
-//   more         tagi_grouped_tc.cu    tensor cores, tiles of 256 features x up to 128 rows (up to NARROW_ROWS; forward and state
-//                                      pass) or 256 rows
-// Measured on eight experts of 4096 x 4096, forward pass, 4 / 8 / 16 / 32 rows each: few 220 / 307 / 522 / 936 us; thin 371 to
-// 392 us up to 32 rows, 465 us at 40; the kernel after it 546 us at 56. Parameter pass at 7 / 10 / 14 / 20 rows: few 377 /
-// 419 / 486 / 595 us, the wide kernel 503 to 507 us.
-constexpr int FEW_ROWS = 8, FEW_PARAM_ROWS = 14, THIN_ROWS = 48, NARROW_ROWS = 128;
+// Which kernel an expert's rows run on, decided on the device by their number (few: see GroupedArgs):
+//   up to few           tagi_grouped_few.cu   one pass over the weights on the FP32 pipe
+//   up to THIN_ROWS     tagi_grouped_thin.cu  tensor cores, tiles of 128 features (forward and state pass)
+//   up to MIDDLE_ROWS   the same for up to 128 rows, if middle_likely()
+//   more                tagi_grouped_tc.cu    tensor cores, tiles of 256 features x up to 256 rows
+// Measured on eight experts of 4096 x 4096, forward pass, 4 / 8 / 16 / 32 rows each: few 220 / 307 / 522 / 936 us; thin 283 at 16;
+// 56 / 100 / 128 rows: middle 494 / 539 / 604 us, the wide kernel 813 / 843 / 862 us. Parameter pass at 7 / 10 / 14 / 20 rows: few
+// 377 / 419 / 486 / 595 us, the wide kernel 503 to 507 us.
+constexpr int FEW_ROWS = 8, FEW_PARAM_ROWS = 14, THIN_ROWS = 48, MIDDLE_ROWS = 128;
+
+// The middle kernel is tried where the average expert makes 49 to 128 rows likely: one that finds nothing to do takes up to 7 us.
+inline bool middle_likely(int E, int S) { return S > THIN_ROWS && S > THIN_ROWS / 2 * E && S <= (MIDDLE_ROWS + 32) * E; }
 
 // the rows that a pass reads (of weights, activations and deltas) are whole 16-byte groups
 inline bool grouped_aligned(int pass, const GroupedArgs &a) {

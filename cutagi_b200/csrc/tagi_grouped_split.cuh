@@ -110,8 +110,7 @@ __device__ __forceinline__ void mma_small_products(uint32_t d, uint32_t x, uint3
 __device__ __forceinline__ void mma_large_product(uint32_t d, uint32_t x, uint32_t y, uint32_t hi, uint32_t idesc) { GROUPED_LARGE("2"); }
 
 // The lane that issues for a warp whose lanes all run the same code: with values that are the same in all lanes, instructions
-// take them from uniform registers. From a branch that only one lane takes, each MMA cost 104 cycles: its operands are moved there
-// one by one.
+// take them from uniform registers. An MMA issued so costs 37 cycles, from a branch that only one lane takes 104.
 __device__ __forceinline__ bool elected() {
     uint32_t e;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
@@ -132,6 +131,26 @@ __device__ __forceinline__ void mma_stacked_ts(uint32_t d0, uint32_t d1, uint32_
         "@q tcgen05.mma.cta_group::1.kind::f16 [%1], [r], db, %7, t;\n\t"
         "@q tcgen05.mma.cta_group::1.kind::f16 [%2], [s], db, %8, t;\n\t}"
         ::"r"(d0), "r"(d1), "r"(d2), "r"(x), "r"(y), "r"(hi), "r"(idesc3), "r"(idesc2), "r"(idesc1), "r"(accumulate), "n"(AP), "n"(2 * AP), "r"(lead)
+        : "memory");
+}
+
+// The same sixteen steps as six products into one accumulator: B's parts bp units of 16 bytes apart, the five small products
+// (accumulate == 0: the first overwrites the accumulator), and the large one.
+#define GROUPED_TS(A, B, P) "mov.b64 db, {" B ", %4};\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], [" A "], db, %5, " P ";\n\t"
+template <uint32_t AP>
+__device__ __forceinline__ void mma_small_products_ts(uint32_t d, uint32_t x, uint32_t y, uint32_t bp, uint32_t hi, uint32_t idesc, uint32_t accumulate, uint32_t lead) {
+    asm volatile(
+        "{\n\t.reg .pred p, t, q;\n\t.reg .b32 r, s, u, w;\n\t.reg .b64 db;\n\t"
+        "setp.ne.b32 q, %9, 0;\n\tsetp.ne.b32 p, %6, 0;\n\tsetp.eq.b32 t, 0, 0;\n\tadd.u32 r, %1, %7;\n\tadd.u32 s, %1, %8;\n\tadd.u32 u, %2, %3;\n\tadd.u32 w, u, %3;\n\t"
+        GROUPED_TS("s", "%2", "p") GROUPED_TS("%1", "w", "t") GROUPED_TS("r", "u", "t") GROUPED_TS("r", "%2", "t") GROUPED_TS("%1", "u", "t") "}"
+        ::"r"(d), "r"(x), "r"(y), "r"(bp), "r"(hi), "r"(idesc), "r"(accumulate), "n"(AP), "n"(2 * AP), "r"(lead)
+        : "memory");
+}
+__device__ __forceinline__ void mma_large_product_ts(uint32_t d, uint32_t x, uint32_t y, uint32_t hi, uint32_t idesc, uint32_t lead) {
+    asm volatile(
+        "{\n\t.reg .pred t, q;\n\t.reg .b64 db;\n\tsetp.ne.b32 q, %5, 0;\n\tsetp.eq.b32 t, 0, 0;\n\tmov.b64 db, {%2, %3};\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, t;\n\t}"
+        ::"r"(d), "r"(x), "r"(y), "r"(hi), "r"(idesc), "r"(lead)
         : "memory");
 }
 

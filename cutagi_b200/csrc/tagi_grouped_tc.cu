@@ -10,22 +10,21 @@
 //
 // Shape of the work. Rows of the tensor-core tile are features (of the weights: always many), columns are the expert's
 // rows (ragged: any width in steps of 32), so a thin expert costs a narrow tile. Two CTAs of a cluster share a tile of
-// 256 features x up to 256 columns, or 128 (cta_group::2); every accumulator lane is a feature, so stores run along memory.
+// 256 features x up to 256 columns (cta_group::2); every accumulator lane is a feature, so stores run along memory.
 // The mean and the variance are two accumulations over different operands (forward: mu_w.mu_a; mu_w^2.var_a followed by
 // var_w.(mu_a^2 + var_a) as one contraction of twice the length), which neighbouring pairs do at the same time: mu_w is
 // fetched from HBM for one and found in L2 by the other.
 //
-// Roles. Four warps (narrow tiles: eight) fetch A from global memory into registers, as many B (gathered rows, ragged edges and
-// any alignment cost nothing extra there), a chunk at a time; they form squares, split, and store the parts to shared memory in
-// the swizzled layouts the tensor core reads. Eight summing warps add each chunk's accumulator to their registers and write
-// finished tiles out. One
+// Roles. Four warps fetch A from global memory into registers, four B (gathered rows, ragged edges and any alignment cost
+// nothing extra there), a chunk at a time; they form squares, split, and store the parts to shared memory in the swizzled layouts
+// the tensor core reads. Eight summing warps add each chunk's accumulator to their registers and write finished tiles out. One
 // thread issues the MMAs, and a warp works out the items ahead of the others. Two slots of 64 contraction steps hold 2 x 96
 // KiB of operands and two accumulators of 256 columns fill tensor memory; a slot's "full" barrier counts the converters
 // (operands written) and the summing warps (accumulator read), its "done" barrier the MMAs' completion. Nothing stops at a
 // tile's end: the next tile's operands are converted while the last one's chunks multiply and its sums are written.
 //
-// Bound by the tensor cores (and the power cap) from about 250 rows an expert on; by the converters with fewer (wide tiles, 100
-// rows: 5000 cycles a chunk, 1200 to issue its loads, 1500 until the values are there, 1200 to split and store them); by the output of
+// Bound by the tensor cores (and the power cap) from about 250 rows an expert on; by the converters with fewer (100 rows: 5000
+// cycles a chunk, 1200 to issue its loads, 1500 until the values are there, 1200 to split and store them); by the output of
 // the tiles in the parameter pass of few rows (12 bytes a weight).
 #include "tagi_grouped_plan.cuh"
 #include "tagi_grouped_split.cuh"
@@ -35,22 +34,14 @@
 namespace tagi {
 namespace {
 
-// NARROW: tiles of up to 128 columns. Their sums need half the registers; with those each operand has twice the warps, which is
-// what the converters' time depends on (a chunk 3600 cycles instead of 5000).
-template <bool NARROW>
-struct Shape {
-    static constexpr int WIDTH = NARROW ? 128 : 256, PER = WIDTH / 2;   // columns of a tile at most, and of a summing warp
-    static constexpr int CONVERTERS = NARROW ? 8 : 4;                   // warps of A, and of B
-    static constexpr int TASKS = 64 / CONVERTERS;                       // times four values: a thread's part of A of a chunk
-    static constexpr int SUMMERS = 8, FIRST_B = SUMMERS + CONVERTERS, ISSUER = FIRST_B + CONVERTERS;   // warps; then three more
-    static constexpr int THREADS = 32 * (ISSUER + 4);
-    // Registers of a thread: all are launched with the same number; each warpgroup then takes what its role needs.
-    static constexpr int LAUNCH_REGS = NARROW ? 72 : 96, SUMMER_REGS = NARROW ? 96 : 144, A_REGS = 80, B_REGS = NARROW ? 56 : 88,
-                         ISSUER_REGS = NARROW ? 40 : 24;
-    static_assert(SUMMERS * SUMMER_REGS + CONVERTERS * (A_REGS + B_REGS) + 4 * ISSUER_REGS <= (ISSUER + 4) * LAUNCH_REGS,
-                  "more registers than the launch has");
-};
-constexpr int SUMMERS = Shape<false>::SUMMERS;
+constexpr int SUMMERS = 8, CONVERTERS = 4, FIRST_B = SUMMERS + CONVERTERS, ISSUER = FIRST_B + CONVERTERS;   // warps (of A, and of B); then three more
+constexpr int THREADS = 32 * (ISSUER + 4);
+constexpr int WIDTH = 256, PER = WIDTH / 2;     // columns of a tile at most, and of a summing warp
+constexpr int TASKS = 16;                       // times four values: a converter thread's part of its operand of a chunk
+// Registers of a thread: all are launched with the same number; each warpgroup then takes what its role needs.
+constexpr int LAUNCH_REGS = 96, SUMMER_REGS = 144, A_REGS = 80, B_REGS = 88, ISSUER_REGS = 24;
+static_assert(SUMMERS * SUMMER_REGS + CONVERTERS * (A_REGS + B_REGS) + 4 * ISSUER_REGS <= (ISSUER + 4) * LAUNCH_REGS,
+              "more registers than the launch has");
 constexpr int KC = 64;                          // contraction steps of a chunk
 constexpr uint32_t PART = 128 * KC * 2;         // one bf16 part of 128 rows (or columns) of a chunk: 16 KiB
 constexpr uint32_t SLOT = 6 * PART;             // hi, mid, lo of A, then of B
@@ -87,7 +78,7 @@ struct Shared {                 // behind the slots
 static_assert(offsetof(Shared, rows) % 16 == 0 && sizeof(Shared) % 8 == 0, "rows are read 16 bytes at a time");
 
 // The mean or the variance of tile t.
-template <int PASS, bool NARROW>
+template <int PASS>
 __device__ __forceinline__ void tile_item(const GroupedArgs &a, const int *before, int t, int kind, Item &it) {
     it.kind = kind;
     int lo = 0, hi = a.E - 1;   // the last expert whose tiles begin at or before t
@@ -100,7 +91,7 @@ __device__ __forceinline__ void tile_item(const GroupedArgs &a, const int *befor
     expert_rows(a, lo, r0, r1);
     const int l = t - before[lo], mt = ((PASS == FWD ? a.N : a.K) + 255) / 256;
     it.m0 = (l % mt) * 256;
-    const int n = l / mt, width = PASS == PARAM ? a.N : r1 - r0, nt = (width + Shape<NARROW>::WIDTH - 1) / Shape<NARROW>::WIDTH;
+    const int n = l / mt, width = PASS == PARAM ? a.N : r1 - r0, nt = (width + WIDTH - 1) / WIDTH;
     it.bn = round_up((width + nt - 1) / nt, PASS == PARAM ? 128 : 32);
     it.cols = min(it.bn, width - n * it.bn);
     it.c0 = n * it.bn + (PASS == PARAM ? 0 : r0);
@@ -114,28 +105,26 @@ __device__ __forceinline__ void tile_item(const GroupedArgs &a, const int *befor
 
 // Item j of pair `pair`. Cut tiles: 3000 rows of 5 experts, 1001 to 1515 features, forward: 267 us whole, 216 us cut; 7288 rows of
 // 2 experts, 16 to 75 features, parameter pass: 174 and 47 us.
-template <int PASS, bool NARROW>
+template <int PASS>
 __device__ __forceinline__ bool get_item(const GroupedArgs &a, Shared &sh, Plan &p, int pair, int pairs, int j, Item &it) {
     Share s;
     auto chunks_of = [&](int i) {
         Item t;
-        tile_item<PASS, NARROW>(a, sh.before, i >> 1, kind_of(i, pairs), t);
+        tile_item<PASS>(a, sh.before, i >> 1, kind_of(i, pairs), t);
         return t.chunks;
     };
     if (!share_of(sh.start, p, pair, pairs, CUT_SAVES, j, chunks_of, s)) return false;
-    tile_item<PASS, NARROW>(a, sh.before, s.i >> 1, kind_of(s.i, pairs), it);
+    tile_item<PASS>(a, sh.before, s.i >> 1, kind_of(s.i, pairs), it);
     if (s.chunks) it.from = s.from, it.chunks = s.chunks, it.part = s.part;
     return true;
 }
 
 // Operands of 128 rows x 64 contraction steps as the tensor core reads them (128-byte swizzle: 16-byte chunk c of line r
-// lies at chunk c ^ (r & 7)), and which groups of four values ("tasks") a thread of an operand's WARPS warps brings there. With
-// four warps:
+// lies at chunk c ^ (r & 7)), and which 16 groups of four values ("tasks") each of an operand's 128 threads brings there.
 //  K-major: line = row, 64 steps of 2 bytes. Task t = 4 g + s: row g * 32 + row(), steps s * 16 + 0..3 + along(); a warp
 //  loads 64 consecutive bytes of eight rows and stores to all banks.
 //  MN-major: line = 64 rows of one step; the 64 lines of rows 0..63 come before those of rows 64..127. Task t: step
 //  4 t + row(), rows along() + 0..3; a warp loads 512 consecutive bytes.
-// With eight, a task's g (K-major) and t (MN-major) stand for twice as many rows and steps.
 // Rows that are not aligned to 16 bytes are read a float at a time, and a warp's loads have to be neighbours all the same (the
 // load unit takes a line of memory at a time). Neither the order of the steps nor that of the features matters to a sum:
 //  forward pass, both operands: the order of step_at(); four lanes read neighbours.
@@ -143,7 +132,7 @@ __device__ __forceinline__ bool get_item(const GroupedArgs &a, Shared &sh, Plan 
 //  row(). A: its steps lie in the same order, and place 4 i + c of the CTA's 128 features holds feature i + 32 c. 3000 rows of 5
 //  experts, 1001 to 1515 features: 168 us; 185 us without. In the other passes this was slower (forward: a thread then has
 //  sixteen gathered rows; parameters: their output is scattered).
-template <bool MN, bool SPREAD, bool WIDE, int WARPS>
+template <bool MN, bool SPREAD, bool WIDE>
 struct Place {
     static constexpr uint32_t KSTEP = (MN ? 16 * 128 : 32) >> 4;             // 16 contraction steps, in 16-byte units
     static constexpr uint32_t LBO = MN ? 64 * 128 : 16;
@@ -157,16 +146,15 @@ struct Place {
     }
     // where task t goes, from base(): the swizzle's exclusive or with the bits of t that change the chunk or the line
     __device__ static uint32_t at(uint32_t base, int t) {
-        return LINE ? base + t * (WARPS * 256) : !MN ? (base ^ ((t & 3) << 5)) + (t >> 2) * (WARPS * 1024)
-               : WARPS == 4 ? (base ^ ((t & 1) << 6)) + t * 512 : base + t * 1024;
+        return LINE ? base + t * 1024 : MN ? (base ^ ((t & 1) << 6)) + t * 512 : (base ^ ((t & 3) << 5)) + (t >> 2) * 4096;
     }
 };
 template <int PASS, bool VEC>
 constexpr bool wide = !VEC && PASS == STATE;
-template <int PASS, bool VEC, bool NARROW>
-using PlaceA = Place<PASS != FWD, !VEC && PASS == FWD, wide<PASS, VEC>, Shape<NARROW>::CONVERTERS>;
-template <int PASS, bool VEC, bool NARROW>
-using PlaceB = Place<PASS == PARAM, !VEC && PASS == FWD, wide<PASS, VEC>, Shape<NARROW>::CONVERTERS>;
+template <int PASS, bool VEC>
+using PlaceA = Place<PASS != FWD, !VEC && PASS == FWD, wide<PASS, VEC>>;
+template <int PASS, bool VEC>
+using PlaceB = Place<PASS == PARAM, !VEC && PASS == FWD, wide<PASS, VEC>>;
 // Item j, as it was handed over; false when the CTA is aborting. release(): this warp needs the record no longer.
 __device__ __forceinline__ bool take(Shared &sh, int j, Item &t) {
     t.chunks = 0;
@@ -196,11 +184,10 @@ using TcParts = Parts<256, 256>;
 
 // A: 128 features of this CTA. A chunk is fetched whole as soon as the registers of the one before have been stored (one
 // latency a chunk: loads that are waited for in turn would cost one each).
-template <int PASS, bool VEC, bool NARROW>
+template <int PASS, bool VEC>
 __device__ __forceinline__ void convert_a(const GroupedArgs &a, Shared &sh, int cta, int w, int lane, uint32_t smem_base) {
-    constexpr int TASKS = Shape<NARROW>::TASKS, WARPS = Shape<NARROW>::CONVERTERS;
     constexpr bool MN = PASS != FWD, WIDE = wide<PASS, VEC>;
-    using P = PlaceA<PASS, VEC, NARROW>;
+    using P = PlaceA<PASS, VEC>;
     const int row = P::row(w, lane), along = P::along(lane);
     const uint32_t to = smem_base + P::base(w, lane);
     float4 v[TASKS];
@@ -239,20 +226,19 @@ __device__ __forceinline__ void convert_a(const GroupedArgs &a, Shared &sh, int 
             __syncwarp();
         }
 #pragma unroll
-        for (int g = 0; g < TASKS / 4; g++) {
-            const float *src = PASS == FWD ? (cu.var && cu.half ? a.var_w : a.mu_w) + base + cu.kc + (size_t)(g * WARPS * 8) * a.K
-                               : PASS == STATE ? a.mu_w + base + (size_t)(cu.kc + (WIDE ? 0 : g * 4 * WARPS)) * a.K : a.x + base;
+        for (int g = 0; g < 4; g++) {
+            const float *src = PASS == FWD ? (cu.var && cu.half ? a.var_w : a.mu_w) + base + cu.kc + (size_t)(g * 32) * a.K
+                               : PASS == STATE ? a.mu_w + base + (size_t)(cu.kc + (WIDE ? 0 : g * 16)) * a.K : a.x + base;
             int4 r = make_int4(-1, -1, -1, -1);
             if (PASS == PARAM) r = *reinterpret_cast<const int4 *>(&sh.rows[w][g * 4]);
 #pragma unroll
             for (int s = 0; s < 4; s++) {
                 const int rs = s == 0 ? r.x : s == 1 ? r.y : s == 2 ? r.z : r.w;
                 if (PASS == FWD) {
-                    v[g * 4 + s] = ld4<VEC, P::STRIDE>(src + s * 16, g * WARPS * 8 < left ? a.K - cu.kc - along - s * 16 : 0);
+                    v[g * 4 + s] = ld4<VEC, P::STRIDE>(src + s * 16, g * 32 < left ? a.K - cu.kc - along - s * 16 : 0);
                 } else if (PASS == STATE) {
-                    // place p = (4 g + s) * WARPS + row; WIDE: step p / 4 + p % 4 * 16
-                    const int k = !WIDE ? s * WARPS + row : WARPS == 4 ? row * 16 + g * 4 + s : (row & 3) * 16 + (g * 4 + s) * 2 + (row >> 2);
-                    v[g * 4 + s] = ld4<VEC, P::STRIDE>(src + (size_t)k * a.K, cu.kc + (WIDE ? 0 : g * 4 * WARPS) + k < a.N ? left : 0);
+                    const int k = WIDE ? row * 16 + g * 4 + s : s * 4 + row;   // place 16 g + 4 s + row; WIDE: step place / 4 + place % 4 * 16
+                    v[g * 4 + s] = ld4<VEC, P::STRIDE>(src + (size_t)k * a.K, cu.kc + (WIDE ? 0 : g * 16) + k < a.N ? left : 0);
                 } else {
                     v[g * 4 + s] = ld4<VEC>(src + (size_t)max(rs, 0) * a.K, rs >= 0 ? left : 0);
                 }
@@ -277,17 +263,15 @@ __device__ __forceinline__ void convert_a(const GroupedArgs &a, Shared &sh, int 
 
 // B: this CTA's half of the tile's columns, as A. In the parameter pass those are the deltas: the pairs of the first features'
 // tile also add them up for the bias.
-template <int PASS, bool VEC, bool NARROW>
+template <int PASS, bool VEC>
 __device__ __forceinline__ void convert_b(const GroupedArgs &a, Shared &sh, int cta, int w, int lane, uint32_t smem_base) {
-    constexpr int WARPS = Shape<NARROW>::CONVERTERS;
     constexpr bool MN = PASS == PARAM;
-    constexpr int FOURS = MN ? 4 : Shape<NARROW>::PER / (WARPS * 8);   // of tasks
-    using P = PlaceB<PASS, VEC, NARROW>;
+    using P = PlaceB<PASS, VEC>;
     const int row = P::row(w, lane), along = P::along(lane);
     const uint32_t to = smem_base + 3 * PART + P::base(w, lane);
-    float4 v[4 * FOURS];
+    float4 v[TASKS];
     Cursor cu;
-    int rows[FOURS];         // forward pass: input rows of the thread's columns
+    int rows[4];             // forward pass: input rows of the thread's four columns
     size_t base = 0;         // state, parameter pass: the thread's first element at contraction step 0
     int left = 0, half_bn = 0, nk = 0, depth = 0;   // left: columns from the thread's first one to the end of the CTA's
     bool sum = false;        // the item's deltas are added up for the bias
@@ -309,7 +293,7 @@ __device__ __forceinline__ void convert_b(const GroupedArgs &a, Shared &sh, int 
         sum = PASS == PARAM && a.var_b != nullptr && t.chunks > 0 && t.m0 == 0;
         if (PASS == FWD) {
 #pragma unroll
-            for (int g = 0; g < FOURS; g++) rows[g] = g * WARPS * 8 < left ? sh.record[j % RECORDS].rows[g * WARPS * 8 + row] : -1;
+            for (int g = 0; g < 4; g++) rows[g] = g * 32 < left ? sh.record[j % RECORDS].rows[g * 32 + row] : -1;
         } else {
             base = PASS == STATE ? (size_t)(t.c0 + n) * a.N + along : (size_t)(t.p0 + row) * a.N + t.c0 + n;
         }
@@ -322,15 +306,15 @@ __device__ __forceinline__ void convert_b(const GroupedArgs &a, Shared &sh, int 
     };
     auto load = [&](int g) {
         const float *src = PASS == FWD ? (!cu.var ? a.a0 : cu.half ? a.second : a.a1) + (size_t)max(rows[g], 0) * a.K + cu.kc + along
-                                       : (cu.var ? a.a1 : a.a0) + base + (PASS == STATE ? (size_t)(g * WARPS * 8) * a.N + cu.kc : (size_t)(cu.kc + g * 16) * a.N);
+                                       : (cu.var ? a.a1 : a.a0) + base + (PASS == STATE ? (size_t)(g * 32) * a.N + cu.kc : (size_t)(cu.kc + g * 16) * a.N);
 #pragma unroll
         for (int s = 0; s < 4; s++) {
             if (P::LINE) {
-                v[g * 4 + s] = ld4<VEC, P::STRIDE>(src + (size_t)(s * WARPS * 2) * a.N, g * WARPS * 8 + s * WARPS * 2 < left ? a.N - cu.kc - along : 0);
+                v[g * 4 + s] = ld4<VEC, P::STRIDE>(src + (size_t)(s * 8) * a.N, g * 32 + s * 8 < left ? a.N - cu.kc - along : 0);
             } else if (PASS == FWD) {
                 v[g * 4 + s] = ld4<VEC, P::STRIDE>(src + s * 16, rows[g] >= 0 ? a.K - cu.kc - along - s * 16 : 0);
             } else if (PASS == STATE) {
-                v[g * 4 + s] = ld4<VEC>(src + s * 16, g * WARPS * 8 < left ? a.N - cu.kc - along - s * 16 : 0);
+                v[g * 4 + s] = ld4<VEC>(src + s * 16, g * 32 < left ? a.N - cu.kc - along - s * 16 : 0);
             } else {
                 v[g * 4 + s] = ld4<VEC>(src + (size_t)(s * 4) * a.N, cu.kc + (g * 4 + s) * 4 + row < depth ? left : 0);
             }
@@ -340,24 +324,24 @@ __device__ __forceinline__ void convert_b(const GroupedArgs &a, Shared &sh, int 
     for (int i = 0; cu.end > 0; i++) {
         const int s = i & 1, lines = half_bn;
 #pragma unroll
-        for (int g = 0; g < FOURS; g++) load(g);
+        for (int g = 0; g < 4; g++) load(g);
         const bool sums = PASS == PARAM && sum;
         const int ended = PASS == PARAM && cu.c + 1 == cu.end ? cu.j : -1;   // the item that ends with this chunk
         advance();
         if (i >= 2 && !mbar_wait(sh.done + s, ((i - 2) >> 1) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_EMPTY)) return;
 #pragma unroll
-        for (int g = 0; g < FOURS; g++)
-            if (MN || g * WARPS * 8 < lines) {   // narrow tiles have no columns for the later groups
+        for (int g = 0; g < 4; g++)
+            if (MN || g * 32 < lines) {   // narrow tiles have no columns for the later groups
 #pragma unroll
                 for (int q = g * 4; q < g * 4 + 4; q++)
-                    if (MN ? along < round_up(lines, 64) : P::LINE ? q * WARPS * 2 + row < lines : g * WARPS * 8 + row < lines) store_split(P::at(to + s * SLOT, q), PART, v[q]);
+                    if (MN ? along < round_up(lines, 64) : P::LINE ? q * 8 < lines : g * 32 + row < lines) store_split(P::at(to + s * SLOT, q), PART, v[q]);
             }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(sh.full + s, 0);
         if (PASS == PARAM && sums) {
 #pragma unroll
-            for (int q = 0; q < 4 * FOURS; q++) {
+            for (int q = 0; q < TASKS; q++) {
                 add2(total.x, total.y, v[q].x, v[q].y);
                 add2(total.z, total.w, v[q].z, v[q].w);
             }
@@ -389,14 +373,12 @@ __device__ __forceinline__ void convert_b(const GroupedArgs &a, Shared &sh, int 
     }
 }
 
-// Experts of more than `above` and at most `upto` rows.
-template <int PASS, bool VEC, bool NARROW>
-__global__ void __launch_bounds__(Shape<NARROW>::THREADS, 1) grouped_tc_kernel(const GroupedArgs a, int above, int upto) {
-    using Sh = Shape<NARROW>;
-    constexpr int FIRST_B = Sh::FIRST_B, ISSUER = Sh::ISSUER, PER = Sh::PER;
+// Experts of more than `above` rows.
+template <int PASS, bool VEC>
+__global__ void __launch_bounds__(THREADS, 1) grouped_tc_kernel(const GroupedArgs a, int above) {
     constexpr bool A_MN = PASS != FWD, B_MN = PASS == PARAM;
-    using PA = PlaceA<PASS, VEC, NARROW>;   // layouts of the operands
-    using PB = PlaceB<PASS, VEC, NARROW>;
+    using PA = PlaceA<PASS, VEC>;   // layouts of the operands
+    using PB = PlaceB<PASS, VEC>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     Shared &sh = *reinterpret_cast<Shared *>(smem_raw + (smem_base - smem_u32(smem_raw)) + 2 * SLOT);
@@ -408,7 +390,7 @@ __global__ void __launch_bounds__(Shape<NARROW>::THREADS, 1) grouped_tc_kernel(c
         for (int e0 = 0; e0 < a.E; e0 += 32) {
             int r0 = 0, r1 = 0;
             if (e0 + lane < a.E) expert_rows(a, e0 + lane, r0, r1);
-            const int v = r1 - r0 > above && r1 - r0 <= upto ? mt * (((PASS == PARAM ? a.N : r1 - r0) + Sh::WIDTH - 1) / Sh::WIDTH) : 0;
+            const int v = r1 - r0 > above ? mt * (((PASS == PARAM ? a.N : r1 - r0) + WIDTH - 1) / WIDTH) : 0;
             int s = v;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -451,7 +433,7 @@ __global__ void __launch_bounds__(Shape<NARROW>::THREADS, 1) grouped_tc_kernel(c
     };
 
     if (warp >= ISSUER) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Sh::ISSUER_REGS));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(ISSUER_REGS));
         // ---------------------------------------------------------------------------------------------- MMA (CTA 0)
         if (warp == ISSUER && lane == 0 && cta == 0) {
             constexpr uint32_t HI = desc_hi(1024, SWZ_128B);
@@ -484,7 +466,7 @@ __global__ void __launch_bounds__(Shape<NARROW>::THREADS, 1) grouped_tc_kernel(c
                 if (j >= RECORDS && !mbar_wait(sh.item_empty + j % RECORDS, (j / RECORDS - 1) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_EMPTY))
                     break;
                 Item t;
-                more = get_item<PASS, NARROW>(a, sh, plan, pair, pairs, j, t);
+                more = get_item<PASS>(a, sh, plan, pair, pairs, j, t);
                 if (!more) t.chunks = 0;
                 if (more && t.part != WHOLE && cta == 0 && lane == 0)
                     *TcParts::piece(a, pairs, pair, t.part) = Piece{1, t.from + t.chunks == (PASS == FWD && t.kind == VAR ? 2 : 1) * t.nk, t.e, t.m0, t.c0, t.cols, t.bn, t.kind};
@@ -503,7 +485,7 @@ __global__ void __launch_bounds__(Shape<NARROW>::THREADS, 1) grouped_tc_kernel(c
         if (warp == ISSUER) tmem_dealloc_pair(sh.tmem, 2 * ACC);
     } else if (warp < SUMMERS) {
         // ------------------------------------------------------------------------------------------- sums and output
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Sh::SUMMER_REGS));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SUMMER_REGS));
         const int quad = warp & 3, group = warp >> 2;
         const uint32_t lane_addr = tmem + ((uint32_t)(quad * 32) << 16);
         float acc[PER];
@@ -612,13 +594,12 @@ __global__ void __launch_bounds__(Shape<NARROW>::THREADS, 1) grouped_tc_kernel(c
     } else {
         // ------------------------------------------------------------------------------------------------- converters
         if (warp < FIRST_B) {
-            if (Sh::A_REGS > Sh::LAUNCH_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Sh::A_REGS));
-            else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Sh::A_REGS));
-            convert_a<PASS, VEC, NARROW>(a, sh, cta, warp - SUMMERS, lane, smem_base);
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(A_REGS));
+            convert_a<PASS, VEC>(a, sh, cta, warp - SUMMERS, lane, smem_base);
             finish();
         } else {
-            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Sh::B_REGS));
-            convert_b<PASS, VEC, NARROW>(a, sh, cta, warp - FIRST_B, lane, smem_base);
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(B_REGS));
+            convert_b<PASS, VEC>(a, sh, cta, warp - FIRST_B, lane, smem_base);
             finish();
         }
     }
@@ -642,15 +623,14 @@ __global__ void __launch_bounds__(256) grouped_second_moment_unaligned_kernel(co
     if (i < n) out[i] = fmaf(__ldg(mu + i), __ldg(mu + i), __ldg(var + i));
 }
 
-template <int PASS, bool NARROW>
-int launch_pass(const GroupedArgs &a, int above, int upto, cudaStream_t st) {
-    using Sh = Shape<NARROW>;
+template <int PASS>
+int launch_pass(const GroupedArgs &a, int above, cudaStream_t st) {
     const bool vec = grouped_aligned(PASS, a);
     const size_t smem = 2 * SLOT + 1024 + sizeof(Shared) + (a.E + 1) * sizeof(int);
     const int pairs = grouped_tc_pairs(PASS, a.E, a.S, a.K, a.N);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2 * pairs);
-    cfg.blockDim = dim3(Sh::THREADS);
+    cfg.blockDim = dim3(THREADS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr;
@@ -660,24 +640,13 @@ int launch_pass(const GroupedArgs &a, int above, int upto, cudaStream_t st) {
     attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    auto k = vec ? grouped_tc_kernel<PASS, true, NARROW> : grouped_tc_kernel<PASS, false, NARROW>;
+    auto k = vec ? grouped_tc_kernel<PASS, true> : grouped_tc_kernel<PASS, false>;
     TAGI_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    TAGI_CUDA(cudaLaunchKernelEx(&cfg, k, a, above, upto));
-    grouped_join_kernel<PASS, 256, 256><<<dim3(pairs, Sh::WIDTH / JOIN_COLUMNS), 256, 0, st>>>(a, pairs, vec ? wide<PASS, true> : wide<PASS, false>);
+    TAGI_CUDA(cudaLaunchKernelEx(&cfg, k, a, above));
+    grouped_join_kernel<PASS, 256, 256><<<dim3(pairs, WIDTH / JOIN_COLUMNS), 256, 0, st>>>(a, pairs, vec ? wide<PASS, true> : wide<PASS, false>);
     TAGI_CUDA(cudaGetLastError());
     return TAGI_OK;
 }
-// Narrow tiles for experts of up to 128 rows, where the average expert makes some likely: a kernel that finds nothing to do takes
-// 7 us with its join. The kernels follow one another and use the same workspace. Eight experts of 4096 x 4096, forward pass, 56 /
-// 100 / 128 rows each: 546 / 653 / 697 us, with wide tiles 813 / 843 / 862 us; state pass 352 / 421 / 454 and 477 / 516 / 529.
-template <int PASS>
-int launch_rows(const GroupedArgs &a, cudaStream_t st) {
-    if (a.S <= THIN_ROWS / 2 * a.E || a.S > (NARROW_ROWS + 32) * a.E) return launch_pass<PASS, false>(a, a.thin, a.S, st);
-    int rc = launch_pass<PASS, true>(a, a.thin, NARROW_ROWS, st);
-    if (rc != TAGI_OK || a.S <= NARROW_ROWS) return rc;
-    return launch_pass<PASS, false>(a, NARROW_ROWS, a.S, st);
-}
-
 }  // namespace
 
 // CTA pairs that may find work: one per SM pair, or as many as there can be chunks
@@ -704,7 +673,10 @@ int grouped_second_moment(const GroupedArgs &a, cudaStream_t st) {
 }
 
 int grouped_tc(int pass, const GroupedArgs &a, cudaStream_t st) {
-    return pass == FWD ? launch_rows<FWD>(a, st) : pass == STATE ? launch_rows<STATE>(a, st) : launch_pass<PARAM, false>(a, a.thin, a.S, st);
+    if (pass == PARAM) return launch_pass<PARAM>(a, FEW_PARAM_ROWS, st);
+    const int above = middle_likely(a.E, a.S) ? MIDDLE_ROWS : THIN_ROWS;   // what tagi_grouped_thin.cu has left
+    if (a.S <= above) return TAGI_OK;
+    return pass == FWD ? launch_pass<FWD>(a, above, st) : launch_pass<STATE>(a, above, st);
 }
 
 int grouped_tc_status(int *out, int reset) {

@@ -1,20 +1,19 @@
-// Linear layers grouped by expert, forward and state pass of experts with few < rows <= thin on the tensor cores:
-// the arithmetic of tagi_grouped_tc.cu for tiles so narrow that the weights' way from HBM, not the multiplication, is what
-// takes the time. Bound: HBM, 8 (forward) or 4 (state) bytes a weight.
+// Linear layers grouped by expert, forward and state pass of experts with 9 to 48 rows, and 49 to 128, on the tensor cores: the
+// arithmetic of tagi_grouped_tc.cu for tiles so narrow that the weights' way from HBM and their conversion, not the
+// multiplication, are what takes the time. Bound: HBM, 8 (forward) or 4 (state) bytes a weight.
 //
-// One CTA computes 128 features x all rows of an expert. The weights come through a ring of eight half-chunks (16 KiB each),
-// so that about 100 KB of each SM are on their way from HBM whatever the converters do: by TMA, or with cp.async, by the 16-byte
-// groups of memory that they lie in, where rows are not multiples of 16 bytes (30 rows of 4 experts of 2047 x 2047, forward: 122
-// us; 4 bytes at a time 140 us; of 2048 x 2048 82 us). Sixteen warps read them, a feature to a lane, and store the values' bf16
-// parts to tensor memory, where the MMAs take that operand from (through shared memory, its parts would be read six times
-// from there). Four more warps fetch and split the rows, which come from L2; eight add up the accumulators of chunks of 64
-// steps; one thread issues the MMAs. Mean and variance of a tile go to neighbouring CTAs at the same time, mu_w first in
-// both, so that it is fetched from HBM once.
+// One CTA computes 128 features x all rows of an expert. The weights come through a ring of six to eight half-chunks (16 KiB
+// each), so that about 100 KB of each SM are on their way from HBM whatever the converters do: by TMA, or with cp.async, by the
+// 16-byte groups of memory that they lie in, where rows are not multiples of 16 bytes (30 rows of 4 experts of 2047 x 2047,
+// forward: 100 us; of 2048 x 2048 66 us). Eight warps read them, a feature to a lane, and store the values' bf16 parts to tensor
+// memory, where the MMAs take that operand from. Eight more fetch and split the rows, which come from L2; eight add up the
+// accumulators of chunks of 64 steps; one issues the MMAs.
 //
-// A thread issues an MMA every 70 cycles at best, and a chunk has to be done in 1380 (32 KiB at an SM's share of HBM), so the
-// six products of 16 steps are three MMAs: the rows' parts lie below each other and count as one operand of up to 3 x 48
-// columns. hi.[hi mid lo] adds to accumulators 0, 1 and 2, mid.[hi mid] to 1 and 2, lo.[hi] to 2: the accumulators hold the
-// terms of one magnitude each and are added up when a chunk is read.
+// Up to 48 rows the six products of 16 steps are three MMAs: the rows' parts lie below each other and count as one operand of up
+// to 3 x 48 columns (STACKED). hi.[hi mid lo] adds to accumulators 0, 1 and 2, mid.[hi mid] to 1 and 2, lo.[hi] to 2: the
+// accumulators hold the terms of one magnitude each and are added up when a chunk is read. The rows' warps take turns at the
+// chunks (four for each: 365 us instead of 283 for 16 rows of 8 experts of 4096 x 4096, forward; HBM alone takes 164 us). With
+// more rows the accumulators do not fit tensor memory three times, and the products are six MMAs into one.
 #include "tagi_grouped_plan.cuh"
 #include "tagi_grouped_split.cuh"
 #include "tagi_tc_tile.cuh"
@@ -26,20 +25,28 @@ namespace thin {
 constexpr int SUMMERS = 8, CONVERT_A = 8, CONVERT_B = 8, LOADERS = 2;
 constexpr int FIRST_A = SUMMERS, FIRST_B = FIRST_A + CONVERT_A, FIRST_LOADER = FIRST_B + CONVERT_B, ISSUER = FIRST_LOADER + LOADERS;
 constexpr int THREADS = 32 * (ISSUER + 2);       // the last warp works out the items
-constexpr int ROWS = 128, COLS = 48, KC = 64, HALF = 32, RING = 8, RECORDS = 4, CTAS = 148;
-constexpr uint32_t SLOT = 3 * COLS * KC * 2;   // the parts of a tile lie bn rows of 128 bytes apart
+constexpr int ROWS = 128, KC = 64, HALF = 32, MAX_RING = 8, RECORDS = 4, CTAS = 148;
+// For tiles of up to COLS columns. STACKED: the rows' parts count as one operand.
+template <int COLS>
+struct Shape {
+    static constexpr bool STACKED = COLS <= 48;
+    static constexpr int ring(bool vec) { return STACKED ? 8 : vec ? 7 : 6; }   // half-chunks
+    static constexpr uint32_t SLOT = 3 * COLS * KC * 2;   // the parts of a tile lie bn rows of 128 bytes apart
+    // tensor-memory columns: two slots of accumulators, two slots of A's parts (two bf16 values a column)
+    static constexpr uint32_t ACC = (STACKED ? 3 : 1) * COLS, A_COL = 2 * ACC;
+    static_assert(SLOT % 1024 == 0, "the swizzle counts lines from multiples of 1024 bytes");
+    static_assert(A_COL + 2 * 3 * (KC / 2) <= 512, "tensor memory");
+};
+// Registers of a thread, not stacked: all are launched with the same number; each warpgroup then takes what its role needs.
+constexpr int LAUNCH_REGS = 72, SUMMER_REGS = 104, CONVERT_REGS = 64, OTHER_REGS = 40;
+static_assert(SUMMERS * SUMMER_REGS + (CONVERT_A + CONVERT_B) * CONVERT_REGS + 4 * OTHER_REGS <= THREADS / 32 * LAUNCH_REGS, "more registers than the launch has");
 // A half-chunk of weights. Lines that do not begin at multiples of 16 bytes take one 16-byte group more, begin up to three floats
 // behind their place, and are not swizzled: a pitch of 36 floats keeps eight lines off each other's banks as well.
 constexpr int FWD_PITCH = HALF + 4, STATE_PITCH = ROWS + 4;   // floats
 __host__ __device__ constexpr uint32_t raw_bytes(bool vec) { return vec ? ROWS * HALF * 4 : ROWS * FWD_PITCH * 4; }
 static_assert(HALF * STATE_PITCH * 4 <= raw_bytes(false), "");
-// tensor-memory columns: two slots of three accumulators, two slots of A's parts (two bf16 values a column)
-constexpr uint32_t ACC = 3 * COLS, A_PART = KC / 2, A_SLOT = 3 * A_PART, A_COL = 2 * ACC, TMEM_COLS = 512;
-static_assert(SLOT % 1024 == 0, "the swizzle counts lines from multiples of 1024 bytes");
-static_assert(A_COL + 2 * A_SLOT <= TMEM_COLS, "");
+constexpr uint32_t A_PART = KC / 2, A_SLOT = 3 * A_PART, TMEM_COLS = 512;
 constexpr int CUT_SAVES = 12;   // chunks that cutting has to save (see tagi_grouped_plan.cuh): a chunk takes 1 us, cutting about 10
-using ThinParts = Parts<ROWS, COLS>;
-static_assert(THIN_ROWS <= COLS, "one tile for all rows of an expert");
 
 __device__ int g_status;  // first wait that ran out
 
@@ -49,8 +56,9 @@ struct Item {
     int kind, depth, nk;          // MEAN or VAR; contraction length; chunks of one contraction
     int from, part;               // first chunk; WHOLE, or which of the CTA's two partial sums the item goes to
 };
+template <int COLS>
 struct Shared {                   // behind the slots and the ring
-    uint64_t full[2], done[2], raw_full[RING], raw_empty[RING], item_full[RECORDS], item_empty[RECORDS];
+    uint64_t full[2], done[2], raw_full[MAX_RING], raw_empty[MAX_RING], item_full[RECORDS], item_empty[RECORDS];
     uint32_t tmem;
     volatile int abort_flag;
     Item item[RECORDS];
@@ -58,11 +66,10 @@ struct Shared {                   // behind the slots and the ring
     int start[2 * CTAS + 2];      // of the tiles that are cut: chunks of those before each
     int before[];                 // tiles of the experts before e, E + 1 entries
 };
-static_assert(sizeof(Shared) % 8 == 0, "");
 
 // Item j of a CTA; chunks == 0: there is none.
-template <int PASS>
-__device__ __forceinline__ void get_item(const GroupedArgs &a, Shared &sh, Plan &p, int j, Item &it) {
+template <int PASS, int COLS>
+__device__ __forceinline__ void get_item(const GroupedArgs &a, Shared<COLS> &sh, Plan &p, int j, Item &it) {
     const int ctas = gridDim.x, *before = sh.before;
     it.depth = PASS == FWD ? a.K : a.N;
     it.nk = (it.depth + KC - 1) / KC;
@@ -87,13 +94,15 @@ __device__ __forceinline__ void get_item(const GroupedArgs &a, Shared &sh, Plan 
     it.chunks = s.chunks ? s.chunks : chunks_of(s.i);
 }
 
-__device__ __forceinline__ bool take(Shared &sh, int j, Item &t) {
+template <int COLS>
+__device__ __forceinline__ bool take(Shared<COLS> &sh, int j, Item &t) {
     t.chunks = 0;
     if (!mbar_wait(sh.item_full + j % RECORDS, (j / RECORDS) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_RAW)) return false;
     t = sh.item[j % RECORDS];
     return true;
 }
-__device__ __forceinline__ void release(Shared &sh, int j, int lane) {
+template <int COLS>
+__device__ __forceinline__ void release(Shared<COLS> &sh, int j, int lane) {
     __syncwarp();
     if (lane == 0) mbar_arrive(sh.item_empty + j % RECORDS);
 }
@@ -113,13 +122,19 @@ __device__ __forceinline__ void copy16(uint32_t dst, const float *src, int bytes
 // of a 16-byte group before whose end lie `floats` of a line's floats (any number)
 __device__ __forceinline__ int bytes_of(int floats) { return min(max(floats, 0), 4) * 4; }
 
-template <int PASS, bool VEC>
+// Experts of more than `above` and at most `upto` rows.
+template <int PASS, bool VEC, int COLS>
 __global__ void __launch_bounds__(THREADS, 1)
-grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_constant__ CUtensorMap var_map, const GroupedArgs a, bool may_cut) {
+grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_constant__ CUtensorMap var_map, const GroupedArgs a, int above, int upto, bool may_cut) {
+    using Sh = Shape<COLS>;
+    using ThinParts = Parts<ROWS, COLS>;
+    constexpr bool STACKED = Sh::STACKED;
+    constexpr int RING = Sh::ring(VEC);
+    constexpr uint32_t SLOT = Sh::SLOT, ACC = Sh::ACC, A_COL = Sh::A_COL;
     constexpr uint32_t RAW = raw_bytes(VEC);
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u, ring = smem_base + 2 * SLOT;
-    Shared &sh = *reinterpret_cast<Shared *>(smem_raw + (smem_base - smem_u32(smem_raw)) + 2 * SLOT + RING * RAW);
+    Shared<COLS> &sh = *reinterpret_cast<Shared<COLS> *>(smem_raw + (smem_base - smem_u32(smem_raw)) + 2 * SLOT + RING * RAW);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (warp == 0) {
         const int mt = ((PASS == FWD ? a.N : a.K) + ROWS - 1) / ROWS;
@@ -127,7 +142,7 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
         for (int e0 = 0; e0 < a.E; e0 += 32) {
             int r0 = 0, r1 = 0;
             if (e0 + lane < a.E) expert_rows(a, e0 + lane, r0, r1);
-            const int v = r1 - r0 > a.few && r1 - r0 <= a.thin ? mt : 0;
+            const int v = r1 - r0 > above && r1 - r0 <= upto ? mt : 0;
             int s = v;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -144,7 +159,7 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
     if (sh.before[a.E] == 0) return;   // no expert of this size
     if (threadIdx.x == 0) {
         for (int s = 0; s < 2; s++) {
-            mbar_init(sh.full + s, SUMMERS + CONVERT_A + CONVERT_B / 2);   // half the converters of B write a slot
+            mbar_init(sh.full + s, SUMMERS + CONVERT_A + (STACKED ? CONVERT_B / 2 : CONVERT_B));   // stacked: B's take turns
             mbar_init(sh.done + s, 1);
         }
         for (int s = 0; s < RING; s++) {
@@ -166,6 +181,7 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
 
     if (warp < SUMMERS) {
         // -------------------------------------------------------------------------------------------- sums and output
+        if (!STACKED) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SUMMER_REGS));
         const int quad = warp & 3, group = warp >> 2;
         const uint32_t lane_addr = tmem + ((uint32_t)(quad * 32) << 16);
         float acc[COLS / 2];
@@ -188,6 +204,12 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
                 for (int g = 0; g < COLS / 2; g += 8)
                     if (g < per) {
                         float v[8], u[8], t[8];
+                        if (!STACKED) {
+                            tmem_ld_32x8(lane_addr + s * ACC + first + g, v);
+#pragma unroll
+                            for (int x = 0; x < 8; x += 2) add2(acc[g + x], acc[g + x + 1], v[x], v[x + 1]);
+                            continue;
+                        }
                         tmem_ld_32x8_async(lane_addr + s * ACC + 2 * it.bn + first + g, v);
                         tmem_ld_32x8_async(lane_addr + s * ACC + it.bn + first + g, u);
                         tmem_ld_32x8_async(lane_addr + s * ACC + first + g, t);
@@ -231,6 +253,7 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
         }
     } else if (warp < FIRST_B) {
         // ------------------------------------------------------------------------------------------ weights, ring -> parts
+        if (!STACKED) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CONVERT_REGS));
         // h: which half of each chunk
         const int w = warp - FIRST_A, quad = w & 3, h = w >> 2, row = quad * 32 + lane;
         Item it;
@@ -249,8 +272,10 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
                 const int r = 2 * i + h, slot = i & 1;
                 const uint32_t to = tmem + ((uint32_t)(quad * 32) << 16) + A_COL + slot * A_SLOT + h * (HALF / 2);
                 const bool square = it.kind == VAR && (PASS == STATE || c < it.nk);
-                ok = mbar_wait(sh.raw_full + r % RING, (r / RING) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_RAW) &&
-                     (i < 2 || mbar_wait(sh.done + slot, ((i - 2) >> 1) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_EMPTY));
+                // the slot first: once it is free, nothing that was to come before this half-chunk in its place of the ring is still to
+                // come, so that the parity tells
+                ok = (i < 2 || mbar_wait(sh.done + slot, ((i - 2) >> 1) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_EMPTY)) &&
+                     mbar_wait(sh.raw_full + r % RING, (r / RING) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_RAW);
                 if (!ok) break;
                 tc_fence_after_sync();
                 const uint32_t raw = ring + (r % RING) * RAW;
@@ -309,8 +334,10 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
         }
     } else if (warp < FIRST_LOADER) {
         // ------------------------------------------------------------------------------- rows, global memory -> parts
-        // a warp loads 64 consecutive bytes of eight rows; two groups of four warps take turns at the chunks
-        const int w = (warp - FIRST_B) & 3, turn = (warp - FIRST_B) >> 2, row = w * 8 + ((lane >> 2) & 3) * 2 + (lane >> 4), along = VEC ? (lane & 3) * 4 : lane & 3;
+        // a warp loads 64 consecutive bytes of eight rows; two groups of four warps take turns at the chunks, or have half the rows
+        if (!STACKED) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CONVERT_REGS));
+        constexpr int TURNS = STACKED ? 2 : 1;
+        const int w = (warp - FIRST_B) & 3, half = (warp - FIRST_B) >> 2, turn = STACKED ? half : 0, row = (STACKED ? 0 : half * 64) + w * 8 + ((lane >> 2) & 3) * 2 + (lane >> 4), along = VEC ? (lane & 3) * 4 : lane & 3;
         const uint32_t to = smem_base + row * 128 + ((((lane & 3) >> 1) ^ (row & 7)) << 4) + (lane & 1) * 8;
         float4 v[8];
         Item it;
@@ -340,11 +367,11 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
         };
         seek();
         if (turn == 1) step();
-        for (int i = turn; it.chunks > 0; i += 2) {
-            const int s = turn, cols = it.bn;
+        for (int i = turn; it.chunks > 0; i += TURNS) {
+            const int s = i & 1, cols = it.bn;
             load();
             step();
-            step();
+            if (STACKED) step();
             if (i >= 2) ok = mbar_wait(sh.done + s, ((i - 2) >> 1) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_EMPTY);
             if (!ok) break;
 #pragma unroll
@@ -354,6 +381,11 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
             __syncwarp();
             if (lane == 0) mbar_arrive(sh.full + s);
         }
+    } else if (!STACKED) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
+    }
+    // the warps that need few registers: a chain of its own, as all of a warpgroup's warps give registers back together
+    if (warp < FIRST_LOADER) {
     } else if (warp < ISSUER) {
         // --------------------------------------------------------------------------------------- weights, HBM -> ring
         // Forward: lines of 32 steps of a feature, 16-byte chunk c of line l at c ^ (l & 7), which is what TMA's 128-byte
@@ -448,8 +480,13 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
                 if (!ok) break;
                 tc_fence_after_sync();
                 const uint32_t x = tm + A_COL + s * A_SLOT, y = desc_lo(base + s * SLOT, 16), d = tm + s * ACC;
-                for (int k = 0; k < steps; k++)
-                    mma_stacked_ts<A_PART>(d, d + bn, d + 2 * bn, x + k * 8, y + k * 2, HI, three, two, one, k, lead);
+                if (STACKED) {
+                    for (int k = 0; k < steps; k++)
+                        mma_stacked_ts<A_PART>(d, d + bn, d + 2 * bn, x + k * 8, y + k * 2, HI, three, two, one, k, lead);
+                } else {
+                    for (int k = 0; k < steps; k++) mma_small_products_ts<A_PART>(d, x + k * 8, y + k * 2, bn * 8, HI, one, k, lead);
+                    for (int k = 0; k < steps; k++) mma_large_product_ts(d, x + k * 8, y + k * 2, HI, one, lead);
+                }
                 if (lead) mma_commit(sh.done + s);
                 __syncwarp();
             }
@@ -461,7 +498,7 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
         for (int j = 0; more; j++) {
             if (j >= RECORDS && !mbar_wait(sh.item_empty + j % RECORDS, (j / RECORDS - 1) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_EMPTY)) break;
             Item t;
-            get_item<PASS>(a, sh, plan, j, t);
+            get_item<PASS, COLS>(a, sh, plan, j, t);
             more = t.chunks > 0;
             if (more && t.part != WHOLE && lane == 0)
                 *ThinParts::piece(a, gridDim.x, blockIdx.x, t.part) =
@@ -500,27 +537,28 @@ struct Grid {
     int ctas;
     bool may_cut;
 };
-Grid grid_of(int pass, int E, int S, int K, int N) {
-    const long mt = ((pass == FWD ? N : K) + ROWS - 1) / ROWS, experts = E < S / (FEW_ROWS + 1) ? E : S / (FEW_ROWS + 1);
-    const long items = 2 * mt * experts, nk = ((pass == FWD ? K : N) + KC - 1) / KC;   // experts with more than `few` rows, at most
+Grid grid_of(int pass, int above, int E, int S, int K, int N) {
+    const long mt = ((pass == FWD ? N : K) + ROWS - 1) / ROWS, experts = E < S / (above + 1) ? E : S / (above + 1);
+    const long items = 2 * mt * experts, nk = ((pass == FWD ? K : N) + KC - 1) / KC;   // experts with more than `above` rows, at most
     const long longest = pass == FWD ? 2 * nk : nk, chunks = pass == FWD ? items / 2 * 3 * nk : items * nk;
     const bool may_cut = items <= CTAS ? longest - chunks / CTAS >= 16 : items < 4 * CTAS && longest >= 48;
     const long most = may_cut ? chunks : items;
     return Grid{(int)(most < 1 ? 1 : most < CTAS ? most : CTAS), may_cut};
 }
 
-template <int PASS>
-int launch_thin(const GroupedArgs &a, cudaStream_t st) {
+template <int PASS, int COLS>
+int launch_thin(const GroupedArgs &a, int above, int upto, cudaStream_t st) {
+    using Sh = Shape<COLS>;
     const bool vec = grouped_aligned(PASS, a);
-    const size_t smem = 2 * SLOT + RING * raw_bytes(vec) + 1024 + sizeof(Shared) + (a.E + 1) * sizeof(int);
-    const Grid g = grid_of(PASS, a.E, a.S, a.K, a.N);
+    const size_t smem = 2 * Sh::SLOT + Sh::ring(vec) * raw_bytes(vec) + 1024 + sizeof(Shared<COLS>) + (a.E + 1) * sizeof(int);
+    const Grid g = grid_of(PASS, above, a.E, a.S, a.K, a.N);
     CUtensorMap mean = {}, var = {};
     int rc;
     if (vec && (rc = make_map(PASS, a, a.mu_w, &mean)) != TAGI_OK) return rc;
     if (vec && PASS == FWD && (rc = make_map(PASS, a, a.var_w, &var)) != TAGI_OK) return rc;
-    auto k = vec ? grouped_thin_kernel<PASS, true> : grouped_thin_kernel<PASS, false>;
+    auto k = vec ? grouped_thin_kernel<PASS, true, COLS> : grouped_thin_kernel<PASS, false, COLS>;
     TAGI_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    k<<<g.ctas, THREADS, smem, st>>>(mean, var, a, g.may_cut);
+    k<<<g.ctas, THREADS, smem, st>>>(mean, var, a, above, upto, g.may_cut);
     TAGI_CUDA(cudaGetLastError());
     if (g.may_cut) {
         grouped_join_kernel<PASS, ROWS, COLS><<<dim3(g.ctas, COLS / JOIN_COLUMNS), ROWS, 0, st>>>(a, g.ctas, false);
@@ -532,11 +570,18 @@ int launch_thin(const GroupedArgs &a, cudaStream_t st) {
 }  // namespace thin
 }  // namespace
 
-int grouped_thin(int pass, const GroupedArgs &a, cudaStream_t st) { return pass == FWD ? thin::launch_thin<FWD>(a, st) : thin::launch_thin<STATE>(a, st); }
+template <int PASS>
+static int launch_all(const GroupedArgs &a, cudaStream_t st) {
+    int rc = thin::launch_thin<PASS, 48>(a, a.few, THIN_ROWS, st);
+    if (rc != TAGI_OK || !middle_likely(a.E, a.S)) return rc;
+    return thin::launch_thin<PASS, 128>(a, THIN_ROWS, MIDDLE_ROWS, st);
+}
+int grouped_thin(int pass, const GroupedArgs &a, cudaStream_t st) { return pass == FWD ? launch_all<FWD>(a, st) : launch_all<STATE>(a, st); }
 
 size_t grouped_thin_parts_bytes(int pass, int E, int S, int K, int N) {
-    const thin::Grid g = thin::grid_of(pass, E, S, K, N);
-    return g.may_cut ? thin::ThinParts::bytes(g.ctas) : 0;
+    const thin::Grid g = thin::grid_of(pass, FEW_ROWS, E, S, K, N), h = thin::grid_of(pass, THIN_ROWS, E, S, K, N);
+    const size_t x = g.may_cut ? Parts<thin::ROWS, 48>::bytes(g.ctas) : 0, y = middle_likely(E, S) && h.may_cut ? Parts<thin::ROWS, 128>::bytes(h.ctas) : 0;
+    return x > y ? x : y;
 }
 
 int grouped_thin_status(int *out, int reset) {
