@@ -55,8 +55,9 @@ __device__ __forceinline__ void copy_first_group(float *dst, const float *src, i
 //   up to THIN_ROWS     tagi_grouped_thin.cu  tensor cores, tiles of 128 features (forward and state pass)
 //   up to MIDDLE_ROWS   the same for up to 128 rows, if middle_likely()
 //   more                tagi_grouped_tc.cu    tensor cores, tiles of 256 features x up to 256 rows
-// Measured on eight experts of 4096 x 4096, forward pass, 4 / 8 / 16 / 32 rows each: few 220 / 307 / 522 / 936 us; thin 283 at 16;
-// 56 / 100 / 128 rows: middle 494 / 539 / 604 us, the wide kernel 813 / 843 / 862 us. Parameter pass at 7 / 10 / 14 / 20 rows: few
+// Measured on eight experts of 4096 x 4096, forward pass, 4 / 8 / 16 / 32 rows each: few 220 / 317 / 522 / 936 us; thin 279 / 314 /
+// 337 us at 16 / 32 / 40; 56 / 100 / 128 rows: middle 494 / 524 / 583 us, the wide kernel 813 / 843 / 862 us. (Of 1001 x 1001, 7 rows:
+// few 48, thin 70 us.) Parameter pass at 7 / 10 / 14 / 20 rows: few
 // 377 / 419 / 486 / 595 us, the wide kernel 503 to 507 us.
 constexpr int FEW_ROWS = 8, FEW_PARAM_ROWS = 14, THIN_ROWS = 48, MIDDLE_ROWS = 128;
 

@@ -463,7 +463,9 @@ __global__ void __launch_bounds__(THREADS, 1) grouped_tc_kernel(const GroupedArg
             bool more = true;
             for (int j = 0; more; j++) {
                 Record &r = sh.record[j % RECORDS];
-                if (j >= RECORDS && !mbar_wait(sh.item_empty + j % RECORDS, (j / RECORDS - 1) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_EMPTY))
+                // the same for all lanes: they look at the rest together
+                if (j >= RECORDS &&
+                    !__all_sync(0xffffffffu, mbar_wait(sh.item_empty + j % RECORDS, (j / RECORDS - 1) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_EMPTY)))
                     break;
                 Item t;
                 more = get_item<PASS>(a, sh, plan, pair, pairs, j, t);

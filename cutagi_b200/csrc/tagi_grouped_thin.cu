@@ -470,13 +470,14 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
         const uint32_t tm = uniform(tmem), base = uniform(smem_base);
         Item it;
         bool ok = true;
-        for (int j = 0, i = 0; ok && take(sh, j, it) && it.chunks > 0; j++) {
+        // (also whether a wait has ended: lanes that part would wait for one another)
+        for (int j = 0, i = 0; ok && __all_sync(0xffffffffu, take(sh, j, it) && it.chunks > 0); j++) {
             release(sh, j, lane);
             const int bn = uniform(it.bn), nk = uniform(it.nk), depth = uniform(it.depth), from = uniform(it.from), end = from + uniform(it.chunks);
             const uint32_t one = make_idesc_bf16(ROWS, bn, 0, 0), two = make_idesc_bf16(ROWS, 2 * bn, 0, 0), three = make_idesc_bf16(ROWS, 3 * bn, 0, 0);
             for (int c = from; c < end; c++, i++) {
                 const int s = i & 1, left = depth - (c >= nk ? c - nk : c) * KC, steps = min(KC / 16, (left + 15) / 16);
-                ok = mbar_wait(sh.full + s, (i >> 1) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_CONV);
+                ok = __all_sync(0xffffffffu, mbar_wait(sh.full + s, (i >> 1) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_CONV));
                 if (!ok) break;
                 tc_fence_after_sync();
                 const uint32_t x = tm + A_COL + s * A_SLOT, y = desc_lo(base + s * SLOT, 16), d = tm + s * ACC;
@@ -496,7 +497,9 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
         Plan plan = make_plan(PASS == FWD, 2 * sh.before[a.E], gridDim.x, may_cut);
         bool more = true;
         for (int j = 0; more; j++) {
-            if (j >= RECORDS && !mbar_wait(sh.item_empty + j % RECORDS, (j / RECORDS - 1) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_EMPTY)) break;
+            if (j >= RECORDS &&
+                !__all_sync(0xffffffffu, mbar_wait(sh.item_empty + j % RECORDS, (j / RECORDS - 1) & 1, &sh.abort_flag, &g_status, ST_TIMEOUT_EMPTY)))
+                break;
             Item t;
             get_item<PASS, COLS>(a, sh, plan, j, t);
             more = t.chunks > 0;
