@@ -7,9 +7,9 @@
 // Forward and state pass: a CTA computes 64 output columns of all the expert's rows. The weights come in slabs of 32
 // contraction steps through a ring of stages filled with cp.async, so that the bytes in flight cost no registers (two CTAs of
 // an SM keep about 100 KB on their way). Where there are too few tiles for that, a cluster of up to eight CTAs cuts the
-// contraction of a tile, and their sums are added through distributed shared memory in the order of the CTAs. Eight warps share a slab, four steps each; a
-// thread multiplies its two columns with all rows, whose entries all lanes read at the same address. The warps' sums are
-// added in a fixed order at the end.
+// contraction of a tile, and their sums are added through distributed shared memory in the order of the CTAs. Eight warps share
+// a slab, four steps each; a thread multiplies its two columns with all rows, whose entries all lanes read at the same address.
+// The warps' sums are added in a fixed order at the end.
 #include "tagi_grouped.h"
 
 namespace tagi {
@@ -20,8 +20,8 @@ static_assert(SLAB == 4 * WARPS, "a warp takes four steps of a slab");
 constexpr int PITCH = SLAB + 4;                          // floats of a weight row in shared memory: no bank conflicts
 constexpr int FWD_WEIGHTS = 2 * OUT * PITCH;
 // Rows that do not begin at multiples of 16 bytes are copied in the 16-byte groups of memory all the same, one more of them,
-// and begin up to three floats behind their place in shared memory. One row of two experts of 4095 x 4095, forward: 74 us,
-// with 4-byte copies 94 us; of 4096 x 4096 55 us.
+// and begin up to three floats behind their place in shared memory. One row of two experts of 4095 x 4095, forward: 70 us,
+// with 4-byte copies 94 us; of 4096 x 4096 57 us.
 __host__ __device__ constexpr int state_pitch(bool vec) { return vec ? OUT : OUT + 4; }
 __host__ __device__ constexpr int weights(int pass, bool vec) { return pass == FWD ? FWD_WEIGHTS : SLAB * state_pitch(vec); }
 __host__ __device__ constexpr int stages(int pass) { return pass == FWD ? 4 : 8; }   // a slab of both is 18 KiB, of means 8
@@ -55,7 +55,10 @@ __device__ __forceinline__ Pair mul2(Pair a, Pair b) {
 // float at the same place in the shared memory of CTA `cta` of the cluster
 __device__ __forceinline__ float remote(const float *p, int cta) {
     float v;
-    asm volatile("{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %1, %2;\n\tld.shared::cluster.f32 %0, [r];\n\t}" : "=f"(v) : "r"(smem_at(p)), "r"(cta) : "memory");
+    asm volatile("{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %1, %2;\n\tld.shared::cluster.f32 %0, [r];\n\t}"
+                 : "=f"(v)
+                 : "r"(smem_at(p)), "r"(cta)
+                 : "memory");
     return v;
 }
 __device__ __forceinline__ void cluster_sync() {
@@ -138,7 +141,7 @@ __device__ __forceinline__ void few_rows_pass(const GroupedArgs &a, int e, int r
                 if (has_extra) copy_group(s + (tid >> 6) * OUT * PITCH + extra * PITCH + GROUPS * 4, more, a.K - at + se - GROUPS * 4);
                 at += SLAB, pv += move;
             } else {
-                const int lm = a.K - at + sm - g, le = a.K - at + se - GROUPS * 4;   // a column behind the end: whatever, but for zeros in lines behind the last
+                const int lm = a.K - at + sm - g, le = a.K - at + se - GROUPS * 4;   // lines behind the last: zeros
                 float *d = s + n * SP + g;
                 if (tensor_begins && slab == 0 && sm != 0) copy_first_group(d, pm, sm, lm);
                 else copy_group(d, pm, k0 + n < a.N ? lm : 0);
@@ -258,8 +261,9 @@ __global__ void __launch_bounds__(THREADS, 2) grouped_few_kernel(const GroupedAr
 }
 
 // -------------------------------------------------------------------------------------------------------- parameters
-// A warp computes PARAM_N output features x 32 lanes of four input features (neighbours, or 32 apart where rows are not aligned: two a lane were slower from eight rows on); a CTA stacks 8 warps along the output features. The
-// prior variances are fetched before the rows are added up; the deltas come from shared memory, at one address for all lanes.
+// A warp computes PARAM_N output features x 32 lanes of four input features (neighbours, or 32 apart where rows are not aligned: two
+// a lane were slower from eight rows on); a CTA stacks 8 warps along the output features. The prior variances are fetched
+// before the rows are added up; the deltas come from shared memory, at one address for all lanes.
 constexpr int PARAM_N = 8, PARAM_OUT = WARPS * PARAM_N;
 
 // Four entries of a row, of which `left` follow from p on: neighbours (VEC: at least one is left), or 32 apart.
@@ -308,7 +312,8 @@ __global__ void __launch_bounds__(THREADS, 2) grouped_few_param_kernel(const Gro
     }
     for (int i = threadIdx.x; i < rows * 2 * PARAM_OUT; i += THREADS) {
         const int n = block_n + i % PARAM_OUT, r = i / (2 * PARAM_OUT);
-        delta[r][(i / PARAM_OUT) & 1][i % PARAM_OUT] = n < a.N ? __ldg(((i / PARAM_OUT) & 1 ? a.a1 : a.a0) + (size_t)(r0 + r) * a.N + n) : 0.f;
+        const float *from = (i / PARAM_OUT) & 1 ? a.a1 : a.a0;
+        delta[r][(i / PARAM_OUT) & 1][i % PARAM_OUT] = n < a.N ? __ldg(from + (size_t)(r0 + r) * a.N + n) : 0.f;
     }
     for (int r = threadIdx.x; r < rows; r += THREADS) input[r] = input_row(a, r0 + r);
     __syncthreads();

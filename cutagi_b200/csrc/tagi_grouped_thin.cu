@@ -337,7 +337,8 @@ grouped_thin_kernel(const __grid_constant__ CUtensorMap mean_map, const __grid_c
         // a warp loads 64 consecutive bytes of eight rows; two groups of four warps take turns at the chunks, or have half the rows
         if (!STACKED) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CONVERT_REGS));
         constexpr int TURNS = STACKED ? 2 : 1;
-        const int w = (warp - FIRST_B) & 3, half = (warp - FIRST_B) >> 2, turn = STACKED ? half : 0, row = (STACKED ? 0 : half * 64) + w * 8 + ((lane >> 2) & 3) * 2 + (lane >> 4), along = VEC ? (lane & 3) * 4 : lane & 3;
+        const int w = (warp - FIRST_B) & 3, half = (warp - FIRST_B) >> 2, turn = STACKED ? half : 0;
+        const int row = (STACKED ? 0 : half * 64) + w * 8 + ((lane >> 2) & 3) * 2 + (lane >> 4), along = VEC ? (lane & 3) * 4 : lane & 3;
         const uint32_t to = smem_base + row * 128 + ((((lane & 3) >> 1) ^ (row & 7)) << 4) + (lane & 1) * 8;
         float4 v[8];
         Item it;

@@ -370,7 +370,7 @@ int tagi_route_fwd(int T, int E, int k, const float *mu_s, const float *var_s, i
     const RouteArgs a{T, E, k, per_block(T), mu_s, var_s, expert, mu_g, var_g, offsets, token, pos, static_cast<int *>(workspace),
                       E % 4 == 0 && aligned16(mu_s)};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    // the smallest group that has a lane for each slot and at most 16 scores a lane (more spill)
+    // the smallest group that has a lane for each slot and at most 16 scores a lane (what 32 warps have registers for)
     if (k <= 8 && E <= 32) return route_launch<8, 4>(a, st);
     if (k <= 8 && E <= 64) return route_launch<8, 8>(a, st);
     if (k <= 8 && E <= 128) return route_launch<8, 16>(a, st);
